@@ -8,25 +8,12 @@
 // then reduce in a fixed order (xor shuffles inside the wave, LDS across the
 // 16 waves).  Ties go to the smaller index and NaN beats every number
 // (the first NaN wins), which is torch's argmax on CUDA/ROCm.
-#include "common.h"
+#include "sample_common.h"
 
 namespace rwkv7mi {
 
 constexpr int AM_THREADS = 1024;
 constexpr int AM_RUNS = 8;  // 8-element runs per lane in flight
-
-// (va, ia) better than (vb, ib)
-__device__ __forceinline__ bool am_better(float va, int64_t ia, float vb, int64_t ib) {
-  const bool na = va != va, nb = vb != vb;
-  if (na || nb) return na && (!nb || ia < ib);
-  return va > vb || (va == vb && ia < ib);
-}
-
-__device__ __forceinline__ bool am_better(float va, int ia, float vb, int ib) {
-  const bool na = va != va, nb = vb != vb;
-  if (na || nb) return na && (!nb || ia < ib);
-  return va > vb || (va == vb && ia < ib);
-}
 
 template <typename T>
 __device__ __forceinline__ void am_run(uint32_t (&w)[4], int64_t base, int64_t n, float& bv, int64_t& bi) {
@@ -136,18 +123,6 @@ constexpr int AP_THREADS = 256;
 constexpr int AP_LOADS = 2;  // 16-byte runs per lane
 template <typename T>
 constexpr int ap_chunk() { return AP_THREADS * AP_LOADS * (16 / (int)sizeof(T)); }
-
-__device__ __forceinline__ void am_wave_best(float& bv, int& bi) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float ov = __shfl_xor(bv, o, 64);
-    const int oi = __shfl_xor(bi, o, 64);
-    if (am_better(ov, oi, bv, bi)) {
-      bv = ov;
-      bi = oi;
-    }
-  }
-}
 
 template <typename T>
 __global__ __launch_bounds__(AP_THREADS) void argmax_part_kernel(const T* __restrict__ x, int n, int64_t ld,

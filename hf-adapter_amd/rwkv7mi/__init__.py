@@ -27,6 +27,13 @@ from .native_quant_mm4 import (
     quantize_model_mm4,
 )
 from .sm70_quant import quantize_w4_groupwise, w4_groupwise_linear
+from .native_quant_mxfp4 import (
+    MXFP4Linear,
+    dequantize_mxfp4,
+    mxfp4_linear,
+    quantize_model_mxfp4,
+    quantize_mxfp4,
+)
 from .native_wkv_fp16 import (
     native_fp16_recurrent_available,
     native_fp16_recurrent_build_error,
@@ -34,7 +41,7 @@ from .native_wkv_fp16 import (
     native_fp16_recurrent_should_use,
     native_fp16_sequence,
 )
-from .sampling import argmax_rows
+from .sampling import argmax_rows, process_logits
 from . import ops as _ops
 
 _ops.register()  # torch.ops.rwkv7mi.*
@@ -62,7 +69,13 @@ __all__ = [
     "quantize_model_mm4",
     "quantize_w4_groupwise",
     "w4_groupwise_linear",
+    "quantize_mxfp4",
+    "dequantize_mxfp4",
+    "mxfp4_linear",
+    "MXFP4Linear",
+    "quantize_model_mxfp4",
     "argmax_rows",
+    "process_logits",
     "native_fp16_recurrent_should_use",
     "native_fp16_recurrent_available",
     "native_fp16_recurrent_build_error",

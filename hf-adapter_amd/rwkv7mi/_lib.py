@@ -6,6 +6,7 @@ if the library is missing every operator raises RuntimeError.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -131,6 +132,14 @@ SIGNATURES = {
         _i32,
         [_c_p] * 6 + [_i64, _i64, _i64, _i64, _i32, _i32, _i32, _c_p],
     ),
+    "rwkv7mi_mxfp4_quantize": (_i32, [_c_p, _i64, _i64, _i64, _i32, _c_p, _c_p, _c_p]),
+    "rwkv7mi_mxfp4_dequantize": (_i32, [_c_p, _c_p, _i64, _i64, _c_p, _i32, _c_p]),
+    "rwkv7mi_mxfp4_linear_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64, _i32, _i32]),
+    "rwkv7mi_mxfp4_linear": (_i32, [_i32] + [_c_p] * 7 + [_i64, _i64, _i64, _i32, _i32, _c_p, _i64, _c_p]),
+    "rwkv7mi_process_logits_workspace_bytes": (_sz, [_i64, _i64]),
+    "rwkv7mi_process_logits": (
+        _i32, [_c_p, _i64, _i64, _i64, _i32, _c_p, _i64, _i32, _c_p, _i32, _i64, _i64, _c_p, _c_p, _c_p, _i32, _c_p, _i64,
+               _c_p, _i64, _c_p, _c_p, _i32, _c_p, _sz, _c_p]),
     "rwkv7mi_attn_norm_mix6": (
         _i32, [_c_p] * 8 + [_i64, _i64, _i64, _f32, _i32, _i32, _c_p],
     ),
@@ -214,6 +223,30 @@ def stream_of(t: torch.Tensor):
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
+def on_device(t: torch.Tensor):
+    """A context in which ``t``'s device is the current one (kernels launch on the
+    current device; no work where it already is)."""
+    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def require_same_device(*tensors: torch.Tensor | None, name: str) -> None:
+    """Every given tensor is on the first one's GPU."""
+    require_gpu(*tensors, name=name)
+    devices = {t.get_device() for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"{name}: tensors on different devices {sorted(devices)}")
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors (any strides) meet."""
+    def ends(t):
+        n = 1 + sum((int(s) - 1) * st for s, st in zip(t.shape, t.stride())) if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+    (a0, a1), (b0, b1) = ends(a), ends(b)
+    return a0 < b1 and b0 < a1
+
+
 def require_gpu(*tensors: torch.Tensor | None, name: str) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
@@ -227,5 +260,6 @@ def require_gpu(*tensors: torch.Tensor | None, name: str) -> None:
 
 __all__ = [
     "F32", "F16", "BF16", "EPI_NONE", "EPI_RELU2", "EPI_RESIDUAL", "LIB_PATH", "SIGNATURES",
-    "load", "call", "dtype_code", "ptr", "stream_of", "require_gpu", "declared_symbols",
+    "load", "call", "dtype_code", "ptr", "stream_of", "require_gpu", "require_same_device", "on_device", "overlap",
+    "declared_symbols",
 ]

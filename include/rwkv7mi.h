@@ -678,6 +678,33 @@ int rwkv7mi_argmax_rows_ws(const void* x, int64_t rows, int64_t n, int64_t ld,
                            int dtype, int64_t* out, int64_t* out2,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/* The logits step of each row of x [rows, V] (rows ldx apart) into out (ldo
+ * apart; x's dtype or fp32; out may be x itself):
+ *   c[t] = sum over the row's history h[0..n-1], h[i] = t, of decay^(n - 1 - i)
+ *   where t is in the history: l = l > 0 ? l / repetition : l * repetition,
+ *                              then l -= presence + frequency c[t]
+ *   l += bias[t];  bit t of the row's words in allowed clear: l = -inf
+ * in fp32, rounded once.  history [rows, L] of 32- or 64-bit tokens (NULL: none;
+ * at most 2^23 a row, those outside 0..V-1 ignored), the first lengths[row] of a
+ * row (NULL: L).  penalties / penalty: the four of repetition, presence,
+ * frequency, decay (decay in 0..1, `decayed` nonzero unless every decay is 1),
+ * each a device array [rows], or NULL for the one value.  bias, allowed: row
+ * strides ldb, lda (0: one row for all; allowed in 32-bit words).
+ * next (NULL: none), next2: the first index of each rounded row's maximum (NaN
+ * counts as the maximum; 0 where nothing is allowed), which needs the workspace.
+ * append: the token also goes behind the row's history, whose length grows by
+ * one, where there is room. */
+size_t rwkv7mi_process_logits_workspace_bytes(int64_t rows, int64_t V);
+int rwkv7mi_process_logits(const void* x, int64_t rows, int64_t V, int64_t ldx,
+                           int dtype, void* out, int64_t ldo, int out_dtype,
+                           void* history, int history_bits, int64_t ldh,
+                           int64_t L, int* lengths,
+                           const float* const* penalties, const float* penalty,
+                           int decayed, const float* bias, int64_t ldb,
+                           const uint32_t* allowed, int64_t lda, int64_t* next,
+                           int64_t* next2, int append, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ LoRA */
 
 /* Bytes of workspace rwkv7mi_lora_multi uses: fp32 split-K partials of one
@@ -758,6 +785,42 @@ int rwkv7mi_w4_matmul_ws(const void* x, const uint8_t* packed,
                          int64_t rows, int64_t O, int64_t I, int64_t group,
                          int epilogue, int act_dtype, int scale_dtype,
                          void* ws, int64_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------ MXFP4 */
+
+/* Microscaled 4-bit floating point (OCP MX): blocks of 32 consecutive inputs of
+ * a row share a scale byte e, 2^(e - 127) (255: NaN); codes are e2m1 (0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6 and the sign), two a byte, the even input in the low nibble.
+ * codes [rows, I/2], scales [rows, I/32]; I % 32 == 0.
+ *
+ * Quantises x [rows, I] of any dtype code, rows ld elements apart (16-byte
+ * aligned): e = max(floor(log2 amax) - 2 + 127, 0), codes to nearest, ties to
+ * even, at most 6.  A block with an infinity or a NaN gets e = 255, codes 0. */
+int rwkv7mi_mxfp4_quantize(const void* x, int64_t rows, int64_t I, int64_t ld,
+                           int dtype, uint8_t* codes, uint8_t* scales,
+                           void* stream);
+/* y [rows, I] = the values of the codes, rounded to dtype. */
+int rwkv7mi_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales,
+                             int64_t rows, int64_t I, void* y, int dtype,
+                             void* stream);
+/* y = epilogue(x W^T + bias) for nprob (1..4) products of one shape: x [rows, I]
+ * and y [rows, O] fp16 / bf16 (bias [O] and residual [rows, O] alike, NULL: none),
+ * W [O, I] in MXFP4, fp32 accumulation.  quantize_input: x is quantised to MXFP4
+ * first and both operands go through the scaled MFMA.  x and the codes 16-byte
+ * aligned, the scales 4-byte.  Needs a 16-byte aligned workspace of
+ * rwkv7mi_mxfp4_linear_workspace_bytes bytes (0: none); calls in flight at once
+ * must not share it.  y may be the residual itself; it must not overlap x. */
+int64_t rwkv7mi_mxfp4_linear_workspace_bytes(int nprob, int64_t rows, int64_t O,
+                                             int64_t I, int act_dtype,
+                                             int quantize_input);
+int rwkv7mi_mxfp4_linear(int nprob, const void* const* x,
+                         const uint8_t* const* codes,
+                         const uint8_t* const* scales,
+                         const void* const* bias, const void* const* residual,
+                         void* const* y, const int* epilogue, int64_t rows,
+                         int64_t O, int64_t I, int act_dtype,
+                         int quantize_input, void* ws, int64_t ws_bytes,
+                         void* stream);
 
 /* ------------------------------------------------ LayerNorm + token shift */
 
