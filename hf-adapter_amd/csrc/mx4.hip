@@ -19,6 +19,7 @@ struct Mx4Quant {
   uint8_t *codes[MX4_MAXPROB], *scales[MX4_MAXPROB];
   int64_t n8, ld;  // runs of 8 values in all, row stride of x
   int row8;        // runs of 8 values in a row
+  int in8;         // of which hold values (PADDED: the rest are zeros)
 };
 
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
@@ -28,15 +29,16 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 
 }  // namespace
 
-template <typename T>
+// PADDED: rows padded to whole supersteps, their scales in the GEMM's order
+template <typename T, bool PADDED>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const Mx4Quant Q) {
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (t >= Q.n8) return;  // (n8 is a multiple of 4: a block's lanes stay together)
   const int p = blockIdx.y;
   const int64_t row = t / Q.row8;
-  const int64_t src = row * Q.ld + (t - row * Q.row8) * 8;
-  float v[8];
-  ld8(static_cast<const T*>(Q.x[p]) + src, v);
+  const int run = (int)(t - row * Q.row8);
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (!PADDED || run < Q.in8) ld8(static_cast<const T*>(Q.x[p]) + row * Q.ld + 8 * (int64_t)run, v);
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
@@ -52,7 +54,11 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const Mx4Quant Q) {
     d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, v[6], v[7], s, 3);
   }
   reinterpret_cast<uint32_t*>(Q.codes[p])[t] = d;
-  if ((t & 3) == 0) Q.scales[p][t >> 2] = (uint8_t)e;
+  if ((t & 3) == 0) {
+    int64_t b = t >> 2;
+    if (PADDED) b = (b & ~15) | (b & 3) << 2 | (b >> 2 & 3);
+    Q.scales[p][b] = (uint8_t)e;
+  }
 }
 
 template <typename T>
@@ -70,23 +76,35 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __r
   st8(y + 8 * t, v);
 }
 
-int mx4_quantize_run(int nprob, const void* const* x, int64_t rows, int64_t I, int64_t ld, int dtype,
-                     uint8_t* const* codes, uint8_t* const* scales, void* stream) {
+static int mx4_quantize_go(int nprob, const void* const* x, int64_t rows, int64_t I, int64_t ld, int dtype, bool padded,
+                           uint8_t* const* codes, uint8_t* const* scales, void* stream) {
   Mx4Quant q{};
   for (int i = 0; i < nprob; ++i) {
     q.x[i] = x[i];
     q.codes[i] = codes[i];
     q.scales[i] = scales[i];
   }
-  q.row8 = (int)(I / 8);
+  q.in8 = (int)(I / 8);
+  q.row8 = padded ? (int)((I + 511) / 512 * 64) : q.in8;
   q.n8 = rows * q.row8;
   q.ld = ld;
   const dim3 grid((unsigned)((q.n8 + 255) / 256), (unsigned)nprob);
   return dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL(mx4_quantize_kernel<T>, grid, dim3(256), 0, as_stream(stream), q);
+    if (padded)
+      hipLaunchKernelGGL((mx4_quantize_kernel<T, true>), grid, dim3(256), 0, as_stream(stream), q);
+    else
+      hipLaunchKernelGGL((mx4_quantize_kernel<T, false>), grid, dim3(256), 0, as_stream(stream), q);
     return check_launch("mx4_quantize_kernel");
   });
+}
+int mx4_quantize_run(int nprob, const void* const* x, int64_t rows, int64_t I, int64_t ld, int dtype,
+                     uint8_t* const* codes, uint8_t* const* scales, void* stream) {
+  return mx4_quantize_go(nprob, x, rows, I, ld, dtype, false, codes, scales, stream);
+}
+int mx4_quantize_padded(int nprob, const void* const* x, int64_t rows, int64_t I, int dtype, uint8_t* const* codes,
+                        uint8_t* const* scales, void* stream) {
+  return mx4_quantize_go(nprob, x, rows, I, I, dtype, true, codes, scales, stream);
 }
 
 }  // namespace rwkv7mi

@@ -35,6 +35,20 @@ struct Mx4Batch {
 // field alone; 255 gives NaN).
 __device__ __forceinline__ float mx4_scale(uint32_t e) { return __uint_as_float(e << 23); }
 
+// fp16 weights are scaled relative to the largest scale byte emax of a run of
+// inputs: a block's codes by 2^(13 + e - emax) (at most 6 x 2^13, exact down to
+// 2^-36 of the largest scale, rounding at 2^-24 below), the sums over the run by
+// the factor 2^(emax - 127 - 13) (NaN for emax = 255) in fp32.
+__device__ __forceinline__ float mx4_relative(uint32_t e, uint32_t emax) {
+  return mx4_scale((uint32_t)max(140 + (int)e - (int)emax, 1));
+}
+__device__ __forceinline__ float mx4_factor(uint32_t emax) {
+  return emax == 255u ? __builtin_nanf("") : ldexpf(1.f, (int)emax - 140);
+}
+__device__ __forceinline__ uint32_t mx4_factor_exponent(float f) {  // emax again
+  return f != f ? 255u : (uint32_t)(ilogbf(f) + 140);
+}
+
 // 8 codes of a dword -> 8 values times the scale, in order
 __device__ __forceinline__ void mx4_decode8(uint32_t d, float s, bf16x8& o) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 0);
@@ -54,14 +68,18 @@ __device__ __forceinline__ void mx4_decode8(uint32_t d, float s, f16x8& o) {
 template <typename T> struct Mx4Types { typedef f16x8 V; };
 template <> struct Mx4Types<__hip_bfloat16> { typedef bf16x8 V; };
 
+__device__ __forceinline__ float mx4_relu2(float v) {
+  v = v < 0.f ? 0.f : v;  // (NaN stays)
+  return v * v;
+}
+
 // v (+ bias) through the epilogue, rounded once
 template <typename T>
 __device__ __forceinline__ void mx4_store(const Mx4Prob& P, int64_t row, int o, int O, float v) {
   const int64_t i = row * O + o;
   if (P.bias) v += ld(static_cast<const T*>(P.bias), o);
   if (P.epilogue == RWKV7MI_EPI_RELU2) {
-    v = v > 0.f ? v : (v != v ? v : 0.f);  // (NaN stays)
-    v = v * v;
+    v = mx4_relu2(v);
   } else if (P.epilogue == RWKV7MI_EPI_RESIDUAL) {
     v += ld(static_cast<const T*>(P.residual), i);
   }
@@ -71,5 +89,20 @@ __device__ __forceinline__ void mx4_store(const Mx4Prob& P, int64_t row, int o, 
 // Quantises nprob inputs of [rows, I] values (row stride ld) into codes / scales (mx4.hip).
 int mx4_quantize_run(int nprob, const void* const* x, int64_t rows, int64_t I, int64_t ld, int dtype,
                      uint8_t* const* codes, uint8_t* const* scales, void* stream);
+// The same into rows padded with zeros to NS = ceil(I / 512) supersteps: codes [rows, 256 NS] bytes, scales
+// [rows, 16 NS] with block 4 h + q of a superstep at byte 4 q + h.
+int mx4_quantize_padded(int nprob, const void* const* x, int64_t rows, int64_t I, int dtype, uint8_t* const* codes,
+                        uint8_t* const* scales, void* stream);
+
+// Products of two MXFP4 operands of many rows (mx4_gemm.hip): x is quantised there.
+bool mx4_gemm_supported(int64_t rows, int64_t O, int64_t I);
+int64_t mx4_gemm_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I);
+int mx4_gemm_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* stream);
+
+// Products through fp16 / bf16 records of the weight and the 256 x 256 GEMM
+// (mm8h.hip): whether it takes these shapes, its workspace, its launches.
+bool mx4h_supported(int64_t rows, int64_t I, int64_t O);
+int64_t mx4h_workspace_bytes(int nprob, int64_t rows, int64_t I, int64_t O);
+int mx4h_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, int64_t ws_bytes, void* stream);
 
 }  // namespace rwkv7mi

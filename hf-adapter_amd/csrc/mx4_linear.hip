@@ -9,10 +9,8 @@
 //  * four v_mfma_f32_16x16x32 where x is 16-bit: MFMA j takes inputs 8 j .. +7
 //    of every lane's block, and so do the rows of x.
 // bf16 holds a scaled code exactly.  fp16 does not for every scale, so there a
-// step's codes are scaled to 2^(13 + e - emax), emax the largest of the four
-// blocks' exponents, and the step's sums by 2^(emax - 13) in fp32: codes whose
-// scale is within 2^36 of the step's largest stay exact (fp16 subnormals), and
-// smaller ones round at 2^-38 of the step's largest weight.
+// step's codes are scaled relative to the largest of its four scales and the
+// step's sums by that one's factor (mx4_common.h).
 #include <algorithm>
 
 #include "mx4_common.h"
@@ -41,15 +39,6 @@ __device__ __forceinline__ uint32_t mx4_exps(const uint8_t* row, int b, int nb) 
 
 __device__ __forceinline__ uint32_t max4(uint32_t v) {
   return max(max(v & 255u, (v >> 8) & 255u), max((v >> 16) & 255u, v >> 24));
-}
-
-// the factor of a step's fp16 sums, 2^(emax - 127 - 13)
-__device__ __forceinline__ float mx4_step_scale(uint32_t emax) {
-  return emax == 255u ? __builtin_nanf("") : ldexpf(1.f, (int)emax - 140);
-}
-// the scale of a block's codes within its step: 2^(13 + e - emax)
-__device__ __forceinline__ float mx4_step_rel(uint32_t e, uint32_t emax) {
-  return mx4_scale((uint32_t)max(140 + (int)e - (int)emax, 1));
 }
 
 }  // namespace
@@ -88,7 +77,7 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Batch B) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) a[j] = ok ? *reinterpret_cast<const u32x4*>(x + 32 * (b + q) + 8 * j) : zero;
       const uint32_t emax = F16 ? max4(ex) : 0u;
-      const float s = F16 ? mx4_step_rel(e, emax) : mx4_scale(e);
+      const float s = F16 ? mx4_relative(e, emax) : mx4_scale(e);
       f32x4 c = F16 ? (f32x4){0.f, 0.f, 0.f, 0.f} : acc;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -96,7 +85,7 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Batch B) {
         mx4_decode8(w[j], s, wv);
         c = mfma16x16x32(__builtin_bit_cast(V, a[j]), wv, c);
       }
-      acc = F16 ? acc + mx4_step_scale(emax) * c : c;
+      acc = F16 ? acc + mx4_factor(emax) * c : c;
     }
   }
 
@@ -130,6 +119,11 @@ static int mx4_rows_run(const Mx4Batch& b, int nprob, void* stream) {
 static int64_t mx4_codes_bytes(int64_t rows, int64_t I) { return (rows * (I / 2) + 255) & ~(int64_t)255; }
 static int64_t mx4_scales_bytes(int64_t rows, int64_t I) { return (rows * (I / MX4_BLOCK) + 255) & ~(int64_t)255; }
 
+// Rows from which a product pays for materialising the weight.
+static bool mx4_prefill(int64_t rows, int64_t I, int64_t O) { return rows > 256 && mx4h_supported(rows, I, O); }
+// Quantised rows of more than one tile of the few-row kernel.
+static bool mx4_gemm(int64_t rows, int64_t I, int64_t O) { return rows > 16 && mx4_gemm_supported(rows, O, I); }
+
 }  // namespace rwkv7mi
 
 using namespace rwkv7mi;
@@ -137,7 +131,9 @@ using namespace rwkv7mi;
 extern "C" int64_t rwkv7mi_mxfp4_linear_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I, int act_dtype,
                                                         int quantize_input) {
   if (nprob < 1 || nprob > MX4_MAXPROB || rows <= 0 || O <= 0 || I <= 0) return 0;
-  return quantize_input ? nprob * (mx4_codes_bytes(rows, I) + mx4_scales_bytes(rows, I)) : 0;
+  if (quantize_input && mx4_gemm(rows, I, O)) return mx4_gemm_workspace_bytes(nprob, rows, O, I);
+  if (quantize_input) return nprob * (mx4_codes_bytes(rows, I) + mx4_scales_bytes(rows, I));
+  return mx4_prefill(rows, I, O) ? mx4h_workspace_bytes(nprob, rows, I, O) : 0;
 }
 
 extern "C" int rwkv7mi_mxfp4_linear(int nprob, const void* const* x, const uint8_t* const* codes,
@@ -170,12 +166,14 @@ extern "C" int rwkv7mi_mxfp4_linear(int nprob, const void* const* x, const uint8
     if (p.epilogue == RWKV7MI_EPI_RESIDUAL && !p.residual) return fail(RWKV7MI_EINVAL, w + ": residual missing");
   }
   const bool bf = act_dtype == RWKV7MI_BF16;
-  if (!quantize_input)
-    return bf ? mx4_rows_run<__hip_bfloat16, false>(b, nprob, stream) : mx4_rows_run<__half, false>(b, nprob, stream);
-  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 15) ||
-      ws_bytes < rwkv7mi_mxfp4_linear_workspace_bytes(nprob, rows, O, I, act_dtype, 1))
+  const int64_t need = rwkv7mi_mxfp4_linear_workspace_bytes(nprob, rows, O, I, act_dtype, quantize_input);
+  if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < need))
     return fail(RWKV7MI_ESIZE, w + ": workspace missing, unaligned or smaller than "
                                    "rwkv7mi_mxfp4_linear_workspace_bytes");
+  if (!quantize_input && mx4_prefill(rows, I, O)) return mx4h_run(b, nprob, act_dtype, ws, ws_bytes, stream);
+  if (!quantize_input)
+    return bf ? mx4_rows_run<__hip_bfloat16, false>(b, nprob, stream) : mx4_rows_run<__half, false>(b, nprob, stream);
+  if (mx4_gemm(rows, I, O)) return mx4_gemm_run(b, nprob, act_dtype, ws, stream);
   uint8_t *xc[MX4_MAXPROB], *xs[MX4_MAXPROB];
   uint8_t* at = static_cast<uint8_t*>(ws);
   for (int i = 0; i < nprob; ++i) {
