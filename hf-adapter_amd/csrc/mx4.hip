@@ -17,7 +17,7 @@ namespace {
 struct Mx4Quant {
   const void* x[MX4_MAXPROB];
   uint8_t *codes[MX4_MAXPROB], *scales[MX4_MAXPROB];
-  int64_t n8, ld;  // runs of 8 values in all, row stride of x
+  int64_t rows, n8, ld;  // rows, runs of 8 values in all, row stride of x
   int row8;        // runs of 8 values in a row
   int in8;         // of which hold values (PADDED: the rest are zeros)
 };
@@ -56,7 +56,8 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const Mx4Quant Q) {
   reinterpret_cast<uint32_t*>(Q.codes[p])[t] = d;
   if ((t & 3) == 0) {
     int64_t b = t >> 2;
-    if (PADDED) b = (b & ~15) | (b & 3) << 2 | (b >> 2 & 3);
+    if (PADDED)  // [superstep][row][16]
+      b = ((run >> 6) * Q.rows + row) * 16 + ((b & 1) << 3 | (b >> 3 & 1) << 2 | (b >> 1 & 3));
     Q.scales[p][b] = (uint8_t)e;
   }
 }
@@ -84,6 +85,7 @@ static int mx4_quantize_go(int nprob, const void* const* x, int64_t rows, int64_
     q.codes[i] = codes[i];
     q.scales[i] = scales[i];
   }
+  q.rows = rows;
   q.in8 = (int)(I / 8);
   q.row8 = padded ? (int)((I + 511) / 512 * 64) : q.in8;
   q.n8 = rows * q.row8;

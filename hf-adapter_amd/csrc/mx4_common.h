@@ -90,7 +90,7 @@ __device__ __forceinline__ void mx4_store(const Mx4Prob& P, int64_t row, int o, 
 int mx4_quantize_run(int nprob, const void* const* x, int64_t rows, int64_t I, int64_t ld, int dtype,
                      uint8_t* const* codes, uint8_t* const* scales, void* stream);
 // The same into rows padded with zeros to NS = ceil(I / 512) supersteps: codes [rows, 256 NS] bytes, scales
-// [rows, 16 NS] with block 4 h + q of a superstep at byte 4 q + h.
+// [NS, rows, 16] with block 8 s + 2 h + u of a superstep at byte 8 u + 4 s + h.
 int mx4_quantize_padded(int nprob, const void* const* x, int64_t rows, int64_t I, int dtype, uint8_t* const* codes,
                         uint8_t* const* scales, void* stream);
 
