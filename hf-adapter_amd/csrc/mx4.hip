@@ -20,6 +20,10 @@ struct Mx4Quant {
   int64_t rows, n8, ld;  // rows, runs of 8 values in all, row stride of x
   int row8;        // runs of 8 values in a row
   int in8;         // of which hold values (PADDED: the rest are zeros)
+  // PADDED: the weights' scales too, in the workgroups from qblocks on
+  const uint8_t* win[MX4_MAXPROB];
+  uint32_t* wout[MX4_MAXPROB];
+  int qblocks, O, nb, NS;
 };
 
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
@@ -29,12 +33,32 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 
 }  // namespace
 
-// PADDED: rows padded to whole supersteps, their scales in the GEMM's order
+// W's scales [O, nb] in the products' order [superstep][column][16], padded to whole
+// supersteps (1.0 there): one thread a dword (the four blocks of lane half u in a step)
+__device__ __forceinline__ void mx4_weight_scales(const Mx4Quant& Q, int p, int64_t t) {
+  if (t >= (int64_t)Q.O * 4 * Q.NS) return;
+  const int o = (int)(t / (4 * Q.NS)), d = (int)(t % (4 * Q.NS)), b0 = 16 * (d >> 2) + 8 * (d & 1) + (d >> 1 & 1);
+  const uint8_t* s = Q.win[p] + (int64_t)o * Q.nb;
+  uint32_t v = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int b = b0 + 2 * i;
+    v |= (b < Q.nb ? (uint32_t)s[b] : 127u) << (8 * i);
+  }
+  Q.wout[p][((int64_t)(d >> 2) * Q.O + o) * 4 + (d & 3)] = v;
+}
+
+// PADDED: rows padded to whole supersteps, their scales in the GEMM's order; the
+// same launch orders the weights' scales (a launch of their own took 4 us)
 template <typename T, bool PADDED>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const Mx4Quant Q) {
+  const int p = blockIdx.y;
+  if (PADDED && (int)blockIdx.x >= Q.qblocks) {
+    mx4_weight_scales(Q, p, (int64_t)(blockIdx.x - Q.qblocks) * 256 + threadIdx.x);
+    return;
+  }
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (t >= Q.n8) return;  // (n8 is a multiple of 4: a block's lanes stay together)
-  const int p = blockIdx.y;
   const int64_t row = t / Q.row8;
   const int run = (int)(t - row * Q.row8);
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -77,9 +101,8 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __r
   st8(y + 8 * t, v);
 }
 
-static int mx4_quantize_go(int nprob, const void* const* x, int64_t rows, int64_t I, int64_t ld, int dtype, bool padded,
-                           uint8_t* const* codes, uint8_t* const* scales, void* stream) {
-  Mx4Quant q{};
+static int mx4_quantize_go(Mx4Quant& q, int nprob, const void* const* x, int64_t rows, int64_t I, int64_t ld, int dtype,
+                           bool padded, uint8_t* const* codes, uint8_t* const* scales, void* stream) {
   for (int i = 0; i < nprob; ++i) {
     q.x[i] = x[i];
     q.codes[i] = codes[i];
@@ -87,10 +110,11 @@ static int mx4_quantize_go(int nprob, const void* const* x, int64_t rows, int64_
   }
   q.rows = rows;
   q.in8 = (int)(I / 8);
-  q.row8 = padded ? (int)((I + 511) / 512 * 64) : q.in8;
+  q.row8 = padded ? q.NS * 64 : q.in8;
   q.n8 = rows * q.row8;
   q.ld = ld;
-  const dim3 grid((unsigned)((q.n8 + 255) / 256), (unsigned)nprob);
+  q.qblocks = (int)((q.n8 + 255) / 256);
+  const dim3 grid((unsigned)(q.qblocks + (padded ? ((int64_t)q.O * 4 * q.NS + 255) / 256 : 0)), (unsigned)nprob);
   return dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     if (padded)
@@ -102,11 +126,22 @@ static int mx4_quantize_go(int nprob, const void* const* x, int64_t rows, int64_
 }
 int mx4_quantize_run(int nprob, const void* const* x, int64_t rows, int64_t I, int64_t ld, int dtype,
                      uint8_t* const* codes, uint8_t* const* scales, void* stream) {
-  return mx4_quantize_go(nprob, x, rows, I, ld, dtype, false, codes, scales, stream);
+  Mx4Quant q{};
+  return mx4_quantize_go(q, nprob, x, rows, I, ld, dtype, false, codes, scales, stream);
 }
-int mx4_quantize_padded(int nprob, const void* const* x, int64_t rows, int64_t I, int dtype, uint8_t* const* codes,
-                        uint8_t* const* scales, void* stream) {
-  return mx4_quantize_go(nprob, x, rows, I, I, dtype, true, codes, scales, stream);
+int mx4_quantize_padded(const Mx4Batch& b, int nprob, int dtype, uint8_t* const* codes, uint8_t* const* scales,
+                        uint8_t* const* wscales, void* stream) {
+  Mx4Quant q{};
+  const void* x[MX4_MAXPROB];
+  for (int i = 0; i < nprob; ++i) {
+    x[i] = b.p[i].x;
+    q.win[i] = b.p[i].ws;
+    q.wout[i] = reinterpret_cast<uint32_t*>(wscales[i]);
+  }
+  q.O = b.O;
+  q.nb = b.I / MX4_BLOCK;
+  q.NS = (b.I + 511) / 512;
+  return mx4_quantize_go(q, nprob, x, b.rows, b.I, b.I, dtype, true, codes, scales, stream);
 }
 
 }  // namespace rwkv7mi

@@ -89,10 +89,11 @@ __device__ __forceinline__ void mx4_store(const Mx4Prob& P, int64_t row, int o, 
 // Quantises nprob inputs of [rows, I] values (row stride ld) into codes / scales (mx4.hip).
 int mx4_quantize_run(int nprob, const void* const* x, int64_t rows, int64_t I, int64_t ld, int dtype,
                      uint8_t* const* codes, uint8_t* const* scales, void* stream);
-// The same into rows padded with zeros to NS = ceil(I / 512) supersteps: codes [rows, 256 NS] bytes, scales
-// [NS, rows, 16] with block 8 s + 2 h + u of a superstep at byte 8 u + 4 s + h.
-int mx4_quantize_padded(int nprob, const void* const* x, int64_t rows, int64_t I, int dtype, uint8_t* const* codes,
-                        uint8_t* const* scales, void* stream);
+// The same for the products of b, rows padded with zeros to NS = ceil(I / 512) supersteps: codes [rows, 256 NS]
+// bytes, scales [NS, rows, 16] with block 8 s + 2 h + u of a superstep at byte 8 u + 4 s + h, and the weights'
+// scales in that order, wscales [NS, O, 16].
+int mx4_quantize_padded(const Mx4Batch& b, int nprob, int dtype, uint8_t* const* codes, uint8_t* const* scales,
+                        uint8_t* const* wscales, void* stream);
 
 // Products of two MXFP4 operands of many rows (mx4_gemm.hip): x is quantised there.
 bool mx4_gemm_supported(int64_t rows, int64_t O, int64_t I);

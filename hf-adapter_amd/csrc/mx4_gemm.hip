@@ -19,8 +19,8 @@
 //    conflicts on gfx950.  Lane n + 32 u reads chunk 2 h + u in sub-step h;
 //  * scales: two steps (16 blocks, a superstep) at a time, global -> LDS, 16 bytes
 //    a row, in the order [u][step][sub-step], so that one dword serves a step's
-//    four sub-steps through the instruction's byte select.  The quantiser writes
-//    x's that way and a pre-pass W's, the rows of a superstep side by side (16
+//    four sub-steps through the instruction's byte select.  The quantiser's launch
+//    writes both that way, the rows of a superstep side by side (16
 //    bytes a row, rows apart, were a third of the kernel's L2 requests);
 //  * x, and both scales, are padded to whole supersteps: x with zeros, so nothing
 //    past I counts (W's codes there are some finite value).
@@ -373,24 +373,6 @@ __global__ __launch_bounds__(256) void mx4_gemm_reduce_kernel(const MgArgs B) {
   }
 }
 
-// W's scales in the products' order [superstep][column][16], padded to whole
-// supersteps (1.0 there): one thread a dword (the four blocks of lane half u in a
-// step)
-__global__ __launch_bounds__(256) void mx4_gemm_scales_kernel(const MgArgs B, uint8_t* out, int64_t each) {
-  const int nb = B.I / MX4_BLOCK;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= (int64_t)B.O * 4 * B.NS) return;
-  const int o = (int)(t / (4 * B.NS)), d = (int)(t % (4 * B.NS)), b0 = 16 * (d >> 2) + 8 * (d & 1) + (d >> 1 & 1);
-  const uint8_t* s = B.p[blockIdx.y].ws + (int64_t)o * nb;
-  uint32_t v = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int b = b0 + 2 * i;
-    v |= (b < nb ? (uint32_t)s[b] : 127u) << (8 * i);
-  }
-  reinterpret_cast<uint32_t*>(out + blockIdx.y * each)[((int64_t)(d >> 2) * B.O + o) * 4 + (d & 3)] = v;
-}
-
 static int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 struct MgPlan {
   int mi, S;                       // rows of a workgroup / 64, K splits
@@ -402,14 +384,42 @@ static MgPlan mg_plan(int nprob, int64_t rows, int64_t O, int64_t I) {
   p.codes = up256(rows * 256 * p.NS);
   p.scales = up256(rows * 16 * p.NS);
   p.pad = up256(O * 16 * p.NS);
-  p.mi = rows <= 64 ? 1 : rows <= 128 ? 2 : 4;
+  // The cheapest by an estimate in us: rounds of 256 workgroups (one a CU), each a
+  // start and an epilogue and its supersteps, slower with the chip busy, and for
+  // splits the second launch and the partials' traffic.  Fitted to 20 shapes from 17 x
+  // 2048 -> 2048 to 7000 x 2048 -> 2048, every tile height and split timed, e.g. 1000 x
+  // 4096 -> 4096: 64 rows a tile 27.7, 128 rows 30.3, 256 rows 38.2; 4000 rows: 83, 63,
+  // 54; 1000 x 16384 -> 4096: 128 rows in two splits 71, unsplit 92.
+  p.mi = 1;
   p.S = 1;
-  const int64_t tiles = nprob * ((rows + 64 * p.mi - 1) / (64 * p.mi)) * ((O + MG_N - 1) / MG_N);
-  while (p.S < 8 && tiles * p.S * 2 <= 256 && p.NS / (p.S * 2) >= 1) p.S *= 2;
-  const int64_t sps = (p.NS + p.S - 1) / p.S;
-  p.S = (int)((p.NS + sps - 1) / sps);  // no empty split
+  double cost = 1e30;
+  for (int mi = 1; mi <= 4; mi *= 2) {
+    const int64_t tiles = nprob * ((rows + 64 * mi - 1) / (64 * mi)) * ((O + MG_N - 1) / MG_N);
+    for (int64_t S = 1; S <= 16 && (S == 1 || tiles * S <= 512); ++S) {
+      const int64_t sps = (p.NS + S - 1) / S;
+      if (S > p.NS || (p.NS + sps - 1) / sps != S) continue;  // no empty split
+      const int64_t rounds = (tiles * S + 255) / 256;
+      const double busy = std::min(1.0, tiles * S / 256.0);
+      const double ends = mi == 1 ? 1.0 : mi == 2 ? 4.0 : 8.0 + 6.0 * busy;
+      const double step = mi == 1 ? 2.1 + 0.3 * busy : mi == 2 ? 2.5 + 0.3 * busy : 2.8 + 0.7 * busy;
+      const double split = S > 1 ? 6.0 + 0.4 * S + 8.0 * nprob * S * rows * O / 7e6 : 0.0;
+      const double t = rounds * (ends + step * sps) + split;
+      if (t < cost) cost = t, p.mi = mi, p.S = (int)S;
+    }
+  }
   p.part = p.S > 1 ? up256((int64_t)nprob * p.S * rows * ((O + 7) / 8 * 8) * 4) : 0;
   return p;
+}
+
+// Tiles of an XCD group along one side: all up to 8, else the 4 to 8 that pad the
+// side least (padding tiles leave some XCDs idle: 300 x 2560 -> 10240, 5 x 40 tiles,
+// 33.7 us in groups of 4 x 8 and 19.7 in 5 x 8).
+static int mg_group(int n) {
+  if (n <= 8) return n;
+  int best = 8;
+  for (int g = 7; g >= 4; --g)
+    if ((n + g - 1) / g * g < (n + best - 1) / best * best) best = g;
+  return best;
 }
 
 bool mx4_gemm_supported(int64_t rows, int64_t O, int64_t I) {
@@ -452,28 +462,21 @@ int mx4_gemm_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* st
   a.NS = (int)pl.NS;
   a.mt = (int)((b.rows + 64 * pl.mi - 1) / (64 * pl.mi));
   a.nt = (int)((b.O + MG_N - 1) / MG_N);
-  a.gm = std::min(a.mt, 4);
-  a.gn = std::min(a.nt, 8);
+  a.gm = mg_group(a.mt);
+  a.gn = mg_group(a.nt);
   a.S = pl.S;
   a.sps = (int)((pl.NS + pl.S - 1) / pl.S);
   a.ldp = (b.O + 7) / 8 * 8;
   uint8_t* at = static_cast<uint8_t*>(ws);
-  const void* x[MX4_MAXPROB];
-  uint8_t *xc[MX4_MAXPROB], *xs[MX4_MAXPROB];
+  uint8_t *xc[MX4_MAXPROB], *xs[MX4_MAXPROB], *wsc[MX4_MAXPROB];
   for (int i = 0; i < nprob; ++i) {
     a.p[i] = b.p[i];
-    x[i] = b.p[i].x;
     a.p[i].xc = xc[i] = at;
     a.p[i].xs = xs[i] = at + pl.codes;
-    at += pl.codes + pl.scales;
+    a.p[i].ws = wsc[i] = xs[i] + pl.scales;
+    at += pl.codes + pl.scales + pl.pad;
   }
-  if (int rc = mx4_quantize_padded(nprob, x, b.rows, b.I, act_dtype, xc, xs, stream)) return rc;
-  const int64_t cells = (int64_t)b.O * 4 * pl.NS;
-  hipLaunchKernelGGL(mx4_gemm_scales_kernel, dim3((unsigned)((cells + 255) / 256), (unsigned)nprob), dim3(256), 0,
-                     as_stream(stream), a, at, pl.pad);
-  if (int rc = check_launch("mx4_gemm_scales_kernel")) return rc;
-  for (int i = 0; i < nprob; ++i) a.p[i].ws = at + i * pl.pad;
-  at += nprob * pl.pad;
+  if (int rc = mx4_quantize_padded(b, nprob, act_dtype, xc, xs, wsc, stream)) return rc;
   a.part = reinterpret_cast<float*>(at);
   const auto go = [&](auto t) {
     using T = decltype(t);
