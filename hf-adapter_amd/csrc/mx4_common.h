@@ -39,14 +39,12 @@ __device__ __forceinline__ float mx4_scale(uint32_t e) { return __uint_as_float(
 // inputs: a block's codes by 2^(13 + e - emax) (at most 6 x 2^13, exact down to
 // 2^-36 of the largest scale, rounding at 2^-24 below), the sums over the run by
 // the factor 2^(emax - 127 - 13) (NaN for emax = 255) in fp32.
-__device__ __forceinline__ float mx4_relative(uint32_t e, uint32_t emax) {
-  return mx4_scale((uint32_t)max(140 + (int)e - (int)emax, 1));
+__device__ __forceinline__ uint32_t mx4_relative_byte(uint32_t e, uint32_t emax) {
+  return (uint32_t)max(140 + (int)e - (int)emax, 1);
 }
+__device__ __forceinline__ float mx4_relative(uint32_t e, uint32_t emax) { return mx4_scale(mx4_relative_byte(e, emax)); }
 __device__ __forceinline__ float mx4_factor(uint32_t emax) {
   return emax == 255u ? __builtin_nanf("") : ldexpf(1.f, (int)emax - 140);
-}
-__device__ __forceinline__ uint32_t mx4_factor_exponent(float f) {  // emax again
-  return f != f ? 255u : (uint32_t)(ilogbf(f) + 140);
 }
 
 // 8 codes of a dword -> 8 values times the scale, in order
@@ -100,10 +98,9 @@ bool mx4_gemm_supported(int64_t rows, int64_t O, int64_t I);
 int64_t mx4_gemm_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I);
 int mx4_gemm_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* stream);
 
-// Products through fp16 / bf16 records of the weight and the 256 x 256 GEMM
-// (mm8h.hip): whether it takes these shapes, its workspace, its launches.
-bool mx4h_supported(int64_t rows, int64_t I, int64_t O);
-int64_t mx4h_workspace_bytes(int nprob, int64_t rows, int64_t I, int64_t O);
-int mx4h_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, int64_t ws_bytes, void* stream);
+// Products with 16-bit rows, many of them (mx4_tile.hip).
+bool mx4_tile_supported(int64_t rows, int64_t O, int64_t I);
+int64_t mx4_tile_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I);
+int mx4_tile_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* stream);
 
 }  // namespace rwkv7mi

@@ -30,31 +30,11 @@
 // ahead go into the same stage, with a whole step to land.  Where the tiles do not
 // fill the chip K is split over workgroups and a second launch adds the fp32
 // partials.
-#include <algorithm>
-
-#include "mx4_common.h"
+#include "mx4_gemm.h"
 
 namespace rwkv7mi {
 
-constexpr int MG_N = 256;
-
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) void* mg_lds_ptr;
-
-struct MgArgs {
-  Mx4Prob p[MX4_MAXPROB];
-  int rows, O, I, NS;      // NS supersteps of 512 inputs
-  int mt, nt, gm, gn;      // row / column tiles, XCD tile group
-  int S, sps;              // K splits, supersteps of each
-  int64_t ldp;             // partials [problem][split][row][ldp]
-  float* part;
-};
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-// the key of x's row r, read by lane r % 32, and of W's column c of a tile
-__device__ __forceinline__ int mg_key(int r) { return (r & 7) ^ ((r >> 3) & 1); }
-__device__ __forceinline__ int mg_wkey(int c) { return mg_key(4 * (c >> 3) + (c & 3)); }
 
 __device__ __forceinline__ i32x8 mg_operand(u32x4 v) {
   return (i32x8){(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
@@ -65,56 +45,14 @@ __device__ __forceinline__ f32x16 mg_mfma(u32x4 a, u32x4 b, f32x16 c, int sa, in
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mg_operand(a), mg_operand(b), c, 4, 4, H, sa, H, sb);
 }
 
-// 8 columns of a row from c0: bias and epilogue, before the rounding
-template <typename T>
-__device__ __forceinline__ void mg_finish8(const Mx4Prob& P, int64_t row, int c0, int O, bool vec, float (&v)[8]) {
-  const int64_t oi = row * O + c0;
-  const bool whole = vec && c0 + 8 <= O;
-  const T* bp = static_cast<const T*>(P.bias);
-  const T* rp = static_cast<const T*>(P.residual) + oi;
-  float r[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = 0.f;
-  if (P.epilogue == RWKV7MI_EPI_RESIDUAL) {
-    if (whole) {
-      ld8(rp, r);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c0 + e < O) r[e] = to_f32(rp[e]);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if (bp && c0 + e < O) v[e] += to_f32(bp[c0 + e]);
-    if (P.epilogue == RWKV7MI_EPI_RELU2) v[e] = mx4_relu2(v[e]);
-    v[e] += r[e];
-  }
-}
-
-// 16-byte rows of y (and of the residual)
-__device__ __forceinline__ bool mg_vec(const Mx4Prob& P, int O) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(P.y) |
-                      (P.epilogue == RWKV7MI_EPI_RESIDUAL ? reinterpret_cast<uintptr_t>(P.residual) : 0);
-  return O % 8 == 0 && !(a & 15);
-}
-
 template <int MI, bool SPLIT, typename T>
 __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
   constexpr int ROWS = 64 * MI, XB = ROWS * 128, STAGE = XB + MG_N * 128;
   constexpr int SX = ROWS * 16, SB = SX + MG_N * 16, NX = 2 * MI;  // scale bytes; x loads a wave and step
   const Mx4Prob& P = B.p[blockIdx.y];
-  const int O = B.O, M = B.rows, NS = B.NS;
-  // XCD-aware tile number: workgroup L runs on XCD L % 8, which takes a run of the
-  // grouped tile order (padding tiles exit)
-  const int ngm = (B.mt + B.gm - 1) / B.gm, ngn = (B.nt + B.gn - 1) / B.gn;
-  const int gsz = B.gm * B.gn, tiles = ngm * ngn * gsz;
-  const int per = (tiles + 7) / 8;
-  const int t = ((int)blockIdx.x % 8) * per + (int)blockIdx.x / 8;
-  if (t >= tiles) return;
-  const int grp = t / gsz, gi = t % gsz;
-  const int tm = grp / ngn * B.gm + gi / B.gn, tn = grp % ngn * B.gn + gi % B.gn;
-  if (tm >= B.mt || tn >= B.nt) return;
+  const int M = B.rows, O = B.O, NS = B.NS;
+  int tm, tn;
+  if (!mg_tile(B, tm, tn)) return;
   const int m0 = tm * ROWS, n0 = tn * MG_N;
 
   extern __shared__ __align__(16) char smem[];  // two stages (x, W), the scales of two supersteps (x, W)
@@ -261,220 +199,53 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the trailing loads have landed before the waves exit
 
-  // Lane: row 32 i + n and, in group j, columns 64 (j / 2) + 16 a + 8 u + 4 (j % 2)
-  // .. +3, a = 0 .. 3.  The sums go through LDS (the stages are done with) in two
-  // halves of 64 columns a wave, and come back as whole rows: 16 lanes a row, 8
-  // columns each, whose bias stays in registers.  (Finished and stored from the MFMA
-  // layout, 32-byte pieces of 32 rows an instruction, the epilogue took as long as
-  // half the main loop.)
-  constexpr int LDT = 128 * 4 + 16;  // a staged row (the 16 bytes spread it over the banks)
-  const bool vec = mg_vec(P, O);
-  const int epi = P.epilogue;
-  const T *bias = static_cast<const T*>(P.bias), *res = static_cast<const T*>(P.residual);
-  T* y = static_cast<T*>(P.y);
-  float* part = SPLIT ? B.part + ((int64_t)blockIdx.y * B.S + blockIdx.z) * M * B.ldp : nullptr;
-  const int ll = 8 * (lane & 15);  // this lane's column of the staged 128, in the tile:
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const f32x16 c = acc[i][2 * p + g];
-          *reinterpret_cast<f32x4*>(smem + (wm + 32 * i + n) * LDT + ((wave & 1) * 64 + 16 * a + 8 * u + 4 * g) * 4) =
-              (f32x4){c[4 * a], c[4 * a + 1], c[4 * a + 2], c[4 * a + 3]};
-        }
-    __syncthreads();
-    const int cl = 128 * (ll >> 6) + 64 * p + (ll & 63), c0 = n0 + cl;
-    if (c0 >= O) continue;
-    const bool whole = vec && c0 + 8 <= O;
-    float bo[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) bo[e] = !SPLIT && bias && c0 + e < O ? to_f32(bias[c0 + e]) : 0.f;
-    // four rows at a time: their LDS reads (and residuals) are in flight together
-    for (int rb = 4 * wave + (lane >> 4); rb < nrow; rb += 64) {
-      float v[4][8], w[4][8];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) ld8(reinterpret_cast<const float*>(smem + (rb + 16 * k) * LDT) + ll, v[k]);
-      if (!SPLIT && epi == RWKV7MI_EPI_RESIDUAL) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int64_t oi = (int64_t)(m0 + min(rb + 16 * k, nrow - 1)) * O + c0;
-          if (whole) {
-            ld8(res + oi, w[k]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[k][e] = c0 + e < O ? to_f32(res[oi + e]) : 0.f;
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = rb + 16 * k;
-        const int64_t row = m0 + r, oi = row * O + c0;
-        if (r >= nrow) break;
-        if constexpr (SPLIT) {
-          st8(part + row * B.ldp + c0, v[k]);
-          continue;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[k][e] += bo[e];
-        if (epi == RWKV7MI_EPI_RELU2) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[k][e] = mx4_relu2(v[k][e]);
-        } else if (epi == RWKV7MI_EPI_RESIDUAL) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[k][e] += w[k][e];
-        }
-        if (whole) {
-          st8(y + oi, v[k]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (c0 + e < O) y[oi + e] = from_f32<T>(v[k][e]);
-        }
-      }
-    }
-  }
+  mg_epilogue<MI, SPLIT, T>(B, P, smem, acc, m0, n0);
 }
 
-// One thread: 8 columns of a row, the S partials in split order
-template <typename T>
-__global__ __launch_bounds__(256) void mx4_gemm_reduce_kernel(const MgArgs B) {
-  const Mx4Prob& P = B.p[blockIdx.y];
-  const int cols = (int)(B.ldp / 8);
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= (int64_t)B.rows * cols) return;
-  const int64_t row = t / cols;
-  const int c0 = 8 * (int)(t % cols);
-  if (c0 >= B.O) return;
-  const int64_t zs = (int64_t)B.rows * B.ldp;
-  const float* p = B.part + (int64_t)blockIdx.y * B.S * zs + row * B.ldp + c0;
-  float v[8];
-  ld8(p, v);
-  for (int z = 1; z < B.S; ++z) {
-    float a[8];
-    ld8(p + z * zs, a);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += a[e];
-  }
-  const bool vec = mg_vec(P, B.O);
-  mg_finish8<T>(P, row, c0, B.O, vec, v);
-  T* y = static_cast<T*>(P.y) + row * B.O + c0;
-  if (vec) {
-    st8(y, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c0 + e < B.O) y[e] = from_f32<T>(v[e]);
-  }
+// Fitted to 20 shapes from 17 x 2048 -> 2048 to 7000 x 2048 -> 2048, every tile height
+// and split timed, e.g. 1000 x 4096 -> 4096: 64 rows a tile 27.7 us, 128 rows 30.3, 256
+// rows 38.2; 4000 rows: 83, 63, 54; 1000 x 16384 -> 4096: 128 rows in two splits 71,
+// unsplit 92.
+static const MgCost MX4_GEMM_COST = {{1.0, 4.0, 8.0}, {0.0, 0.0, 6.0}, {2.1, 2.5, 2.8}, {0.3, 0.3, 0.7}};
+static MgPlan mx4_gemm_plan(int nprob, int64_t rows, int64_t O, int64_t I) {
+  return mg_plan(MX4_GEMM_COST, nprob, rows, O, (I + 511) / 512);
 }
+// workspace bytes: x's codes and scales, W's scales (a problem each)
+static int64_t mx4_gemm_codes(int64_t rows, int64_t I) { return mg_up256(rows * 256 * ((I + 511) / 512)); }
+static int64_t mx4_gemm_scales(int64_t rows, int64_t I) { return mg_up256(rows * 16 * ((I + 511) / 512)); }
 
-static int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
-struct MgPlan {
-  int mi, S;                       // rows of a workgroup / 64, K splits
-  int64_t NS, codes, scales, pad, part;  // workspace bytes: x's codes and scales, W's scales (a problem each), partials
-};
-static MgPlan mg_plan(int nprob, int64_t rows, int64_t O, int64_t I) {
-  MgPlan p{};
-  p.NS = (I + 511) / 512;
-  p.codes = up256(rows * 256 * p.NS);
-  p.scales = up256(rows * 16 * p.NS);
-  p.pad = up256(O * 16 * p.NS);
-  // The cheapest by an estimate in us: rounds of 256 workgroups (one a CU), each a
-  // start and an epilogue and its supersteps, slower with the chip busy, and for
-  // splits the second launch and the partials' traffic.  Fitted to 20 shapes from 17 x
-  // 2048 -> 2048 to 7000 x 2048 -> 2048, every tile height and split timed, e.g. 1000 x
-  // 4096 -> 4096: 64 rows a tile 27.7, 128 rows 30.3, 256 rows 38.2; 4000 rows: 83, 63,
-  // 54; 1000 x 16384 -> 4096: 128 rows in two splits 71, unsplit 92.
-  p.mi = 1;
-  p.S = 1;
-  double cost = 1e30;
-  for (int mi = 1; mi <= 4; mi *= 2) {
-    const int64_t tiles = nprob * ((rows + 64 * mi - 1) / (64 * mi)) * ((O + MG_N - 1) / MG_N);
-    for (int64_t S = 1; S <= 16 && (S == 1 || tiles * S <= 512); ++S) {
-      const int64_t sps = (p.NS + S - 1) / S;
-      if (S > p.NS || (p.NS + sps - 1) / sps != S) continue;  // no empty split
-      const int64_t rounds = (tiles * S + 255) / 256;
-      const double busy = std::min(1.0, tiles * S / 256.0);
-      const double ends = mi == 1 ? 1.0 : mi == 2 ? 4.0 : 8.0 + 6.0 * busy;
-      const double step = mi == 1 ? 2.1 + 0.3 * busy : mi == 2 ? 2.5 + 0.3 * busy : 2.8 + 0.7 * busy;
-      const double split = S > 1 ? 6.0 + 0.4 * S + 8.0 * nprob * S * rows * O / 7e6 : 0.0;
-      const double t = rounds * (ends + step * sps) + split;
-      if (t < cost) cost = t, p.mi = mi, p.S = (int)S;
-    }
-  }
-  p.part = p.S > 1 ? up256((int64_t)nprob * p.S * rows * ((O + 7) / 8 * 8) * 4) : 0;
-  return p;
-}
-
-// Tiles of an XCD group along one side: all up to 8, else the 4 to 8 that pad the
-// side least (padding tiles leave some XCDs idle: 300 x 2560 -> 10240, 5 x 40 tiles,
-// 33.7 us in groups of 4 x 8 and 19.7 in 5 x 8).
-static int mg_group(int n) {
-  if (n <= 8) return n;
-  int best = 8;
-  for (int g = 7; g >= 4; --g)
-    if ((n + g - 1) / g * g < (n + best - 1) / best * best) best = g;
-  return best;
-}
-
-bool mx4_gemm_supported(int64_t rows, int64_t O, int64_t I) {
-  // 32-bit offsets within a tile's 256 rows and columns, and within the scales
-  const int64_t NS = (I + 511) / 512, tiles = (rows + 63) / 64 * ((O + MG_N - 1) / MG_N);
-  return rows > 0 && 256 * 256 * NS < (int64_t)BUF_OOB && 16 * NS * std::max(rows, O) < (int64_t)BUF_OOB && rows <= INT32_MAX / 2 && O <= INT32_MAX / 2 &&
-         tiles < INT32_MAX / 64;
-}
+bool mx4_gemm_supported(int64_t rows, int64_t O, int64_t I) { return mg_supported(rows, O, I); }
 
 int64_t mx4_gemm_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I) {
-  const MgPlan p = mg_plan(nprob, rows, O, I);
-  return nprob * (p.codes + p.scales + p.pad) + p.part;
+  return nprob * (mx4_gemm_codes(rows, I) + mx4_gemm_scales(rows, I) + mx4_gemm_scales(O, I)) +
+         mg_part_bytes(mx4_gemm_plan(nprob, rows, O, I), nprob, rows, O);
 }
 
 template <int MI, typename T>
 static int mg_go(const MgArgs& a, int nprob, void* stream) {
   constexpr int lds = 2 * (64 * MI + MG_N) * (128 + 16);
-  const int64_t tiles = (int64_t)((a.mt + a.gm - 1) / a.gm * a.gm) * ((a.nt + a.gn - 1) / a.gn * a.gn);
-  const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)nprob, (unsigned)a.S);
   static std::atomic<uint64_t> raised[2];
   auto launch = [&](auto kern, std::atomic<uint64_t>& done) {
     if (int rc = raise_dynamic_lds(reinterpret_cast<const void*>(kern), lds, done, "mx4_gemm_kernel")) return rc;
-    hipLaunchKernelGGL(kern, grid, dim3(256), lds, as_stream(stream), a);
-    return check_launch("mx4_gemm_kernel");
+    hipLaunchKernelGGL(kern, mg_grid(a, nprob), dim3(256), lds, as_stream(stream), a);
+    if (int rc = check_launch("mx4_gemm_kernel")) return rc;
+    return mg_reduce<T>(a, nprob, stream);
   };
-  if (a.S == 1) return launch(&mx4_gemm_kernel<MI, false, T>, raised[0]);
-  if (int rc = launch(&mx4_gemm_kernel<MI, true, T>, raised[1])) return rc;
-  const int64_t nthr = (int64_t)a.rows * (a.ldp / 8);
-  hipLaunchKernelGGL(mx4_gemm_reduce_kernel<T>, dim3((unsigned)((nthr + 255) / 256), (unsigned)nprob), dim3(256), 0,
-                     as_stream(stream), a);
-  return check_launch("mx4_gemm_reduce_kernel");
+  return a.S == 1 ? launch(&mx4_gemm_kernel<MI, false, T>, raised[0]) : launch(&mx4_gemm_kernel<MI, true, T>, raised[1]);
 }
 
 int mx4_gemm_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* stream) {
-  const MgPlan pl = mg_plan(nprob, b.rows, b.O, b.I);
+  const MgPlan pl = mx4_gemm_plan(nprob, b.rows, b.O, b.I);
   MgArgs a{};
-  a.rows = b.rows;
-  a.O = b.O;
-  a.I = b.I;
-  a.NS = (int)pl.NS;
-  a.mt = (int)((b.rows + 64 * pl.mi - 1) / (64 * pl.mi));
-  a.nt = (int)((b.O + MG_N - 1) / MG_N);
-  a.gm = mg_group(a.mt);
-  a.gn = mg_group(a.nt);
-  a.S = pl.S;
-  a.sps = (int)((pl.NS + pl.S - 1) / pl.S);
-  a.ldp = (b.O + 7) / 8 * 8;
+  mg_sizes(a, b, pl);
   uint8_t* at = static_cast<uint8_t*>(ws);
   uint8_t *xc[MX4_MAXPROB], *xs[MX4_MAXPROB], *wsc[MX4_MAXPROB];
   for (int i = 0; i < nprob; ++i) {
     a.p[i] = b.p[i];
     a.p[i].xc = xc[i] = at;
-    a.p[i].xs = xs[i] = at + pl.codes;
-    a.p[i].ws = wsc[i] = xs[i] + pl.scales;
-    at += pl.codes + pl.scales + pl.pad;
+    a.p[i].xs = xs[i] = at + mx4_gemm_codes(b.rows, b.I);
+    a.p[i].ws = wsc[i] = xs[i] + mx4_gemm_scales(b.rows, b.I);
+    at = wsc[i] + mx4_gemm_scales(b.O, b.I);
   }
   if (int rc = mx4_quantize_padded(b, nprob, act_dtype, xc, xs, wsc, stream)) return rc;
   a.part = reinterpret_cast<float*>(at);

@@ -1,16 +1,24 @@
 // Products with an MXFP4 weight: y = epilogue(x W^T + bias), fp16 / bf16 rows
 // x, or the same rows quantised to MXFP4 on the way.
 //
-// mx4_rows_kernel: a workgroup of NW waves computes 16 rows x 16 outputs; the
-// waves share K, and their fp32 sums meet in LDS in wave order.  A wave advances
-// 128 inputs (four blocks) a step: lane n + 16 q holds block q of output n, 16
-// bytes of codes and one scale byte, which is the operand of
+// mx4_rows_kernel, 16 rows a tile: the nw waves of a workgroup share K in units of
+// 512 inputs and go through groups of 16 outputs, a grid apart; a group's fp32 sums
+// meet in LDS in wave order.  A unit is four steps of 128 inputs (four blocks): lane
+// n + 16 q holds block q of output n, 16 bytes of codes and one scale byte, which is
+// the operand of
 //  * one v_mfma_scale_f32_16x16x128_f8f6f4 where x is MXFP4 too, or
 //  * four v_mfma_f32_16x16x32 where x is 16-bit: MFMA j takes inputs 8 j .. +7
 //    of every lane's block, and so do the rows of x.
-// bf16 holds a scaled code exactly.  fp16 does not for every scale, so there a
-// step's codes are scaled relative to the largest of its four scales and the
-// step's sums by that one's factor (mx4_common.h).
+// A wave has one unit: its part of x stays in registers for all its groups, and the
+// next group's codes and scales are loaded before this one's MFMAs.  Above 16 units
+// (K > 8192) the units go over several workgroups, and a second launch adds their
+// sums (16 x 16384 -> 4096 with two units a wave, x reloaded, 25.6 us).  What does
+// not carry weights is kept out of the loads' way: a group's scales are loaded once
+// by the workgroup, through LDS, a group ahead (by each wave 1.4 us more at 1 x 4096
+// -> 16384, 13.1 us then), and up to four 16-bit rows of x by whole instructions,
+// through LDS (in the operand's layout, most lanes idle, 2.6 us more).  bf16 holds a scaled code exactly.  fp16 does
+// not for every scale, so there a step's codes are scaled relative to the largest of
+// its four scales and the step's sums by that one's factor (mx4_common.h).
 #include <algorithm>
 
 #include "mx4_common.h"
@@ -25,104 +33,231 @@ __device__ __forceinline__ i32x8 mx4_operand(u32x4 v) {
   return (i32x8){(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
 }
 
-// exponent bytes of the four blocks of one step, block q in byte q; blocks past
-// the row read 0.  WHOLE: I % 128 == 0 (a step's bytes are an aligned dword).
-template <bool WHOLE>
-__device__ __forceinline__ uint32_t mx4_exps(const uint8_t* row, int b, int nb) {
-  if constexpr (WHOLE) return *reinterpret_cast<const uint32_t*>(row + b);
-  uint32_t v = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (b + i < nb) v |= (uint32_t)row[b + i] << (8 * i);
-  return v;
-}
-
 __device__ __forceinline__ uint32_t max4(uint32_t v) {
   return max(max(v & 255u, (v >> 8) & 255u), max((v >> 16) & 255u, v >> 24));
 }
 
-}  // namespace
-
-template <typename T, bool A4, bool WHOLE>
-__global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Batch B) {
-  using V = typename Mx4Types<T>::V;
-  constexpr bool F16 = std::is_same<T, __half>::value && !A4;
-  const Mx4Prob& P = B.p[blockIdx.z];
-  const int I = B.I, O = B.O, nb = I / MX4_BLOCK;
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
-  const int o0 = blockIdx.x * 16, row0 = blockIdx.y * 16;
-  // rows and outputs past the end repeat the last one; their sums are not stored
-  const int o = min(o0 + n, O - 1), row = min(row0 + n, B.rows - 1);
-  const uint8_t* wc = P.wc + (int64_t)o * (I / 2);
-  const uint8_t* ws = P.ws + (int64_t)o * nb;
-  const T* x = A4 ? nullptr : static_cast<const T*>(P.x) + (int64_t)row * I;
-  const uint8_t* xc = A4 ? P.xc + (int64_t)row * (I / 2) : nullptr;
-  const uint8_t* xs = A4 ? P.xs + (int64_t)row * nb : nullptr;
-
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const u32x4 zero = {0u, 0u, 0u, 0u};
-  for (int b = 4 * wave; b < nb; b += 4 * nw) {
-    const bool ok = WHOLE || b + q < nb;
-    const u32x4 w = ok ? *reinterpret_cast<const u32x4*>(wc + 16 * (b + q)) : zero;
-    const uint32_t ex = mx4_exps<WHOLE>(ws, b, nb);
-    const uint32_t e = (ex >> (8 * q)) & 255u;
-    if constexpr (A4) {
-      const u32x4 a = ok ? *reinterpret_cast<const u32x4*>(xc + 16 * (b + q)) : zero;
-      const uint32_t ea = (mx4_exps<WHOLE>(xs, b, nb) >> (8 * q)) & 255u;
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(a), mx4_operand(w), acc, 4, 4, 0, (int)ea, 0,
-                                                             (int)e);
+// The scale bytes of a row's unit (16 blocks from b), a dword a step, block q of it
+// in byte q; blocks past the row read 0.  SC: 2 where I % 512 == 0 (16 aligned
+// bytes), 1 where I % 128 == 0 (aligned dwords), else bytes.
+template <int SC>
+__device__ __forceinline__ u32x4 mx4_unit_scales(const uint8_t* row, int b, int nb) {
+  if constexpr (SC == 2) return *reinterpret_cast<const u32x4*>(row + b);
+  u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    if constexpr (SC == 1) {
+      if (b + 4 * s < nb) v[s] = *reinterpret_cast<const uint32_t*>(row + b + 4 * s);
     } else {
-      u32x4 a[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) a[j] = ok ? *reinterpret_cast<const u32x4*>(x + 32 * (b + q) + 8 * j) : zero;
-      const uint32_t emax = F16 ? max4(ex) : 0u;
-      const float s = F16 ? mx4_relative(e, emax) : mx4_scale(e);
-      f32x4 c = F16 ? (f32x4){0.f, 0.f, 0.f, 0.f} : acc;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        V wv;
-        mx4_decode8(w[j], s, wv);
-        c = mfma16x16x32(__builtin_bit_cast(V, a[j]), wv, c);
-      }
-      acc = F16 ? acc + mx4_factor(emax) * c : c;
+      for (int i = 0; i < 4; ++i)
+        if (b + 4 * s + i < nb) v[s] |= (uint32_t)row[b + 4 * s + i] << (8 * i);
     }
   }
+  return v;
+}
 
-  // lane: output n, rows 4 q .. +3
-  __shared__ float part[16][16][17];
+}  // namespace
+
+struct Mx4Rows {
+  Mx4Batch b;
+  int S;        // workgroups that share K
+  float* part;  // S > 1: [problem][split][row][O]
+};
+
+// FEW: 16-bit rows, at most four
+template <typename T, bool A4, int SC, bool FEW>
+__global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Rows R) {
+  using V = typename Mx4Types<T>::V;
+  constexpr bool F16 = std::is_same<T, __half>::value && !A4;
+  const Mx4Batch& B = R.b;
+  const Mx4Prob& P = B.p[blockIdx.z / R.S];
+  const int I = B.I, O = B.O, nb = I / MX4_BLOCK, groups = (O + 15) / 16;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
+  const int row0 = blockIdx.y * 16;
+  const bool mine = row0 + n < B.rows;
+  const int64_t row = min(row0 + n, B.rows - 1);
+  const T* x = A4 ? nullptr : static_cast<const T*>(P.x) + row * I + 32 * q;
+  const uint8_t* xc = A4 ? P.xc + row * (I / 2) + 16 * q : nullptr;
+  const uint8_t* xs = A4 ? P.xs + row * nb : nullptr;
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  constexpr int NX = A4 ? 1 : 4;  // 16-byte pieces of x a step
+
+  // [group's parity][output][wave] scales, then [group's parity][wave][row][output]
+  // sums in the memory that first holds [wave][row][16-byte piece] of x
+  extern __shared__ __align__(16) char smem[];
+  u32x4* const scale = reinterpret_cast<u32x4*>(smem);
+  char* const lower = smem + 512 * nw;
+  typedef float Sums[16][17];
+  Sums* const part = reinterpret_cast<Sums*>(lower);
+  u32x4* const xl = reinterpret_cast<u32x4*>(lower) + wave * (FEW ? B.rows : 0) * 64;
+
+  u32x4 w[4], wn[4], a[4][NX], ea = zero;
+  const int u0 = (int)(blockIdx.z % R.S) * nw;
+  const int b0 = 16 * (u0 + wave);  // (waves past the last unit add zeros)
+  const bool has = b0 < nb;
+  auto load_w = [&](int g, u32x4 (&w)[4]) {
+    const int64_t o = min(16 * g + n, O - 1);  // (outputs past the end repeat the last one and are not stored)
+    const uint8_t* wc = P.wc + o * (I / 2) + 16 * (b0 + q);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) part[wave][4 * q + i][n] = acc[i];
+    for (int s = 0; s < 4; ++s)
+      w[s] = SC == 2 || b0 + 4 * s + q < nb ? *reinterpret_cast<const u32x4*>(wc + 64 * s) : zero;
+  };
+  // thread t: the scales of output t / nw, unit t % nw of the group
+  const int so = tid / nw, su = tid % nw, sb = 16 * (u0 + su);
+  const bool scales = tid < 16 * nw && sb < nb;
+  auto load_s = [&](int g) {
+    return mx4_unit_scales<SC>(P.ws + (int64_t)min(16 * g + so, O - 1) * nb, sb, nb);
+  };
+  u32x4 sn = zero;
+  if (has) load_w(blockIdx.x, w);
+  if (scales) scale[so * nw + su] = load_s(blockIdx.x);
+  if (has) {
+    if constexpr (FEW) {
+      // piece `lane` of each row's unit, 8 inputs
+      const T* xr = static_cast<const T*>(P.x) + 32 * b0 + 8 * lane;
+      const bool in = SC == 2 || 32 * b0 + 8 * lane < I;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r < B.rows) xl[64 * r + lane] = in ? *reinterpret_cast<const u32x4*>(xr + (int64_t)r * I) : zero;
+      const int r = min(n, B.rows - 1);  // (rows past the end repeat the last one and are not stored)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int j = 0; j < NX; ++j) a[s][j] = xl[64 * r + 16 * s + 4 * q + j];
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+#pragma unroll
+        for (int j = 0; j < NX; ++j) a[s][j] = zero;
+        if (mine && (SC == 2 || b0 + 4 * s + q < nb)) {
+          if constexpr (A4) {
+            a[s][0] = *reinterpret_cast<const u32x4*>(xc + 16 * (b0 + 4 * s));
+          } else {
+#pragma unroll
+            for (int j = 0; j < NX; ++j) a[s][j] = *reinterpret_cast<const u32x4*>(x + 32 * (b0 + 4 * s) + 8 * j);
+          }
+        }
+      }
+      if constexpr (A4) {
+        if (mine) ea = mx4_unit_scales<SC>(xs, b0, nb);
+      }
+    }
+  }
   __syncthreads();
-  for (int t = tid; t < 256; t += blockDim.x) {
-    const int r = t >> 4, c = t & 15;
-    if (row0 + r >= B.rows || o0 + c >= O) continue;
-    float v = part[0][r][c];
-    for (int w = 1; w < nw; ++w) v += part[w][r][c];
-    mx4_store<T>(P, row0 + r, o0 + c, O, v);
+  int par = 0;
+  for (int g = blockIdx.x; g < groups; g += gridDim.x, par ^= 1) {
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const bool next = g + (int)gridDim.x < groups;
+    if (next && scales) sn = load_s(g + gridDim.x);
+    if (has) {
+      if (next) load_w(g + gridDim.x, wn);
+      const u32x4 e = scale[(16 * par + n) * nw + wave];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const uint32_t ew = e[s], eb = (ew >> (8 * q)) & 255u;
+        if constexpr (A4) {
+          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(a[s][0]), mx4_operand(w[s]), acc, 4, 4, 0,
+                                                                 (int)((ea[s] >> (8 * q)) & 255u), 0, (int)eb);
+        } else {
+          const uint32_t emax = F16 ? max4(ew) : 0u;
+          const float sc = F16 ? mx4_relative(eb, emax) : mx4_scale(eb);
+          f32x4 c = F16 ? (f32x4){0.f, 0.f, 0.f, 0.f} : acc;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            V wv;
+            mx4_decode8(w[s][j], sc, wv);
+            c = mfma16x16x32(__builtin_bit_cast(V, a[s][j]), wv, c);
+          }
+          acc = F16 ? acc + mx4_factor(emax) * c : c;
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) w[s] = wn[s];
+    }
+    if (next && scales) scale[(16 * (par ^ 1) + so) * nw + su] = sn;
+    // lane: output n, rows 4 q .. +3.  (A wave is at most one group ahead of the
+    // readers of the other half.)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[par * nw + wave][4 * q + i][n] = acc[i];
+    __syncthreads();
+    for (int z = tid; z < 256; z += blockDim.x) {
+      const int r = z >> 4, c = z & 15;
+      if (row0 + r >= B.rows || 16 * g + c >= O) continue;
+      float v = part[par * nw][r][c];
+      for (int k = 1; k < nw; ++k) v += part[par * nw + k][r][c];
+      if (R.S > 1)
+        R.part[((int64_t)blockIdx.z * B.rows + row0 + r) * O + 16 * g + c] = v;
+      else
+        mx4_store<T>(P, row0 + r, 16 * g + c, O, v);
+    }
   }
 }
 
+// One thread an output: its S partial sums in split order
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_rows_reduce_kernel(const Mx4Rows R) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, each = (int64_t)R.b.rows * R.b.O;
+  if (t >= each) return;
+  const float* p = R.part + blockIdx.y * R.S * each + t;
+  float v = p[0];
+  for (int z = 1; z < R.S; ++z) v += p[z * each];
+  mx4_store<T>(R.b.p[blockIdx.y], t / R.b.O, (int)(t % R.b.O), R.b.O, v);
+}
+
+// Workgroups that share K: up to 16 units of 512 inputs in one, 8 where there are
+// more (16 x 16384 -> 4096: 21.0 us with 8, 21.8 with 16; 1 row 15.9 and 16.7).
+static int mx4_rows_splits(int64_t I) { return I <= 8192 ? 1 : (int)((I + 4095) / 4096); }
+static int64_t mx4_rows_part_bytes(int nprob, int64_t rows, int64_t O, int64_t I) {
+  const int S = mx4_rows_splits(I);
+  return S > 1 ? nprob * S * rows * O * 4 : 0;
+}
+
 template <typename T, bool A4>
-static int mx4_rows_run(const Mx4Batch& b, int nprob, void* stream) {
-  const int steps = (b.I + 127) / 128;
-  const int nw = steps >= 64 ? 16 : steps >= 16 ? 8 : 4;
-  const dim3 grid((unsigned)((b.O + 15) / 16), (unsigned)((b.rows + 15) / 16), (unsigned)nprob);
-  if (b.I % 128 == 0)
-    hipLaunchKernelGGL((mx4_rows_kernel<T, A4, true>), grid, dim3(64 * nw), 0, as_stream(stream), b);
-  else
-    hipLaunchKernelGGL((mx4_rows_kernel<T, A4, false>), grid, dim3(64 * nw), 0, as_stream(stream), b);
-  return check_launch("mx4_rows_kernel");
+static int mx4_rows_run(const Mx4Batch& b, int nprob, void* part, void* stream) {
+  Mx4Rows r{b, mx4_rows_splits(b.I), static_cast<float*>(part)};
+  const int units = (b.I + 511) / 512, nw = (units + r.S - 1) / r.S;
+  const int groups = (b.O + 15) / 16, tiles = (b.rows + 15) / 16;
+  // 16 waves a CU fit by registers: no more workgroups than run at once
+  const int64_t most = std::max<int64_t>(1, 256 * (16 / nw) / ((int64_t)tiles * nprob * r.S));
+  const dim3 grid((unsigned)std::min<int64_t>(groups, most), (unsigned)tiles, (unsigned)(nprob * r.S));
+  // (16-byte scale reads need the rows of scales to start 16-byte aligned)
+  bool wide = b.I % 512 == 0;
+  for (int i = 0; i < nprob; ++i)
+    if ((reinterpret_cast<uintptr_t>(b.p[i].ws) | reinterpret_cast<uintptr_t>(b.p[i].xs)) & 15) wide = false;
+  const int lds = nw * (512 + std::max(2 * 16 * 17 * 4, !A4 && b.rows <= 4 ? 1024 * b.rows : 0));
+  const auto go = [&](auto sc) {
+    static std::atomic<uint64_t> raised[2];
+    const auto launch = [&](auto kern, std::atomic<uint64_t>& done) {
+      if (lds > 65536)
+        if (int rc = raise_dynamic_lds(reinterpret_cast<const void*>(kern), 16 * (512 + 4096), done, "mx4_rows_kernel"))
+          return rc;
+      hipLaunchKernelGGL(kern, grid, dim3(64 * nw), lds, as_stream(stream), r);
+      return check_launch("mx4_rows_kernel");
+    };
+    return !A4 && b.rows <= 4 ? launch(&mx4_rows_kernel<T, A4, decltype(sc)::value, !A4>, raised[0])
+                              : launch(&mx4_rows_kernel<T, A4, decltype(sc)::value, false>, raised[1]);
+  };
+  if (int rc = wide               ? go(std::integral_constant<int, 2>{})
+               : b.I % 128 == 0 ? go(std::integral_constant<int, 1>{})
+                                : go(std::integral_constant<int, 0>{}))
+    return rc;
+  if (r.S == 1) return RWKV7MI_OK;
+  const int64_t each = (int64_t)b.rows * b.O;
+  hipLaunchKernelGGL(mx4_rows_reduce_kernel<T>, dim3((unsigned)((each + 255) / 256), (unsigned)nprob), dim3(256), 0,
+                     as_stream(stream), r);
+  return check_launch("mx4_rows_reduce_kernel");
 }
 
 // bytes of one quantised input, each part on a 256-byte boundary
 static int64_t mx4_codes_bytes(int64_t rows, int64_t I) { return (rows * (I / 2) + 255) & ~(int64_t)255; }
 static int64_t mx4_scales_bytes(int64_t rows, int64_t I) { return (rows * (I / MX4_BLOCK) + 255) & ~(int64_t)255; }
 
-// Rows from which a product pays for materialising the weight.
-static bool mx4_prefill(int64_t rows, int64_t I, int64_t O) { return rows > 256 && mx4h_supported(rows, I, O); }
-// Quantised rows of more than one tile of the few-row kernel.
-static bool mx4_gemm(int64_t rows, int64_t I, int64_t O) { return rows > 16 && mx4_gemm_supported(rows, O, I); }
+// More rows than a tile of the few-row kernel: the 64- to 256-row tiles.
+static bool mx4_many(int64_t rows, int64_t I, int64_t O, int quantize_input) {
+  return rows > 16 && (quantize_input ? mx4_gemm_supported(rows, O, I) : mx4_tile_supported(rows, O, I));
+}
 
 }  // namespace rwkv7mi
 
@@ -131,9 +266,10 @@ using namespace rwkv7mi;
 extern "C" int64_t rwkv7mi_mxfp4_linear_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I, int act_dtype,
                                                         int quantize_input) {
   if (nprob < 1 || nprob > MX4_MAXPROB || rows <= 0 || O <= 0 || I <= 0) return 0;
-  if (quantize_input && mx4_gemm(rows, I, O)) return mx4_gemm_workspace_bytes(nprob, rows, O, I);
-  if (quantize_input) return nprob * (mx4_codes_bytes(rows, I) + mx4_scales_bytes(rows, I));
-  return mx4_prefill(rows, I, O) ? mx4h_workspace_bytes(nprob, rows, I, O) : 0;
+  if (mx4_many(rows, I, O, quantize_input))
+    return quantize_input ? mx4_gemm_workspace_bytes(nprob, rows, O, I) : mx4_tile_workspace_bytes(nprob, rows, O, I);
+  const int64_t part = mx4_rows_part_bytes(nprob, rows, O, I);
+  return part + (quantize_input ? nprob * (mx4_codes_bytes(rows, I) + mx4_scales_bytes(rows, I)) : 0);
 }
 
 extern "C" int rwkv7mi_mxfp4_linear(int nprob, const void* const* x, const uint8_t* const* codes,
@@ -170,10 +306,11 @@ extern "C" int rwkv7mi_mxfp4_linear(int nprob, const void* const* x, const uint8
   if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < need))
     return fail(RWKV7MI_ESIZE, w + ": workspace missing, unaligned or smaller than "
                                    "rwkv7mi_mxfp4_linear_workspace_bytes");
-  if (!quantize_input && mx4_prefill(rows, I, O)) return mx4h_run(b, nprob, act_dtype, ws, ws_bytes, stream);
+  if (mx4_many(rows, I, O, quantize_input))
+    return quantize_input ? mx4_gemm_run(b, nprob, act_dtype, ws, stream) : mx4_tile_run(b, nprob, act_dtype, ws, stream);
   if (!quantize_input)
-    return bf ? mx4_rows_run<__hip_bfloat16, false>(b, nprob, stream) : mx4_rows_run<__half, false>(b, nprob, stream);
-  if (mx4_gemm(rows, I, O)) return mx4_gemm_run(b, nprob, act_dtype, ws, stream);
+    return bf ? mx4_rows_run<__hip_bfloat16, false>(b, nprob, ws, stream)
+              : mx4_rows_run<__half, false>(b, nprob, ws, stream);
   uint8_t *xc[MX4_MAXPROB], *xs[MX4_MAXPROB];
   uint8_t* at = static_cast<uint8_t*>(ws);
   for (int i = 0; i < nprob; ++i) {
@@ -182,5 +319,5 @@ extern "C" int rwkv7mi_mxfp4_linear(int nprob, const void* const* x, const uint8
     at = xs[i] + mx4_scales_bytes(rows, I);
   }
   if (int rc = mx4_quantize_run(nprob, x, rows, I, I, act_dtype, xc, xs, stream)) return rc;
-  return bf ? mx4_rows_run<__hip_bfloat16, true>(b, nprob, stream) : mx4_rows_run<__half, true>(b, nprob, stream);
+  return bf ? mx4_rows_run<__hip_bfloat16, true>(b, nprob, at, stream) : mx4_rows_run<__half, true>(b, nprob, at, stream);
 }

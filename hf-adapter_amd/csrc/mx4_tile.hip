@@ -1,0 +1,280 @@
+// MXFP4 weights times 16-bit rows, more than 16 of them: y = epilogue(x W^T + bias),
+// fp16 / bf16 x.
+//
+// The tile of mx4_gemm.h on v_mfma_f32_32x32x16: lane n + 32 u holds 8 inputs of a row.
+// K advances 64 inputs a step, four sub-steps; lane half u takes the block of inputs
+// 32 u .. +31, 8 a sub-step, so a lane's scale holds for a step:
+//  * x: global -> LDS directly, 128 bytes a row, two stages; lane n + 32 u reads chunk
+//    4 u + h in sub-step h;
+//  * W codes: global -> LDS directly, 128 bytes (four steps) a column, two stages; a
+//    lane reads 16 bytes a step, one dword a sub-step, which four conversions turn into
+//    its operand during the sub-step before;
+//  * W's scales: 8 steps (a superstep) at a time, global -> LDS, 16 bytes a column in
+//    the order [u][step], written by a pre-pass.  fp16 columns are scaled relative to
+//    their largest scale (mx4_common.h), which the pre-pass finds, and the sums by its
+//    factor.
+// A stage of x is read to the end in its step's third sub-step: one barrier there, and
+// the loads two steps ahead go into the same stage.  A stage of W is free a sub-step
+// later in its last step, and its loads go out two a step over the next four.  Inputs
+// past I are zeros of x (W's codes there are some finite value).  Where the tiles do
+// not fill the chip K is split over workgroups and a second launch adds the partials.
+#include "mx4_gemm.h"
+
+namespace rwkv7mi {
+
+__device__ __forceinline__ f32x16 mt_mfma(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mt_mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+template <int MI, bool SPLIT, typename T>
+__global__ __launch_bounds__(256, 1) void mx4_tile_kernel(const MgArgs B) {
+  using V = typename Mx4Types<T>::V;
+  constexpr int ROWS = 64 * MI, XB = ROWS * 128, WB = MG_N * 128, SB = MG_N * 16;  // bytes of a stage of x, W, scales
+  constexpr int NX = 2 * MI;                                                       // x loads a wave and step
+  const Mx4Prob& P = B.p[blockIdx.y];
+  const int M = B.rows, O = B.O, I = B.I, NS = B.NS;
+  int tm, tn;
+  if (!mg_tile(B, tm, tn)) return;
+  const int m0 = tm * ROWS, n0 = tn * MG_N;
+
+  extern __shared__ __align__(16) char smem[];  // two stages each: x, W, scales
+  char* const wst = smem + 2 * XB;
+  char* const scl = wst + 2 * WB;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, u = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int S0 = SPLIT ? (int)blockIdx.z * B.sps : 0;
+  const int S1 = SPLIT ? min(NS, S0 + B.sps) : NS;
+  const int s0 = 8 * S0, nsteps = min(8 * S1, (I + 63) / 64) - s0;  // (the last superstep may be short)
+
+  // descriptors end at the tile's last row / column: past them zeros
+  const int nrow = min(ROWS, M - m0), ncol = min(MG_N, O - n0);
+  const int ldx = 2 * I, ldw = I / 2;
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(static_cast<const char*>(P.x) + (int64_t)m0 * ldx, (uint32_t)(nrow * ldx));
+  const __amdgpu_buffer_rsrc_t wr = make_rsrc(P.wc + (int64_t)n0 * ldw, (uint32_t)(ncol * ldw));
+  const __amdgpu_buffer_rsrc_t wsr = make_rsrc(P.ws, (uint32_t)(NS * O * 16));
+
+  // round v of a stage: rows 32 v + 8 w .. +7 of x (W), lane l at row + l / 8, chunk
+  // position l % 8
+  const int lr = 8 * wave + (lane >> 3);
+  auto issue_x = [&](int s, int v) {
+    const int r = 32 * v + lr, c = (lane & 7) ^ mg_key(r);
+    const int vo = 64 * (s0 + s) + 8 * c < I ? r * ldx + 16 * c : (int)BUF_OOB;
+    const int so = s < nsteps ? 128 * (s0 + s) : (int)BUF_OOB;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (mg_lds_ptr)(smem + (s & 1) * XB + (32 * v + 8 * wave) * 128), 16, vo, so,
+                                             0, 0);
+  };
+  auto issue_w = [&](int f, int v) {  // stage f: steps 4 f .. +3
+    const int r = 32 * v + lr, vo = r * ldw + 16 * ((lane & 7) ^ mg_wkey(r));
+    const int so = 4 * f < nsteps ? 128 * (s0 / 4 + f) : (int)BUF_OOB;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (mg_lds_ptr)(wst + (f & 1) * WB + (32 * v + 8 * wave) * 128), 16, vo, so, 0,
+                                             0);
+  };
+  auto issue_s = [&](int s) {  // scales of superstep s: 64 columns a wave
+    const int so = s < S1 - S0 ? 16 * ((S0 + s) * O + n0 + 64 * wave) : (int)BUF_OOB;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(wsr, (mg_lds_ptr)(scl + (s & 1) * SB + 64 * wave * 16), 16, 16 * lane, so, 0, 0);
+  };
+
+  const int wm = 32 * MI * (wave >> 1), wn = 128 * (wave & 1);  // the wave's rows and columns in the tile
+  const int wcol = 8 * (n >> 2) + (n & 3), key = mg_key(n);
+  auto ld_x = [&](int s, int h, int i) {
+    return *reinterpret_cast<const V*>(smem + (s & 1) * XB + (wm + 32 * i + n) * 128 + 16 * ((4 * u + h) ^ key));
+  };
+  auto col = [&](int j) { return wn + 64 * (j >> 1) + 4 * (j & 1) + wcol; };
+  auto ld_w = [&](int s, int j) {  // the lane's block of step s
+    return *reinterpret_cast<const u32x4*>(wst + (s >> 2 & 1) * WB + col(j) * 128 + 16 * ((2 * (s & 3) + u) ^ key));
+  };
+  auto ld_s = [&](int s, int j) {  // its scale byte
+    return (uint32_t) * reinterpret_cast<const uint8_t*>(scl + (s >> 3 & 1) * SB + col(j) * 16 + 8 * u + (s & 7));
+  };
+
+  f32x16 acc[MI][4];
+  V xa[2][MI], wa[2][4];     // operands of two sub-steps
+  u32x4 wc[4], wcn[4];       // codes of this step and the next
+  uint32_t sc[4], scn[4];    // their scale bytes
+
+  // Sub-step H of step s (operand set H & 1): its MFMAs; the next sub-step's x operands
+  // are read and its W operands made meanwhile, and in H = 3 load(l), l = 0 .. NX + 1,
+  // issues the global loads.
+  auto substep = [&](auto hc, int s, auto&& load) {
+    constexpr int H = decltype(hc)::value, A = H & 1, HN = (H + 1) & 3, L = H == 3 ? NX + 2 : 0;
+    constexpr int TILES = MI * 4;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = 4 * i + j;
+        acc[i][j] = mt_mfma(wa[A][j], xa[A][i], acc[i][j]);
+        // x's reads over the first half, W's conversions over all of it
+#pragma unroll
+        for (int r = min(MI, k * 2 * MI / TILES); r < min(MI, (k + 1) * 2 * MI / TILES); ++r)
+          xa[A ^ 1][r] = ld_x(H == 3 ? s + 1 : s, HN, r);
+        if (H == 3 && i == 0) wc[j] = wcn[j], sc[j] = scn[j];
+#pragma unroll
+        for (int r = k * 4 / TILES; r < (k + 1) * 4 / TILES; ++r) mx4_decode8(wc[r][HN], mx4_scale(sc[r]), wa[A ^ 1][r]);
+#pragma unroll
+        for (int l = k * L / TILES; l < (k + 1) * L / TILES; ++l) load(l);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  // every wave's operand reads and loads so far have landed, for all to see
+  auto meet = [&]() {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto none = [](int) {};
+
+  issue_s(0);
+#pragma unroll
+  for (int v = 0; v < 8; ++v) issue_w(0, v);
+#pragma unroll
+  for (int v = 0; v < NX; ++v) issue_x(0, v);
+#pragma unroll
+  for (int v = 0; v < NX; ++v) issue_x(1, v);
+#pragma unroll
+  for (int v = 0; v < 2; ++v) issue_w(1, v);  // (steps 0 to 2 issue the rest)
+  meet();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    wc[j] = ld_w(0, j);
+    sc[j] = ld_s(0, j);
+    mx4_decode8(wc[j][0], mx4_scale(sc[j]), wa[0][j]);
+  }
+#pragma unroll
+  for (int i = 0; i < MI; ++i) xa[0][i] = ld_x(0, 0, i);
+  // (separate zeros: sums that start as one shared value are moved from register to
+  // register every turn of the loop)
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+      asm volatile("" : "+a"(acc[i][j]));
+    }
+  for (int s = 0; s < nsteps; ++s) {
+    substep(std::integral_constant<int, 0>{}, s, none);
+    substep(std::integral_constant<int, 1>{}, s, none);
+    substep(std::integral_constant<int, 2>{}, s, none);
+    meet();  // x of step s read to its end, x of step s + 1 (and its codes and scales) there
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      wcn[j] = ld_w(s + 1, j);
+      scn[j] = ld_s(s + 1, j);
+    }
+    if ((s & 7) == 3) issue_s((s >> 3) + 1);
+    // W two stages ahead: a stage's last codes were read for its last step, in the third
+    // sub-step of the step before
+    const int f = (s + 1) / 4 + 1, v0 = 2 * ((s + 1) & 3);
+    substep(std::integral_constant<int, 3>{}, s, [&](int l) {
+      if (l < NX)
+        issue_x(s + 2, l);
+      else
+        issue_w(f, v0 + l - NX);
+    });
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the trailing loads have landed before the waves exit
+
+  mg_epilogue<MI, SPLIT, T>(B, P, smem, acc, m0, n0);
+}
+
+// The pre-pass, a wave a column: its scales [superstep][column][16] in the order
+// [u][step], 1.0 behind its end; for fp16 relative to the largest, and that one's factor.
+struct MtScales {
+  const uint8_t* in[MX4_MAXPROB];
+  uint32_t* out[MX4_MAXPROB];
+  float* cs[MX4_MAXPROB];
+  int O, nb, NS;
+};
+template <bool REL>
+__global__ __launch_bounds__(256) void mx4_tile_scales_kernel(const MtScales S) {
+  const int o = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, p = blockIdx.y;
+  if (o >= S.O) return;
+  const uint8_t* in = S.in[p] + (int64_t)o * S.nb;
+  uint32_t m = 0;
+  if (REL) {
+    for (int i = lane; i < S.nb; i += 64) m = max(m, (uint32_t)in[i]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 64));
+    if (lane == 0) S.cs[p][o] = mx4_factor(m);
+  }
+  for (int d = lane; d < 4 * S.NS; d += 64) {
+    const int b0 = 16 * (d >> 2) + 8 * (d & 1) + (d >> 1 & 1);
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int b = b0 + 2 * i;
+      const uint32_t e = b < S.nb ? in[b] : 127u;
+      v |= (REL ? mx4_relative_byte(b < S.nb ? e : m, m) : e) << (8 * i);
+    }
+    S.out[p][((int64_t)(d >> 2) * S.O + o) * 4 + (d & 3)] = v;
+  }
+}
+
+static const MgCost MX4_TILE_COST = {{1.0, 4.0, 8.0}, {0.0, 0.0, 6.0}, {4.5, 7.0, 13.0}, {0.5, 1.0, 4.0}};
+static MgPlan mx4_tile_plan(int nprob, int64_t rows, int64_t O, int64_t I) {
+  return mg_plan(MX4_TILE_COST, nprob, rows, O, (I + 511) / 512);
+}
+static int64_t mx4_tile_scales(int64_t O, int64_t I) { return mg_up256(O * 16 * ((I + 511) / 512)); }
+
+bool mx4_tile_supported(int64_t rows, int64_t O, int64_t I) { return mg_supported(rows, O, I); }
+
+int64_t mx4_tile_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I) {
+  return nprob * (mx4_tile_scales(O, I) + mg_up256(4 * O)) +
+         mg_part_bytes(mx4_tile_plan(nprob, rows, O, I), nprob, rows, O);
+}
+
+template <int MI, typename T>
+static int mt_go(const MgArgs& a, int nprob, void* stream) {
+  // (the epilogue's staging, 64 MI rows of 528 bytes, fits in it)
+  constexpr int lds = 2 * (64 * MI * 128 + MG_N * (128 + 16));
+  static_assert(lds >= 64 * MI * 528, "epilogue staging");
+  static std::atomic<uint64_t> raised[2];
+  auto launch = [&](auto kern, std::atomic<uint64_t>& done) {
+    if (int rc = raise_dynamic_lds(reinterpret_cast<const void*>(kern), lds, done, "mx4_tile_kernel")) return rc;
+    hipLaunchKernelGGL(kern, mg_grid(a, nprob), dim3(256), lds, as_stream(stream), a);
+    if (int rc = check_launch("mx4_tile_kernel")) return rc;
+    return mg_reduce<T>(a, nprob, stream);
+  };
+  return a.S == 1 ? launch(&mx4_tile_kernel<MI, false, T>, raised[0]) : launch(&mx4_tile_kernel<MI, true, T>, raised[1]);
+}
+
+int mx4_tile_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* stream) {
+  const MgPlan pl = mx4_tile_plan(nprob, b.rows, b.O, b.I);
+  const bool f16 = act_dtype == RWKV7MI_F16;
+  MgArgs a{};
+  mg_sizes(a, b, pl);
+  MtScales s{};
+  s.O = b.O;
+  s.nb = b.I / MX4_BLOCK;
+  s.NS = a.NS;
+  uint8_t* at = static_cast<uint8_t*>(ws);
+  for (int i = 0; i < nprob; ++i) {
+    a.p[i] = b.p[i];
+    s.in[i] = b.p[i].ws;
+    s.out[i] = reinterpret_cast<uint32_t*>(at);
+    a.p[i].ws = at;
+    at += mx4_tile_scales(b.O, b.I);
+    s.cs[i] = reinterpret_cast<float*>(at);
+    a.cs[i] = f16 ? s.cs[i] : nullptr;
+    at += mg_up256(4 * (int64_t)b.O);
+  }
+  a.part = reinterpret_cast<float*>(at);
+  const dim3 grid((unsigned)((b.O + 3) / 4), (unsigned)nprob);
+  if (f16)
+    hipLaunchKernelGGL(mx4_tile_scales_kernel<true>, grid, dim3(256), 0, as_stream(stream), s);
+  else
+    hipLaunchKernelGGL(mx4_tile_scales_kernel<false>, grid, dim3(256), 0, as_stream(stream), s);
+  if (int rc = check_launch("mx4_tile_scales_kernel")) return rc;
+  const auto go = [&](auto t) {
+    using T = decltype(t);
+    return pl.mi == 1 ? mt_go<1, T>(a, nprob, stream) : pl.mi == 2 ? mt_go<2, T>(a, nprob, stream)
+                                                                   : mt_go<4, T>(a, nprob, stream);
+  };
+  return f16 ? go(__half{}) : go(__hip_bfloat16{});
+}
+
+}  // namespace rwkv7mi

@@ -83,7 +83,8 @@ def test_quantize_strides_and_ranks():
 # ------------------------------------------------------------------ products
 SHAPES = [(1, 32, 1), (1, 64, 17), (2, 96, 40), (16, 128, 16), (17, 160, 33), (1, 4096, 48), (5, 1056, 65),
           (33, 1024, 100), (40, 512, 300), (64, 2048, 96), (65, 288, 130), (129, 640, 257), (200, 2560, 512),
-          (257, 1024, 520), (300, 96, 70), (520, 768, 264)]
+          (257, 1024, 520), (300, 96, 70), (520, 768, 264),
+          (2, 8704, 30), (9, 16384, 40), (16, 8224, 24)]
 
 
 def _case(rows, n, m, dt, seed, *, lo=112, hi=122):
