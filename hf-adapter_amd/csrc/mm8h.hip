@@ -50,6 +50,7 @@
 
 #include "dense_common.h"
 #include "mm8t_common.h"
+#include "mx4_common.h"
 
 namespace rwkv7mi {
 
@@ -69,6 +70,7 @@ struct MhProb {
   void* y;
   int epilogue;
   int vec;  // O % 8 == 0 and y (and the residual) 16-byte aligned: 16-byte output rows
+  const float* cs;  // MX instances: a factor per column, before the bias (null: none)
 };
 struct MhBatch {
   MhProb p[MM8T_MAXPROB];
@@ -193,8 +195,13 @@ __global__ __launch_bounds__(256) void mm8h_dequant_kernel(const MhDeqBatch D) {
   }
 }
 
+template <bool MX>
+__device__ __forceinline__ float mh_relu(float w) {
+  return MX ? (w < 0.f ? 0.f : w) : fmaxf(w, 0.f);
+}
+
 // The tail of a column vector run: y = epilogue(v + bias), 8 columns from c0
-template <typename TA>
+template <typename TA, bool MX>
 __device__ __forceinline__ void mh_store8(const MhProb& P, int64_t row, int c0, int O, float (&v)[8]) {
   using E = typename MhTypes<TA>::E;
   using V = typename MhTypes<TA>::V;
@@ -210,7 +217,7 @@ __device__ __forceinline__ void mh_store8(const MhProb& P, int64_t row, int c0, 
     for (int e = 0; e < 8; ++e) {
       float w = v[e];
       if (P.epilogue == RWKV7MI_EPI_RELU2) {
-        w = fmaxf(w, 0.f);
+        w = mh_relu<MX>(w);
         w = w * w;
       }
       o8[e] = (E)w;
@@ -222,7 +229,7 @@ __device__ __forceinline__ void mh_store8(const MhProb& P, int64_t row, int c0, 
       if (c0 + e >= O) continue;
       float w = v[e];
       if (P.epilogue == RWKV7MI_EPI_RELU2) {
-        w = fmaxf(w, 0.f);
+        w = mh_relu<MX>(w);
         w = w * w;
       } else if (P.epilogue == RWKV7MI_EPI_RESIDUAL) {
         w += ld(reinterpret_cast<const TA*>(P.residual), oi + e);
@@ -234,7 +241,7 @@ __device__ __forceinline__ void mh_store8(const MhProb& P, int64_t row, int c0, 
 
 // S > 1: one thread adds the S fp32 partials of 8 columns of a row in split
 // order and applies the epilogue.  Memory-bound: 4 S + 2 (+ 2) bytes a value.
-template <typename TA>
+template <typename TA, bool MX>
 __global__ __launch_bounds__(256) void mm8h_reduce_kernel(const MhBatch B) {
   const MhProb& P = B.p[blockIdx.y];
   const int cols = (int)(B.ldp / 8);
@@ -253,17 +260,22 @@ __global__ __launch_bounds__(256) void mm8h_reduce_kernel(const MhBatch B) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += a[e];
   }
+  if constexpr (MX) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) if (P.cs && c0 + e < B.O) v[e] *= P.cs[c0 + e];
+  }
   const TA* bp = reinterpret_cast<const TA*>(P.bias);
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] += bp && c0 + e < B.O ? to_f32(bp[c0 + e]) : 0.f;
-  mh_store8<TA>(P, row, c0, B.O, v);
+  mh_store8<TA, MX>(P, row, c0, B.O, v);
 }
 
 // FULLK: I is a multiple of 64 (no step ends inside a 16-byte chunk's range).
 // SPLIT: blockIdx.z takes B.sps of the steps and leaves fp32 partial tiles (an
 // instance of its own: the bounds and the second epilogue cost the unsplit
-// kernel 4%)
-template <bool FULLK, bool SPLIT, typename TA>
+// kernel 4%).  MX: the records are an MXFP4 weight's: a factor per column (fp16
+// rows are scaled by a power of two each), and relu^2 keeps a NaN
+template <bool FULLK, bool SPLIT, typename TA, bool MX>
 __global__ __launch_bounds__(MH_THREADS, 1) void mm8h_gemm_kernel(const MhBatch B) {
   using E = typename MhTypes<TA>::E;
   using V = typename MhTypes<TA>::V;
@@ -435,9 +447,13 @@ __global__ __launch_bounds__(MH_THREADS, 1) void mm8h_gemm_kernel(const MhBatch 
   for (int p = 0; p < 2; ++p) {
     const int c0 = n0 + 64 * wave + 32 * p + 8 * kg;
     if (c0 >= O) continue;
-    float bo[8];
+    float bo[8], co[MX ? 8 : 1];
 #pragma unroll
     for (int e = 0; e < 8; ++e) bo[e] = bp && c0 + e < O ? to_f32(bp[c0 + e]) : 0.f;
+    if constexpr (MX) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) co[e] = P.cs && c0 + e < O ? P.cs[c0 + e] : 1.f;
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int64_t row = m0 + 16 * i + n;
@@ -445,8 +461,13 @@ __global__ __launch_bounds__(MH_THREADS, 1) void mm8h_gemm_kernel(const MhBatch 
       float v[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        v[e] = acc[i][2 * p][e] + bo[e];
-        v[4 + e] = acc[i][2 * p + 1][e] + bo[4 + e];
+        if constexpr (MX) {
+          v[e] = acc[i][2 * p][e] * co[e] + bo[e];
+          v[4 + e] = acc[i][2 * p + 1][e] * co[4 + e] + bo[4 + e];
+        } else {
+          v[e] = acc[i][2 * p][e] + bo[e];
+          v[4 + e] = acc[i][2 * p + 1][e] + bo[4 + e];
+        }
       }
       const int64_t oi = row * O + c0;
       if (vec && c0 + 8 <= O) {
@@ -460,7 +481,7 @@ __global__ __launch_bounds__(MH_THREADS, 1) void mm8h_gemm_kernel(const MhBatch 
         for (int e = 0; e < 8; ++e) {
           float w = v[e];
           if (P.epilogue == RWKV7MI_EPI_RELU2) {
-            w = fmaxf(w, 0.f);
+            w = mh_relu<MX>(w);
             w = w * w;
           }
           o8[e] = (E)w;
@@ -472,7 +493,7 @@ __global__ __launch_bounds__(MH_THREADS, 1) void mm8h_gemm_kernel(const MhBatch 
           if (c0 + e >= O) continue;
           float w = v[e];
           if (P.epilogue == RWKV7MI_EPI_RELU2) {
-            w = fmaxf(w, 0.f);
+            w = mh_relu<MX>(w);
             w = w * w;
           } else if (P.epilogue == RWKV7MI_EPI_RESIDUAL) {
             w += ld(reinterpret_cast<const TA*>(P.residual), oi + e);
@@ -567,7 +588,7 @@ static int64_t mh_part_bytes(int64_t nprob, int64_t rows, int64_t O) {
   return nprob * rows * ((O + 31) / 32 * 32) * 4;
 }
 // the GEMM over prepared W_hat records (b.p[i].wt), with the tile grid set here
-template <typename TA>
+template <typename TA, bool MX = false>
 static int mh_gemm_launch(MhBatch& b, int nprob, int64_t rows, int64_t I, int64_t O, void* ws, int64_t ws_bytes,
                           void* stream, const std::string& w) {
   b.rows = (int)rows;
@@ -595,14 +616,14 @@ static int mh_gemm_launch(MhBatch& b, int nprob, int64_t rows, int64_t I, int64_
                        as_stream(stream), b);
     if (int rc = check_launch("mm8h_gemm_kernel")) return rc;
     if (b.S == 1) return (int)RWKV7MI_OK;
-    hipLaunchKernelGGL(mm8h_reduce_kernel<TA>, dim3((unsigned)((rows * (b.ldp / 8) + 255) / 256), (unsigned)nprob),
+    hipLaunchKernelGGL((mm8h_reduce_kernel<TA, MX>), dim3((unsigned)((rows * (b.ldp / 8) + 255) / 256), (unsigned)nprob),
                        dim3(256), 0, as_stream(stream), b);
     return check_launch("mm8h_reduce_kernel");
   };
   static std::atomic<uint64_t> raised[3];
-  if (b.S > 1) return launch(&mm8h_gemm_kernel<true, true, TA>, raised[0]);
-  return I % 64 == 0 ? launch(&mm8h_gemm_kernel<true, false, TA>, raised[1])
-                     : launch(&mm8h_gemm_kernel<false, false, TA>, raised[2]);
+  if (b.S > 1) return launch(&mm8h_gemm_kernel<true, true, TA, MX>, raised[0]);
+  return I % 64 == 0 ? launch(&mm8h_gemm_kernel<true, false, TA, MX>, raised[1])
+                     : launch(&mm8h_gemm_kernel<false, false, TA, MX>, raised[2]);
 }
 
 double mm8h_estimate_us(int64_t nprob, int64_t rows, int64_t I, int64_t O) {
@@ -755,9 +776,9 @@ extern "C" int rwkv7mi_dense_gemm_prefill_ws(int nprob, const void* const* x, co
     if (S == 1) return RWKV7MI_OK;
     const dim3 rgrid((unsigned)((rows * (t.ldp / 8) + 255) / 256), (unsigned)nprob);
     if (act_dtype == RWKV7MI_BF16)
-      hipLaunchKernelGGL(mm8h_reduce_kernel<__hip_bfloat16>, rgrid, dim3(256), 0, as_stream(stream), t);
+      hipLaunchKernelGGL((mm8h_reduce_kernel<__hip_bfloat16, false>), rgrid, dim3(256), 0, as_stream(stream), t);
     else
-      hipLaunchKernelGGL(mm8h_reduce_kernel<__half>, rgrid, dim3(256), 0, as_stream(stream), t);
+      hipLaunchKernelGGL((mm8h_reduce_kernel<__half, false>), rgrid, dim3(256), 0, as_stream(stream), t);
     return check_launch("mm8h_reduce_kernel");
   }
   const int64_t per_prob = mh_weight_bytes(1, I, O);
@@ -786,3 +807,125 @@ extern "C" int rwkv7mi_dense_gemm_prefill_ws(int nprob, const void* const* x, co
   if (int rc = check_launch("mm8h_relayout_kernel")) return rc;
   return mh_gemm_launch<__half>(b, nprob, rows, I, O, ws, ws_bytes, stream, w);
 }
+
+namespace rwkv7mi {
+
+// ---- MXFP4 weights: the same records, then the same GEMM.  fp16 rows are scaled
+// relative to their largest scale and the sums by its factor per column
+// (mx4_common.h).
+struct Mx4hBatch {
+  const uint8_t *codes[MX4_MAXPROB], *scales[MX4_MAXPROB];
+  void* out[MX4_MAXPROB];
+  float* cs[MX4_MAXPROB];  // fp16: the columns' factors
+  int I, O, SB;
+};
+
+// one wave a row: the largest scale byte as the column's factor
+__global__ __launch_bounds__(256) void mx4h_factor_kernel(const Mx4hBatch D) {
+  const int o = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, nb = D.I / MX4_BLOCK;
+  if (o >= D.O) return;
+  const uint8_t* s = D.scales[blockIdx.y] + (int64_t)o * nb;
+  int m = 0;
+  for (int i = lane; i < nb; i += 64) m = max(m, (int)s[i]);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) m = max(m, __shfl_xor(m, d, 64));
+  if (lane == 0) D.cs[blockIdx.y][o] = mx4_factor((uint32_t)m);
+}
+
+// one thread per (column group, step, lane): 8 bytes of codes -> its two records.
+// Bound by the 2 bytes a weight it writes.
+template <typename TA>
+__global__ __launch_bounds__(256) void mx4h_dequant_kernel(const Mx4hBatch D) {
+  using V = typename MhTypes<TA>::V;
+  const int p = blockIdx.y;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int ngroups = 2 * ((D.O + 31) / 32);
+  if (t >= (int64_t)ngroups * D.SB * 64) return;
+  const int lane = (int)(t & 63);
+  const int64_t gs = t >> 6;
+  const int sb = (int)(gs % D.SB), g = (int)(gs / D.SB);
+  const int n = lane & 15, kg = lane >> 4;
+  const int o = 32 * (g >> 1) + 8 * (n >> 2) + 4 * (g & 1) + (n & 3);
+  const int k0 = 64 * sb + 16 * kg;
+  uint2 c = make_uint2(0u, 0u);
+  float s = 0.f;
+  if (o < D.O && k0 < D.I) {  // I % 32 == 0: the lane's 16 inputs are of one block
+    c = *reinterpret_cast<const uint2*>(D.codes[p] + (int64_t)o * (D.I / 2) + k0 / 2);
+    const uint32_t e = D.scales[p][(int64_t)o * (D.I / MX4_BLOCK) + k0 / MX4_BLOCK];
+    if constexpr (std::is_same<TA, __half>::value)
+      s = mx4_relative(e, mx4_factor_emax(D.cs[p][o]));
+    else
+      s = mx4_scale(e);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    V v;
+    mx4_decode8(h ? c.y : c.x, s, v);
+    *reinterpret_cast<V*>(static_cast<char*>(D.out[p]) + gs * MH_REC + h * 1024 + 16 * lane) = v;
+  }
+}
+
+static int64_t mx4h_factor_bytes(int nprob, int64_t O) { return (nprob * O * 4 + 255) & ~(int64_t)255; }
+// rows of one GEMM: x's descriptor ends below 2^31 bytes
+static int64_t mx4h_chunk(int64_t rows, int64_t I) {
+  return std::min<int64_t>(rows, (((int64_t)1 << 31) - 1) / (2 * I) / MH_M * MH_M);
+}
+
+bool mx4h_supported(int64_t rows, int64_t I, int64_t O) {
+  return mx4h_chunk(rows, I) > 0 && 4 * ((I + 63) / 64) * MH_REC < (int64_t)MM8T_OOB &&
+         (O + MH_N - 1) / MH_N * ((mx4h_chunk(rows, I) + MH_M - 1) / MH_M) < INT32_MAX / 64;
+}
+
+int64_t mx4h_workspace_bytes(int nprob, int64_t rows, int64_t I, int64_t O) {
+  return mx4h_factor_bytes(nprob, O) +
+         rwkv7mi_mm8t_gemm_prefill_split_ws_bytes(nprob, mx4h_chunk(rows, I), I, O);
+}
+
+template <typename TA>
+static int mx4h_go(const Mx4Batch& m, int nprob, char* ws, int64_t ws_bytes, void* stream) {
+  constexpr bool F16 = std::is_same<TA, __half>::value;
+  const std::string w("mxfp4_linear");
+  const int64_t I = m.I, O = m.O, fb = mx4h_factor_bytes(nprob, O), per = mh_weight_bytes(1, I, O);
+  Mx4hBatch d{};
+  d.I = m.I;
+  d.O = m.O;
+  d.SB = (int)((I + 63) / 64);
+  for (int i = 0; i < nprob; ++i) {
+    d.codes[i] = m.p[i].wc;
+    d.scales[i] = m.p[i].ws;
+    d.cs[i] = reinterpret_cast<float*>(ws) + i * O;
+    d.out[i] = ws + fb + i * per;
+  }
+  if (F16) {
+    hipLaunchKernelGGL(mx4h_factor_kernel, dim3((unsigned)((O + 3) / 4), (unsigned)nprob), dim3(256), 0,
+                       as_stream(stream), d);
+    if (int rc = check_launch("mx4h_factor_kernel")) return rc;
+  }
+  const int64_t recs = (2 * ((O + 31) / 32)) * (int64_t)d.SB * 64;
+  hipLaunchKernelGGL(mx4h_dequant_kernel<TA>, dim3((unsigned)((recs + 255) / 256), (unsigned)nprob), dim3(256), 0,
+                     as_stream(stream), d);
+  if (int rc = check_launch("mx4h_dequant_kernel")) return rc;
+  const int64_t step = mx4h_chunk(m.rows, I);
+  for (int64_t r = 0; r < m.rows; r += step) {
+    MhBatch b{};
+    for (int i = 0; i < nprob; ++i) {
+      const Mx4Prob& p = m.p[i];
+      const char* res = static_cast<const char*>(p.residual);
+      if (int rc = mh_prob(w, b.p[i], static_cast<const char*>(p.x) + r * I * 2, d.out[i], p.bias,
+                           res ? res + r * O * 2 : nullptr, static_cast<char*>(p.y) + r * O * 2, p.epilogue, O))
+        return rc;
+      b.p[i].cs = F16 ? d.cs[i] : nullptr;
+    }
+    if (int rc = mh_gemm_launch<TA, true>(b, nprob, std::min<int64_t>(step, m.rows - r), I, O, ws + fb, ws_bytes - fb,
+                                        stream, w))
+      return rc;
+  }
+  return RWKV7MI_OK;
+}
+
+int mx4h_run(const Mx4Batch& m, int nprob, int act_dtype, void* ws, int64_t ws_bytes, void* stream) {
+  return act_dtype == RWKV7MI_BF16 ? mx4h_go<__hip_bfloat16>(m, nprob, static_cast<char*>(ws), ws_bytes, stream)
+                                   : mx4h_go<__half>(m, nprob, static_cast<char*>(ws), ws_bytes, stream);
+}
+
+}  // namespace rwkv7mi

@@ -47,6 +47,10 @@ __device__ __forceinline__ float mx4_factor(uint32_t emax) {
   return emax == 255u ? __builtin_nanf("") : ldexpf(1.f, (int)emax - 140);
 }
 
+__device__ __forceinline__ uint32_t mx4_factor_emax(float f) {  // emax again
+  return f != f ? 255u : (uint32_t)(ilogbf(f) + 140);
+}
+
 // 8 codes of a dword -> 8 values times the scale, in order
 __device__ __forceinline__ void mx4_decode8(uint32_t d, float s, bf16x8& o) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 0);
@@ -102,5 +106,11 @@ int mx4_gemm_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* st
 bool mx4_tile_supported(int64_t rows, int64_t O, int64_t I);
 int64_t mx4_tile_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I);
 int mx4_tile_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* stream);
+
+// Products through fp16 / bf16 records of the weight and the 256 x 256 GEMM of
+// mm8h.hip: whether it takes these shapes, its workspace, its launches.
+bool mx4h_supported(int64_t rows, int64_t I, int64_t O);
+int64_t mx4h_workspace_bytes(int nprob, int64_t rows, int64_t I, int64_t O);
+int mx4h_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, int64_t ws_bytes, void* stream);
 
 }  // namespace rwkv7mi

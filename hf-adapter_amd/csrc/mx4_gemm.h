@@ -1,7 +1,7 @@
 // What the two many-row MXFP4 products share (mx4_gemm.hip: 4-bit rows, mx4_tile.hip:
-// 16-bit rows): the 64 MI x 256 tile of a 256-lane workgroup, four waves of 32 MI x 128
-// in tiles of 32x32 MFMAs, W as the A operand, its numbering, its epilogue, the plan of
-// tile heights and K splits.
+// 16-bit rows): the 64 MI x 256 tile of a workgroup, two rows of WC waves of 32 MI x 256
+// / WC in tiles of 32x32 MFMAs, W as the A operand, its numbering, its epilogue, the
+// plan of tile heights and K splits.
 #pragma once
 #include <algorithm>
 
@@ -81,57 +81,66 @@ __device__ __forceinline__ bool mg_vec(const Mx4Prob& P, int O) {
 }
 
 // The tile's end.  Lane: row 32 i + n and, in group j, columns 64 (j / 2) + 16 a + 8 u
-// + 4 (j % 2) .. +3, a = 0 .. 3.  The sums go through LDS (the stages are done with) in two
-// halves of 64 columns a wave, and come back as whole rows: 16 lanes a row, 8
+// + 4 (j % 2) .. +3, a = 0 .. 3.  The sums go through LDS (the stages are done with),
+// two row tiles a wave at a time, and come back as whole rows: 32 lanes a row, 8
 // columns each, whose bias stays in registers.  (Finished and stored from the MFMA
-// layout, 32-byte pieces of 32 rows an instruction, the epilogue took as long as
-// half the main loop.)
-template <int MI, bool SPLIT, typename T>
-__device__ __forceinline__ void mg_epilogue(const MgArgs& B, const Mx4Prob& P, char* smem, const f32x16 (&acc)[MI][4], int m0,
-                                            int n0) {
+// layout, 32-byte pieces of 32 rows an instruction, the epilogue of the 4-bit rows took
+// as long as half their main loop.)
+constexpr int MG_LDT = MG_N * 4 + 16;  // a staged row (the 16 bytes spread it over the banks)
+constexpr int mg_staging(int mi) { return (mi < 2 ? 64 : 128) * MG_LDT; }
+
+template <int MI, int WC, bool SPLIT, typename T>
+__device__ __forceinline__ void mg_epilogue(const MgArgs& B, const Mx4Prob& P, char* smem, const f32x16 (&acc)[MI][8 / WC],
+                                            int m0, int n0) {
+  constexpr int W = 2 * WC, RT = MI < 2 ? 1 : 2;  // waves; row tiles a wave and pass
   const int O = B.O, M = B.rows, nrow = min(64 * MI, M - m0);
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, u = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = 32 * MI * (wave >> 1);
-  constexpr int LDT = 128 * 4 + 16;  // a staged row (the 16 bytes spread it over the banks)
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave / WC, wn = MG_N / WC * (wave % WC);
   const bool vec = mg_vec(P, O);
   const int epi = P.epilogue;
   const T *bias = static_cast<const T*>(P.bias), *res = static_cast<const T*>(P.residual);
   T* y = static_cast<T*>(P.y);
   const float* cs = SPLIT ? nullptr : B.cs[blockIdx.y];
   float* part = SPLIT ? B.part + ((int64_t)blockIdx.y * B.S + blockIdx.z) * M * B.ldp : nullptr;
-  const int ll = 8 * (lane & 15);  // this lane's column of the staged 128
+  const int cl = 8 * (lane & 31), c0 = n0 + cl;
+  const bool whole = vec && c0 + 8 <= O;
+  float bo[8], co[8];
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
+  for (int e = 0; e < 8; ++e) {
+    bo[e] = !SPLIT && bias && c0 + e < O ? to_f32(bias[c0 + e]) : 0.f;
+    co[e] = cs && c0 + e < O ? cs[c0 + e] : 1.f;
+  }
+#pragma unroll
+  for (int p = 0; p < MI / RT; ++p) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
+      for (int j = 0; j < 8 / WC; ++j)
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const f32x16 c = acc[i][2 * p + g];
-          *reinterpret_cast<f32x4*>(smem + (wm + 32 * i + n) * LDT + ((wave & 1) * 64 + 16 * a + 8 * u + 4 * g) * 4) =
+        for (int a = 0; a < 4; ++a) {
+          const f32x16 c = acc[RT * p + i][j];
+          *reinterpret_cast<f32x4*>(smem + (32 * (RT * wr + i) + n) * MG_LDT +
+                                    (wn + 64 * (j >> 1) + 16 * a + 8 * u + 4 * (j & 1)) * 4) =
               (f32x4){c[4 * a], c[4 * a + 1], c[4 * a + 2], c[4 * a + 3]};
         }
     __syncthreads();
-    const int cl = 128 * (ll >> 6) + 64 * p + (ll & 63), c0 = n0 + cl;
     if (c0 >= O) continue;
-    const bool whole = vec && c0 + 8 <= O;
-    float bo[8], co[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bo[e] = !SPLIT && bias && c0 + e < O ? to_f32(bias[c0 + e]) : 0.f;
-      co[e] = cs && c0 + e < O ? cs[c0 + e] : 1.f;
-    }
-    // four rows at a time: their LDS reads (and residuals) are in flight together
-    for (int rb = 4 * wave + (lane >> 4); rb < nrow; rb += 64) {
+    // four rows at a time: their LDS reads (and residuals) are in flight together;
+    // staged row s is row s + 32 (MI - RT) (s / (32 RT)) + 32 RT p of the tile
+    for (int sb = 2 * wave + (lane >> 5); sb < 64 * RT; sb += 8 * W) {
       float v[4][8], w[4][8];
+      int r[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) ld8(reinterpret_cast<const float*>(smem + (rb + 16 * k) * LDT) + ll, v[k]);
+      for (int k = 0; k < 4; ++k) {
+        const int s = sb + 2 * W * k;
+        r[k] = s + 32 * (MI - RT) * (s / (32 * RT)) + 32 * RT * p;
+        ld8(reinterpret_cast<const float*>(smem + s * MG_LDT) + cl, v[k]);
+      }
       if (!SPLIT && epi == RWKV7MI_EPI_RESIDUAL) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int64_t oi = (int64_t)(m0 + min(rb + 16 * k, nrow - 1)) * O + c0;
+          const int64_t oi = (int64_t)(m0 + min(r[k], nrow - 1)) * O + c0;
           if (whole) {
             ld8(res + oi, w[k]);
           } else {
@@ -142,9 +151,8 @@ __device__ __forceinline__ void mg_epilogue(const MgArgs& B, const Mx4Prob& P, c
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int r = rb + 16 * k;
-        const int64_t row = m0 + r, oi = row * O + c0;
-        if (r >= nrow) break;
+        if (r[k] >= nrow) continue;
+        const int64_t row = m0 + r[k], oi = row * O + c0;
         if constexpr (SPLIT) {
           st8(part + row * B.ldp + c0, v[k]);
           continue;

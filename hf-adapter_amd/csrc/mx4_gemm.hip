@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the trailing loads have landed before the waves exit
 
-  mg_epilogue<MI, SPLIT, T>(B, P, smem, acc, m0, n0);
+  mg_epilogue<MI, 2, SPLIT, T>(B, P, smem, acc, m0, n0);
 }
 
 // Fitted to 20 shapes from 17 x 2048 -> 2048 to 7000 x 2048 -> 2048, every tile height
@@ -223,7 +223,7 @@ int64_t mx4_gemm_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I) 
 
 template <int MI, typename T>
 static int mg_go(const MgArgs& a, int nprob, void* stream) {
-  constexpr int lds = 2 * (64 * MI + MG_N) * (128 + 16);
+  constexpr int lds = std::max(2 * (64 * MI + MG_N) * (128 + 16), mg_staging(MI));
   static std::atomic<uint64_t> raised[2];
   auto launch = [&](auto kern, std::atomic<uint64_t>& done) {
     if (int rc = raise_dynamic_lds(reinterpret_cast<const void*>(kern), lds, done, "mx4_gemm_kernel")) return rc;

@@ -254,9 +254,18 @@ static int mx4_rows_run(const Mx4Batch& b, int nprob, void* part, void* stream) 
 static int64_t mx4_codes_bytes(int64_t rows, int64_t I) { return (rows * (I / 2) + 255) & ~(int64_t)255; }
 static int64_t mx4_scales_bytes(int64_t rows, int64_t I) { return (rows * (I / MX4_BLOCK) + 255) & ~(int64_t)255; }
 
-// More rows than a tile of the few-row kernel: the 64- to 256-row tiles.
-static bool mx4_many(int64_t rows, int64_t I, int64_t O, int quantize_input) {
-  return rows > 16 && (quantize_input ? mx4_gemm_supported(rows, O, I) : mx4_tile_supported(rows, O, I));
+// Which kernel takes a product: up to 16 rows (and what the others' offsets cannot
+// hold) the few-row kernel, above it the 64- to 256-row tiles.  16-bit rows from 1024
+// tiles of 256 x 256 on write the weight out in 16 bits and run the GEMM of mm8h.hip:
+// without conversions between its MFMAs it holds a higher clock over such long calls
+// (16384 x 4096 -> 16384 1672 us, on the tiles 2000), and the pass over the weight
+// is small against them (1000 rows, 256 tiles: 150 and 145).
+enum Mx4Route { MX4_ROWS, MX4_TILE, MX4_GEMM, MX4_PREFILL };
+static Mx4Route mx4_route(int64_t rows, int64_t I, int64_t O, int quantize_input) {
+  if (rows <= 16) return MX4_ROWS;
+  if (quantize_input) return mx4_gemm_supported(rows, O, I) ? MX4_GEMM : MX4_ROWS;
+  if ((rows + 255) / 256 * ((O + 255) / 256) >= 1024 && mx4h_supported(rows, I, O)) return MX4_PREFILL;
+  return mx4_tile_supported(rows, O, I) ? MX4_TILE : MX4_ROWS;
 }
 
 }  // namespace rwkv7mi
@@ -266,8 +275,10 @@ using namespace rwkv7mi;
 extern "C" int64_t rwkv7mi_mxfp4_linear_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I, int act_dtype,
                                                         int quantize_input) {
   if (nprob < 1 || nprob > MX4_MAXPROB || rows <= 0 || O <= 0 || I <= 0) return 0;
-  if (mx4_many(rows, I, O, quantize_input))
-    return quantize_input ? mx4_gemm_workspace_bytes(nprob, rows, O, I) : mx4_tile_workspace_bytes(nprob, rows, O, I);
+  const Mx4Route route = mx4_route(rows, I, O, quantize_input);
+  if (route == MX4_PREFILL) return mx4h_workspace_bytes(nprob, rows, I, O);
+  if (route == MX4_GEMM) return mx4_gemm_workspace_bytes(nprob, rows, O, I);
+  if (route == MX4_TILE) return mx4_tile_workspace_bytes(nprob, rows, O, I);
   const int64_t part = mx4_rows_part_bytes(nprob, rows, O, I);
   return part + (quantize_input ? nprob * (mx4_codes_bytes(rows, I) + mx4_scales_bytes(rows, I)) : 0);
 }
@@ -306,8 +317,10 @@ extern "C" int rwkv7mi_mxfp4_linear(int nprob, const void* const* x, const uint8
   if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < need))
     return fail(RWKV7MI_ESIZE, w + ": workspace missing, unaligned or smaller than "
                                    "rwkv7mi_mxfp4_linear_workspace_bytes");
-  if (mx4_many(rows, I, O, quantize_input))
-    return quantize_input ? mx4_gemm_run(b, nprob, act_dtype, ws, stream) : mx4_tile_run(b, nprob, act_dtype, ws, stream);
+  const Mx4Route route = mx4_route(rows, I, O, quantize_input);
+  if (route == MX4_PREFILL) return mx4h_run(b, nprob, act_dtype, ws, ws_bytes, stream);
+  if (route == MX4_GEMM) return mx4_gemm_run(b, nprob, act_dtype, ws, stream);
+  if (route == MX4_TILE) return mx4_tile_run(b, nprob, act_dtype, ws, stream);
   if (!quantize_input)
     return bf ? mx4_rows_run<__hip_bfloat16, false>(b, nprob, ws, stream)
               : mx4_rows_run<__half, false>(b, nprob, ws, stream);

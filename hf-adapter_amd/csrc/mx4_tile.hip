@@ -1,23 +1,27 @@
 // MXFP4 weights times 16-bit rows, more than 16 of them: y = epilogue(x W^T + bias),
 // fp16 / bf16 x.
 //
-// The tile of mx4_gemm.h on v_mfma_f32_32x32x16: lane n + 32 u holds 8 inputs of a row.
-// K advances 64 inputs a step, four sub-steps; lane half u takes the block of inputs
-// 32 u .. +31, 8 a sub-step, so a lane's scale holds for a step:
-//  * x: global -> LDS directly, 128 bytes a row, two stages; lane n + 32 u reads chunk
-//    4 u + h in sub-step h;
-//  * W codes: global -> LDS directly, 128 bytes (four steps) a column, two stages; a
-//    lane reads 16 bytes a step, one dword a sub-step, which four conversions turn into
-//    its operand during the sub-step before;
+// The tile of mx4_gemm.h with eight waves (two a SIMD, so that one's conversions and
+// waits hide behind the other's MFMAs: 16384 x 4096 -> 16384 2.14 -> 1.98 ms) on
+// v_mfma_f32_32x32x16: lane n + 32 u holds 8 inputs of a row.  K advances 64 inputs a
+// step, four sub-steps; lane half u takes the block of inputs 32 u .. +31, 8 a sub-step,
+// so a lane's scale holds for a step:
+//  * x: global -> LDS directly, 128 bytes a row, a ring of NXS stages; lane n + 32 u reads
+//    chunk 4 u + h in sub-step h;
+//  * W codes: global -> LDS directly, 128 bytes (four steps) a column, two stages; a lane
+//    reads 16 bytes a step, one dword a sub-step, which four conversions turn into its
+//    operand during the sub-step before (a ring of 64-byte stages, 16384 x 4096 ->
+//    16384: 2.04 ms);
 //  * W's scales: 8 steps (a superstep) at a time, global -> LDS, 16 bytes a column in
 //    the order [u][step], written by a pre-pass.  fp16 columns are scaled relative to
 //    their largest scale (mx4_common.h), which the pre-pass finds, and the sums by its
 //    factor.
 // A stage of x is read to the end in its step's third sub-step: one barrier there, and
-// the loads two steps ahead go into the same stage.  A stage of W is free a sub-step
-// later in its last step, and its loads go out two a step over the next four.  Inputs
-// past I are zeros of x (W's codes there are some finite value).  Where the tiles do
-// not fill the chip K is split over workgroups and a second launch adds the partials.
+// the loads a ring ahead go into the same stage; the barrier waits for the loads of the
+// next step only, by count (with two stages every load had to land within a step: 64 x
+// 16384 -> 4096 took 0.85 us a step).  Inputs past I are zeros of x (W's codes there are
+// some finite value).  Where the tiles do not fill the chip K is split over workgroups
+// and a second launch adds the partials.
 #include "mx4_gemm.h"
 
 namespace rwkv7mi {
@@ -29,19 +33,29 @@ __device__ __forceinline__ f32x16 mt_mfma(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+constexpr int MT_WC = 4, MT_WAVES = 2 * MT_WC;
+// x stages: what W's two leave room for, and W's loads, four steps ahead, are waited for
+constexpr int mt_xstages(int mi) { return mi <= 2 ? 5 : 2; }
+constexpr int mt_lds(int mi) {
+  return std::max(mt_xstages(mi) * 64 * mi * 128 + 2 * MG_N * (128 + 16), mg_staging(mi));
+}
+static_assert(mt_lds(1) <= 163840 && mt_lds(2) <= 163840 && mt_lds(4) <= 163840, "LDS of a CU");
+
 template <int MI, bool SPLIT, typename T>
-__global__ __launch_bounds__(256, 1) void mx4_tile_kernel(const MgArgs B) {
+__global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MgArgs B) {
   using V = typename Mx4Types<T>::V;
   constexpr int ROWS = 64 * MI, XB = ROWS * 128, WB = MG_N * 128, SB = MG_N * 16;  // bytes of a stage of x, W, scales
-  constexpr int NX = 2 * MI;                                                       // x loads a wave and step
+  constexpr int NXS = mt_xstages(MI);
+  constexpr int NJ = 8 / MT_WC, RND = 8 * MT_WAVES;  // column groups of a wave; rows a round of loads
+  constexpr int NX = ROWS / RND, NW = MG_N / RND;    // loads of a wave a stage of x, of W
   const Mx4Prob& P = B.p[blockIdx.y];
   const int M = B.rows, O = B.O, I = B.I, NS = B.NS;
   int tm, tn;
   if (!mg_tile(B, tm, tn)) return;
   const int m0 = tm * ROWS, n0 = tn * MG_N;
 
-  extern __shared__ __align__(16) char smem[];  // two stages each: x, W, scales
-  char* const wst = smem + 2 * XB;
+  extern __shared__ __align__(16) char smem[];  // the stages of x, W and (two) the scales
+  char* const wst = smem + NXS * XB;
   char* const scl = wst + 2 * WB;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, u = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -56,31 +70,31 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(const MgArgs B) {
   const __amdgpu_buffer_rsrc_t wr = make_rsrc(P.wc + (int64_t)n0 * ldw, (uint32_t)(ncol * ldw));
   const __amdgpu_buffer_rsrc_t wsr = make_rsrc(P.ws, (uint32_t)(NS * O * 16));
 
-  // round v of a stage: rows 32 v + 8 w .. +7 of x (W), lane l at row + l / 8, chunk
+  // round v of a stage: rows RND v + 8 w .. +7 of x (W), lane l at row + l / 8, chunk
   // position l % 8
   const int lr = 8 * wave + (lane >> 3);
-  auto issue_x = [&](int s, int v) {
-    const int r = 32 * v + lr, c = (lane & 7) ^ mg_key(r);
+  auto issue_x = [&](int s, int st, int v) {
+    const int r = RND * v + lr, c = (lane & 7) ^ mg_key(r);
     const int vo = 64 * (s0 + s) + 8 * c < I ? r * ldx + 16 * c : (int)BUF_OOB;
     const int so = s < nsteps ? 128 * (s0 + s) : (int)BUF_OOB;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (mg_lds_ptr)(smem + (s & 1) * XB + (32 * v + 8 * wave) * 128), 16, vo, so,
-                                             0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (mg_lds_ptr)(smem + st * XB + (RND * v + 8 * wave) * 128), 16, vo, so, 0, 0);
   };
-  auto issue_w = [&](int f, int v) {  // stage f: steps 4 f .. +3
-    const int r = 32 * v + lr, vo = r * ldw + 16 * ((lane & 7) ^ mg_wkey(r));
+  auto issue_w = [&](int f, int v) {  // steps 4 f .. +3
+    const int r = RND * v + lr, vo = r * ldw + 16 * ((lane & 7) ^ mg_wkey(r));
     const int so = 4 * f < nsteps ? 128 * (s0 / 4 + f) : (int)BUF_OOB;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (mg_lds_ptr)(wst + (f & 1) * WB + (32 * v + 8 * wave) * 128), 16, vo, so, 0,
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (mg_lds_ptr)(wst + (f & 1) * WB + (RND * v + 8 * wave) * 128), 16, vo, so, 0,
                                              0);
   };
-  auto issue_s = [&](int s) {  // scales of superstep s: 64 columns a wave
-    const int so = s < S1 - S0 ? 16 * ((S0 + s) * O + n0 + 64 * wave) : (int)BUF_OOB;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(wsr, (mg_lds_ptr)(scl + (s & 1) * SB + 64 * wave * 16), 16, 16 * lane, so, 0, 0);
+  const int cw = wave % 4;
+  auto issue_s = [&](int s) {  // scales of superstep s: 64 columns a wave (twice)
+    const int so = s < S1 - S0 ? 16 * ((S0 + s) * O + n0 + 64 * cw) : (int)BUF_OOB;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(wsr, (mg_lds_ptr)(scl + (s & 1) * SB + 64 * cw * 16), 16, 16 * lane, so, 0, 0);
   };
 
-  const int wm = 32 * MI * (wave >> 1), wn = 128 * (wave & 1);  // the wave's rows and columns in the tile
+  const int wm = 32 * MI * (wave / MT_WC), wn = MG_N / MT_WC * (wave % MT_WC);  // the wave's rows and columns in the tile
   const int wcol = 8 * (n >> 2) + (n & 3), key = mg_key(n);
-  auto ld_x = [&](int s, int h, int i) {
-    return *reinterpret_cast<const V*>(smem + (s & 1) * XB + (wm + 32 * i + n) * 128 + 16 * ((4 * u + h) ^ key));
+  auto ld_x = [&](int st, int h, int i) {
+    return *reinterpret_cast<const V*>(smem + st * XB + (wm + 32 * i + n) * 128 + 16 * ((4 * u + h) ^ key));
   };
   auto col = [&](int j) { return wn + 64 * (j >> 1) + 4 * (j & 1) + wcol; };
   auto ld_w = [&](int s, int j) {  // the lane's block of step s
@@ -90,38 +104,39 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(const MgArgs B) {
     return (uint32_t) * reinterpret_cast<const uint8_t*>(scl + (s >> 3 & 1) * SB + col(j) * 16 + 8 * u + (s & 7));
   };
 
-  f32x16 acc[MI][4];
-  V xa[2][MI], wa[2][4];     // operands of two sub-steps
-  u32x4 wc[4], wcn[4];       // codes of this step and the next
-  uint32_t sc[4], scn[4];    // their scale bytes
+  f32x16 acc[MI][NJ];
+  V xa[2][MI], wa[2][NJ];     // operands of two sub-steps
+  u32x4 wc[NJ], wcn[NJ];      // codes of this step and the next
+  uint32_t sc[NJ], scn[NJ];   // their scale bytes
 
   // Sub-step H of step s (operand set H & 1): its MFMAs; the next sub-step's x operands
-  // are read and its W operands made meanwhile, and in H = 3 load(l), l = 0 .. NX + 1,
-  // issues the global loads.
-  auto substep = [&](auto hc, int s, auto&& load) {
-    constexpr int H = decltype(hc)::value, A = H & 1, HN = (H + 1) & 3, L = H == 3 ? NX + 2 : 0;
-    constexpr int TILES = MI * 4;
+  // are read (from stage st) and its W operands made meanwhile, and in H = 3 load(l), l =
+  // 0 .. NX - 1, issues x's loads.
+  auto substep = [&](auto hc, int st, auto&& load) {
+    constexpr int H = decltype(hc)::value, A = H & 1, HN = (H + 1) & 3, L = H == 3 ? NX : 0;
+    constexpr int TILES = MI * NJ;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = 4 * i + j;
+      for (int j = 0; j < NJ; ++j) {
+        const int k = NJ * i + j;
         acc[i][j] = mt_mfma(wa[A][j], xa[A][i], acc[i][j]);
         // x's reads over the first half, W's conversions over all of it
 #pragma unroll
         for (int r = min(MI, k * 2 * MI / TILES); r < min(MI, (k + 1) * 2 * MI / TILES); ++r)
-          xa[A ^ 1][r] = ld_x(H == 3 ? s + 1 : s, HN, r);
+          xa[A ^ 1][r] = ld_x(st, HN, r);
         if (H == 3 && i == 0) wc[j] = wcn[j], sc[j] = scn[j];
 #pragma unroll
-        for (int r = k * 4 / TILES; r < (k + 1) * 4 / TILES; ++r) mx4_decode8(wc[r][HN], mx4_scale(sc[r]), wa[A ^ 1][r]);
+        for (int r = k * NJ / TILES; r < (k + 1) * NJ / TILES; ++r) mx4_decode8(wc[r][HN], mx4_scale(sc[r]), wa[A ^ 1][r]);
 #pragma unroll
         for (int l = k * L / TILES; l < (k + 1) * L / TILES; ++l) load(l);
         __builtin_amdgcn_sched_barrier(0);
       }
   };
-  // every wave's operand reads and loads so far have landed, for all to see
-  auto meet = [&]() {
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+  // every wave's operand reads, and all its loads but the newest NL, have landed, for all to see
+  auto meet = [&](auto nl) {
+    constexpr int NL = decltype(nl)::value;
+    __builtin_amdgcn_s_waitcnt(0x0070 | (NL & 15) | (NL >> 4) << 14);  // vmcnt(NL), lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -129,16 +144,14 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(const MgArgs B) {
 
   issue_s(0);
 #pragma unroll
-  for (int v = 0; v < 8; ++v) issue_w(0, v);
+  for (int v = 0; v < 2 * NW; ++v) issue_w(v / NW, v % NW);
 #pragma unroll
-  for (int v = 0; v < NX; ++v) issue_x(0, v);
+  for (int s = 0; s < NXS; ++s)
 #pragma unroll
-  for (int v = 0; v < NX; ++v) issue_x(1, v);
+    for (int v = 0; v < NX; ++v) issue_x(s, s, v);
+  meet(std::integral_constant<int, 0>{});
 #pragma unroll
-  for (int v = 0; v < 2; ++v) issue_w(1, v);  // (steps 0 to 2 issue the rest)
-  meet();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < NJ; ++j) {
     wc[j] = ld_w(0, j);
     sc[j] = ld_s(0, j);
     mx4_decode8(wc[j][0], mx4_scale(sc[j]), wa[0][j]);
@@ -150,35 +163,36 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(const MgArgs B) {
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NJ; ++j) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
       asm volatile("" : "+a"(acc[i][j]));
     }
+  int st = 0;  // the stage of x of step s
   for (int s = 0; s < nsteps; ++s) {
-    substep(std::integral_constant<int, 0>{}, s, none);
-    substep(std::integral_constant<int, 1>{}, s, none);
-    substep(std::integral_constant<int, 2>{}, s, none);
-    meet();  // x of step s read to its end, x of step s + 1 (and its codes and scales) there
+    substep(std::integral_constant<int, 0>{}, st, none);
+    substep(std::integral_constant<int, 1>{}, st, none);
+    substep(std::integral_constant<int, 2>{}, st, none);
+    // x of step s read to its end, x of step s + 1 (and its codes and scales) there: of
+    // the loads of NXS - 2 steps, x's at least, none is waited for
+    meet(std::integral_constant<int, (NXS - 2) * NX>{});
+    const int sn = st == NXS - 1 ? 0 : st + 1;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NJ; ++j) {
       wcn[j] = ld_w(s + 1, j);
       scn[j] = ld_s(s + 1, j);
     }
-    if ((s & 7) == 3) issue_s((s >> 3) + 1);
-    // W two stages ahead: a stage's last codes were read for its last step, in the third
-    // sub-step of the step before
-    const int f = (s + 1) / 4 + 1, v0 = 2 * ((s + 1) & 3);
-    substep(std::integral_constant<int, 3>{}, s, [&](int l) {
-      if (l < NX)
-        issue_x(s + 2, l);
-      else
-        issue_w(f, v0 + l - NX);
-    });
+    if ((s & 7) == 0) issue_s((s >> 3) + 1);
+    if ((s & 3) == 3) {  // a stage of W's last codes were read a step ago
+#pragma unroll
+      for (int v = 0; v < NW; ++v) issue_w(s / 4 + 2, v);
+    }
+    substep(std::integral_constant<int, 3>{}, sn, [&](int l) { issue_x(s + NXS, st, l); });
+    st = sn;
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the trailing loads have landed before the waves exit
 
-  mg_epilogue<MI, SPLIT, T>(B, P, smem, acc, m0, n0);
+  mg_epilogue<MI, MT_WC, SPLIT, T>(B, P, smem, acc, m0, n0);
 }
 
 // The pre-pass, a wave a column: its scales [superstep][column][16] in the order
@@ -214,7 +228,11 @@ __global__ __launch_bounds__(256) void mx4_tile_scales_kernel(const MtScales S) 
   }
 }
 
-static const MgCost MX4_TILE_COST = {{1.0, 4.0, 8.0}, {0.0, 0.0, 6.0}, {4.5, 7.0, 13.0}, {0.5, 1.0, 4.0}};
+// Fitted to 19 shapes from 17 x 2048 -> 2048 to 7000 x 2048 -> 2048, every tile height and
+// split timed, e.g. 1000 x 4096 -> 4096: 64 rows a tile 49.2 us, 128 rows 59.7, 256 rows
+// in four splits 64.0; 4000 rows: 178, 136, 119; 64 x 16384 -> 4096: 64 rows in 16 splits
+// 36.4, unsplit 154.
+static const MgCost MX4_TILE_COST = {{1.0, 4.0, 5.5}, {0.0, 0.0, 3.5}, {4.6, 6.3, 9.5}, {0.9, 0.5, 3.5}};
 static MgPlan mx4_tile_plan(int nprob, int64_t rows, int64_t O, int64_t I) {
   return mg_plan(MX4_TILE_COST, nprob, rows, O, (I + 511) / 512);
 }
@@ -229,13 +247,11 @@ int64_t mx4_tile_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I) 
 
 template <int MI, typename T>
 static int mt_go(const MgArgs& a, int nprob, void* stream) {
-  // (the epilogue's staging, 64 MI rows of 528 bytes, fits in it)
-  constexpr int lds = 2 * (64 * MI * 128 + MG_N * (128 + 16));
-  static_assert(lds >= 64 * MI * 528, "epilogue staging");
+  constexpr int lds = mt_lds(MI);
   static std::atomic<uint64_t> raised[2];
   auto launch = [&](auto kern, std::atomic<uint64_t>& done) {
     if (int rc = raise_dynamic_lds(reinterpret_cast<const void*>(kern), lds, done, "mx4_tile_kernel")) return rc;
-    hipLaunchKernelGGL(kern, mg_grid(a, nprob), dim3(256), lds, as_stream(stream), a);
+    hipLaunchKernelGGL(kern, mg_grid(a, nprob), dim3(64 * MT_WAVES), lds, as_stream(stream), a);
     if (int rc = check_launch("mx4_tile_kernel")) return rc;
     return mg_reduce<T>(a, nprob, stream);
   };

@@ -84,7 +84,8 @@ def test_quantize_strides_and_ranks():
 SHAPES = [(1, 32, 1), (1, 64, 17), (2, 96, 40), (16, 128, 16), (17, 160, 33), (1, 4096, 48), (5, 1056, 65),
           (33, 1024, 100), (40, 512, 300), (64, 2048, 96), (65, 288, 130), (129, 640, 257), (200, 2560, 512),
           (257, 1024, 520), (300, 96, 70), (520, 768, 264),
-          (2, 8704, 30), (9, 16384, 40), (16, 8224, 24)]
+          (2, 8704, 30), (9, 16384, 40), (16, 8224, 24),
+          (4, 8192, 40), (2, 7680, 24), (700, 608, 1100)]
 
 
 def _case(rows, n, m, dt, seed, *, lo=112, hi=122):
@@ -114,6 +115,25 @@ def test_linear_against_64_bits(rows, n, m, dtype, quantize_input):
                               quantize_input=quantize_input).cpu().double()
         worst = ((got - want).abs() - bound).max().item()
         assert worst <= 0, (epilogue, worst)
+
+
+@pytest.mark.parametrize("dtype,epilogue", [("fp16", "relu2"), ("bf16", "residual")])
+def test_linear_of_a_prefill_batch(dtype, epilogue):
+    """1024 tiles of 256 x 256 and more, ragged on both sides and in K: the weight in 16 bits."""
+    import rwkv7mi as mi
+
+    rows, n, m, dt = 4001, 96, 16325, DTYPES[dtype]
+    x, codes, scales, g = _case(rows, n, m, dt, 3)
+    scales[7, 1] = 60
+    x, codes, scales = x.cuda(), codes.cuda(), scales.cuda()
+    bias = torch.randn(m, generator=g).to(dt).cuda()
+    residual = torch.randn(rows, m, generator=g).to(dt).cuda() if epilogue == "residual" else None
+    got = mi.mxfp4_linear(x, codes, scales, bias=bias, residual=residual, epilogue=epilogue)
+    w = ref.values(codes, scales)
+    for r in (0, 255, 1300, 3990):  # a few rows of several tiles, all columns
+        rs = slice(r, min(r + 40, rows))
+        want, bound = ref.product(x[rs], w, bias, None if residual is None else residual[rs], epilogue)
+        assert ((got[rs].cpu().double() - want).abs() <= bound).all()
 
 
 @pytest.mark.parametrize("rows", [1, 24, 90, 400])
