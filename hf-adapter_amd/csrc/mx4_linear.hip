@@ -334,3 +334,10 @@ extern "C" int rwkv7mi_mxfp4_linear(int nprob, const void* const* x, const uint8
   if (int rc = mx4_quantize_run(nprob, x, rows, I, I, act_dtype, xc, xs, stream)) return rc;
   return bf ? mx4_rows_run<__hip_bfloat16, true>(b, nprob, at, stream) : mx4_rows_run<__half, true>(b, nprob, at, stream);
 }
+
+extern "C" int rwkv7mi_mxfp4_linear1(const void* x, const uint8_t* codes, const uint8_t* scales, const void* bias,
+                                     const void* residual, void* y, int epilogue, int64_t rows, int64_t O, int64_t I,
+                                     int act_dtype, int quantize_input, void* ws, int64_t ws_bytes, void* stream) {
+  return rwkv7mi_mxfp4_linear(1, &x, &codes, &scales, &bias, &residual, &y, &epilogue, rows, O, I, act_dtype,
+                              quantize_input, ws, ws_bytes, stream);
+}

@@ -137,9 +137,10 @@ SIGNATURES = {
     "rwkv7mi_mxfp4_linear_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64, _i32, _i32]),
     "rwkv7mi_mxfp4_linear": (_i32, [_i32] + [_c_p] * 7 + [_i64, _i64, _i64, _i32, _i32, _c_p, _i64, _c_p]),
     "rwkv7mi_process_logits_workspace_bytes": (_sz, [_i64, _i64]),
+    "rwkv7mi_mxfp4_linear1": (_i32, [_c_p] * 6 + [_i32, _i64, _i64, _i64, _i32, _i32, _c_p, _i64, _c_p]),
     "rwkv7mi_process_logits": (
-        _i32, [_c_p, _i64, _i64, _i64, _i32, _c_p, _i64, _i32, _c_p, _i32, _i64, _i64, _c_p, _c_p, _c_p, _i32, _c_p, _i64,
-               _c_p, _i64, _c_p, _c_p, _i32, _c_p, _sz, _c_p]),
+        _i32, [_c_p, _i64, _i64, _i64, _i32, _c_p, _i64, _i32, _c_p, _i32, _i64, _i64, _c_p] + [_c_p, _f32] * 4
+        + [_c_p, _i64, _c_p, _i64, _c_p, _c_p, _i32, _c_p, _sz, _c_p]),
     "rwkv7mi_attn_norm_mix6": (
         _i32, [_c_p] * 8 + [_i64, _i64, _i64, _f32, _i32, _i32, _c_p],
     ),
@@ -223,18 +224,25 @@ def stream_of(t: torch.Tensor):
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(t: torch.Tensor):
     """A context in which ``t``'s device is the current one (kernels launch on the
     current device; no work where it already is)."""
-    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def require_same_device(*tensors: torch.Tensor | None, name: str) -> None:
     """Every given tensor is on the first one's GPU."""
-    require_gpu(*tensors, name=name)
-    devices = {t.get_device() for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"{name}: tensors on different devices {sorted(devices)}")
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != dev or dev < 0):
+            require_gpu(*tensors, name=name)
+            raise ValueError(f"{name}: tensors on different devices "
+                             f"{sorted({t.get_device() for t in tensors if t is not None})}")
+    if _lib is None:
+        load()
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:

@@ -42,16 +42,21 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise ValueError("quantize_mxfp4: the last dimension must be a multiple of 32")
     code = _lib.dtype_code(x)
     _lib.require_gpu(x, name="quantize_mxfp4")
-    lead, width = x.shape[:-1], int(x.shape[-1])
-    x2 = x.detach().reshape(-1, width)
-    rows, step = int(x2.shape[0]), 16 // x2.element_size()
-    if x2.stride(1) != 1 or (rows > 1 and (x2.stride(0) < width or x2.stride(0) % step)) or x2.data_ptr() % 16:
-        x2 = _aligned(x2, 16)
-    codes = torch.empty((*lead, width // 2), device=x.device, dtype=torch.uint8)
-    scales = torch.empty((*lead, width // BLOCK), device=x.device, dtype=torch.uint8)
-    with _lib.on_device(x2):
-        _lib.call("rwkv7mi_mxfp4_quantize", _lib.ptr(x2), rows, width, int(x2.stride(0)) if rows > 1 else width, code,
-                  _lib.ptr(codes), _lib.ptr(scales), _lib.stream_of(x2))
+    lead, width = x.shape[:-1], x.shape[-1]
+    rows = x.numel() // width
+    ld = width
+    if not x.is_contiguous():
+        x = x.reshape(rows, width)
+        ld = x.stride(0)
+        if x.stride(1) != 1 or ld < width or ld % (16 // x.element_size()):
+            x, ld = x.contiguous(), width
+    if x.data_ptr() % 16:
+        x, ld = x.contiguous().clone(), width
+    codes = x.new_empty((*lead, width // 2), dtype=torch.uint8)
+    scales = x.new_empty((*lead, width // BLOCK), dtype=torch.uint8)
+    with _lib.on_device(x):
+        _lib.call("rwkv7mi_mxfp4_quantize", x.data_ptr(), rows, width, ld, code, codes.data_ptr(), scales.data_ptr(),
+                  _lib.stream_of(x))
     return codes, scales
 
 
@@ -62,19 +67,19 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor,
     _check_packed(codes, scales, "dequantize_mxfp4")
     _lib.require_same_device(codes, scales, name="dequantize_mxfp4")
     codes, scales = _aligned(codes, 4), scales.contiguous()
-    width = 2 * int(codes.shape[-1])
-    out = torch.empty((*codes.shape[:-1], width), device=codes.device, dtype=out_dtype)
+    width = 2 * codes.shape[-1]
+    out = codes.new_empty((*codes.shape[:-1], width), dtype=out_dtype)
     with _lib.on_device(codes):
-        _lib.call("rwkv7mi_mxfp4_dequantize", _lib.ptr(codes), _lib.ptr(scales), out.numel() // width, width,
-                  _lib.ptr(out), _lib.dtype_code(out), _lib.stream_of(codes))
+        _lib.call("rwkv7mi_mxfp4_dequantize", codes.data_ptr(), scales.data_ptr(), out.numel() // width, width,
+                  out.data_ptr(), _lib.dtype_code(out), _lib.stream_of(codes))
     return out
 
 
 def _check_packed(codes, scales, who):
     if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise ValueError(f"{who}: codes and scales are uint8")
-    if (codes.dim() < 1 or codes.dim() != scales.dim() or codes.shape[:-1] != scales.shape[:-1]
-            or int(scales.shape[-1]) == 0 or int(codes.shape[-1]) != 16 * int(scales.shape[-1])):
+    cs, ss = codes.shape, scales.shape
+    if not cs or len(cs) != len(ss) or cs[:-1] != ss[:-1] or ss[-1] == 0 or cs[-1] != 16 * ss[-1]:
         raise ValueError(f"{who}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not match "
                          "([..., I/2] and [..., I/32])")
 
@@ -149,34 +154,56 @@ def mxfp4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, 
     as :func:`quantize_mxfp4` does, and both operands run as codes.  ``out`` (contiguous,
     ``x``'s dtype) may be the residual itself, not overlap ``x``.
     """
-    if epilogue not in EPILOGUES:
+    epi = EPILOGUES.get(epilogue)
+    if epi is None:
         raise ValueError(f"mxfp4: unknown epilogue {epilogue!r}; expected one of {', '.join(EPILOGUES)}")
-    if (epilogue == "residual") != (residual is not None):
+    if (epi == _lib.EPI_RESIDUAL) != (residual is not None):
         raise ValueError("mxfp4: the residual goes with epilogue='residual'")
-    if x.dim() < 1:
+    shape, cshape = x.shape, codes.shape
+    if not shape:
         raise ValueError("mxfp4: x must be [..., I]")
     _check_packed(codes, scales, "mxfp4")
     _lib.require_same_device(x, codes, scales, bias, out, residual, name="mxfp4_linear")
-    if codes.dim() != 2 or 2 * int(codes.shape[1]) != int(x.shape[-1]):
-        raise ValueError(f"mxfp4: x has {x.shape[-1]} features but codes are {tuple(codes.shape)}")
-    m = int(codes.shape[0])
-    lead = x.shape[:-1]
-    x2 = _aligned(x.reshape(-1, int(x.shape[-1])), 16)
-    if out is None:
-        out2 = torch.empty((int(x2.shape[0]), m), device=x.device, dtype=x.dtype)
-    else:
-        if tuple(out.shape) != (*lead, m) or not out.is_contiguous():
-            raise ValueError("mxfp4: out must be a contiguous [..., O] tensor")
-        out2 = out.view(-1, m)
-    if residual is not None:
-        if tuple(residual.shape) != (*lead, m):
-            raise ValueError("mxfp4: residual must have out's shape")
-        residual = residual.reshape(-1, m).contiguous()
+    n = shape[-1]
+    if len(cshape) != 2 or 2 * cshape[1] != n:
+        raise ValueError(f"mxfp4: x has {n} features but codes are {tuple(cshape)}")
+    dt = x.dtype
+    if dt is not torch.float16 and dt is not torch.bfloat16:
+        raise ValueError(f"mxfp4: fp16 or bf16 activations, got {dt}")
+    m, rows, want = cshape[0], x.numel() // n, (*shape[:-1], cshape[0])
+    if not x.is_contiguous() or x.data_ptr() % 16:
+        x = _aligned(x, 16)
+    if not codes.is_contiguous() or codes.data_ptr() % 16:
+        codes = _aligned(codes, 16)
+    if not scales.is_contiguous() or scales.data_ptr() % 4:
+        scales = _aligned(scales, 4)
     if bias is not None:
-        bias = bias.reshape(-1).to(x.dtype).contiguous()
-    mxfp4_linear_multi_into([x2], [(_aligned(codes, 16), _aligned(scales, 4))], [out2], biases=[bias],
-                            residuals=[residual], epilogues=[EPILOGUES[epilogue]], quantize_input=quantize_input)
-    return out if out is not None else out2.view(*lead, m)
+        if bias.numel() != m:
+            raise ValueError(f"mxfp4: bias must hold {m} entries")
+        bias = bias.to(dt).contiguous()
+    if residual is not None:
+        if tuple(residual.shape) != want or residual.dtype is not dt:
+            raise ValueError("mxfp4: residual must have out's shape and dtype")
+        residual = residual.contiguous()
+    if out is None:
+        out = x.new_empty(want)
+    else:
+        if tuple(out.shape) != want or not out.is_contiguous() or out.dtype is not dt:
+            raise ValueError("mxfp4: out must be a contiguous [..., O] tensor of x's dtype")
+        if _lib.overlap(out, x):
+            raise ValueError("mxfp4: out overlaps an input")
+        if residual is not None and residual.data_ptr() != out.data_ptr() and _lib.overlap(out, residual):
+            raise ValueError("mxfp4: out overlaps the residual without being it")
+    if rows == 0 or m == 0:
+        return out
+    quant, code = int(bool(quantize_input)), _lib.dtype_code(x)
+    need = _scratch(1, rows, m, n, code, quant, x.get_device())
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    with _lib.on_device(x):
+        _lib.call("rwkv7mi_mxfp4_linear1", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), _lib.ptr(bias),
+                  _lib.ptr(residual), out.data_ptr(), epi, rows, m, n, code, quant, _lib.ptr(ws), need,
+                  _lib.stream_of(x))
+    return out
 
 
 class MXFP4Linear(torch.nn.Module):

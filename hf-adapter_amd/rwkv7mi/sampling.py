@@ -6,7 +6,7 @@ can end with its next tokens; and the logits step before it
 mask, with the greedy token of what they leave."""
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
 
 import torch
@@ -52,16 +52,23 @@ def argmax_rows(logits: torch.Tensor, *, out: torch.Tensor | None = None,
     return out
 
 
+@functools.lru_cache(maxsize=4096)
+def _process_workspace(rows: int, n: int) -> int:
+    return int(_lib.load().rwkv7mi_process_logits_workspace_bytes(rows, n))
+
+
 def process_logits_workspace_bytes(rows: int, n: int) -> int:
     """Workspace bytes of :func:`process_logits` with ``next_tokens``."""
-    return int(_lib.load().rwkv7mi_process_logits_workspace_bytes(int(rows), int(n)))
+    return _process_workspace(int(rows), int(n))
 
 
-def _row_values(value, rows: int, device, name: str, lo: float, hi: float, *, open_lo: bool = False):
+def _row_values(value, rows: int, name: str, lo: float, hi: float, *, open_lo: bool = False):
     """A penalty as ``(device tensor [rows] or None, float)``; numbers are checked
     against ``lo``..``hi`` (``open_lo``: above ``lo``)."""
     if isinstance(value, torch.Tensor):
-        if int(value.numel()) not in (1, rows) or value.dim() > 1 or not value.is_floating_point():
+        if value.dtype is torch.float32 and value.shape == (rows,) and value.is_contiguous():
+            return value, 0.0
+        if value.numel() not in (1, rows) or value.dim() > 1 or not value.is_floating_point():
             raise ValueError(f"process_logits: {name} must be a number or a floating-point tensor of one value per row")
         return value.to(torch.float32).expand(rows).contiguous(), 0.0
     value = float(value)
@@ -111,33 +118,39 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     (:func:`process_logits_workspace_bytes`) is allocated when not given and needed.
     """
     name = "process_logits"
-    if logits.dim() != 2 or int(logits.shape[1]) == 0:
+    if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"{name}: logits must be [rows, n]")
-    _lib.require_same_device(logits, history, lengths, bias, allowed, out, next_tokens, next_tokens2, workspace, name=name)
-    rows, n = (int(s) for s in logits.shape)
+    rows, n = logits.shape
     dt = _lib.dtype_code(logits)
-    if logits.stride(1) != 1 and n > 1:
+    big = math.inf
+    rep, rep_v = _row_values(repetition_penalty, rows, "repetition_penalty", 0.0, big, open_lo=True)
+    pres, pres_v = _row_values(presence_penalty, rows, "presence_penalty", -big, big)
+    freq, freq_v = _row_values(frequency_penalty, rows, "frequency_penalty", -big, big)
+    dec, dec_v = _row_values(penalty_decay, rows, "penalty_decay", 0.0, 1.0)
+    _lib.require_same_device(logits, history, lengths, rep, pres, freq, dec, bias, allowed, out, next_tokens, next_tokens2,
+                             workspace, name=name)
+    if n > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
     if out is None:
-        out = torch.empty((rows, n), device=logits.device, dtype=logits.dtype)
+        out = logits.new_empty((rows, n))
     elif (tuple(out.shape) != (rows, n) or out.dtype not in (logits.dtype, torch.float32)
-          or (out.stride(1) != 1 and n > 1) or (rows > 1 and out.stride(0) < n)):
+          or (n > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < n)):
         raise ValueError(f"{name}: out must be [rows, n] with dense rows, of logits' dtype or fp32")
     elif _lib.overlap(out, logits) and not (out.data_ptr() == logits.data_ptr() and out.dtype == logits.dtype
                                             and (rows == 1 or out.stride(0) == logits.stride(0))):
         raise ValueError(f"{name}: out overlaps logits without being them")
     bits, ldh, cap = 64, 0, 0
     if history is not None:
-        if (history.dim() != 2 or int(history.shape[0]) != rows or history.dtype not in (torch.int32, torch.int64)):
+        if history.dim() != 2 or history.shape[0] != rows or history.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{name}: history must be an int32 or int64 [rows, L] tensor")
-        cap, bits = int(history.shape[1]), 8 * history.element_size()
-        if history.stride(1) != 1 and cap > 1:
+        cap, bits = history.shape[1], 8 * history.element_size()
+        if cap > 1 and history.stride(1) != 1:
             if append:
                 raise ValueError(f"{name}: appending needs a history of dense rows")
             history = history.contiguous()
-        ldh = int(history.stride(0))
+        ldh = history.stride(0)
     if lengths is not None:
-        if history is None or int(lengths.numel()) != rows or lengths.dim() != 1 or lengths.dtype != torch.int32:
+        if history is None or lengths.shape != (rows,) or lengths.dtype is not torch.int32:
             raise ValueError(f"{name}: lengths must be int32 [rows], with a history")
         if not lengths.is_contiguous():
             if append:
@@ -145,37 +158,33 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
             lengths = lengths.contiguous()
     if append and (history is None or lengths is None or next_tokens is None):
         raise ValueError(f"{name}: append needs history, lengths and next_tokens")
-    big = math.inf
-    values = [_row_values(repetition_penalty, rows, logits.device, "repetition_penalty", 0.0, big, open_lo=True),
-              _row_values(presence_penalty, rows, logits.device, "presence_penalty", -big, big),
-              _row_values(frequency_penalty, rows, logits.device, "frequency_penalty", -big, big),
-              _row_values(penalty_decay, rows, logits.device, "penalty_decay", 0.0, 1.0)]
     ldb = lda = 0
     if bias is not None:
         bias, ldb = _shared_rows(bias.to(torch.float32), rows, n, "bias")
     if allowed is not None:
-        if allowed.dtype != torch.int32:
+        if allowed.dtype is not torch.int32:
             raise ValueError(f"{name}: allowed must hold int32 words")
         allowed, lda = _shared_rows(allowed, rows, (n + 31) // 32, "allowed")
-    for t in (next_tokens, next_tokens2):
-        if t is not None and (t.dtype != torch.int64 or int(t.numel()) != rows or not t.is_contiguous()):
-            raise ValueError(f"{name}: next_tokens must be a contiguous int64 tensor of one entry per row")
-    if next_tokens2 is not None and next_tokens is None:
+    need = 0
+    if next_tokens is not None:
+        for t in (next_tokens, next_tokens2):
+            if t is not None and (t.dtype is not torch.int64 or t.numel() != rows or not t.is_contiguous()):
+                raise ValueError(f"{name}: next_tokens must be a contiguous int64 tensor of one entry per row")
+        need = _process_workspace(rows, n)
+    elif next_tokens2 is not None:
         raise ValueError(f"{name}: next_tokens2 is a second copy of next_tokens")
-    need = process_logits_workspace_bytes(rows, n) if next_tokens is not None else 0
     if workspace is None:
-        workspace = torch.empty(need, device=logits.device, dtype=torch.uint8) if need else None
+        workspace = logits.new_empty(need, dtype=torch.uint8) if need else None
     elif (not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need
           or workspace.data_ptr() % 8):
         raise ValueError(f"{name}: workspace must be contiguous, 8-byte aligned, "
                          "of at least process_logits_workspace_bytes bytes")
-    decayed = int(values[3][0] is not None or values[3][1] != 1.0)
+    ptr = _lib.ptr
     with _lib.on_device(logits):
-        _lib.call("rwkv7mi_process_logits", _lib.ptr(logits), rows, n, int(logits.stride(0)), dt, _lib.ptr(out),
-                  int(out.stride(0)), _lib.dtype_code(out), _lib.ptr(history), bits, ldh, cap, _lib.ptr(lengths),
-                  _lib.ptr_array([t for t, _ in values]), (ctypes.c_float * 4)(*[v for _, v in values]), decayed,
-                  _lib.ptr(bias), ldb, _lib.ptr(allowed), lda, _lib.ptr(next_tokens), _lib.ptr(next_tokens2),
-                  int(bool(append)), _lib.ptr(workspace), need, _lib.stream_of(logits))
+        _lib.call("rwkv7mi_process_logits", logits.data_ptr(), rows, n, logits.stride(0), dt, out.data_ptr(),
+                  out.stride(0), _lib.dtype_code(out), ptr(history), bits, ldh, cap, ptr(lengths), ptr(rep), rep_v,
+                  ptr(pres), pres_v, ptr(freq), freq_v, ptr(dec), dec_v, ptr(bias), ldb, ptr(allowed), lda,
+                  ptr(next_tokens), ptr(next_tokens2), 1 if append else 0, ptr(workspace), need, _lib.stream_of(logits))
     return out
 
 

@@ -686,9 +686,8 @@ int rwkv7mi_argmax_rows_ws(const void* x, int64_t rows, int64_t n, int64_t ld,
  *   l += bias[t];  bit t of the row's words in allowed clear: l = -inf
  * in fp32, rounded once.  history [rows, L] of 32- or 64-bit tokens (NULL: none;
  * at most 2^23 a row, those outside 0..V-1 ignored), the first lengths[row] of a
- * row (NULL: L).  penalties / penalty: the four of repetition, presence,
- * frequency, decay (decay in 0..1, `decayed` nonzero unless every decay is 1),
- * each a device array [rows], or NULL for the one value.  bias, allowed: row
+ * row (NULL: L).  Each penalty (decay in 0..1) is a device array [rows], or with
+ * NULL the one value for every row.  bias, allowed: row
  * strides ldb, lda (0: one row for all; allowed in 32-bit words).
  * next (NULL: none), next2: the first index of each rounded row's maximum (NaN
  * counts as the maximum; 0 where nothing is allowed), which needs the workspace.
@@ -699,8 +698,11 @@ int rwkv7mi_process_logits(const void* x, int64_t rows, int64_t V, int64_t ldx,
                            int dtype, void* out, int64_t ldo, int out_dtype,
                            void* history, int history_bits, int64_t ldh,
                            int64_t L, int* lengths,
-                           const float* const* penalties, const float* penalty,
-                           int decayed, const float* bias, int64_t ldb,
+                           const float* repetition_rows, float repetition,
+                           const float* presence_rows, float presence,
+                           const float* frequency_rows, float frequency,
+                           const float* decay_rows, float decay,
+                           const float* bias, int64_t ldb,
                            const uint32_t* allowed, int64_t lda, int64_t* next,
                            int64_t* next2, int append, void* workspace,
                            size_t workspace_bytes, void* stream);
@@ -821,6 +823,13 @@ int rwkv7mi_mxfp4_linear(int nprob, const void* const* x,
                          int64_t O, int64_t I, int act_dtype,
                          int quantize_input, void* ws, int64_t ws_bytes,
                          void* stream);
+/* The same for one product. */
+int rwkv7mi_mxfp4_linear1(const void* x, const uint8_t* codes,
+                          const uint8_t* scales, const void* bias,
+                          const void* residual, void* y, int epilogue,
+                          int64_t rows, int64_t O, int64_t I, int act_dtype,
+                          int quantize_input, void* ws, int64_t ws_bytes,
+                          void* stream);
 
 /* ------------------------------------------------ LayerNorm + token shift */
 

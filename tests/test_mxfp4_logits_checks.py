@@ -62,16 +62,15 @@ def test_empty_calls_launch_nothing():
 
 
 def _logits(x=A, rows=2, n=100, ldx=100, dt=1, out=A, ldo=100, odt=1, hist=None, bits=64, ldh=8, cap=8, lengths=None,
-            pen=True, bias=None, ldb=0, allowed=None, lda=0, nxt=None, nxt2=None, append=0, ws=None, nws=0):
-    arr = _arr(0, 0, 0, 0) if pen else None
-    val = (ctypes.c_float * 4)(2.0, 0.0, 0.0, 1.0) if pen else None
-    return _lib().rwkv7mi_process_logits(x, rows, n, ldx, dt, out, ldo, odt, hist, bits, ldh, cap, lengths, arr, val, 0,
-                                         bias, ldb, allowed, lda, nxt, nxt2, append, ws, nws, None)
+            bias=None, ldb=0, allowed=None, lda=0, nxt=None, nxt2=None, append=0, ws=None, nws=0):
+    return _lib().rwkv7mi_process_logits(x, rows, n, ldx, dt, out, ldo, odt, hist, bits, ldh, cap, lengths, None, 2.0,
+                                         None, 0.0, None, 0.0, None, 1.0, bias, ldb, allowed, lda, nxt, nxt2, append, ws,
+                                         nws, None)
 
 
 @pytest.mark.parametrize("kw", [dict(rows=-1), dict(n=0), dict(ldx=-1), dict(ldo=50), dict(dt=5), dict(odt=2), dict(x=0),
                                 dict(out=0), dict(bits=16), dict(hist=A, cap=-1), dict(hist=A, cap=(1 << 23) + 1),
-                                dict(hist=A, pen=False), dict(ldb=-1), dict(lda=-4), dict(nxt2=A), dict(rows=1 << 16),
+                                dict(ldb=-1), dict(lda=-4), dict(nxt2=A), dict(rows=1 << 16),
                                 dict(append=1), dict(append=1, hist=A, nxt=A), dict(append=1, hist=A, lengths=A),
                                 dict(append=1, hist=A, lengths=A, nxt=A, ldh=0)])
 def test_logits_entry_refuses(kw):
