@@ -41,7 +41,7 @@ from .native_wkv_fp16 import (
     native_fp16_recurrent_should_use,
     native_fp16_sequence,
 )
-from .sampling import argmax_rows, process_logits
+from .sampling import NativeLogitsProcessor, argmax_rows, process_logits
 from . import ops as _ops
 
 _ops.register()  # torch.ops.rwkv7mi.*
@@ -75,6 +75,7 @@ __all__ = [
     "MXFP4Linear",
     "quantize_model_mxfp4",
     "argmax_rows",
+    "NativeLogitsProcessor",
     "process_logits",
     "native_fp16_recurrent_should_use",
     "native_fp16_recurrent_available",

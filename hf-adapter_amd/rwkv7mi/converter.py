@@ -16,8 +16,8 @@ from a directory the reference converter wrote: the same keys, its
 
 Prepacked checkpoint (the per-module loader metadata of
 docs/quantization/VLLM_QUANTIZATION_PORTING.md:411-430): the MM8 modules'
-bytes in the GEMV's blocked layout with their scales, ``prepacked.safetensors``,
-and ``manifest.json`` with one entry per module (format, features, dtypes,
+bytes in the GEMV's blocked layout with their scales, or the MXFP4 modules' codes
+and block scales, ``prepacked.safetensors``, and ``manifest.json`` with one entry per module (format, features, dtypes,
 epilogue, sha256 of the source weight, packer version) validated before any
 GPU buffer is allocated, so loading skips quantisation.
 
@@ -46,6 +46,10 @@ DTYPES = {
 
 PREPACKED_FORMAT = "rwkv7mi.mm8_blocked.v1"
 PACKER_VERSION = "rwkv7mi-mm8-1"
+MXFP4_FORMAT = "rwkv7mi.mxfp4.v1"
+MXFP4_PACKER_VERSION = "rwkv7mi-mxfp4-1"
+_PACKERS = {PREPACKED_FORMAT: PACKER_VERSION, MXFP4_FORMAT: MXFP4_PACKER_VERSION}
+_FIELDS = {PREPACKED_FORMAT: ("w_blk", "mx", "rx", "my", "ry"), MXFP4_FORMAT: ("codes", "scales")}
 # the reference converter's fills for layer 0's optional pre-norm
 _ALLOWED_MISSING = ("model.layers.0.pre_norm.weight", "model.layers.0.pre_norm.bias")
 
@@ -261,14 +265,16 @@ def load_hf_directory(path) -> tuple:
 
 
 def load_pretrained(path, *, device="cuda", dtype=torch.float16, use_native_mm8: bool | None = None,
-                    native_mm8_policy: str | None = None, native_mm8_min_params: int | None = None):
+                    native_mm8_policy: str | None = None, native_mm8_min_params: int | None = None,
+                    use_native_mxfp4: bool | None = None, native_mxfp4_policy: str | None = None,
+                    native_mxfp4_min_params: int | None = None, native_mxfp4_quantize_input: bool | None = None):
     """A :class:`NativeRWKV7ForCausalLM` from a converted directory; with a
-    ``manifest.json`` next to it the MM8 modules come prepacked."""
+    ``manifest.json`` next to it the MM8 or MXFP4 modules come prepacked."""
     from .model import NativeRWKV7ForCausalLM
 
     p = Path(path)
     if (p / "manifest.json").exists():
-        return load_prepacked(p, device=device, dtype=dtype)
+        return load_prepacked(p, device=device, dtype=dtype, native_mxfp4_quantize_input=native_mxfp4_quantize_input)
     cfg, state = load_hf_directory(p)
     if use_native_mm8 is not None:
         cfg.use_native_mm8 = bool(use_native_mm8)
@@ -276,6 +282,14 @@ def load_pretrained(path, *, device="cuda", dtype=torch.float16, use_native_mm8:
         cfg.native_mm8_policy = native_mm8_policy
     if native_mm8_min_params is not None:
         cfg.native_mm8_min_params = int(native_mm8_min_params)
+    if use_native_mxfp4 is not None:
+        cfg.use_native_mxfp4 = bool(use_native_mxfp4)
+    if native_mxfp4_policy is not None:
+        cfg.native_mxfp4_policy = native_mxfp4_policy
+    if native_mxfp4_min_params is not None:
+        cfg.native_mxfp4_min_params = int(native_mxfp4_min_params)
+    if native_mxfp4_quantize_input is not None:
+        cfg.native_mxfp4_quantize_input = bool(native_mxfp4_quantize_input)
     return NativeRWKV7ForCausalLM(cfg, state, device=device, dtype=dtype)
 
 
@@ -289,32 +303,39 @@ _EPILOGUE = {"ffn.key": "relu2", "ffn.value": "residual", "attn.o_proj": "residu
 
 def save_prepacked(model, output, *, source_state: Dict[str, torch.Tensor] | None = None) -> dict:
     """Write ``prepacked.safetensors`` (the model's MM8 modules in the blocked
-    layout: ``<module>.w_blk``, ``.mx``, ``.rx``, ``.my``, ``.ry``), the
+    layout: ``<module>.w_blk``, ``.mx``, ``.rx``, ``.my``, ``.ry``; or its MXFP4
+    modules: ``<module>.codes``, ``.scales``; a model with both is refused), the
     remaining (dense) parameters in ``model.safetensors``, ``config.json`` and
     ``manifest.json``.  ``source_state`` (the unquantised HF state dict)
     supplies each module's ``source_weight_sha256``."""
     from safetensors.torch import save_file
 
-    from .model import QuantLinear
+    from .model import BlockFloatLinear, QuantLinear
 
+    mx = [lin for _, lin in model.named_linears() if isinstance(lin, BlockFloatLinear)]
+    if mx and any(isinstance(lin, QuantLinear) for _, lin in model.named_linears()):
+        raise ValueError("a model with both MM8 and MXFP4 modules cannot be prepacked")
+    if any(lin.m.bias is not None for lin in mx):
+        raise ValueError("MXFP4 modules with a bias cannot be prepacked")
     out = Path(output)
     out.mkdir(parents=True, exist_ok=True)
     cfg = model.config
     packed: Dict[str, torch.Tensor] = {}
-    manifest = {"format": PREPACKED_FORMAT, "packer_version": PACKER_VERSION, "modules": []}
+    fmt = MXFP4_FORMAT if mx else PREPACKED_FORMAT
+    manifest = {"format": fmt, "packer_version": _PACKERS[fmt], "modules": []}
     dense = dict(model.dense_state_dict())
     for name, lin in model.named_linears():
-        if not isinstance(lin, QuantLinear):
+        if not isinstance(lin, BlockFloatLinear if mx else QuantLinear):
             continue
         m = lin.m
-        for field in ("w_blk", "mx", "rx", "my", "ry"):
+        for field in _FIELDS[fmt]:
             packed[f"{name}.{field}"] = getattr(m, field).detach().cpu().contiguous()
         entry = {
-            "format": PREPACKED_FORMAT, "module": name, "input_features": int(m.in_features),
+            "format": fmt, "module": name, "input_features": int(m.in_features),
             "output_features": int(m.out_features), "activation_dtype": str(model.dtype).replace("torch.", ""),
-            "scale_dtype": str(m.mx.dtype).replace("torch.", ""),
+            "scale_dtype": "uint8" if mx else str(m.mx.dtype).replace("torch.", ""),
             "epilogue": next((v for k, v in _EPILOGUE.items() if name.endswith(k)), "none"),
-            "blocked_shape": list(m.w_blk.shape), "packer_version": PACKER_VERSION,
+            "blocked_shape": list((m.codes if mx else m.w_blk).shape), "packer_version": _PACKERS[fmt],
         }
         if source_state is not None and name + ".weight" in source_state:
             entry["source_weight_sha256"] = _sha256(source_state[name + ".weight"])
@@ -324,8 +345,13 @@ def save_prepacked(model, output, *, source_state: Dict[str, torch.Tensor] | Non
     save_file({k: v.detach().cpu().contiguous() for k, v in dense.items()}, str(out / "model.safetensors"),
               metadata={"format": "pt"})
     cj = _config_json(cfg, str(model.dtype).replace("torch.", ""))
-    cj.update({"use_native_mm8": True, "native_mm8_policy": cfg.native_mm8_policy,
-               "native_mm8_min_params": cfg.native_mm8_min_params})
+    if mx:
+        cj.update({"use_native_mxfp4": True, "native_mxfp4_policy": cfg.native_mxfp4_policy,
+                   "native_mxfp4_min_params": cfg.native_mxfp4_min_params,
+                   "native_mxfp4_quantize_input": mx[0].m.quantize_input})
+    else:
+        cj.update({"use_native_mm8": True, "native_mm8_policy": cfg.native_mm8_policy,
+                   "native_mm8_min_params": cfg.native_mm8_min_params})
     (out / "config.json").write_text(json.dumps(cj, indent=2) + "\n")
     (out / "manifest.json").write_text(json.dumps(manifest, indent=2) + "\n")
     return manifest
@@ -335,41 +361,51 @@ def validate_manifest(manifest: dict, cfg, dtype: torch.dtype) -> None:
     """Check every entry against the config before any GPU buffer exists."""
     from .native_quant_mm8 import mm8_block_shape
 
-    if manifest.get("format") != PREPACKED_FORMAT:
-        raise ValueError(f"unsupported prepacked format {manifest.get('format')!r} (expected {PREPACKED_FORMAT})")
-    if manifest.get("packer_version") != PACKER_VERSION:
-        raise ValueError(f"prepacked by {manifest.get('packer_version')!r}; this build reads {PACKER_VERSION!r}")
+    fmt = manifest.get("format")
+    if fmt not in _PACKERS:
+        raise ValueError(f"unsupported prepacked format {fmt!r} (expected {PREPACKED_FORMAT} or {MXFP4_FORMAT})")
+    packer = _PACKERS[fmt]
+    if manifest.get("packer_version") != packer:
+        raise ValueError(f"prepacked by {manifest.get('packer_version')!r}; this build reads {packer!r}")
+    if fmt == MXFP4_FORMAT and dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"MXFP4 modules need an fp16 or bf16 model, got {dtype}")
     from .model import parameter_shapes
 
     shapes = parameter_shapes(cfg)
     seen = set()
     for e in manifest.get("modules", []):
         name = e.get("module", "")
-        if e.get("format") != PREPACKED_FORMAT:
+        if e.get("format") != fmt:
             raise ValueError(f"{name}: format {e.get('format')!r}")
         if name + ".weight" not in shapes:
             raise ValueError(f"{name}: not a linear of this config")
         o, i = shapes[name + ".weight"]
         if (e.get("input_features"), e.get("output_features")) != (i, o):
             raise ValueError(f"{name}: features {(e.get('input_features'), e.get('output_features'))} vs ({i}, {o})")
-        if list(e.get("blocked_shape", [])) != list(mm8_block_shape(i, o)):
-            raise ValueError(f"{name}: blocked shape {e.get('blocked_shape')} vs {list(mm8_block_shape(i, o))}")
+        blocked = [o, i // 2] if fmt == MXFP4_FORMAT else list(mm8_block_shape(i, o))
+        if list(e.get("blocked_shape", [])) != blocked:
+            raise ValueError(f"{name}: blocked shape {e.get('blocked_shape')} vs {blocked}")
         dname = str(dtype).replace("torch.", "")
-        if e.get("activation_dtype") != dname:
-            raise ValueError(f"{name}: packed for {e.get('activation_dtype')} activations, loading {dtype}")
-        if e.get("scale_dtype") != dname:  # the kernels read mx / rx / my / ry in the activation dtype
-            raise ValueError(f"{name}: scales stored as {e.get('scale_dtype')}, the kernels need {dname}")
-        if e.get("packer_version") != PACKER_VERSION:
-            raise ValueError(f"{name}: packer {e.get('packer_version')!r}, this build reads {PACKER_VERSION!r}")
+        if fmt == MXFP4_FORMAT:  # codes and scales do not depend on the activations' type
+            if e.get("scale_dtype") != "uint8" or i % 32:
+                raise ValueError(f"{name}: MXFP4 needs uint8 scales and inputs divisible by 32")
+        else:
+            if e.get("activation_dtype") != dname:
+                raise ValueError(f"{name}: packed for {e.get('activation_dtype')} activations, loading {dtype}")
+            if e.get("scale_dtype") != dname:  # the kernels read mx / rx / my / ry in the activation dtype
+                raise ValueError(f"{name}: scales stored as {e.get('scale_dtype')}, the kernels need {dname}")
+        if e.get("packer_version") != packer:
+            raise ValueError(f"{name}: packer {e.get('packer_version')!r}, this build reads {packer!r}")
         if name in seen:
             raise ValueError(f"{name}: listed twice")
         seen.add(name)
 
 
 def load_prepacked(path, *, device="cuda", dtype=torch.float16,
-                   source_state: Dict[str, torch.Tensor] | None = None):
+                   source_state: Dict[str, torch.Tensor] | None = None,
+                   native_mxfp4_quantize_input: bool | None = None):
     """The model from a prepacked directory: the manifest is validated, then
-    the MM8 modules are built from the stored bytes (no quantisation).  Each
+    the MM8 or MXFP4 modules are built from the stored bytes (no quantisation).  Each
     stored tensor must have the dtype the manifest declares.  With
     ``source_state`` (the unquantised HF state dict), every module's
     ``source_weight_sha256`` is checked against it."""
@@ -377,25 +413,34 @@ def load_prepacked(path, *, device="cuda", dtype=torch.float16,
 
     from .model import NativeRWKV7ForCausalLM
     from .native_quant_mm8 import MM8Linear
+    from .native_quant_mxfp4 import MXFP4Linear
 
     p = Path(path)
     cj = json.loads((p / "config.json").read_text())
     cfg = config_from_json(cj)
-    cfg.use_native_mm8 = True
-    cfg.native_mm8_policy = cj.get("native_mm8_policy", cfg.native_mm8_policy)
-    cfg.native_mm8_min_params = int(cj.get("native_mm8_min_params", cfg.native_mm8_min_params))
     manifest = json.loads((p / "manifest.json").read_text())
+    fmt = manifest.get("format")
+    if fmt == MXFP4_FORMAT:
+        cfg.use_native_mxfp4 = True
+        cfg.native_mxfp4_policy = cj.get("native_mxfp4_policy", cfg.native_mxfp4_policy)
+        cfg.native_mxfp4_min_params = int(cj.get("native_mxfp4_min_params", cfg.native_mxfp4_min_params))
+        cfg.native_mxfp4_quantize_input = bool(cj.get("native_mxfp4_quantize_input", False)
+                                               if native_mxfp4_quantize_input is None else native_mxfp4_quantize_input)
+    else:
+        cfg.use_native_mm8 = True
+        cfg.native_mm8_policy = cj.get("native_mm8_policy", cfg.native_mm8_policy)
+        cfg.native_mm8_min_params = int(cj.get("native_mm8_min_params", cfg.native_mm8_min_params))
     validate_manifest(manifest, cfg, dtype)
     packed = load_file(str(p / "prepacked.safetensors"))
     state = load_file(str(p / "model.safetensors"))
     prebuilt = {}
     for e in manifest["modules"]:
         n = e["module"]
-        missing = [f for f in ("w_blk", "mx", "rx", "my", "ry") if f"{n}.{f}" not in packed]
+        missing = [f for f in _FIELDS[fmt] if f"{n}.{f}" not in packed]
         if missing:
             raise ValueError(f"{n}: prepacked.safetensors lacks {missing}")
-        t = {f: packed[f"{n}.{f}"] for f in ("w_blk", "mx", "rx", "my", "ry")}
-        for f in ("mx", "rx", "my", "ry"):
+        t = {f: packed[f"{n}.{f}"] for f in _FIELDS[fmt]}
+        for f in ("scales",) if fmt == MXFP4_FORMAT else ("mx", "rx", "my", "ry"):
             if str(t[f].dtype).replace("torch.", "") != e["scale_dtype"]:
                 raise ValueError(f"{n}.{f}: stored as {t[f].dtype}, manifest says {e['scale_dtype']}")
         if source_state is not None:
@@ -405,6 +450,14 @@ def load_prepacked(path, *, device="cuda", dtype=torch.float16,
                 raise ValueError(f"{n}: cannot verify the source weight (no digest or no source tensor)")
             if _sha256(src) != want:
                 raise ValueError(f"{n}: source weight digest differs from the one it was packed from")
+        if fmt == MXFP4_FORMAT:
+            if (list(t["codes"].shape) != e["blocked_shape"]
+                    or list(t["scales"].shape) != [e["output_features"], e["input_features"] // 32]):
+                raise ValueError(f"{n}: codes {list(t['codes'].shape)} and scales {list(t['scales'].shape)} do not "
+                                 "match the manifest")
+            prebuilt[n] = MXFP4Linear.from_packed(t["codes"].to(device), t["scales"].to(device),
+                                                  quantize_input=cfg.native_mxfp4_quantize_input)
+            continue
         prebuilt[n] = MM8Linear.from_packed(t["w_blk"].to(device), t["mx"].to(device), t["rx"].to(device),
                                            t["my"].to(device), t["ry"].to(device), e["input_features"],
                                            e["output_features"])
@@ -417,10 +470,10 @@ def convert(args: argparse.Namespace) -> Path:
     weights = torch.load(args.input, weights_only=True, map_location="cpu", mmap=bool(args.low_memory))
     cfg, state = convert_state_dict(weights, dtype)
     out = save_hf_directory(args.output, cfg, state, dtype_name=dtype_name)
-    if args.prepack_mm8:
+    if args.prepack_mm8 or args.prepack_mxfp4:
         from .model import NativeRWKV7ForCausalLM
 
-        cfg.use_native_mm8 = True
+        cfg.use_native_mm8, cfg.use_native_mxfp4 = bool(args.prepack_mm8), bool(args.prepack_mxfp4)
         model = NativeRWKV7ForCausalLM(cfg, state, device=args.device, dtype=dtype)
         save_prepacked(model, out, source_state=state)
     print(f"Saved RWKV-7 model to: {out}")
@@ -434,8 +487,11 @@ def build_parser(prog: str | None = None) -> argparse.ArgumentParser:
     ap.add_argument("--output", required=True, help="output directory")
     ap.add_argument("--precision", choices=sorted(DTYPES), default="fp16")
     ap.add_argument("--low-memory", action="store_true", help="memory-map the checkpoint")
-    ap.add_argument("--prepack-mm8", action="store_true",
-                    help="also write the MM8 modules prepacked (needs a GPU: the packer is a HIP kernel)")
+    pack = ap.add_mutually_exclusive_group()
+    pack.add_argument("--prepack-mm8", action="store_true",
+                      help="also write the MM8 modules prepacked (needs a GPU: the packer is a HIP kernel)")
+    pack.add_argument("--prepack-mxfp4", action="store_true",
+                      help="also write the MXFP4 modules prepacked (needs a GPU; fp16 or bf16)")
     ap.add_argument("--device", default="cuda")
     return ap
 

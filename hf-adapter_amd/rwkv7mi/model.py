@@ -40,10 +40,11 @@ from .fused_recurrent_update import fused_recurrent_output_prepare_raw
 from .native_wkv_fp16 import (native_fp16_recurrent_output_prepare_raw, native_fp16_recurrent_should_use,
                               native_fp16_sequence)
 from .fused_time_mix import fused_attn_sequence_shift_mix, fused_ffn_sequence_shift_mix
-from .sampling import argmax_rows, argmax_workspace_bytes
+from .sampling import argmax_rows, argmax_workspace_bytes, process_logits, process_logits_workspace_bytes
 from .native_quant_mm8 import (GEMM_ROWS, GEMV_ROWS, MM8Linear, is_blocked, mm8_gemm_workspace_bytes, mm8_lnmix_multi_into,
                                mm8_many_rows_into, mm8_matmul_multi_into, mm8_matmul_multi_lora_into,
                                mm8_matmul_partials, mm8_prefill_workspace_bytes, mm8_rows_reserve_bytes, mm8t_workspace_bytes)
+from .native_quant_mxfp4 import BLOCK as MXFP4_BLOCK, MXFP4Linear, mxfp4_linear, mxfp4_linear_multi_into, quantize_mxfp4
 from .native_quant_policy import should_quantize_linear
 from .self_chunk_rwkv7 import _run_chunk, check_wkv7_chunk_status
 
@@ -70,7 +71,12 @@ class NativeRWKV7Config(_PretrainedConfig):
     """The fields of the reference's ``NativeRWKV7Config`` that shape the
     inference path (rwkv7_hf/model_config.py:25-101), as a Hugging Face
     config of the same ``model_type``, so converted directories and
-    ``AutoConfig`` read it.  Only head size 64 has kernels here."""
+    ``AutoConfig`` read it.  Only head size 64 has kernels here.
+
+    ``use_native_mxfp4`` holds the projections (``native_mxfp4_policy``: every one of at
+    least ``native_mxfp4_min_params`` weights, or the head alone) in MXFP4;
+    ``native_mxfp4_quantize_input`` also quantises their inputs, for prompts and decode
+    alike.  It goes with fp16 and bf16 models and not with ``use_native_mm8``."""
 
     model_type = "rwkv7_native"
 
@@ -79,7 +85,9 @@ class NativeRWKV7Config(_PretrainedConfig):
                  decay_low_rank_dim: int = 64, a_low_rank_dim: int = 64, gate_low_rank_dim: int = 128,
                  v_low_rank_dim: int = 32, norm_eps: float = 1e-5, use_native_mm8: bool = False,
                  native_mm8_min_params: int = 8_000_000, native_mm8_policy: str = "memory",
-                 attention_hidden_size: int | None = None, extra: dict | None = None, **kwargs):
+                 attention_hidden_size: int | None = None, extra: dict | None = None,
+                 use_native_mxfp4: bool = False, native_mxfp4_min_params: int = 8_000_000,
+                 native_mxfp4_policy: str = "memory", native_mxfp4_quantize_input: bool = False, **kwargs):
         kwargs.setdefault("tie_word_embeddings", False)  # RWKV keeps an independent output head
         kwargs.pop("num_attention_heads", None)
         if _PretrainedConfig is not object:
@@ -105,6 +113,10 @@ class NativeRWKV7Config(_PretrainedConfig):
         self.use_native_mm8 = bool(use_native_mm8)
         self.native_mm8_min_params = int(native_mm8_min_params)
         self.native_mm8_policy = native_mm8_policy
+        self.use_native_mxfp4 = bool(use_native_mxfp4)
+        self.native_mxfp4_min_params = int(native_mxfp4_min_params)
+        self.native_mxfp4_policy = native_mxfp4_policy
+        self.native_mxfp4_quantize_input = bool(native_mxfp4_quantize_input)
         self.extra = dict(extra or {})
 
     @property
@@ -320,9 +332,41 @@ class QuantLinear:
             return outs
         if all(isinstance(l, DenseLinear) for l in lins) and DenseLinear.apply_group(lins, xs, outs):
             return outs
+        if all(isinstance(l, BlockFloatLinear) for l in lins) and BlockFloatLinear.apply_group(lins, xs, outs):
+            return outs
         for l, x2, o in zip(lins, xs, outs):
             l.apply(x2, o)
         return outs
+
+
+class BlockFloatLinear:
+    """MXFP4 Linear over an :class:`MXFP4Linear`: the few-row kernel, the tile kernel or the
+    prefill GEMM by the product's shape, and the 4-bit x 4-bit GEMM where the module
+    quantises its input; relu^2 and residual inside.  Its scratch comes from torch's
+    allocator, so a captured step keeps its own."""
+
+    def __init__(self, mx: MXFP4Linear):
+        self.m = mx
+        self.out_features, self.in_features = mx.out_features, mx.in_features
+
+    def apply(self, x2, out, *, act=ACT_NONE, residual=None):
+        if act not in (0, 3) or (act == 3 and residual is not None):
+            raise ValueError("BlockFloatLinear: unsupported activation / residual combination")
+        return mxfp4_linear(x2, self.m.codes, self.m.scales, bias=self.m.bias, out=out, residual=residual,
+                            epilogue="relu2" if act == 3 else "none" if residual is None else "residual",
+                            quantize_input=self.m.quantize_input)
+
+    @staticmethod
+    def apply_group(lins, xs, outs) -> bool:
+        """``[l.apply(x, o) for ...]`` as one launch; False (nothing run) when the products
+        do not share a shape and a treatment of their inputs."""
+        if (len(lins) > 4 or len({(l.in_features, l.out_features, l.m.quantize_input) for l in lins}) != 1
+                or any(q.dtype != xs[0].dtype or q.shape != xs[0].shape or not q.is_contiguous()
+                       or q.data_ptr() % 16 for q in xs)):
+            return False
+        mxfp4_linear_multi_into(list(xs), [(l.m.codes, l.m.scales) for l in lins], list(outs),
+                                biases=[l.m.bias for l in lins], quantize_input=lins[0].m.quantize_input)
+        return True
 
 
 # ------------------------------------------------------------------ cache
@@ -875,7 +919,9 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
         self.layers = []
 
     def _finish_init(self):
-        self._rwkv7_native_mm_quantization = "mm8" if self._replaced else None
+        kinds = [name for name, cls in (("mm8", QuantLinear), ("mxfp4", BlockFloatLinear))
+                 if any(isinstance(lin, cls) for lin in self._linears())]
+        self._rwkv7_native_mm_quantization = "+".join(kinds) or None
         self._rwkv7_native_mm_replaced_modules = self._replaced
         self._graph_runners: dict[int, "NativeGraphRunner"] = {}
 
@@ -883,9 +929,14 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
                  device="cuda", dtype=torch.float16, prepacked: dict | None = None):
         """``weights``: HF-named parameters (see :func:`parameter_shapes`);
         None gives the seeded random init (as ``cls(config)`` does for the
-        reference).  ``prepacked``: module name -> :class:`MM8Linear` built
-        from a prepacked checkpoint; those modules' ``.weight`` entries are not
-        read."""
+        reference).  ``prepacked``: module name -> :class:`MM8Linear` or
+        :class:`MXFP4Linear` built from a prepacked checkpoint; those modules'
+        ``.weight`` entries are not read."""
+        if config.use_native_mxfp4:
+            if config.use_native_mm8:
+                raise ValueError("use_native_mm8 and use_native_mxfp4 exclude each other")
+            if dtype not in (torch.float16, torch.bfloat16):
+                raise ValueError(f"use_native_mxfp4 needs an fp16 or bf16 model, got {dtype}")
         if weights is None:
             weights = _LazyWeights(config, 0, device, dtype)
         self._init_common(config, device, dtype)
@@ -898,8 +949,14 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
         def linear(name):
             if prepacked is not None and name in prepacked:
                 self._replaced += 1
-                return QuantLinear(prepacked[name])
+                m = prepacked[name]
+                return BlockFloatLinear(m) if isinstance(m, MXFP4Linear) else QuantLinear(m)
             w = get(name + ".weight")
+            if cfg.use_native_mxfp4 and int(w.shape[1]) % MXFP4_BLOCK == 0 and should_quantize_linear(
+                    name, int(w.numel()), min_params=cfg.native_mxfp4_min_params, policy=cfg.native_mxfp4_policy):
+                self._replaced += 1
+                return BlockFloatLinear(MXFP4Linear.from_packed(*quantize_mxfp4(w),
+                                                                quantize_input=cfg.native_mxfp4_quantize_input))
             if cfg.use_native_mm8 and should_quantize_linear(name, int(w.numel()),
                                                              min_params=cfg.native_mm8_min_params,
                                                              policy=cfg.native_mm8_policy):
@@ -951,15 +1008,15 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
         ``(i, H, N, eps, has_pre, pre_w, pre_b, an_w, an_b, fn_w, fn_b, x_r, x_w,
         x_k, x_v, x_a, x_g, k_k, k_a, r_k, Rw, Kw, Vw, Ow, w1, w2, w0, a1, a2, a0,
         v1, v2, v0, g1, g2, gn_w, gn_b, fx_k, fK, fV, RKVw)``.  Quantized
-        projections stay callables (their ``MM8Linear`` modules), dense ones are
-        ``[out, in]`` weights; layer 0's missing V LoRA and pre-norm are zeros of
+        projections stay callables (their ``MM8Linear`` or ``MXFP4Linear`` modules), dense ones
+        are ``[out, in]`` weights; layer 0's missing V LoRA and pre-norm are zeros of
         the reference's shapes, and the stacked-RKV slot is empty.  Returns
         ``(packs, H, N, eps)``; the tensors are the model's own (no copies)."""
         cfg = self.config
         H, N, D, A = cfg.num_heads, cfg.head_dim, cfg.hidden_size, cfg.attention_hidden_size
         eps = float(N * 1e-5)
         dev, dt = self.device, self.dtype
-        op = lambda lin: lin.m if isinstance(lin, QuantLinear) else lin.weight
+        op = lambda lin: lin.weight if isinstance(lin, DenseLinear) else lin.m
         packs = []
         for L in self.layers:
             has_pre = 1 if L.pre is not None else 0
@@ -990,7 +1047,8 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
         """A model over operands in the reference's 41-entry pack layout (see
         :meth:`extract_graph_packs`): the tensors are used as given (no copies
         when they already have the device and dtype); a projection is an
-        ``MM8Linear`` module (fused MM8 route) or an ``[out, in]`` weight."""
+        ``MM8Linear`` module (fused MM8 route), an ``MXFP4Linear`` module or an
+        ``[out, in]`` weight."""
         if len(packs) != config.num_hidden_layers:
             raise ValueError(f"{len(packs)} packs for {config.num_hidden_layers} layers")
         self = cls.__new__(cls)
@@ -1002,9 +1060,12 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
             if isinstance(x, MM8Linear):
                 self._replaced += 1
                 return QuantLinear(x)
+            if isinstance(x, MXFP4Linear):
+                self._replaced += 1
+                return BlockFloatLinear(x)
             if isinstance(x, torch.Tensor):
                 return DenseLinear(t(x))
-            raise TypeError(f"pack projection must be an MM8Linear or a weight tensor, got {type(x)!r}")
+            raise TypeError(f"pack projection must be an MM8Linear, an MXFP4Linear or a weight tensor, got {type(x)!r}")
 
         for pk in packs:
             if len(pk) != 41:
@@ -1077,7 +1138,7 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
             for L in self.layers:
                 if isinstance(L.r_proj, QuantLinear):
                     pneed = max(pneed, mm8_prefill_workspace_bytes(3, L.r_proj.in_features, L.r_proj.out_features, rows))
-                elif L.r_proj.weight.dtype != torch.float32:
+                elif isinstance(L.r_proj, DenseLinear) and L.r_proj.weight.dtype != torch.float32:
                     pneed = max(pneed, mm8_prefill_workspace_bytes(3, L.r_proj.in_features, L.r_proj.out_features))
             for lin in self._linears():
                 if isinstance(lin, QuantLinear):
@@ -1100,7 +1161,7 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
 
     def dense_state_dict(self) -> dict:
         """HF-named tensors of every parameter the model holds unquantised
-        (the dense linears' ``.weight`` included, the MM8 modules' excluded)."""
+        (the dense linears' ``.weight`` included, the quantised modules' excluded)."""
         sd = {"model.embeddings.weight": self.emb, "model.norm.weight": self.norm[0], "model.norm.bias": self.norm[1]}
         for L in self.layers:
             p = f"model.layers.{L.idx}."
@@ -1652,13 +1713,16 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
     def from_pretrained(cls, pretrained_model_name_or_path, *model_args, config=None, device=None,
                         device_map=None, torch_dtype=None, dtype=None, use_native_mm8: bool | None = None,
                         native_mm8_policy: str | None = None, native_mm8_min_params: int | None = None,
+                        use_native_mxfp4: bool | None = None, native_mxfp4_policy: str | None = None,
+                        native_mxfp4_min_params: int | None = None, native_mxfp4_quantize_input: bool | None = None,
                         **kwargs):
         """A model from a converted directory (``config.json`` +
-        ``*.safetensors``, or a prepacked MM8 directory with ``manifest.json``),
+        ``*.safetensors``, or a prepacked MM8 or MXFP4 directory with ``manifest.json``),
         as ``AutoModelForCausalLM.from_pretrained`` would give the reference's.
         ``dtype`` / ``torch_dtype``: ``"auto"`` reads ``config.json``;
         default fp16.  ``device`` / a single-device ``device_map``: default
-        ``cuda``.  The ``use_native_mm8`` family overrides the config."""
+        ``cuda``.  The ``use_native_mm8`` and ``use_native_mxfp4`` families
+        override the config."""
         import json
         from pathlib import Path
 
@@ -1675,12 +1739,19 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
             device = device_map if isinstance(device_map, (str, torch.device)) and device_map != "auto" else "cuda"
         if config is not None and use_native_mm8 is None:
             use_native_mm8 = getattr(config, "use_native_mm8", None)
+        if config is not None and use_native_mxfp4 is None:
+            use_native_mxfp4 = getattr(config, "use_native_mxfp4", None)
+            if use_native_mxfp4 and native_mxfp4_quantize_input is None:
+                native_mxfp4_quantize_input = getattr(config, "native_mxfp4_quantize_input", None)
         return load_pretrained(path, device=device, dtype=want, use_native_mm8=use_native_mm8,
-                               native_mm8_policy=native_mm8_policy, native_mm8_min_params=native_mm8_min_params)
+                               native_mm8_policy=native_mm8_policy, native_mm8_min_params=native_mm8_min_params,
+                               use_native_mxfp4=use_native_mxfp4, native_mxfp4_policy=native_mxfp4_policy,
+                               native_mxfp4_min_params=native_mxfp4_min_params,
+                               native_mxfp4_quantize_input=native_mxfp4_quantize_input)
 
     def save_pretrained(self, save_directory, **kwargs):
         """Write a directory :meth:`from_pretrained` reads: a prepacked MM8
-        directory when any projection is quantised, else ``config.json`` +
+        or MXFP4 directory when any projection is quantised, else ``config.json`` +
         ``model.safetensors``."""
         from .converter import save_hf_directory, save_prepacked
 
@@ -1691,13 +1762,29 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
                               dtype_name=str(self.dtype).replace("torch.", ""))
 
     @torch.no_grad()
-    def generate_greedy(self, input_ids: torch.Tensor, max_new_tokens: int, *, use_graph: bool = True):
+    def generate_greedy(self, input_ids: torch.Tensor, max_new_tokens: int, *, use_graph: bool = True,
+                        repetition_penalty=1.0, presence_penalty=0.0, frequency_penalty=0.0, penalty_decay=1.0,
+                        bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None):
         """Greedy generation without GenerationMixin's per-step host work: the
         decode graph computes each step's argmax and feeds it to its own next
         replay.  Returns ``[B, T + max_new_tokens]``, the ids
         ``generate(input_ids, max_new_tokens=..., do_sample=False)`` gives
-        with no end-of-sequence token."""
+        with no end-of-sequence token.
+
+        With any of the penalties, ``bias`` or ``allowed`` (those of
+        :func:`~.sampling.process_logits`, over the prompt and what was generated), one
+        :func:`process_logits` after each step picks the token instead, appends it to the
+        ids on the device and feeds it to the next replay."""
         B = int(input_ids.shape[0])
+        plain = bias is None and allowed is None and not any(
+            isinstance(v, torch.Tensor) or v != d
+            for v, d in ((repetition_penalty, 1.0), (presence_penalty, 0.0), (frequency_penalty, 0.0)))
+        if not plain:
+            return self._generate_processed(
+                input_ids, max_new_tokens, use_graph, repetition_penalty=repetition_penalty,
+                presence_penalty=presence_penalty, frequency_penalty=frequency_penalty, penalty_decay=penalty_decay,
+                bias=None if bias is None else bias.to(self.device, torch.float32),
+                allowed=None if allowed is None else allowed.to(self.device))
         out0 = self.forward(input_ids)
         logits, cache = out0.logits, out0.past_key_values
         nxt = argmax_rows(logits[:, -1])
@@ -1711,6 +1798,34 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
                 nxt = argmax_rows(lg)
             out.append(nxt[:, None])
         return torch.cat(out, 1)
+
+    def _generate_processed(self, input_ids, max_new_tokens, use_graph, **how):
+        """:meth:`generate_greedy` through :func:`process_logits`: the ids returned are the
+        history buffer it appends to."""
+        B, T = (int(s) for s in input_ids.shape)
+        dev, V = self.device, self.config.vocab_size
+        ids = torch.empty(B, T + max(int(max_new_tokens), 1), dtype=torch.long, device=dev)
+        ids[:, :T] = input_ids
+        lengths = torch.full((B,), T, dtype=torch.int32, device=dev)
+        nxt = torch.empty(B, dtype=torch.long, device=dev)
+        scores = torch.empty(B, V, dtype=torch.float32, device=dev)
+        ws = torch.empty(process_logits_workspace_bytes(B, V), dtype=torch.uint8, device=dev)
+
+        def pick(logits, nxt2=None):
+            process_logits(logits, history=ids, lengths=lengths, out=scores, next_tokens=nxt, next_tokens2=nxt2,
+                           append=True, workspace=ws, **how)
+
+        out0 = self.forward(input_ids)
+        cache = out0.past_key_values
+        pick(out0.logits[:, -1])
+        runner = self.graph_runner(B) if use_graph else None
+        for t in range(int(max_new_tokens) - 1):
+            if runner is not None:
+                runner.replay_greedy(cache, nxt if t == 0 else None)
+                pick(runner.logits, runner.tokens)
+            else:
+                pick(self.forward(nxt[:, None], past_key_values=cache, use_graph=False).logits[:, -1])
+        return ids
 
 
 class _LazyWeights(dict):

@@ -96,7 +96,7 @@ def mxfp4_linear_multi_into(xs, weights, outs, *, biases=None, residuals=None, e
     """Up to four products of one shape in one launch: ``outs[i] = epilogue(xs[i] @ W_i^T
     (+ bias) (+ residual))`` with ``xs[i] [rows, I]`` and ``outs[i] [rows, O]`` contiguous
     and of one type (fp16 or bf16), ``weights[i] = (codes [O, I/2], scales [O, I/32])``.
-    A residual may be its output's own memory; no output overlaps an input.  The call's
+    A residual may be its output's own memory; no output overlaps an input or another output.  The call's
     scratch is its own (torch's allocator; under capture the graph's pool)."""
     k = len(xs)
     biases, residuals = biases or [None] * k, residuals or [None] * k
@@ -131,7 +131,10 @@ def mxfp4_linear_multi_into(xs, weights, outs, *, biases=None, residuals=None, e
         _lib.require_same_device(x0, x, c, s, o, b, r, name="mxfp4_linear")
         if any(_lib.overlap(o, t) for t in xs):
             raise ValueError("mxfp4: out overlaps an input")
-    if rows == 0:
+    for i, o in enumerate(outs):
+        if any(t is not None and j != i and _lib.overlap(o, t) for side in (outs, residuals) for j, t in enumerate(side)):
+            raise ValueError("mxfp4: out overlaps another product's out or residual")
+    if rows == 0 or m == 0:
         return outs
     need = _scratch(k, rows, m, n, _lib.dtype_code(x0), int(bool(quantize_input)), x0.get_device())
     ws = torch.empty(need, dtype=torch.uint8, device=x0.device) if need else None

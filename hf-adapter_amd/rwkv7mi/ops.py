@@ -47,6 +47,16 @@ SCHEMAS = {
         "mm8_matmul_out(Tensor x, Tensor w_u8, Tensor mx, Tensor rx, Tensor my, Tensor ry, Tensor(a!) out) -> ()",
     "quantize_mm8":
         "quantize_mm8(Tensor weight) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+    "quantize_mxfp4":
+        "quantize_mxfp4(Tensor x) -> (Tensor, Tensor)",
+    "dequantize_mxfp4":
+        "dequantize_mxfp4(Tensor codes, Tensor scales, ScalarType out_dtype) -> Tensor",
+    "mxfp4_linear":
+        "mxfp4_linear(Tensor x, Tensor codes, Tensor scales, bool quantize_input) -> Tensor",
+    "process_logits":
+        "process_logits(Tensor logits, Tensor? history, Tensor? lengths, float repetition_penalty,"
+        " float presence_penalty, float frequency_penalty, float penalty_decay, Tensor? bias, Tensor? allowed)"
+        " -> (Tensor, Tensor)",
     "w4_groupwise_linear":
         "w4_groupwise_linear(Tensor x, Tensor q, Tensor scales, int out_features, int in_features, int group_size)"
         " -> Tensor",
@@ -73,7 +83,7 @@ SCHEMAS = {
 
 def _cuda_impls():
     from . import fused_decode_norm_mix as fdm
-    from . import fused_lora, fused_output, fused_prefill, fused_time_mix, native_quant_mm8, sm70_quant
+    from . import fused_lora, fused_output, fused_prefill, fused_time_mix, native_quant_mm8, native_quant_mxfp4, sampling, sm70_quant
     from .fused_recurrent_update import fused_recurrent_output_prepare_raw, fused_recurrent_update
     from .self_chunk_rwkv7 import _run_chunk
     from .fused_recurrent_update import _as_bthn, _check_state
@@ -121,6 +131,21 @@ def _cuda_impls():
     def quant8(weight):
         return native_quant_mm8.quantize_mm8(weight)
 
+    def quant4(x):
+        return native_quant_mxfp4.quantize_mxfp4(x)
+
+    def dequant4(codes, scales, out_dtype):
+        return native_quant_mxfp4.dequantize_mxfp4(codes, scales, out_dtype=out_dtype)
+
+    def linear4(x, codes, scales, quantize_input):
+        return native_quant_mxfp4.mxfp4_linear(x, codes, scales, quantize_input=quantize_input)
+
+    def logits_step(logits, history, lengths, rep, pres, freq, decay, bias, allowed):
+        nxt = torch.empty(logits.shape[0], dtype=torch.long, device=logits.device)
+        return sampling.process_logits(logits, history=history, lengths=lengths, repetition_penalty=rep,
+                                       presence_penalty=pres, frequency_penalty=freq, penalty_decay=decay, bias=bias,
+                                       allowed=allowed, next_tokens=nxt), nxt
+
     def w4g(x, q, scales, out_features, in_features, group_size):
         return sm70_quant.w4_groupwise_linear(x, q, scales, out_features, in_features, group_size=group_size)
 
@@ -151,7 +176,8 @@ def _cuda_impls():
         "fused_recurrent_update": update, "fused_recurrent_update_": update_,
         "fused_recurrent_output_prepare_raw": prep_raw, "fused_recurrent_output_prepare_raw_": prep_raw_,
         "chunk_scan": chunk, "chunk_scan_": chunk_, "mm8_matmul": mm8, "mm8_matmul_out": mm8_out,
-        "quantize_mm8": quant8, "w4_groupwise_linear": w4g, "attn_norm_mix6_": mix6_,
+        "quantize_mm8": quant8, "quantize_mxfp4": quant4, "dequantize_mxfp4": dequant4, "mxfp4_linear": linear4,
+        "process_logits": logits_step, "w4_groupwise_linear": w4g, "attn_norm_mix6_": mix6_,
         "ffn_add_norm_mix_": ffn_mix_, "wavg_lora": wavg, "state_prep": sprep, "output_prepare": oprep,
         "seq_shift_mix": shift,
     }
@@ -178,6 +204,20 @@ def _fake_impls():
         return (weight.new_empty((n, m), dtype=torch.uint8), weight.new_empty(m), weight.new_empty(m),
                 weight.new_empty((n, 1)), weight.new_empty((n, 1)))
 
+    def quant4(x):
+        n = x.shape[-1]
+        return (x.new_empty((*x.shape[:-1], n // 2), dtype=torch.uint8),
+                x.new_empty((*x.shape[:-1], n // 32), dtype=torch.uint8))
+
+    def dequant4(codes, scales, out_dtype):
+        return codes.new_empty((*codes.shape[:-1], 2 * codes.shape[-1]), dtype=out_dtype)
+
+    def linear4(x, codes, scales, quantize_input):
+        return x.new_empty((*x.shape[:-1], codes.shape[0]))
+
+    def logits_step(logits, history, lengths, rep, pres, freq, decay, bias, allowed):
+        return logits.new_empty(logits.shape), logits.new_empty(logits.shape[0], dtype=torch.long)
+
     def w4g(x, q, scales, out_features, in_features, group_size):
         return x.new_empty((*x.shape[:-1], int(out_features)))
 
@@ -199,7 +239,8 @@ def _fake_impls():
         "fused_recurrent_update": update, "fused_recurrent_update_": none,
         "fused_recurrent_output_prepare_raw": prep_raw, "fused_recurrent_output_prepare_raw_": none,
         "chunk_scan": chunk, "chunk_scan_": none, "mm8_matmul": mm8, "mm8_matmul_out": none,
-        "quantize_mm8": quant8, "w4_groupwise_linear": w4g, "attn_norm_mix6_": none, "ffn_add_norm_mix_": none,
+        "quantize_mm8": quant8, "quantize_mxfp4": quant4, "dequantize_mxfp4": dequant4, "mxfp4_linear": linear4,
+        "process_logits": logits_step, "w4_groupwise_linear": w4g, "attn_norm_mix6_": none, "ffn_add_norm_mix_": none,
         "wavg_lora": wavg, "state_prep": sprep, "output_prepare": oprep, "seq_shift_mix": shift,
     }
 

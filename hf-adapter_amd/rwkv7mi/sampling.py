@@ -188,4 +188,23 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     return out
 
 
-__all__ = ["argmax_rows", "argmax_workspace_bytes", "process_logits", "process_logits_workspace_bytes"]
+class NativeLogitsProcessor:
+    """:func:`process_logits` as an entry of ``generate(logits_processor=[...])``: the ids so
+    far (the prompt from ``prompt_ignore_length`` on) are the history.  ``allowed`` may be a
+    callable that gives the words for ``input_ids``, for a mask that follows the text."""
+
+    def __init__(self, *, repetition_penalty=1.0, presence_penalty=0.0, frequency_penalty=0.0, penalty_decay=1.0,
+                 bias: torch.Tensor | None = None, allowed=None, prompt_ignore_length: int = 0):
+        if int(prompt_ignore_length) < 0:
+            raise ValueError("NativeLogitsProcessor: prompt_ignore_length must not be negative")
+        self.how = dict(repetition_penalty=repetition_penalty, presence_penalty=presence_penalty,
+                        frequency_penalty=frequency_penalty, penalty_decay=penalty_decay)
+        self.bias, self.allowed, self.skip = bias, allowed, int(prompt_ignore_length)
+
+    def __call__(self, input_ids: torch.Tensor, scores: torch.Tensor) -> torch.Tensor:
+        allowed = self.allowed(input_ids) if callable(self.allowed) else self.allowed
+        return process_logits(scores, history=input_ids[:, self.skip:], allowed=allowed, bias=self.bias, **self.how)
+
+
+__all__ = ["argmax_rows", "argmax_workspace_bytes", "process_logits", "process_logits_workspace_bytes",
+           "NativeLogitsProcessor"]

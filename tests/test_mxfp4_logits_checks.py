@@ -108,3 +108,52 @@ def test_python_refusals_before_any_device_work():
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+def test_model_config_refusals():
+    from rwkv7mi.model import NativeRWKV7Config, NativeRWKV7ForCausalLM
+
+    def cfg(**kw):
+        return NativeRWKV7Config(vocab_size=64, hidden_size=64, num_hidden_layers=1, use_native_mxfp4=True, **kw)
+
+    with pytest.raises(ValueError, match="exclude each other"):
+        NativeRWKV7ForCausalLM(cfg(use_native_mm8=True), device="cpu")
+    with pytest.raises(ValueError, match="fp16 or bf16"):
+        NativeRWKV7ForCausalLM(cfg(), device="cpu", dtype=torch.float32)
+    back = NativeRWKV7Config(**{k: v for k, v in cfg(native_mxfp4_quantize_input=True).to_dict().items()
+                                if k != "model_type"})
+    assert back.use_native_mxfp4 and back.native_mxfp4_quantize_input
+
+
+def test_prepacked_manifest_refusals():
+    from rwkv7mi.converter import MXFP4_FORMAT, MXFP4_PACKER_VERSION, PACKER_VERSION, validate_manifest
+    from rwkv7mi.model import NativeRWKV7Config
+
+    cfg = NativeRWKV7Config(vocab_size=64, hidden_size=64, num_hidden_layers=1)
+    entry = {"format": MXFP4_FORMAT, "module": "lm_head", "input_features": 64, "output_features": 64,
+             "activation_dtype": "float16", "scale_dtype": "uint8", "blocked_shape": [64, 32],
+             "packer_version": MXFP4_PACKER_VERSION}
+
+    def check(dtype=torch.bfloat16, top=MXFP4_PACKER_VERSION, **kw):
+        validate_manifest({"format": MXFP4_FORMAT, "packer_version": top, "modules": [{**entry, **kw}]}, cfg, dtype)
+
+    check()
+    check(torch.float16)
+    for bad in (dict(dtype=torch.float32), dict(top=PACKER_VERSION), dict(blocked_shape=[64, 64]),
+                dict(scale_dtype="float16"), dict(format="rwkv7mi.mm8_blocked.v1"), dict(input_features=32)):
+        with pytest.raises(ValueError):
+            check(**bad)
+
+
+def test_fake_kernels_give_shapes():
+    import rwkv7mi  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        codes, scales = torch.ops.rwkv7mi.quantize_mxfp4(torch.empty(7, 96, dtype=torch.float16))
+        assert codes.shape == (7, 48) and scales.shape == (7, 3) and codes.dtype == scales.dtype == torch.uint8
+        assert torch.ops.rwkv7mi.dequantize_mxfp4(codes, scales, torch.bfloat16).shape == (7, 96)
+        y = torch.ops.rwkv7mi.mxfp4_linear(torch.empty(2, 5, 96, dtype=torch.float16), codes, scales, True)
+        assert y.shape == (2, 5, 7)
+        out, nxt = torch.ops.rwkv7mi.process_logits(y[0], None, None, 1.0, 0.0, 0.0, 1.0, None, None)
+        assert out.shape == (5, 7) and nxt.shape == (5,) and nxt.dtype == torch.int64
