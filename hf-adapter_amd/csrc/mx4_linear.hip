@@ -1,7 +1,7 @@
 // Products with an MXFP4 weight: y = epilogue(x W^T + bias), fp16 / bf16 rows
 // x, or the same rows quantised to MXFP4 on the way.
 //
-// mx4_rows_kernel, 16 rows a tile: the nw waves of a workgroup share K in units of
+// mx4_rows_kernel, 16 rows a tile, few of them: the nw waves of a workgroup share K in units of
 // 512 inputs and go through groups of 16 outputs, a grid apart; a group's fp32 sums
 // meet in LDS in wave order.  A unit is four steps of 128 inputs (four blocks): lane
 // n + 16 q holds block q of output n, 16 bytes of codes and one scale byte, which is
@@ -254,15 +254,23 @@ static int mx4_rows_run(const Mx4Batch& b, int nprob, void* part, void* stream) 
 static int64_t mx4_codes_bytes(int64_t rows, int64_t I) { return (rows * (I / 2) + 255) & ~(int64_t)255; }
 static int64_t mx4_scales_bytes(int64_t rows, int64_t I) { return (rows * (I / MX4_BLOCK) + 255) & ~(int64_t)255; }
 
-// Which kernel takes a product: up to 16 rows (and what the others' offsets cannot
-// hold) the few-row kernel, above it the 64- to 256-row tiles.  16-bit rows from 1024
+// Which kernel takes a product.  The few-row kernel: up to 16 rows, and more while its
+// passes over the weight, one a 16-row tile, cost less than the tiles' other launches
+// (16-bit rows on it and on the tiles: 64 x 4096 -> 4096 16.0 and 22.7 us, 40 x 8192 ->
+// 2048 16.8 and 22.7, 128 x 768 -> 768 4.6 and 14.2, 64 x 4096 -> 16384 33.9 and 36.1,
+// 96 rows 48.4 and 43.0, 256 x 4096 -> 4096 31.8 and 30.2; two tiles at any size, 32 x
+// 4096 -> 65536 59 and 74, 48 rows 84 and 76; past 256 rows its passes over x count too,
+// 1000 x 1024 -> 4096 31.6 and 20.2.  MXFP4 rows, whose tiles need no conversions: 128 x
+// 4096 -> 4096 16.4 and 19.7, 64 x 4096 -> 16384 26.7 and 26.0); and what the others'
+// offsets cannot hold.  Else the 64- to 256-row tiles.  16-bit rows from 1024
 // tiles of 256 x 256 on write the weight out in 16 bits and run the GEMM of mm8h.hip:
 // without conversions between its MFMAs it holds a higher clock over such long calls
-// (16384 x 4096 -> 16384 1672 us, on the tiles 2000), and the pass over the weight
-// is small against them (1000 rows, 256 tiles: 150 and 145).
+// (16384 x 4096 -> 16384 1636 us, on the tiles 2000), and the pass over the weight
+// is small against them (1000 rows, 256 tiles: 150 and 114).
 enum Mx4Route { MX4_ROWS, MX4_TILE, MX4_GEMM, MX4_PREFILL };
 static Mx4Route mx4_route(int64_t rows, int64_t I, int64_t O, int quantize_input) {
-  if (rows <= 16) return MX4_ROWS;
+  const bool few = rows <= 256 && (rows + 15) / 16 * (O * I) <= (quantize_input ? 1 << 27 : 1 << 28);
+  if (rows <= 16 || few || (rows <= 32 && !quantize_input)) return MX4_ROWS;
   if (quantize_input) return mx4_gemm_supported(rows, O, I) ? MX4_GEMM : MX4_ROWS;
   if ((rows + 255) / 256 * ((O + 255) / 256) >= 1024 && mx4h_supported(rows, I, O)) return MX4_PREFILL;
   return mx4_tile_supported(rows, O, I) ? MX4_TILE : MX4_ROWS;

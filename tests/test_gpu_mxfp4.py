@@ -85,7 +85,10 @@ SHAPES = [(1, 32, 1), (1, 64, 17), (2, 96, 40), (16, 128, 16), (17, 160, 33), (1
           (33, 1024, 100), (40, 512, 300), (64, 2048, 96), (65, 288, 130), (129, 640, 257), (200, 2560, 512),
           (257, 1024, 520), (300, 96, 70), (520, 768, 264),
           (2, 8704, 30), (9, 16384, 40), (16, 8224, 24),
-          (4, 8192, 40), (2, 7680, 24), (700, 608, 1100)]
+          (4, 8192, 40), (2, 7680, 24), (700, 608, 1100),
+          (256, 2080, 40), (100, 9248, 30), (128, 768, 200), (250, 32, 9),
+          (257, 32, 1), (258, 160, 33), (270, 288, 130), (300, 640, 257), (290, 1056, 65), (321, 2080, 300),
+          (260, 8224, 24), (300, 16384, 40)]
 
 
 def _case(rows, n, m, dt, seed, *, lo=112, hi=122):
