@@ -9,16 +9,22 @@
 //  * one v_mfma_scale_f32_16x16x128_f8f6f4 where x is MXFP4 too, or
 //  * four v_mfma_f32_16x16x32 where x is 16-bit: MFMA j takes inputs 8 j .. +7
 //    of every lane's block, and so do the rows of x.
-// A wave has one unit: its part of x stays in registers for all its groups, and the
-// next group's codes and scales are loaded before this one's MFMAs.  Above 16 units
-// (K > 8192) the units go over several workgroups, and a second launch adds their
-// sums (16 x 16384 -> 4096 with two units a wave, x reloaded, 25.6 us).  What does
-// not carry weights is kept out of the loads' way: a group's scales are loaded once
-// by the workgroup, through LDS, a group ahead (by each wave 1.4 us more at 1 x 4096
-// -> 16384, 13.1 us then), and up to four 16-bit rows of x by whole instructions,
-// through LDS (in the operand's layout, most lanes idle, 2.6 us more).  bf16 holds a scaled code exactly.  fp16 does
-// not for every scale, so there a step's codes are scaled relative to the largest of
-// its four scales and the step's sums by that one's factor (mx4_common.h).
+// A wave has one unit: its part of x stays in registers for all its groups (32 rows of
+// it from 17 rows on, whose codes are then converted once: 64 x 4096 -> 4096 16.1 ->
+// 14.6 us), and the next group's codes and scales are loaded before this one's MFMAs.
+// Above the 16 units (8 with 32 rows) that a CU's registers hold the units go over
+// several workgroups, and a second launch adds their sums (16 x 16384 -> 4096 with two
+// units a wave, x reloaded, 25.6 us).  What does not carry weights is kept out of the
+// loads' way: a group's scales are loaded once by the workgroup, through LDS, a group
+// ahead (by each wave 1.4 us more at 1 x 4096 -> 16384, 13.1 us then), and 16-bit rows
+// by whole lines, through LDS (in the operand's layout, 16 bytes of 64 lines an
+// instruction, 17.3 us for 14.6 at 16 x 4096 -> 16384).  bf16 holds a scaled code
+// exactly.  fp16 does not for every scale, so there a step's codes are scaled relative
+// to the largest of its four scales and the step's sums by that one's factor
+// (mx4_common.h).
+//
+// The weight's bytes bound it: 1 x 4096 -> 16384 11.9 us (36 MB; 9.5 from the caches),
+// 8 x 4096 -> 65536 35 us, 4.0 TB/s of the 5.4 that a copy reaches.
 #include <algorithm>
 
 #include "mx4_common.h"
@@ -65,9 +71,9 @@ struct Mx4Rows {
   float* part;  // S > 1: [problem][split][row][O]
 };
 
-// FEW: 16-bit rows, at most four
-template <typename T, bool A4, int SC, bool FEW>
-__global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Rows R) {
+// RT: 16-row tiles a wave
+template <typename T, bool A4, int SC, int RT>
+__global__ __launch_bounds__(RT > 1 ? 512 : 1024) void mx4_rows_kernel(const Mx4Rows R) {
   using V = typename Mx4Types<T>::V;
   constexpr bool F16 = std::is_same<T, __half>::value && !A4;
   const Mx4Batch& B = R.b;
@@ -75,25 +81,20 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Rows R) {
   const int I = B.I, O = B.O, nb = I / MX4_BLOCK, groups = (O + 15) / 16;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
-  const int row0 = blockIdx.y * 16;
-  const bool mine = row0 + n < B.rows;
-  const int64_t row = min(row0 + n, B.rows - 1);
-  const T* x = A4 ? nullptr : static_cast<const T*>(P.x) + row * I + 32 * q;
-  const uint8_t* xc = A4 ? P.xc + row * (I / 2) + 16 * q : nullptr;
-  const uint8_t* xs = A4 ? P.xs + row * nb : nullptr;
+  const int row0 = blockIdx.y * 16 * RT;
   const u32x4 zero = {0u, 0u, 0u, 0u};
   constexpr int NX = A4 ? 1 : 4;  // 16-byte pieces of x a step
 
   // [group's parity][output][wave] scales, then [group's parity][wave][row][output]
-  // sums in the memory that first holds [wave][row][16-byte piece] of x
+  // sums in the memory that first holds [wave][row][16-byte piece] of a step of x
   extern __shared__ __align__(16) char smem[];
   u32x4* const scale = reinterpret_cast<u32x4*>(smem);
   char* const lower = smem + 512 * nw;
-  typedef float Sums[16][17];
+  typedef float Sums[16 * RT][17];
   Sums* const part = reinterpret_cast<Sums*>(lower);
-  u32x4* const xl = reinterpret_cast<u32x4*>(lower) + wave * (FEW ? B.rows : 0) * 64;
+  u32x4* const xl = reinterpret_cast<u32x4*>(lower) + wave * 256;
 
-  u32x4 w[4], wn[4], a[4][NX], ea = zero;
+  u32x4 w[4], wn[4], a[RT][4][NX], ea = zero;
   const int u0 = (int)(blockIdx.z % R.S) * nw;
   const int b0 = 16 * (u0 + wave);  // (waves past the last unit add zeros)
   const bool has = b0 < nb;
@@ -114,41 +115,51 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Rows R) {
   if (has) load_w(blockIdx.x, w);
   if (scales) scale[so * nw + su] = load_s(blockIdx.x);
   if (has) {
-    if constexpr (FEW) {
-      // piece `lane` of each row's unit, 8 inputs
-      const T* xr = static_cast<const T*>(P.x) + 32 * b0 + 8 * lane;
-      const bool in = SC == 2 || 32 * b0 + 8 * lane < I;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (r < B.rows) xl[64 * r + lane] = in ? *reinterpret_cast<const u32x4*>(xr + (int64_t)r * I) : zero;
-      const int r = min(n, B.rows - 1);  // (rows past the end repeat the last one and are not stored)
+    if constexpr (A4) {
+      const bool mine = row0 + n < B.rows;
+      const int64_t row = min(row0 + n, B.rows - 1);
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int j = 0; j < NX; ++j) a[s][j] = xl[64 * r + 16 * s + 4 * q + j];
+        a[0][s][0] = mine && (SC == 2 || b0 + 4 * s + q < nb)
+                         ? *reinterpret_cast<const u32x4*>(P.xc + row * (I / 2) + 16 * (b0 + 4 * s + q)) : zero;
+      ea = mine ? mx4_unit_scales<SC>(P.xs + row * nb, b0, nb) : zero;
     } else {
+      // load v of a step: lane, piece lane % 16 of row 4 v + lane / 16.  (Rows past the end
+      // hold anything and are not stored.)
+      const T* x = static_cast<const T*>(P.x) + 32 * b0 + 8 * n;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int j = 0; j < NX; ++j) a[s][j] = zero;
-        if (mine && (SC == 2 || b0 + 4 * s + q < nb)) {
-          if constexpr (A4) {
-            a[s][0] = *reinterpret_cast<const u32x4*>(xc + 16 * (b0 + 4 * s));
-          } else {
+        for (int v = 0; v < 4; ++v) {
+          const int r = row0 + 16 * t + 4 * v + q;
 #pragma unroll
-            for (int j = 0; j < NX; ++j) a[s][j] = *reinterpret_cast<const u32x4*>(x + 32 * (b0 + 4 * s) + 8 * j);
+          for (int s = 0; s < 4; ++s) a[t][s][v] = zero;
+          if (r < B.rows) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              if (SC == 2 || 32 * b0 + 128 * s + 8 * n < I)
+                a[t][s][v] = *reinterpret_cast<const u32x4*>(x + (int64_t)r * I + 128 * s);
           }
         }
-      }
-      if constexpr (A4) {
-        if (mine) ea = mx4_unit_scales<SC>(xs, b0, nb);
-      }
+      // piece p of row r at p ^ r: rows of 256 bytes without bank conflicts either way
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (row0 + 16 * t + 4 * v < B.rows) xl[16 * (4 * v + q) + (n ^ (4 * v + q))] = a[t][s][v];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) a[t][s][j] = xl[16 * n + ((4 * q + j) ^ n)];
+        }
     }
   }
   __syncthreads();
   int par = 0;
   for (int g = blockIdx.x; g < groups; g += gridDim.x, par ^= 1) {
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    f32x4 acc[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const bool next = g + (int)gridDim.x < groups;
     if (next && scales) sn = load_s(g + gridDim.x);
     if (has) {
@@ -158,31 +169,35 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Rows R) {
       for (int s = 0; s < 4; ++s) {
         const uint32_t ew = e[s], eb = (ew >> (8 * q)) & 255u;
         if constexpr (A4) {
-          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(a[s][0]), mx4_operand(w[s]), acc, 4, 4, 0,
-                                                                 (int)((ea[s] >> (8 * q)) & 255u), 0, (int)eb);
+          acc[0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(a[0][s][0]), mx4_operand(w[s]), acc[0], 4, 4,
+                                                                    0, (int)((ea[s] >> (8 * q)) & 255u), 0, (int)eb);
         } else {
           const uint32_t emax = F16 ? max4(ew) : 0u;
           const float sc = F16 ? mx4_relative(eb, emax) : mx4_scale(eb);
-          f32x4 c = F16 ? (f32x4){0.f, 0.f, 0.f, 0.f} : acc;
+          f32x4 c[RT];
+#pragma unroll
+          for (int t = 0; t < RT; ++t) c[t] = F16 ? (f32x4){0.f, 0.f, 0.f, 0.f} : acc[t];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             V wv;
             mx4_decode8(w[s][j], sc, wv);
-            c = mfma16x16x32(__builtin_bit_cast(V, a[s][j]), wv, c);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) c[t] = mfma16x16x32(__builtin_bit_cast(V, a[t][s][j]), wv, c[t]);
           }
-          acc = F16 ? acc + mx4_factor(emax) * c : c;
+#pragma unroll
+          for (int t = 0; t < RT; ++t) acc[t] = F16 ? acc[t] + mx4_factor(emax) * c[t] : c[t];
         }
       }
 #pragma unroll
       for (int s = 0; s < 4; ++s) w[s] = wn[s];
     }
     if (next && scales) scale[(16 * (par ^ 1) + so) * nw + su] = sn;
-    // lane: output n, rows 4 q .. +3.  (A wave is at most one group ahead of the
+    // lane: output n, rows 4 q .. +3 of each tile.  (A wave is at most one group ahead of the
     // readers of the other half.)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[par * nw + wave][4 * q + i][n] = acc[i];
+    for (int i = 0; i < 4 * RT; ++i) part[par * nw + wave][16 * (i >> 2) + 4 * q + (i & 3)][n] = acc[i >> 2][i & 3];
     __syncthreads();
-    for (int z = tid; z < 256; z += blockDim.x) {
+    for (int z = tid; z < 256 * RT; z += blockDim.x) {
       const int r = z >> 4, c = z & 15;
       if (row0 + r >= B.rows || 16 * g + c >= O) continue;
       float v = part[par * nw][r][c];
@@ -208,36 +223,45 @@ __global__ __launch_bounds__(256) void mx4_rows_reduce_kernel(const Mx4Rows R) {
 
 // Workgroups that share K: up to 16 units of 512 inputs in one, 8 where there are
 // more (16 x 16384 -> 4096: 21.0 us with 8, 21.8 with 16; 1 row 15.9 and 16.7).
-static int mx4_rows_splits(int64_t I) { return I <= 8192 ? 1 : (int)((I + 4095) / 4096); }
-static int64_t mx4_rows_part_bytes(int nprob, int64_t rows, int64_t O, int64_t I) {
-  const int S = mx4_rows_splits(I);
+static int mx4_rows_tiles(int64_t rows, bool A4) { return rows <= 16 || A4 ? 1 : 2; }
+static int mx4_rows_splits(int64_t rows, int64_t I, bool A4) {
+  return I <= (mx4_rows_tiles(rows, A4) > 1 ? 4096 : 8192) ? 1 : (int)((I + 4095) / 4096);
+}
+static int64_t mx4_rows_part_bytes(int nprob, int64_t rows, int64_t O, int64_t I, bool A4) {
+  const int S = mx4_rows_splits(rows, I, A4);
   return S > 1 ? nprob * S * rows * O * 4 : 0;
 }
 
+// LDS bytes a wave: its scales, and its sums or its part of x
+static int mx4_rows_lds(int rt, bool A4) { return 512 + std::max(2 * 16 * rt * 17 * 4, A4 ? 0 : 4096); }
+
 template <typename T, bool A4>
 static int mx4_rows_run(const Mx4Batch& b, int nprob, void* part, void* stream) {
-  Mx4Rows r{b, mx4_rows_splits(b.I), static_cast<float*>(part)};
-  const int units = (b.I + 511) / 512, nw = (units + r.S - 1) / r.S;
-  const int groups = (b.O + 15) / 16, tiles = (b.rows + 15) / 16;
-  // 16 waves a CU fit by registers: no more workgroups than run at once
-  const int64_t most = std::max<int64_t>(1, 256 * (16 / nw) / ((int64_t)tiles * nprob * r.S));
+  Mx4Rows r{b, mx4_rows_splits(b.rows, b.I, A4), static_cast<float*>(part)};
+  const int units = (b.I + 511) / 512, nw = (units + r.S - 1) / r.S, rt = mx4_rows_tiles(b.rows, A4);
+  const int groups = (b.O + 15) / 16, tiles = (b.rows + 16 * rt - 1) / (16 * rt);
+  // 16 waves a CU fit by registers (8 with two tiles of 16-bit rows): no more workgroups than run at once
+  const int fit = rt > 1 ? 8 : 16;
+  const int64_t most = std::max<int64_t>(1, 256 * (fit / nw) / ((int64_t)tiles * nprob * r.S));
   const dim3 grid((unsigned)std::min<int64_t>(groups, most), (unsigned)tiles, (unsigned)(nprob * r.S));
   // (16-byte scale reads need the rows of scales to start 16-byte aligned)
   bool wide = b.I % 512 == 0;
   for (int i = 0; i < nprob; ++i)
     if ((reinterpret_cast<uintptr_t>(b.p[i].ws) | reinterpret_cast<uintptr_t>(b.p[i].xs)) & 15) wide = false;
-  const int lds = nw * (512 + std::max(2 * 16 * 17 * 4, !A4 && b.rows <= 4 ? 1024 * b.rows : 0));
+  const int lds = nw * mx4_rows_lds(rt, A4);
   const auto go = [&](auto sc) {
+    constexpr int SC = decltype(sc)::value;
     static std::atomic<uint64_t> raised[2];
     const auto launch = [&](auto kern, std::atomic<uint64_t>& done) {
       if (lds > 65536)
-        if (int rc = raise_dynamic_lds(reinterpret_cast<const void*>(kern), 16 * (512 + 4096), done, "mx4_rows_kernel"))
+        if (int rc = raise_dynamic_lds(reinterpret_cast<const void*>(kern), 16 * mx4_rows_lds(1, A4), done, "mx4_rows_kernel"))
           return rc;
       hipLaunchKernelGGL(kern, grid, dim3(64 * nw), lds, as_stream(stream), r);
       return check_launch("mx4_rows_kernel");
     };
-    return !A4 && b.rows <= 4 ? launch(&mx4_rows_kernel<T, A4, decltype(sc)::value, !A4>, raised[0])
-                              : launch(&mx4_rows_kernel<T, A4, decltype(sc)::value, false>, raised[1]);
+    if constexpr (!A4)
+      if (rt == 2) return launch(&mx4_rows_kernel<T, A4, SC, 2>, raised[1]);
+    return launch(&mx4_rows_kernel<T, A4, SC, 1>, raised[0]);
   };
   if (int rc = wide               ? go(std::integral_constant<int, 2>{})
                : b.I % 128 == 0 ? go(std::integral_constant<int, 1>{})
@@ -255,22 +279,23 @@ static int64_t mx4_codes_bytes(int64_t rows, int64_t I) { return (rows * (I / 2)
 static int64_t mx4_scales_bytes(int64_t rows, int64_t I) { return (rows * (I / MX4_BLOCK) + 255) & ~(int64_t)255; }
 
 // Which kernel takes a product.  The few-row kernel: up to 16 rows, and more while its
-// passes over the weight, one a 16-row tile, cost less than the tiles' other launches
-// (16-bit rows on it and on the tiles: 64 x 4096 -> 4096 16.0 and 22.7 us, 40 x 8192 ->
-// 2048 16.8 and 22.7, 128 x 768 -> 768 4.6 and 14.2, 64 x 4096 -> 16384 33.9 and 36.1,
-// 96 rows 48.4 and 43.0, 256 x 4096 -> 4096 31.8 and 30.2; two tiles at any size, 32 x
-// 4096 -> 65536 59 and 74, 48 rows 84 and 76; past 256 rows its passes over x count too,
-// 1000 x 1024 -> 4096 31.6 and 20.2.  MXFP4 rows, whose tiles need no conversions: 128 x
-// 4096 -> 4096 16.4 and 19.7, 64 x 4096 -> 16384 26.7 and 26.0); and what the others'
-// offsets cannot hold.  Else the 64- to 256-row tiles.  16-bit rows from 1024
+// passes over the weight, one a tile of 32 rows (16 in MXFP4), cost less than the other
+// kernels' pre-pass and split sums.  16-bit rows on it and on the larger tiles: 64 x 4096
+// -> 4096 11.2 and 22.7 us, 128 x 768 -> 768 5.5 and 14.2, 256 x 4096 -> 4096 24.9 and
+// 29.9, 96 x 4096 -> 16384 42.0 and 43.0, 128 rows 49.0 and 46.7, 512 x 4096 -> 4096 44.4
+// and 40.3; 32 rows at any size, 32 x 4096 -> 65536 52 and 74; past 512 rows its passes
+// over x count too, 1000 x 1024 -> 4096 27.5 and 20.3.  MXFP4 rows: 128 x 4096 -> 4096
+// 16.6 and 19.7, 64 x 4096 -> 16384 26.0 and 26.0.  And what the others' offsets
+// cannot hold.  Else the 64- to 256-row tiles.  16-bit rows from 1024
 // tiles of 256 x 256 on write the weight out in 16 bits and run the GEMM of mm8h.hip:
 // without conversions between its MFMAs it holds a higher clock over such long calls
 // (16384 x 4096 -> 16384 1636 us, on the tiles 2000), and the pass over the weight
 // is small against them (1000 rows, 256 tiles: 150 and 114).
 enum Mx4Route { MX4_ROWS, MX4_TILE, MX4_GEMM, MX4_PREFILL };
 static Mx4Route mx4_route(int64_t rows, int64_t I, int64_t O, int quantize_input) {
-  const bool few = rows <= 256 && (rows + 15) / 16 * (O * I) <= (quantize_input ? 1 << 27 : 1 << 28);
-  if (rows <= 16 || few || (rows <= 32 && !quantize_input)) return MX4_ROWS;
+  const bool few = quantize_input ? rows <= 256 && (rows + 15) / 16 * (O * I) <= 1 << 27
+                                  : rows <= 32 || (rows <= 512 && (rows + 31) / 32 * (O * I) <= 3 << 26);
+  if (rows <= 16 || few) return MX4_ROWS;
   if (quantize_input) return mx4_gemm_supported(rows, O, I) ? MX4_GEMM : MX4_ROWS;
   if ((rows + 255) / 256 * ((O + 255) / 256) >= 1024 && mx4h_supported(rows, I, O)) return MX4_PREFILL;
   return mx4_tile_supported(rows, O, I) ? MX4_TILE : MX4_ROWS;
@@ -287,7 +312,7 @@ extern "C" int64_t rwkv7mi_mxfp4_linear_workspace_bytes(int nprob, int64_t rows,
   if (route == MX4_PREFILL) return mx4h_workspace_bytes(nprob, rows, I, O);
   if (route == MX4_GEMM) return mx4_gemm_workspace_bytes(nprob, rows, O, I);
   if (route == MX4_TILE) return mx4_tile_workspace_bytes(nprob, rows, O, I);
-  const int64_t part = mx4_rows_part_bytes(nprob, rows, O, I);
+  const int64_t part = mx4_rows_part_bytes(nprob, rows, O, I, quantize_input);
   return part + (quantize_input ? nprob * (mx4_codes_bytes(rows, I) + mx4_scales_bytes(rows, I)) : 0);
 }
 

@@ -1,4 +1,4 @@
-// MXFP4 weights times 16-bit rows, more than 16 of them: y = epilogue(x W^T + bias),
+// MXFP4 weights times many 16-bit rows: y = epilogue(x W^T + bias),
 // fp16 / bf16 x.
 //
 // The tile of mx4_gemm.h with eight waves (two a SIMD, so that one's conversions and

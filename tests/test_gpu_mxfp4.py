@@ -86,9 +86,9 @@ SHAPES = [(1, 32, 1), (1, 64, 17), (2, 96, 40), (16, 128, 16), (17, 160, 33), (1
           (257, 1024, 520), (300, 96, 70), (520, 768, 264),
           (2, 8704, 30), (9, 16384, 40), (16, 8224, 24),
           (4, 8192, 40), (2, 7680, 24), (700, 608, 1100),
-          (256, 2080, 40), (100, 9248, 30), (128, 768, 200), (250, 32, 9),
-          (257, 32, 1), (258, 160, 33), (270, 288, 130), (300, 640, 257), (290, 1056, 65), (321, 2080, 300),
-          (260, 8224, 24), (300, 16384, 40)]
+          (256, 2080, 40), (100, 9248, 30), (128, 768, 200), (250, 32, 9), (400, 544, 70),
+          (513, 32, 1), (514, 160, 33), (520, 288, 130), (530, 640, 257), (600, 1056, 65), (521, 2080, 300),
+          (516, 8224, 24), (515, 16384, 40)]
 
 
 def _case(rows, n, m, dt, seed, *, lo=112, hi=122):
@@ -139,7 +139,27 @@ def test_linear_of_a_prefill_batch(dtype, epilogue):
         assert ((got[rs].cpu().double() - want).abs() <= bound).all()
 
 
-@pytest.mark.parametrize("rows", [1, 24, 90, 400])
+@pytest.mark.parametrize("quantize_input", [False, True])
+@pytest.mark.parametrize("rows,n,m", [(5000, 1056, 1030), (5000, 2080, 2070), (2000, 8224, 1030), (4100, 8224, 1030),
+                                      (1500, 16384, 2050)])
+def test_linear_of_larger_tiles(rows, n, m, quantize_input):
+    """128- and 256-row tiles, whole and split in K, ragged on all sides."""
+    import rwkv7mi as mi
+
+    x, codes, scales, g = _case(rows, n, m, torch.float16, n)
+    bias = torch.randn(m, generator=g).half()
+    got = mi.mxfp4_linear(x.cuda(), codes.cuda(), scales.cuda(), bias=bias.cuda(), epilogue="relu2",
+                          quantize_input=quantize_input).cpu().double()
+    w = ref.values(codes, scales)
+    for r in (0, 120, 250, rows - 20):  # a few rows of several tiles, all columns
+        xr = x[r:r + 20]
+        if quantize_input:
+            xr = ref.values(*[t if i else ref.pack(t) for i, t in enumerate(ref.quantize(xr))]).half()
+        want, bound = ref.product(xr, w, bias, None, "relu2")
+        assert ((got[r:r + 20] - want).abs() <= bound).all(), r
+
+
+@pytest.mark.parametrize("rows", [1, 24, 90, 400, 600])
 def test_linear_fp16_scales_far_apart(rows):
     """fp16 rows with block scales over 2^-100..2^-7: a row's largest scale is brought to
     2^13, where fp16's grid is 2^-24: smaller weights are off by at most half a step,
@@ -162,7 +182,7 @@ def test_linear_fp16_scales_far_apart(rows):
 
 
 @pytest.mark.parametrize("quantize_input", [False, True])
-@pytest.mark.parametrize("rows", [1, 20, 70, 300])
+@pytest.mark.parametrize("rows", [1, 20, 70, 300, 600])
 def test_linear_nan_scale_stays_in_its_output(rows, quantize_input):
     import rwkv7mi as mi
 
@@ -176,7 +196,7 @@ def test_linear_nan_scale_stays_in_its_output(rows, quantize_input):
 
 
 @pytest.mark.parametrize("quantize_input", [False, True])
-@pytest.mark.parametrize("rows", [3, 70, 300])
+@pytest.mark.parametrize("rows", [3, 70, 300, 600])
 def test_linear_bad_rows_stay_in_their_rows(rows, quantize_input):
     import rwkv7mi as mi
 
@@ -235,7 +255,7 @@ def test_linear_strides_ranks_and_out():
 
 
 @pytest.mark.parametrize("quantize_input", [False, True])
-@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("rows", [1, 40, 300, 600])
 def test_linear_in_a_graph_and_on_another_stream(rows, quantize_input):
     import rwkv7mi as mi
 
