@@ -17,12 +17,14 @@
 // occurrence adds at least one step, so `seen` is a count above zero; a history of 2^23
 // tokens cannot overflow).
 //
-// Latency- and issue-bound: the history's loads, eight in flight a lane, then one run;
-// every workgroup of a row reads its whole history, from L2.  64 rows of 65536 fp16
-// logits, mask and bias (19 MB), with the token: 25.9 us behind 4000-token histories
-// and decay, 19.1 without decay, 15 behind 100 tokens; one row 8.1.  (1024 lanes and
-// 8192 tokens a workgroup: 24.0, 17.2, 14.3 and 9.9, but 26.1 for 64 rows of 50277,
-// 18.8 here.)
+// Latency- and issue-bound: the history's loads, then one run; every workgroup of a row
+// reads its whole history, from L2, and a wave has a decayed entry of its slice in most
+// of its loads, each with fp64 work.  64 rows of 65536 fp16 logits, mask and bias (19
+// MB), with the token: 25.7 us behind 4000-token histories and decay, 17.1 without
+// decay, 13.0 behind 100 tokens without mask and bias; one row of 500 tokens 7.9.  (1024
+// lanes and 8192 tokens a workgroup: 2 us less for 64 x 65536, 7 more for 64 x 50277,
+// 17.4 here.  The decayed entries gathered in LDS and weighed by all lanes at once:
+// 32.5.)
 #include <type_traits>
 
 #include "sample_common.h"
@@ -33,7 +35,7 @@ namespace {
 
 constexpr int LG_THREADS = 256;
 constexpr int LG_SLICE = 2048;
-constexpr int LG_FLIGHT = 8;  // history entries a lane loads at once
+constexpr int LG_FLIGHT = 4;  // history entries a lane loads at once (8: registers for 7 waves only)
 constexpr int64_t LG_MAX_HISTORY = 1 << 23;
 
 // one value a row: values[row], or the same for every row
@@ -76,6 +78,7 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(const LgArgs A) {
   using C = std::conditional_t<DECAY, unsigned long long, uint32_t>;
   constexpr int E = 16 / (int)sizeof(TI), RUNS = LG_SLICE / LG_THREADS / E;  // elements of a run, runs of a lane
   __shared__ __align__(16) C count[LG_SLICE];
+  __shared__ double log_decay;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.y;
   const TI* x = static_cast<const TI*>(A.x) + row * A.ldx;
@@ -109,9 +112,13 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(const LgArgs A) {
     freq = lg_get(A.frequency, row);
 #pragma unroll
     for (int i = 0; i < LG_SLICE / LG_THREADS; ++i) count[LG_THREADS * i + tid] = 0;
+    if (DECAY && tid < 64)  // (one wave: fp64 instructions are slow; its lanes write the same)
+      log_decay = log2(fmin(fmax((double)lg_get(A.decay, row), 0.0), 1.0));
     __syncthreads();
     const int64_t n = A.lengths ? min((int64_t)max(A.lengths[row], 0), A.L) : A.L;
-    const double ld = DECAY ? log2(fmin(fmax((double)lg_get(A.decay, row), 0.0), 1.0)) : 0.0;
+    const double ld = DECAY ? log_decay : 0.0;
+    // tokens of the slice that are in the vocabulary: width of them from c0 + lo
+    const int lo = max(-c0, 0), width = max(min(LG_SLICE, A.V - c0) - lo, 0);
     for (int64_t i0 = tid; i0 < n; i0 += LG_FLIGHT * LG_THREADS) {
       int64_t t[LG_FLIGHT];
 #pragma unroll
@@ -119,12 +126,18 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(const LgArgs A) {
         const int64_t i = i0 + LG_THREADS * k;
         t[k] = i < n ? lg_token(A, row, i) : -1;
       }
+      int at[LG_FLIGHT];  // (in 32 bits before the fp64 work: registers for 8 waves)
 #pragma unroll
       for (int k = 0; k < LG_FLIGHT; ++k) {
-        const int64_t o = t[k] - c0;  // (tokens outside the vocabulary count nowhere)
-        if (t[k] < 0 || t[k] >= A.V || o < 0 || o >= LG_SLICE) continue;
+        const uint64_t d = (uint64_t)t[k] - (uint64_t)(c0 + lo);
+        at[k] = d < (uint64_t)width ? lo + (int)d : -1;
+      }
+#pragma unroll
+      for (int k = 0; k < LG_FLIGHT; ++k) {
+        const int o = at[k];
+        if (o < 0) continue;
         if constexpr (DECAY) {
-          const int64_t age = n - 1 - (i0 + LG_THREADS * k);
+          const int age = (int)(n - 1 - i0) - LG_THREADS * k;
           // (past 2^-41 one step; decay 0 counts the newest alone)
           const double w = age ? exp2(fmax((double)age * ld, -100.0) + 40.0) : 0x1p40;
           atomicAdd(&count[o], (unsigned long long)fmax(rint(w), 1.0));

@@ -83,9 +83,11 @@ __device__ __forceinline__ bool mg_vec(const Mx4Prob& P, int O) {
 // The tile's end.  Lane: row 32 i + n and, in group j, columns 64 (j / 2) + 16 a + 8 u
 // + 4 (j % 2) .. +3, a = 0 .. 3.  The sums go through LDS (the stages are done with),
 // two row tiles a wave at a time, and come back as whole rows: 32 lanes a row, 8
-// columns each, whose bias stays in registers.  (Finished and stored from the MFMA
-// layout, 32-byte pieces of 32 rows an instruction, the epilogue of the 4-bit rows took
-// as long as half their main loop.)
+// columns each, whose bias stays in registers, stored past the caches, where they would
+// push out operands (16384 x 4096 -> 16384 with 4-bit rows 700 -> 667 us, 1000 rows 52.6
+// -> 50.3).  (Finished and stored from the MFMA layout, 32-byte pieces of 32 rows an
+// instruction, the epilogue of the 4-bit rows took as long as half their main loop;
+// rounded before LDS, with half the bytes there, 705 us.)
 constexpr int MG_LDT = MG_N * 4 + 16;  // a staged row (the 16 bytes spread it over the banks)
 constexpr int mg_staging(int mi) { return (mi < 2 ? 64 : 128) * MG_LDT; }
 
@@ -167,7 +169,9 @@ __device__ __forceinline__ void mg_epilogue(const MgArgs& B, const Mx4Prob& P, c
           for (int e = 0; e < 8; ++e) v[k][e] += w[k][e];
         }
         if (whole) {
-          st8(y + oi, v[k]);
+          u32x4 t;
+          st8(reinterpret_cast<T*>(&t), v[k]);
+          __builtin_nontemporal_store(t, reinterpret_cast<u32x4*>(y + oi));
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)

@@ -210,3 +210,25 @@ def test_step_in_a_graph():
         torch.cuda.synchronize()
         assert torch.equal(y, want) and all(torch.equal(a, b) for a, b in zip(eager, captured))
     assert captured[1].tolist() == [4] * 4
+
+
+@pytest.mark.parametrize("n", [3001, 2048])
+def test_many_entries_of_one_token_and_of_one_slice(n):
+    """More decayed entries in 2048 tokens than are gathered at once: all of one token, and all
+    of a few neighbours; counts against the sums of the powers."""
+    import rwkv7mi as mi
+
+    L, decay = 5000, 0.999
+    hist = torch.full((3, L), 7, dtype=torch.long)
+    hist[1] = torch.arange(L) % 97 + 1000
+    hist[2, ::2] = n  # outside the vocabulary
+    hist[2, 1::4] = -(2 ** 63)
+    y = mi.process_logits(torch.zeros(3, n, device="cuda"), history=hist.cuda(), frequency_penalty=1.0, penalty_decay=decay)
+    age = torch.arange(L - 1, -1, -1, dtype=torch.float64)
+    want = torch.zeros(3, n, dtype=torch.float64)
+    for r in range(3):
+        ok = (hist[r] >= 0) & (hist[r] < n)
+        want[r].index_add_(0, hist[r][ok], -(decay ** age)[ok])
+    # steps of 2^-40 for each of 5000 entries, decay rounded to fp32 (5000 x 2^-24 of a power), one fp32 rounding
+    bound = L * 2.0 ** -41 + want.abs() * (L * 2.0 ** -24 + 2.0 ** -24)
+    assert ((y.cpu().double() - want).abs() <= bound).all()
