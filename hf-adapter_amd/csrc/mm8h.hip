@@ -812,7 +812,7 @@ namespace rwkv7mi {
 
 // ---- MXFP4 weights: the same records, then the same GEMM.  fp16 rows are scaled
 // relative to their largest scale and the sums by its factor per column
-// (mx4_common.h).  16384 x 4096 -> 16384: 1.64 ms, 1.34 PFLOP/s, 17 us of it the records.
+// (mx4_common.h).  16384 x 4096 -> 16384: 1.64 ms, 1.34 PFLOP/s, 40 us of it the records (170 MB).
 struct Mx4hBatch {
   const uint8_t *codes[MX4_MAXPROB], *scales[MX4_MAXPROB];
   void* out[MX4_MAXPROB];
