@@ -154,7 +154,8 @@ static int mx4_shape(const char* who, int64_t rows, int64_t I) {
   const std::string w(who);
   if (rows < 0 || I <= 0) return fail(RWKV7MI_EINVAL, w + ": bad shape");
   if (I % MX4_BLOCK) return fail(RWKV7MI_EINVAL, w + ": the row length must be a multiple of 32");
-  if (I > INT32_MAX || (rows && rows > ((int64_t)1 << 38) / I)) return fail(RWKV7MI_EINVAL, w + ": too large");
+  // (a launch holds fewer than 2^32 lanes of 8 values)
+  if (I > INT32_MAX || rows > (((int64_t)1 << 35) - 2048) / I) return fail(RWKV7MI_EINVAL, w + ": too large");
   return RWKV7MI_OK;
 }
 

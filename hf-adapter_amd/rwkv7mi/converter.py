@@ -321,11 +321,13 @@ def save_prepacked(model, output, *, source_state: Dict[str, torch.Tensor] | Non
     out.mkdir(parents=True, exist_ok=True)
     cfg = model.config
     packed: Dict[str, torch.Tensor] = {}
-    fmt = MXFP4_FORMAT if mx else PREPACKED_FORMAT
+    # (with no module large enough, the format the config names)
+    four = bool(mx) or (cfg.use_native_mxfp4 and not model._rwkv7_native_mm_replaced_modules)
+    fmt = MXFP4_FORMAT if four else PREPACKED_FORMAT
     manifest = {"format": fmt, "packer_version": _PACKERS[fmt], "modules": []}
     dense = dict(model.dense_state_dict())
     for name, lin in model.named_linears():
-        if not isinstance(lin, BlockFloatLinear if mx else QuantLinear):
+        if not isinstance(lin, BlockFloatLinear if four else QuantLinear):
             continue
         m = lin.m
         for field in _FIELDS[fmt]:
@@ -333,9 +335,9 @@ def save_prepacked(model, output, *, source_state: Dict[str, torch.Tensor] | Non
         entry = {
             "format": fmt, "module": name, "input_features": int(m.in_features),
             "output_features": int(m.out_features), "activation_dtype": str(model.dtype).replace("torch.", ""),
-            "scale_dtype": "uint8" if mx else str(m.mx.dtype).replace("torch.", ""),
+            "scale_dtype": "uint8" if four else str(m.mx.dtype).replace("torch.", ""),
             "epilogue": next((v for k, v in _EPILOGUE.items() if name.endswith(k)), "none"),
-            "blocked_shape": list((m.codes if mx else m.w_blk).shape), "packer_version": _PACKERS[fmt],
+            "blocked_shape": list((m.codes if four else m.w_blk).shape), "packer_version": _PACKERS[fmt],
         }
         if source_state is not None and name + ".weight" in source_state:
             entry["source_weight_sha256"] = _sha256(source_state[name + ".weight"])
@@ -345,10 +347,10 @@ def save_prepacked(model, output, *, source_state: Dict[str, torch.Tensor] | Non
     save_file({k: v.detach().cpu().contiguous() for k, v in dense.items()}, str(out / "model.safetensors"),
               metadata={"format": "pt"})
     cj = _config_json(cfg, str(model.dtype).replace("torch.", ""))
-    if mx:
+    if four:
         cj.update({"use_native_mxfp4": True, "native_mxfp4_policy": cfg.native_mxfp4_policy,
                    "native_mxfp4_min_params": cfg.native_mxfp4_min_params,
-                   "native_mxfp4_quantize_input": mx[0].m.quantize_input})
+                   "native_mxfp4_quantize_input": mx[0].m.quantize_input if mx else cfg.native_mxfp4_quantize_input})
     else:
         cj.update({"use_native_mm8": True, "native_mm8_policy": cfg.native_mm8_policy,
                    "native_mm8_min_params": cfg.native_mm8_min_params})

@@ -932,7 +932,8 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
         reference).  ``prepacked``: module name -> :class:`MM8Linear` or
         :class:`MXFP4Linear` built from a prepacked checkpoint; those modules'
         ``.weight`` entries are not read."""
-        if config.use_native_mxfp4:
+        mxfp4 = bool(getattr(config, "use_native_mxfp4", False))
+        if mxfp4:
             if config.use_native_mm8:
                 raise ValueError("use_native_mm8 and use_native_mxfp4 exclude each other")
             if dtype not in (torch.float16, torch.bfloat16):
@@ -952,7 +953,7 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
                 m = prepacked[name]
                 return BlockFloatLinear(m) if isinstance(m, MXFP4Linear) else QuantLinear(m)
             w = get(name + ".weight")
-            if cfg.use_native_mxfp4 and int(w.shape[1]) % MXFP4_BLOCK == 0 and should_quantize_linear(
+            if mxfp4 and int(w.shape[1]) % MXFP4_BLOCK == 0 and should_quantize_linear(
                     name, int(w.numel()), min_params=cfg.native_mxfp4_min_params, policy=cfg.native_mxfp4_policy):
                 self._replaced += 1
                 return BlockFloatLinear(MXFP4Linear.from_packed(*quantize_mxfp4(w),
@@ -1741,8 +1742,11 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
             use_native_mm8 = getattr(config, "use_native_mm8", None)
         if config is not None and use_native_mxfp4 is None:
             use_native_mxfp4 = getattr(config, "use_native_mxfp4", None)
-            if use_native_mxfp4 and native_mxfp4_quantize_input is None:
-                native_mxfp4_quantize_input = getattr(config, "native_mxfp4_quantize_input", None)
+        if config is not None and use_native_mxfp4:
+            given = lambda value, name: getattr(config, name, None) if value is None else value
+            native_mxfp4_policy = given(native_mxfp4_policy, "native_mxfp4_policy")
+            native_mxfp4_min_params = given(native_mxfp4_min_params, "native_mxfp4_min_params")
+            native_mxfp4_quantize_input = given(native_mxfp4_quantize_input, "native_mxfp4_quantize_input")
         return load_pretrained(path, device=device, dtype=want, use_native_mm8=use_native_mm8,
                                native_mm8_policy=native_mm8_policy, native_mm8_min_params=native_mm8_min_params,
                                use_native_mxfp4=use_native_mxfp4, native_mxfp4_policy=native_mxfp4_policy,

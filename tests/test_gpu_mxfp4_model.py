@@ -295,3 +295,25 @@ def test_grouped_outputs_must_not_overlap():
         mxfp4_linear_multi_into([x, x], [w, w], [o, o])
     with pytest.raises(ValueError, match="another product"):
         mxfp4_linear_multi_into([x, x], [w, w], [o, torch.zeros_like(o)], residuals=[None, o])
+
+
+def test_settings_from_a_config_and_a_model_with_nothing_replaced(tmp_path):
+    from rwkv7mi.converter import save_hf_directory, save_prepacked
+    from rwkv7mi.model import BlockFloatLinear, NativeRWKV7ForCausalLM
+
+    cfg, w, model = _model(native_mxfp4_min_params=10 ** 9)
+    assert model._rwkv7_native_mm_quantization is None
+    plain = tmp_path / "plain"
+    save_hf_directory(plain, cfg, w)
+    head = _cfg(True, native_mxfp4_policy="head")
+    m = NativeRWKV7ForCausalLM.from_pretrained(plain, config=head)
+    assert [n for n, lin in m.named_linears() if isinstance(lin, BlockFloatLinear)] == ["lm_head"]
+    assert m.lm_head.m.quantize_input
+    m = NativeRWKV7ForCausalLM.from_pretrained(plain, use_native_mxfp4=True, native_mxfp4_min_params=0)
+    assert all(isinstance(lin, BlockFloatLinear) for _, lin in m.named_linears())
+    empty = tmp_path / "empty"
+    assert save_prepacked(model, empty)["modules"] == []
+    again = NativeRWKV7ForCausalLM.from_pretrained(empty)
+    assert again.config.use_native_mxfp4 and not again.config.use_native_mm8
+    ids = torch.randint(0, cfg.vocab_size, (1, 5), device="cuda")
+    assert torch.equal(again(ids).logits, model(ids).logits)

@@ -24,7 +24,8 @@ A = 1 << 20  # an aligned address that is never read
 
 @pytest.mark.parametrize("rows,n,ld,dtype,x", [(2, 33, 33, 1, A), (2, 0, 0, 1, A), (-1, 32, 32, 1, A), (2, 32, 16, 1, A),
                                                (2, 32, 32, 7, A), (2, 32, 32, 1, 0), (2, 32, 32, 1, A + 2),
-                                               (2, 32, 36, 1, A), (1 << 40, 1 << 20, 1 << 20, 1, A)])
+                                               (2, 32, 36, 1, A), (1 << 40, 1 << 20, 1 << 20, 1, A),
+                                               (1 << 20, 1 << 15, 1 << 15, 1, A)])
 def test_quantize_entry_refuses(rows, n, ld, dtype, x):
     assert _lib().rwkv7mi_mxfp4_quantize(x, rows, n, ld, dtype, A, A, None) == -1
 
