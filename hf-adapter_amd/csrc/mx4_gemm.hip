@@ -11,7 +11,7 @@
 // consecutive columns (column of group g, lane n: 64 (g / 2) + 8 (n / 4) + 4 (g % 2)
 // + n % 4): 16-byte stores.  K advances 256 inputs a step, four sub-steps of two
 // blocks each:
-//  * codes of x and W: global -> LDS directly, 128 bytes a row, two stages.  Whole
+//  * codes of x and W: global -> LDS directly, 128 bytes a row, two or three stages.  Whole
 //    cache lines: 64-byte pieces straight into the operand registers stalled on
 //    lines still on their way (16384 x 4096 -> 16384, 1.0 ms; without those loads
 //    0.5).  A row's 16-byte chunk c sits at c ^ key, the key from the lane that
@@ -26,8 +26,8 @@
 //    past I counts (W's codes there are some finite value).
 //
 // A sub-step's operands are read during the one before.  So a stage is read to the
-// end in its step's third sub-step: one barrier there, and the loads two steps
-// ahead go into the same stage, with a whole step to land.  Where the tiles do not
+// end in its step's third sub-step: one barrier there, and the loads a ring ahead go
+// into the same stage, with a whole step or two to land.  Where the tiles do not
 // fill the chip K is split over workgroups and a second launch adds the fp32
 // partials.
 //
@@ -49,9 +49,17 @@ __device__ __forceinline__ f32x16 mg_mfma(u32x4 a, u32x4 b, f32x16 c, int sa, in
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mg_operand(a), mg_operand(b), c, 4, 4, H, sa, H, sb);
 }
 
+// Stages of codes: what LDS has room for (two with 64 and 128 rows too: 300 x 2560 ->
+// 10240 22.2 us for 18.1, 200 x 4096 -> 16384 30.4 for 24.8).
+constexpr int mg_stages(int mi) { return mi <= 2 ? 3 : 2; }
+constexpr int mg_lds(int mi) {
+  return std::max(mg_stages(mi) * (64 * mi + MG_N) * 128 + 2 * (64 * mi + MG_N) * 16, mg_staging(mi));
+}
+static_assert(mg_lds(1) <= 163840 && mg_lds(2) <= 163840 && mg_lds(4) <= 163840, "LDS of a CU");
+
 template <int MI, bool SPLIT, typename T>
 __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
-  constexpr int ROWS = 64 * MI, XB = ROWS * 128, STAGE = XB + MG_N * 128;
+  constexpr int ROWS = 64 * MI, XB = ROWS * 128, STAGE = XB + MG_N * 128, NST = mg_stages(MI);
   constexpr int SX = ROWS * 16, SB = SX + MG_N * 16, NX = 2 * MI;  // scale bytes; x loads a wave and step
   const Mx4Prob& P = B.p[blockIdx.y];
   const int M = B.rows, O = B.O, NS = B.NS;
@@ -59,8 +67,8 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
   if (!mg_tile(B, tm, tn)) return;
   const int m0 = tm * ROWS, n0 = tn * MG_N;
 
-  extern __shared__ __align__(16) char smem[];  // two stages (x, W), the scales of two supersteps (x, W)
-  char* const scl = smem + 2 * STAGE;
+  extern __shared__ __align__(16) char smem[];  // the stages (x, W), the scales of two supersteps (x, W)
+  char* const scl = smem + NST * STAGE;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, u = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int S0 = SPLIT ? (int)blockIdx.z * B.sps : 0;
@@ -75,20 +83,20 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
   const __amdgpu_buffer_rsrc_t xsr = make_rsrc(P.xs, (uint32_t)(NS * M * 16));
   const __amdgpu_buffer_rsrc_t wsr = make_rsrc(P.ws, (uint32_t)(NS * O * 16));
 
-  // codes of step s, round v: rows 32 v + 8 w .. +7 of x (W), lane l at row + l / 8,
+  // codes of step s into stage st, round v: rows 32 v + 8 w .. +7 of x (W), lane l at row + l / 8,
   // chunk position l % 8
   const int lr = 8 * wave + (lane >> 3);
-  auto issue_x = [&](int s, int v) {
+  auto issue_x = [&](int s, int st, int v) {
     const int r = 32 * v + lr, vo = r * ldx + 16 * ((lane & 7) ^ mg_key(r));
     const int so = s < nsteps ? 128 * (s0 + s) : (int)BUF_OOB;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (mg_lds_ptr)(smem + (s & 1) * STAGE + (32 * v + 8 * wave) * 128), 16, vo,
-                                             so, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (mg_lds_ptr)(smem + st * STAGE + (32 * v + 8 * wave) * 128), 16, vo, so, 0,
+                                             0);
   };
-  auto issue_w = [&](int s, int v) {
+  auto issue_w = [&](int s, int st, int v) {
     const int r = 32 * v + lr, vo = r * ldw + 16 * ((lane & 7) ^ mg_wkey(r));
     const int so = s < nsteps ? 128 * (s0 + s) : (int)BUF_OOB;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (mg_lds_ptr)(smem + (s & 1) * STAGE + XB + (32 * v + 8 * wave) * 128), 16,
-                                             vo, so, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (mg_lds_ptr)(smem + st * STAGE + XB + (32 * v + 8 * wave) * 128), 16, vo,
+                                             so, 0, 0);
   };
   // scales of superstep s: 64 rows of x (waves past the tile's rows repeat them), 64 columns
   const int xw = wave % MI;
@@ -103,11 +111,11 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
 
   const int wm = 32 * MI * (wave >> 1), wn = 128 * (wave & 1);  // the wave's rows and columns in the tile
   const int wcol = 8 * (n >> 2) + (n & 3), key = mg_key(n);
-  auto ldx_op = [&](int s, int h, int i) {
-    return *reinterpret_cast<const u32x4*>(smem + (s & 1) * STAGE + (wm + 32 * i + n) * 128 + 16 * ((2 * h + u) ^ key));
+  auto ldx_op = [&](int st, int h, int i) {
+    return *reinterpret_cast<const u32x4*>(smem + st * STAGE + (wm + 32 * i + n) * 128 + 16 * ((2 * h + u) ^ key));
   };
-  auto ldw_op = [&](int s, int h, int j) {
-    return *reinterpret_cast<const u32x4*>(smem + (s & 1) * STAGE + XB + (wn + 64 * (j >> 1) + 4 * (j & 1) + wcol) * 128 +
+  auto ldw_op = [&](int st, int h, int j) {
+    return *reinterpret_cast<const u32x4*>(smem + st * STAGE + XB + (wn + 64 * (j >> 1) + 4 * (j & 1) + wcol) * 128 +
                                            16 * ((2 * h + u) ^ key));
   };
   auto ldx_sc = [&](int s, int i) {
@@ -123,13 +131,12 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
   int sx[MI], sw[4], sxn[MI], swn[4];  // scales of this step and the next
 
   // Sub-step H of step s (operand set H & 1): its MFMAs, the reads of the next
-  // sub-step's operands over the first three quarters, and load(l) for l in L0 .. L1 - 1
+  // sub-step's operands (from stage st) over the first three quarters, and load(l) for l in L0 .. L1 - 1
   // spread over them.
   constexpr int LOADS = NX + 8, LCUT = LOADS / 2;  // the loads of a step: before and behind the cut
-  auto substep = [&](auto hc, int s, auto&& load, int L0, int L1) {
+  auto substep = [&](auto hc, int s, int st, auto&& load, int L0, int L1) {
     constexpr int H = decltype(hc)::value, A = H & 1, HN = (H + 1) & 3;
     constexpr int TILES = MI * 4, READS = MI + 4, Q = TILES * 3 / 4;
-    const int sn = H == 3 ? s + 1 : s;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -140,14 +147,14 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
 #pragma unroll
         for (int r = r0; r < r1; ++r) {  // W's first: every MFMA of the first row tile takes one
           if (r < 4)
-            wa[A ^ 1][r] = ldw_op(sn, HN, r);
+            wa[A ^ 1][r] = ldw_op(st, HN, r);
           else
-            xa[A ^ 1][r - 4] = ldx_op(sn, HN, r - 4);
+            xa[A ^ 1][r - 4] = ldx_op(st, HN, r - 4);
           if (H == 3) {
             if (r < 4)
-              swn[r] = ldw_sc(sn, r);
+              swn[r] = ldw_sc(s + 1, r);
             else
-              sxn[r - 4] = ldx_sc(sn, r - 4);
+              sxn[r - 4] = ldx_sc(s + 1, r - 4);
           }
         }
 #pragma unroll
@@ -155,26 +162,26 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
         __builtin_amdgcn_sched_barrier(0);
       }
   };
-  auto loads = [&](int s) {
-    return [&, s](int l) {
+  auto loads = [&](int s, int st) {
+    return [&, s, st](int l) {
       if (l < NX)
-        issue_x(s, l);
+        issue_x(s, st, l);
       else
-        issue_w(s, l - NX);
+        issue_w(s, st, l - NX);
     };
   };
-  // every wave's operand reads and loads so far have landed, for all to see
-  auto meet = [&]() {
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+  // every wave's operand reads, and all its loads but the newest NL, have landed, for all to see
+  auto meet = [&](auto nl) {
+    constexpr int NL = decltype(nl)::value;
+    __builtin_amdgcn_s_waitcnt(0x0070 | (NL & 15) | (NL >> 4) << 14);  // vmcnt(NL), lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
   issue_s(0);
 #pragma unroll
-  for (int l = 0; l < LOADS; ++l) loads(0)(l);
-#pragma unroll
-  for (int l = 0; l < LCUT; ++l) loads(1)(l);  // (step 0 issues the rest)
-  meet();
+  for (int l = 0; l < (NST - 1) * LOADS + LCUT; ++l)  // (step 0 issues the rest)
+    loads(l / LOADS, l / LOADS)(l % LOADS);
+  meet(std::integral_constant<int, (NST - 2) * LOADS + LCUT>{});
 #pragma unroll
   for (int j = 0; j < 4; ++j) wa[0][j] = ldw_op(0, 0, j), sw[j] = ldw_sc(0, j);
 #pragma unroll
@@ -189,13 +196,18 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
       asm volatile("" : "+a"(acc[i][j]));
     }
+  int st = 0;  // the stage of step s
   for (int s = 0; s < nsteps; ++s) {
-    substep(std::integral_constant<int, 0>{}, s, loads(s + 1), LCUT, LOADS);
-    substep(std::integral_constant<int, 1>{}, s, loads(s), 0, 0);
-    substep(std::integral_constant<int, 2>{}, s, loads(s), 0, 0);
-    meet();  // stage s read to its end, step s + 1 (and its scales) there
+    const int sn = st == NST - 1 ? 0 : st + 1, sp = st == 0 ? NST - 1 : st - 1;
+    substep(std::integral_constant<int, 0>{}, s, st, loads(s + NST - 1, sp), LCUT, LOADS);
+    substep(std::integral_constant<int, 1>{}, s, st, loads(s, st), 0, 0);
+    substep(std::integral_constant<int, 2>{}, s, st, loads(s, st), 0, 0);
+    // step s read to its end, step s + 1 (and its scales) there: of the loads NST - 2
+    // steps further none is waited for
+    meet(std::integral_constant<int, (NST - 2) * LOADS>{});
     if ((s & 1) == 0) issue_s((s >> 1) + 1);
-    substep(std::integral_constant<int, 3>{}, s, loads(s + 2), 0, LCUT);
+    substep(std::integral_constant<int, 3>{}, s, sn, loads(s + NST, st), 0, LCUT);
+    st = sn;
 #pragma unroll
     for (int i = 0; i < MI; ++i) sx[i] = sxn[i];
 #pragma unroll
@@ -227,7 +239,7 @@ int64_t mx4_gemm_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I) 
 
 template <int MI, typename T>
 static int mg_go(const MgArgs& a, int nprob, void* stream) {
-  constexpr int lds = std::max(2 * (64 * MI + MG_N) * (128 + 16), mg_staging(MI));
+  constexpr int lds = mg_lds(MI);
   static std::atomic<uint64_t> raised[2];
   auto launch = [&](auto kern, std::atomic<uint64_t>& done) {
     if (int rc = raise_dynamic_lds(reinterpret_cast<const void*>(kern), lds, done, "mx4_gemm_kernel")) return rc;
