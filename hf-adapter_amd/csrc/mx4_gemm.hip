@@ -218,11 +218,11 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
   mg_epilogue<MI, 2, SPLIT, T>(B, P, smem, acc, m0, n0);
 }
 
-// Fitted to 20 shapes from 17 x 2048 -> 2048 to 7000 x 2048 -> 2048, every tile height
-// and split timed, e.g. 1000 x 4096 -> 4096: 64 rows a tile 27.7 us, 128 rows 30.3, 256
-// rows 38.2; 4000 rows: 83, 63, 54; 1000 x 16384 -> 4096: 128 rows in two splits 71,
-// unsplit 92.
-static const MgCost MX4_GEMM_COST = {{1.0, 4.0, 8.0}, {0.0, 0.0, 6.0}, {2.1, 2.5, 2.8}, {0.3, 0.3, 0.7}};
+// Fitted to 18 shapes from 200 x 4096 -> 16384 to 7000 x 2048 -> 2048, every tile height
+// and split timed, e.g. 1000 x 4096 -> 4096: 64 rows a tile 24.3 us, 128 rows 28.7, 256
+// rows in two splits 38.2; 4000 rows: 78.5, 60.5, 54.9; 1500 x 16384 -> 2048: 128 rows
+// in two splits 60.0, unsplit 71.0, 64 rows unsplit 61.8.
+static const MgCost MX4_GEMM_COST = {{0.4, 3.4, 6.8}, {1.6, 0.0, 0.0}, {1.6, 1.8, 2.2}, {0.0, 0.4, 1.4}};
 static MgPlan mx4_gemm_plan(int nprob, int64_t rows, int64_t O, int64_t I) {
   return mg_plan(MX4_GEMM_COST, nprob, rows, O, (I + 511) / 512);
 }

@@ -141,7 +141,7 @@ def test_linear_of_a_prefill_batch(dtype, epilogue):
 
 @pytest.mark.parametrize("quantize_input", [False, True])
 @pytest.mark.parametrize("rows,n,m", [(5000, 1056, 1030), (5000, 2080, 2070), (2000, 8224, 1030), (4100, 8224, 1030),
-                                      (1500, 16384, 2050)])
+                                      (1500, 16384, 2050), (2451, 13792, 1618)])
 def test_linear_of_larger_tiles(rows, n, m, quantize_input):
     """128- and 256-row tiles, whole and split in K, ragged on all sides."""
     import rwkv7mi as mi
