@@ -51,6 +51,10 @@ __device__ __forceinline__ uint32_t mx4_factor_emax(float f) {  // emax again
   return f != f ? 255u : (uint32_t)(ilogbf(f) + 140);
 }
 
+__device__ __forceinline__ uint32_t mx4_max4(uint32_t v) {  // the largest byte
+  return max(max(v & 255u, (v >> 8) & 255u), max((v >> 16) & 255u, v >> 24));
+}
+
 // 8 codes of a dword -> 8 values times the scale, in order
 __device__ __forceinline__ void mx4_decode8(uint32_t d, float s, bf16x8& o) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 0);

@@ -16,7 +16,6 @@ typedef __attribute__((address_space(3))) void* mg_lds_ptr;
 
 struct MgArgs {
   Mx4Prob p[MX4_MAXPROB];  // (ws: the scales in the products' order [superstep][column][16])
-  const float* cs[MX4_MAXPROB];  // a factor per column, before the bias (null: none)
   int rows, O, I, NS;      // NS supersteps of 512 inputs
   int mt, nt, gm, gn;      // row / column tiles, XCD tile group
   int S, sps;              // K splits, supersteps of each
@@ -91,9 +90,10 @@ __device__ __forceinline__ bool mg_vec(const Mx4Prob& P, int O) {
 constexpr int MG_LDT = MG_N * 4 + 16;  // a staged row (the 16 bytes spread it over the banks)
 constexpr int mg_staging(int mi) { return (mi < 2 ? 64 : 128) * MG_LDT; }
 
+// cs: a factor per column of the tile, before the bias (in LDS; null: none).
 template <int MI, int WC, bool SPLIT, typename T>
 __device__ __forceinline__ void mg_epilogue(const MgArgs& B, const Mx4Prob& P, char* smem, const f32x16 (&acc)[MI][8 / WC],
-                                            int m0, int n0) {
+                                            int m0, int n0, const float* cs) {
   constexpr int W = 2 * WC, RT = MI < 2 ? 1 : 2;  // waves; row tiles a wave and pass
   const int O = B.O, M = B.rows, nrow = min(64 * MI, M - m0);
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, u = lane >> 5;
@@ -102,7 +102,6 @@ __device__ __forceinline__ void mg_epilogue(const MgArgs& B, const Mx4Prob& P, c
   const int epi = P.epilogue;
   const T *bias = static_cast<const T*>(P.bias), *res = static_cast<const T*>(P.residual);
   T* y = static_cast<T*>(P.y);
-  const float* cs = SPLIT ? nullptr : B.cs[blockIdx.y];
   float* part = SPLIT ? B.part + ((int64_t)blockIdx.y * B.S + blockIdx.z) * M * B.ldp : nullptr;
   const int cl = 8 * (lane & 31), c0 = n0 + cl;
   const bool whole = vec && c0 + 8 <= O;
@@ -110,7 +109,7 @@ __device__ __forceinline__ void mg_epilogue(const MgArgs& B, const Mx4Prob& P, c
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     bo[e] = !SPLIT && bias && c0 + e < O ? to_f32(bias[c0 + e]) : 0.f;
-    co[e] = cs && c0 + e < O ? cs[c0 + e] : 1.f;
+    co[e] = cs ? cs[cl + e] : 1.f;
   }
 #pragma unroll
   for (int p = 0; p < MI / RT; ++p) {
@@ -156,6 +155,8 @@ __device__ __forceinline__ void mg_epilogue(const MgArgs& B, const Mx4Prob& P, c
         if (r[k] >= nrow) continue;
         const int64_t row = m0 + r[k], oi = row * O + c0;
         if constexpr (SPLIT) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[k][e] *= co[e];
           st8(part + row * B.ldp + c0, v[k]);
           continue;
         }
@@ -201,10 +202,6 @@ __global__ __launch_bounds__(256) void mg_reduce_kernel(const MgArgs B) {
     ld8(p + z * zs, a);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += a[e];
-  }
-  if (const float* cs = B.cs[blockIdx.y]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= c0 + e < B.O ? cs[c0 + e] : 1.f;
   }
   const bool vec = mg_vec(P, B.O);
   mg_finish8<T>(P, row, c0, B.O, vec, v);
@@ -263,7 +260,7 @@ static inline int64_t mg_part_bytes(const MgPlan& p, int nprob, int64_t rows, in
   return p.S > 1 ? mg_up256((int64_t)nprob * p.S * rows * ((O + 7) / 8 * 8) * 4) : 0;
 }
 
-// the launch's sizes (p and cs are the caller's)
+// the launch's sizes (p is the caller's)
 static inline void mg_sizes(MgArgs& a, const Mx4Batch& b, const MgPlan& pl) {
   a.rows = b.rows;
   a.O = b.O;

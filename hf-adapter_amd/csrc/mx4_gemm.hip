@@ -31,7 +31,7 @@
 // fill the chip K is split over workgroups and a second launch adds the fp32
 // partials.
 //
-// 16384 x 4096 -> 16384: 667 us with the quantiser, 3.3 PFLOP/s.  The main loop alone
+// 16384 x 4096 -> 16384: 642 to 685 us with the quantiser, 3.3 PFLOP/s.  The main loop alone
 // takes 500: random codes at 4.8 PFLOP/s draw the card's power limit (7.4 with constant
 // ones), and then all CUs write their tiles, 537 MB, at about the same time.
 #include "mx4_gemm.h"
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(const MgArgs B) {
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the trailing loads have landed before the waves exit
 
-  mg_epilogue<MI, 2, SPLIT, T>(B, P, smem, acc, m0, n0);
+  mg_epilogue<MI, 2, SPLIT, T>(B, P, smem, acc, m0, n0, nullptr);
 }
 
 // Fitted to 18 shapes from 200 x 4096 -> 16384 to 7000 x 2048 -> 2048, every tile height

@@ -39,10 +39,6 @@ __device__ __forceinline__ i32x8 mx4_operand(u32x4 v) {
   return (i32x8){(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
 }
 
-__device__ __forceinline__ uint32_t max4(uint32_t v) {
-  return max(max(v & 255u, (v >> 8) & 255u), max((v >> 16) & 255u, v >> 24));
-}
-
 // The scale bytes of a row's unit (16 blocks from b), a dword a step, block q of it
 // in byte q; blocks past the row read 0.  SC: 2 where I % 512 == 0 (16 aligned
 // bytes), 1 where I % 128 == 0 (aligned dwords), else bytes.
@@ -172,7 +168,7 @@ __global__ __launch_bounds__(RT > 1 ? 512 : 1024) void mx4_rows_kernel(const Mx4
           acc[0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(a[0][s][0]), mx4_operand(w[s]), acc[0], 4, 4,
                                                                     0, (int)((ea[s] >> (8 * q)) & 255u), 0, (int)eb);
         } else {
-          const uint32_t emax = F16 ? max4(ew) : 0u;
+          const uint32_t emax = F16 ? mx4_max4(ew) : 0u;
           const float sc = F16 ? mx4_relative(eb, emax) : mx4_scale(eb);
           f32x4 c[RT];
 #pragma unroll
@@ -279,14 +275,14 @@ static int64_t mx4_codes_bytes(int64_t rows, int64_t I) { return (rows * (I / 2)
 static int64_t mx4_scales_bytes(int64_t rows, int64_t I) { return (rows * (I / MX4_BLOCK) + 255) & ~(int64_t)255; }
 
 // Which kernel takes a product.  The few-row kernel: up to 16 rows, and more while its
-// passes over the weight, one a tile of 32 rows (16 in MXFP4), cost less than the other
-// kernels' pre-pass and split sums.  16-bit rows on it and on the larger tiles: 64 x 4096
-// -> 4096 11.2 and 22.7 us, 128 x 768 -> 768 5.5 and 14.2, 256 x 4096 -> 4096 24.9 and
-// 29.9, 96 x 4096 -> 16384 42.0 and 43.0, 128 rows 49.0 and 46.7, 512 x 4096 -> 4096 44.4
-// and 40.3; 32 rows at any size, 32 x 4096 -> 65536 52 and 74; past 512 rows its passes
-// over x count too, 1000 x 1024 -> 4096 27.5 and 20.3.  MXFP4 rows: 128 x 4096 -> 4096
-// 16.6 and 19.7, 64 x 4096 -> 16384 26.0 and 26.0.  And what the others' offsets
-// cannot hold.  Else the 64- to 256-row tiles.  16-bit rows from 1024
+// passes over the weight, one a tile of 32 rows (16 in MXFP4), cost less than the larger
+// tiles' start and split sums.  16-bit rows on it and on the larger tiles: 128 x 4096 ->
+// 4096 16.5 and 23.4 us, 40 x 8192 -> 2048 13.1 and 19.5, 64 x 4096 -> 16384 28.7 and
+// 29.8, 256 x 4096 -> 4096 25.6 and 26.7, 96 x 4096 -> 16384 41.5 and 36.2, 128 x 16384
+// -> 4096 51.7 and 40.0; 32 rows at any size, 32 x 4096 -> 65536 52.5 and 57.3; past 512
+// rows its passes over x count too, 1000 x 1024 -> 4096 27.5 and 20.3.  MXFP4 rows: 128 x
+// 4096 -> 4096 16.6 and 19.7, 64 x 4096 -> 16384 26.0 and 26.0.  And what the others'
+// offsets cannot hold.  Else the 64- to 256-row tiles.  16-bit rows from 1024
 // tiles of 256 x 256 on write the weight out in 16 bits and run the GEMM of mm8h.hip:
 // without conversions between its MFMAs it holds a higher clock over such long calls
 // (16384 x 4096 -> 16384 1636 us, on the tiles 2000), and the pass over the weight
@@ -294,7 +290,7 @@ static int64_t mx4_scales_bytes(int64_t rows, int64_t I) { return (rows * (I / M
 enum Mx4Route { MX4_ROWS, MX4_TILE, MX4_GEMM, MX4_PREFILL };
 static Mx4Route mx4_route(int64_t rows, int64_t I, int64_t O, int quantize_input) {
   const bool few = quantize_input ? rows <= 256 && (rows + 15) / 16 * (O * I) <= 1 << 27
-                                  : rows <= 32 || (rows <= 512 && (rows + 31) / 32 * (O * I) <= 3 << 26);
+                                  : rows <= 32 || (rows <= 512 && (rows + 31) / 32 * (O * I) <= 1 << 27);
   if (rows <= 16 || few) return MX4_ROWS;
   if (quantize_input) return mx4_gemm_supported(rows, O, I) ? MX4_GEMM : MX4_ROWS;
   if ((rows + 255) / 256 * ((O + 255) / 256) >= 1024 && mx4h_supported(rows, I, O)) return MX4_PREFILL;

@@ -12,10 +12,12 @@
 //    reads 16 bytes a step, one dword a sub-step, which four conversions turn into its
 //    operand during the sub-step before (a ring of 64-byte stages, 16384 x 4096 ->
 //    16384: 2.04 ms);
-//  * W's scales: 8 steps (a superstep) at a time, global -> LDS, 16 bytes a column in
-//    the order [u][step], written by a pre-pass.  fp16 columns are scaled relative to
-//    their largest scale (mx4_common.h), which the pre-pass finds, and the sums by its
-//    factor.
+//  * W's scales: 8 steps (a superstep) at a time, global -> LDS, 16 bytes a column; for
+//    rows of scales that are not whole dwords (I % 128) from a copy that a pre-pass lays
+//    out.  fp16 columns are scaled relative to the largest scale of the workgroup's part
+//    of them (mx4_common.h), which it reads first, while the ring fills, and the sums by
+//    its factor (with the pre-pass at all sizes: 64 x 4096 -> 65536 76 us for 59, 1000 x
+//    4096 -> 16384 122.6 for 121.0, 4000 x 4096 -> 4096 116 for 120).
 // A stage of x is read to the end in its step's third sub-step: one barrier there, and
 // the loads a ring ahead go into the same stage; the barrier waits for the loads of the
 // next step only, by count (with two stages every load had to land within a step: 64 x
@@ -23,7 +25,7 @@
 // some finite value).  Where the tiles do not fill the chip K is split over workgroups
 // and a second launch adds the partials.
 //
-// Bound by the MFMAs and the conversions beside them: 1000 x 4096 -> 16384 114 us, 1.18
+// Bound by the MFMAs and the conversions beside them: 1000 x 4096 -> 16384 112 us, 1.20
 // PFLOP/s, as much as a large library product of 16-bit operands reaches.
 #include "mx4_gemm.h"
 
@@ -41,11 +43,18 @@ constexpr int MT_WC = 4, MT_WAVES = 2 * MT_WC;
 constexpr int mt_xstages(int mi) { return mi <= 2 ? 5 : 2; }
 constexpr int mt_lds(int mi) {
   return std::max(mt_xstages(mi) * 64 * mi * 128 + 2 * MG_N * (128 + 16), mg_staging(mi));
-}
-static_assert(mt_lds(1) <= 163840 && mt_lds(2) <= 163840 && mt_lds(4) <= 163840, "LDS of a CU");
+}  // (then the columns' factors)
+struct MtArgs {
+  MgArgs g;
+  int laid;  // p.ws: the pre-pass's copy, [superstep][column][16]
+};
+static_assert(mt_lds(1) + 4 * MG_N <= 163840 && mt_lds(2) + 4 * MG_N <= 163840 && mt_lds(4) + 4 * MG_N <= 163840,
+              "LDS of a CU");
 
 template <int MI, bool SPLIT, typename T>
-__global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MgArgs B) {
+__global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MtArgs A) {
+  const MgArgs& B = A.g;
+  constexpr bool F16 = std::is_same<T, __half>::value;
   using V = typename Mx4Types<T>::V;
   constexpr int ROWS = 64 * MI, XB = ROWS * 128, WB = MG_N * 128, SB = MG_N * 16;  // bytes of a stage of x, W, scales
   constexpr int NXS = mt_xstages(MI);
@@ -60,6 +69,7 @@ __global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MgArgs
   extern __shared__ __align__(16) char smem[];  // the stages of x, W and (two) the scales
   char* const wst = smem + NXS * XB;
   char* const scl = wst + 2 * WB;
+  float* const factor = reinterpret_cast<float*>(smem + mt_lds(MI));
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, u = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int S0 = SPLIT ? (int)blockIdx.z * B.sps : 0;
@@ -71,7 +81,9 @@ __global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MgArgs
   const int ldx = 2 * I, ldw = I / 2;
   const __amdgpu_buffer_rsrc_t xr = make_rsrc(static_cast<const char*>(P.x) + (int64_t)m0 * ldx, (uint32_t)(nrow * ldx));
   const __amdgpu_buffer_rsrc_t wr = make_rsrc(P.wc + (int64_t)n0 * ldw, (uint32_t)(ncol * ldw));
-  const __amdgpu_buffer_rsrc_t wsr = make_rsrc(P.ws, (uint32_t)(NS * O * 16));
+  const int nb = I / MX4_BLOCK;
+  const uint8_t* const ws = A.laid ? P.ws : P.ws + (int64_t)n0 * nb;
+  const __amdgpu_buffer_rsrc_t wsr = make_rsrc(ws, (uint32_t)(A.laid ? NS * O * 16 : ncol * nb));
 
   // round v of a stage: rows RND v + 8 w .. +7 of x (W), lane l at row + l / 8, chunk
   // position l % 8
@@ -88,10 +100,11 @@ __global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MgArgs
     __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (mg_lds_ptr)(wst + (f & 1) * WB + (RND * v + 8 * wave) * 128), 16, vo, so, 0,
                                              0);
   };
-  const int cw = wave % 4;
-  auto issue_s = [&](int s) {  // scales of superstep s: 64 columns a wave (twice)
-    const int so = s < S1 - S0 ? 16 * ((S0 + s) * O + n0 + 64 * cw) : (int)BUF_OOB;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(wsr, (mg_lds_ptr)(scl + (s & 1) * SB + 64 * cw * 16), 16, 16 * lane, so, 0, 0);
+  auto issue_s = [&](int s) {  // scales of superstep s: 64 columns a wave of the first four
+    if (wave >= MG_N / 64) return;
+    const int at = A.laid ? 16 * ((S0 + s) * O + n0) : 16 * (S0 + s), so = s < S1 - S0 ? at : (int)BUF_OOB;
+    const int vo = (64 * wave + lane) * (A.laid ? 16 : nb);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(wsr, (mg_lds_ptr)(scl + (s & 1) * SB + 64 * wave * 16), 16, vo, so, 0, 0);
   };
 
   const int wm = 32 * MI * (wave / MT_WC), wn = MG_N / MT_WC * (wave % MT_WC);  // the wave's rows and columns in the tile
@@ -103,8 +116,10 @@ __global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MgArgs
   auto ld_w = [&](int s, int j) {  // the lane's block of step s
     return *reinterpret_cast<const u32x4*>(wst + (s >> 2 & 1) * WB + col(j) * 128 + 16 * ((2 * (s & 3) + u) ^ key));
   };
+  uint32_t emax[NJ];  // (of the lane's columns)
   auto ld_s = [&](int s, int j) {  // its scale byte
-    return (uint32_t) * reinterpret_cast<const uint8_t*>(scl + (s >> 3 & 1) * SB + col(j) * 16 + 8 * u + (s & 7));
+    const uint32_t e = *reinterpret_cast<const uint8_t*>(scl + (s >> 3 & 1) * SB + col(j) * 16 + 2 * (s & 7) + u);
+    return F16 ? mx4_relative_byte(e, emax[j]) : e;
   };
 
   f32x16 acc[MI][NJ];
@@ -152,7 +167,34 @@ __global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MgArgs
   for (int s = 0; s < NXS; ++s)
 #pragma unroll
     for (int v = 0; v < NX; ++v) issue_x(s, s, v);
+  if constexpr (F16) {
+    // the largest scale of column tid / 2, every other 8 bytes a thread
+    const int c = tid >> 1, b0 = 16 * S0 + 8 * (tid & 1), be = min(16 * S1, nb);
+    uint32_t m = 0;
+    if (A.laid) {
+      for (int s = S0; s < S1; ++s) {
+        const uint2 d = *reinterpret_cast<const uint2*>(P.ws + 16 * ((int64_t)s * O + min(n0 + c, O - 1)) + 8 * (tid & 1));
+        m = max(m, max(mx4_max4(d.x), mx4_max4(d.y)));
+      }
+    } else {
+      const uint8_t* col = ws + (int64_t)min(c, ncol - 1) * nb;
+#pragma unroll 4
+      for (int s = S0; s < S1; ++s) {  // (past the end the last dword again)
+        const int b = b0 + 16 * (s - S0);
+        const uint32_t d0 = *reinterpret_cast<const uint32_t*>(col + min(b, be - 4));
+        const uint32_t d1 = *reinterpret_cast<const uint32_t*>(col + min(b + 4, be - 4));
+        m = max(m, max(mx4_max4(d0), mx4_max4(d1)));
+      }
+    }
+    m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
+    if (!(tid & 1)) factor[c] = mx4_factor(m);
+    __syncthreads();
+  }
   meet(std::integral_constant<int, 0>{});
+  if constexpr (F16) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) emax[j] = mx4_factor_emax(factor[col(j)]);
+  }
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     wc[j] = ld_w(0, j);
@@ -195,40 +237,26 @@ __global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MgArgs
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the trailing loads have landed before the waves exit
 
-  mg_epilogue<MI, MT_WC, SPLIT, T>(B, P, smem, acc, m0, n0);
+  mg_epilogue<MI, MT_WC, SPLIT, T>(B, P, smem, acc, m0, n0, F16 ? factor : nullptr);
 }
 
-// The pre-pass, a wave a column: its scales [superstep][column][16] in the order
-// [u][step], 1.0 behind its end; for fp16 relative to the largest, and that one's factor.
+// The pre-pass: the scales [superstep][column][16], 0 behind a column's end.  One thread
+// a superstep of a column.
 struct MtScales {
   const uint8_t* in[MX4_MAXPROB];
-  uint32_t* out[MX4_MAXPROB];
-  float* cs[MX4_MAXPROB];
+  u32x4* out[MX4_MAXPROB];
   int O, nb, NS;
 };
-template <bool REL>
 __global__ __launch_bounds__(256) void mx4_tile_scales_kernel(const MtScales S) {
-  const int o = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, p = blockIdx.y;
-  if (o >= S.O) return;
-  const uint8_t* in = S.in[p] + (int64_t)o * S.nb;
-  uint32_t m = 0;
-  if (REL) {
-    for (int i = lane; i < S.nb; i += 64) m = max(m, (uint32_t)in[i]);
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= (int64_t)S.O * S.NS) return;
+  const int o = (int)(t / S.NS), b0 = 16 * (int)(t % S.NS);
+  const uint8_t* in = S.in[blockIdx.y] + (int64_t)o * S.nb;
+  u32x4 v = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int d = 32; d; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 64));
-    if (lane == 0) S.cs[p][o] = mx4_factor(m);
-  }
-  for (int d = lane; d < 4 * S.NS; d += 64) {
-    const int b0 = 16 * (d >> 2) + 8 * (d & 1) + (d >> 1 & 1);
-    uint32_t v = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int b = b0 + 2 * i;
-      const uint32_t e = b < S.nb ? in[b] : 127u;
-      v |= (REL ? mx4_relative_byte(b < S.nb ? e : m, m) : e) << (8 * i);
-    }
-    S.out[p][((int64_t)(d >> 2) * S.O + o) * 4 + (d & 3)] = v;
-  }
+  for (int i = 0; i < 16; ++i)
+    if (b0 + i < S.nb) v[i >> 2] |= (uint32_t)in[b0 + i] << (8 * (i & 3));
+  S.out[blockIdx.y][(int64_t)(b0 >> 4) * S.O + o] = v;
 }
 
 // Fitted to 19 shapes from 17 x 2048 -> 2048 to 7000 x 2048 -> 2048, every tile height and
@@ -239,33 +267,38 @@ static const MgCost MX4_TILE_COST = {{1.0, 4.0, 5.5}, {0.0, 0.0, 3.5}, {4.6, 6.3
 static MgPlan mx4_tile_plan(int nprob, int64_t rows, int64_t O, int64_t I) {
   return mg_plan(MX4_TILE_COST, nprob, rows, O, (I + 511) / 512);
 }
-static int64_t mx4_tile_scales(int64_t O, int64_t I) { return mg_up256(O * 16 * ((I + 511) / 512)); }
+static bool mx4_tile_laid(int64_t I) { return I % (4 * MX4_BLOCK) != 0; }
+static int64_t mx4_tile_scales(int64_t O, int64_t I) {
+  return mx4_tile_laid(I) ? mg_up256(O * 16 * ((I + 511) / 512)) : 0;
+}
 
 bool mx4_tile_supported(int64_t rows, int64_t O, int64_t I) { return mg_supported(rows, O, I); }
 
 int64_t mx4_tile_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I) {
-  return nprob * (mx4_tile_scales(O, I) + mg_up256(4 * O)) +
+  return nprob * mx4_tile_scales(O, I) +
          mg_part_bytes(mx4_tile_plan(nprob, rows, O, I), nprob, rows, O);
 }
 
 template <int MI, typename T>
-static int mt_go(const MgArgs& a, int nprob, void* stream) {
-  constexpr int lds = mt_lds(MI);
+static int mt_go(const MtArgs& a, int nprob, void* stream) {
+  constexpr int lds = mt_lds(MI) + 4 * MG_N;
   static std::atomic<uint64_t> raised[2];
   auto launch = [&](auto kern, std::atomic<uint64_t>& done) {
     if (int rc = raise_dynamic_lds(reinterpret_cast<const void*>(kern), lds, done, "mx4_tile_kernel")) return rc;
-    hipLaunchKernelGGL(kern, mg_grid(a, nprob), dim3(64 * MT_WAVES), lds, as_stream(stream), a);
+    hipLaunchKernelGGL(kern, mg_grid(a.g, nprob), dim3(64 * MT_WAVES), lds, as_stream(stream), a);
     if (int rc = check_launch("mx4_tile_kernel")) return rc;
-    return mg_reduce<T>(a, nprob, stream);
+    return mg_reduce<T>(a.g, nprob, stream);
   };
-  return a.S == 1 ? launch(&mx4_tile_kernel<MI, false, T>, raised[0]) : launch(&mx4_tile_kernel<MI, true, T>, raised[1]);
+  return a.g.S == 1 ? launch(&mx4_tile_kernel<MI, false, T>, raised[0]) : launch(&mx4_tile_kernel<MI, true, T>, raised[1]);
 }
 
 int mx4_tile_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* stream) {
   const MgPlan pl = mx4_tile_plan(nprob, b.rows, b.O, b.I);
   const bool f16 = act_dtype == RWKV7MI_F16;
-  MgArgs a{};
+  MtArgs m{};
+  MgArgs& a = m.g;
   mg_sizes(a, b, pl);
+  m.laid = mx4_tile_laid(b.I);
   MtScales s{};
   s.O = b.O;
   s.nb = b.I / MX4_BLOCK;
@@ -273,25 +306,22 @@ int mx4_tile_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* st
   uint8_t* at = static_cast<uint8_t*>(ws);
   for (int i = 0; i < nprob; ++i) {
     a.p[i] = b.p[i];
+    if (!m.laid) continue;
     s.in[i] = b.p[i].ws;
-    s.out[i] = reinterpret_cast<uint32_t*>(at);
+    s.out[i] = reinterpret_cast<u32x4*>(at);
     a.p[i].ws = at;
     at += mx4_tile_scales(b.O, b.I);
-    s.cs[i] = reinterpret_cast<float*>(at);
-    a.cs[i] = f16 ? s.cs[i] : nullptr;
-    at += mg_up256(4 * (int64_t)b.O);
   }
   a.part = reinterpret_cast<float*>(at);
-  const dim3 grid((unsigned)((b.O + 3) / 4), (unsigned)nprob);
-  if (f16)
-    hipLaunchKernelGGL(mx4_tile_scales_kernel<true>, grid, dim3(256), 0, as_stream(stream), s);
-  else
-    hipLaunchKernelGGL(mx4_tile_scales_kernel<false>, grid, dim3(256), 0, as_stream(stream), s);
-  if (int rc = check_launch("mx4_tile_scales_kernel")) return rc;
+  if (m.laid) {
+    const dim3 grid((unsigned)(((int64_t)b.O * a.NS + 255) / 256), (unsigned)nprob);
+    hipLaunchKernelGGL(mx4_tile_scales_kernel, grid, dim3(256), 0, as_stream(stream), s);
+    if (int rc = check_launch("mx4_tile_scales_kernel")) return rc;
+  }
   const auto go = [&](auto t) {
     using T = decltype(t);
-    return pl.mi == 1 ? mt_go<1, T>(a, nprob, stream) : pl.mi == 2 ? mt_go<2, T>(a, nprob, stream)
-                                                                   : mt_go<4, T>(a, nprob, stream);
+    return pl.mi == 1 ? mt_go<1, T>(m, nprob, stream) : pl.mi == 2 ? mt_go<2, T>(m, nprob, stream)
+                                                                   : mt_go<4, T>(m, nprob, stream);
   };
   return f16 ? go(__half{}) : go(__hip_bfloat16{});
 }
