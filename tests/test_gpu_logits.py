@@ -232,3 +232,40 @@ def test_many_entries_of_one_token_and_of_one_slice(n):
     # steps of 2^-40 for each of 5000 entries, decay rounded to fp32 (5000 x 2^-24 of a power), one fp32 rounding
     bound = L * 2.0 ** -41 + want.abs() * (L * 2.0 ** -24 + 2.0 ** -24)
     assert ((y.cpu().double() - want).abs() <= bound).all()
+
+
+def test_settings_of_one_row_shared_and_two_streams():
+    """Every penalty as a tensor of one value, one bias and mask for all rows, an expanded row
+    of logits, and two steps at once on two streams with a history each."""
+    import rwkv7mi as mi
+
+    g = torch.Generator().manual_seed(3)
+    n = 2500
+    row = torch.randn(1, n, generator=g).cuda()
+    hist = torch.randint(0, n, (4, 50), generator=g).cuda()
+    bias = torch.randn(n, generator=g).cuda()
+    words = torch.randint(-2 ** 31, 2 ** 31, ((n + 31) // 32,), generator=g).to(torch.int32).cuda()
+    one = lambda v: torch.tensor(v, device="cuda")
+    want = mi.process_logits(row.repeat(4, 1), history=hist, repetition_penalty=1.3, presence_penalty=0.5,
+                             frequency_penalty=0.25, penalty_decay=0.75, bias=bias.repeat(4, 1), allowed=words.repeat(4, 1))
+    got = mi.process_logits(row.expand(4, n), history=hist, repetition_penalty=one(1.3), presence_penalty=one(0.5),
+                            frequency_penalty=one(0.25), penalty_decay=one(0.75), bias=bias, allowed=words)
+    assert torch.equal(got, want)
+    sides = []
+    for k in range(2):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        state = (torch.zeros(4, 80, dtype=torch.long, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"),
+                 torch.zeros(4, dtype=torch.long, device="cuda"))
+        sides.append((s, state))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, (h, lengths, nxt) in sides:
+            with torch.cuda.stream(s):
+                mi.process_logits(row.expand(4, n), history=h, lengths=lengths, presence_penalty=3.0, next_tokens=nxt,
+                                  append=True)
+    torch.cuda.synchronize()
+    (_, a), (_, b) = sides
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and a[1].tolist() == [20] * 4
+    order = torch.argsort(row[0], descending=True, stable=True)
+    assert a[0][0, 0] == order[0]

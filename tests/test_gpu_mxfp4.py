@@ -319,3 +319,54 @@ def test_quantize_model_swaps_eligible_linears():
     assert mi.quantize_model_mxfp4(net, min_params=1, quantize_input=True) == 2
     assert isinstance(net[0], mi.MXFP4Linear) and net[0].quantize_input and isinstance(net[2], torch.nn.Linear)
     assert net(x).shape == (4, 8)
+
+
+@pytest.mark.parametrize("quantize_input", [False, True])
+@pytest.mark.parametrize("rows", [1, 40, 600])
+@pytest.mark.parametrize("n", [512, 640])
+def test_scales_on_any_dword_and_outputs_on_any_element(rows, n, quantize_input):
+    """Scales that start 4, 8 and 12 bytes behind a 16-byte boundary, and an output and a
+    residual that start on an odd element: the same bits."""
+    import rwkv7mi as mi
+
+    m = 264
+    x, codes, scales, g = _case(rows, n, m, torch.float16, rows + n)
+    x, codes, scales = x.cuda(), codes.cuda(), scales.cuda()
+    res = torch.randn(rows, m, generator=g).half().cuda()
+    want = mi.mxfp4_linear(x, codes, scales, residual=res, epilogue="residual", quantize_input=quantize_input)
+    for off in (4, 8, 12):
+        moved = torch.zeros(scales.numel() + 16, dtype=torch.uint8, device="cuda")[off:off + scales.numel()]
+        moved = moved.view_as(scales).copy_(scales)
+        buf = torch.full((rows * m + 2,), 5.0, dtype=torch.float16, device="cuda")
+        out = buf[1:-1].view(rows, m)
+        out.copy_(res)  # in place of the residual
+        got = mi.mxfp4_linear(x, codes, moved, residual=out, epilogue="residual", out=out, quantize_input=quantize_input)
+        assert torch.equal(got, want) and buf[0] == 5 and buf[-1] == 5
+
+
+@pytest.mark.parametrize("quantize_input", [False, True])
+@pytest.mark.parametrize("rows", [40, 600])
+def test_calls_on_two_streams_and_one_tensor_in_every_place(rows, quantize_input):
+    """Two split products at once on two streams, and one weight and one input in all four
+    places of a launch."""
+    import rwkv7mi as mi
+    from rwkv7mi.native_quant_mxfp4 import mxfp4_linear_multi_into
+
+    x, codes, scales, _ = _case(rows, 8704, 40, torch.float16, rows)
+    x, codes, scales = x.cuda(), codes.cuda(), scales.cuda()
+    want = mi.mxfp4_linear(x, codes, scales, quantize_input=quantize_input)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(mi.mxfp4_linear(x, codes, scales, quantize_input=quantize_input))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for side in got for y in side)
+    outs = [torch.empty_like(want) for _ in range(4)]
+    mxfp4_linear_multi_into([x] * 4, [(codes, scales)] * 4, outs, quantize_input=quantize_input)
+    again = [torch.empty_like(want) for _ in range(4)]
+    mxfp4_linear_multi_into([x] * 4, [(codes, scales)] * 4, again, quantize_input=quantize_input)
+    assert all(torch.equal(o, outs[0]) for o in outs + again)
