@@ -109,6 +109,7 @@ int mx4_gemm_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* st
 // Products with 16-bit rows, many of them (mx4_tile.hip).
 bool mx4_tile_supported(int64_t rows, int64_t O, int64_t I);
 int64_t mx4_tile_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I);
+double mx4_tile_us(int nprob, int64_t rows, int64_t O, int64_t I);  // an estimate
 int mx4_tile_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* stream);
 
 // Products through fp16 / bf16 records of the weight and the 256 x 256 GEMM of

@@ -103,13 +103,15 @@ __device__ __forceinline__ void mg_epilogue(const MgArgs& B, const Mx4Prob& P, c
   const T *bias = static_cast<const T*>(P.bias), *res = static_cast<const T*>(P.residual);
   T* y = static_cast<T*>(P.y);
   float* part = SPLIT ? B.part + ((int64_t)blockIdx.y * B.S + blockIdx.z) * M * B.ldp : nullptr;
-  const int cl = 8 * (lane & 31), c0 = n0 + cl;
-  const bool whole = vec && c0 + 8 <= O;
+  // columns c0 + 8 l .. (one run), or, where rows do not start on 16 bytes, every 32nd from
+  // l on, so that a store's lanes lie side by side (6319 x 1440 -> 7307, 4-bit rows, 114 -> 83 us)
+  const bool whole = SPLIT || vec;
+  const int step = whole ? 1 : 32, cl = whole ? 8 * (lane & 31) : lane & 31, c0 = n0 + cl;
   float bo[8], co[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    bo[e] = !SPLIT && bias && c0 + e < O ? to_f32(bias[c0 + e]) : 0.f;
-    co[e] = cs ? cs[cl + e] : 1.f;
+    bo[e] = !SPLIT && bias && c0 + e * step < O ? to_f32(bias[c0 + e * step]) : 0.f;
+    co[e] = cs ? cs[cl + e * step] : 1.f;
   }
 #pragma unroll
   for (int p = 0; p < MI / RT; ++p) {
@@ -129,57 +131,70 @@ __device__ __forceinline__ void mg_epilogue(const MgArgs& B, const Mx4Prob& P, c
     if (c0 >= O) continue;
     // four rows at a time: their LDS reads (and residuals) are in flight together;
     // staged row s is row s + 32 (MI - RT) (s / (32 RT)) + 32 RT p of the tile
-    for (int sb = 2 * wave + (lane >> 5); sb < 64 * RT; sb += 8 * W) {
-      float v[4][8], w[4][8];
-      int r[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int s = sb + 2 * W * k;
-        r[k] = s + 32 * (MI - RT) * (s / (32 * RT)) + 32 * RT * p;
-        ld8(reinterpret_cast<const float*>(smem + s * MG_LDT) + cl, v[k]);
-      }
-      if (!SPLIT && epi == RWKV7MI_EPI_RESIDUAL) {
+    const auto finish = [&](auto run) {
+      constexpr bool RUN = decltype(run)::value;
+      for (int sb = 2 * wave + (lane >> 5); sb < 64 * RT; sb += 8 * W) {
+        float v[4][8], w[4][8];
+        int r[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int64_t oi = (int64_t)(m0 + min(r[k], nrow - 1)) * O + c0;
-          if (whole) {
-            ld8(res + oi, w[k]);
+          const int s = sb + 2 * W * k;
+          r[k] = s + 32 * (MI - RT) * (s / (32 * RT)) + 32 * RT * p;
+          const float* at = reinterpret_cast<const float*>(smem + s * MG_LDT) + cl;
+          if constexpr (RUN) {
+            ld8(at, v[k]);
           } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[k][e] = c0 + e < O ? to_f32(res[oi + e]) : 0.f;
+            for (int e = 0; e < 8; ++e) v[k][e] = at[32 * e];
+          }
+        }
+        if (!SPLIT && epi == RWKV7MI_EPI_RESIDUAL) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int64_t oi = (int64_t)(m0 + min(r[k], nrow - 1)) * O + c0;
+            if constexpr (RUN) {
+              ld8(res + oi, w[k]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[k][e] = c0 + 32 * e < O ? to_f32(res[oi + 32 * e]) : 0.f;
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (r[k] >= nrow) continue;
+          const int64_t row = m0 + r[k], oi = row * O + c0;
+          if constexpr (SPLIT) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] *= co[e];
+            st8(part + row * B.ldp + c0, v[k]);
+            continue;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[k][e] = v[k][e] * co[e] + bo[e];
+          if (epi == RWKV7MI_EPI_RELU2) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] = mx4_relu2(v[k][e]);
+          } else if (epi == RWKV7MI_EPI_RESIDUAL) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] += w[k][e];
+          }
+          if constexpr (RUN) {
+            u32x4 t;
+            st8(reinterpret_cast<T*>(&t), v[k]);
+            __builtin_nontemporal_store(t, reinterpret_cast<u32x4*>(y + oi));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (c0 + 32 * e < O) y[oi + 32 * e] = from_f32<T>(v[k][e]);
           }
         }
       }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (r[k] >= nrow) continue;
-        const int64_t row = m0 + r[k], oi = row * O + c0;
-        if constexpr (SPLIT) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[k][e] *= co[e];
-          st8(part + row * B.ldp + c0, v[k]);
-          continue;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[k][e] = v[k][e] * co[e] + bo[e];
-        if (epi == RWKV7MI_EPI_RELU2) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[k][e] = mx4_relu2(v[k][e]);
-        } else if (epi == RWKV7MI_EPI_RESIDUAL) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[k][e] += w[k][e];
-        }
-        if (whole) {
-          u32x4 t;
-          st8(reinterpret_cast<T*>(&t), v[k]);
-          __builtin_nontemporal_store(t, reinterpret_cast<u32x4*>(y + oi));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (c0 + e < O) y[oi + e] = from_f32<T>(v[k][e]);
-        }
-      }
-    }
+    };
+    if (whole)
+      finish(std::true_type{});
+    else if constexpr (!SPLIT)
+      finish(std::false_type{});
   }
 }
 
@@ -237,10 +252,10 @@ struct MgCost {
 };
 struct MgPlan {
   int mi, S;
+  double us;
 };
 static inline MgPlan mg_plan(const MgCost& c, int nprob, int64_t rows, int64_t O, int64_t NS) {
-  MgPlan p{1, 1};
-  double cost = 1e30;
+  MgPlan p{1, 1, 1e30};
   for (int k = 0; k < 3; ++k) {
     const int mi = 1 << k;
     const int64_t tiles = nprob * ((rows + 64 * mi - 1) / (64 * mi)) * ((O + MG_N - 1) / MG_N);
@@ -251,7 +266,7 @@ static inline MgPlan mg_plan(const MgCost& c, int nprob, int64_t rows, int64_t O
       const double busy = std::min(1.0, tiles * S / 256.0);
       const double split = S > 1 ? 6.0 + 0.4 * S + 8.0 * nprob * S * rows * O / 7e6 : 0.0;
       const double t = rounds * (c.ends[k] + c.ends_busy[k] * busy + (c.step[k] + c.step_busy[k] * busy) * sps) + split;
-      if (t < cost) cost = t, p.mi = mi, p.S = (int)S;
+      if (t < p.us) p = MgPlan{mi, (int)S, t};
     }
   }
   return p;

@@ -31,7 +31,7 @@
 // fill the chip K is split over workgroups and a second launch adds the fp32
 // partials.
 //
-// 16384 x 4096 -> 16384: 642 to 685 us with the quantiser, 3.3 PFLOP/s.  The main loop alone
+// 16384 x 4096 -> 16384: 610 to 690 us with the quantiser, 3.4 PFLOP/s.  The main loop alone
 // takes 500: random codes at 4.8 PFLOP/s draw the card's power limit (7.4 with constant
 // ones), and then all CUs write their tiles, 537 MB, at about the same time.
 #include "mx4_gemm.h"

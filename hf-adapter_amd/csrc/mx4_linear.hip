@@ -274,27 +274,38 @@ static int mx4_rows_run(const Mx4Batch& b, int nprob, void* part, void* stream) 
 static int64_t mx4_codes_bytes(int64_t rows, int64_t I) { return (rows * (I / 2) + 255) & ~(int64_t)255; }
 static int64_t mx4_scales_bytes(int64_t rows, int64_t I) { return (rows * (I / MX4_BLOCK) + 255) & ~(int64_t)255; }
 
-// Which kernel takes a product.  The few-row kernel: up to 16 rows, and more while its
-// passes over the weight, one a tile of 32 rows (16 in MXFP4), cost less than the larger
-// tiles' start and split sums.  16-bit rows on it and on the larger tiles: 128 x 4096 ->
-// 4096 16.5 and 23.4 us, 40 x 8192 -> 2048 13.1 and 19.5, 64 x 4096 -> 16384 28.7 and
-// 29.8, 256 x 4096 -> 4096 25.6 and 26.7, 96 x 4096 -> 16384 41.5 and 36.2, 128 x 16384
-// -> 4096 51.7 and 40.0; 32 rows at any size, 32 x 4096 -> 65536 52.5 and 57.3; past 512
-// rows its passes over x count too, 1000 x 1024 -> 4096 27.5 and 20.3.  MXFP4 rows: 128 x
-// 4096 -> 4096 16.6 and 19.7, 64 x 4096 -> 16384 26.0 and 26.0.  And what the others'
-// offsets cannot hold.  Else the 64- to 256-row tiles.  16-bit rows from 1024
+// A call of the few-row kernel with 17 to 512 16-bit rows, in us: a start and its
+// workgroups' rounds of a group of outputs each, which take about the same time at any K
+// (fitted to 24 shapes: 128 x 4096 -> 4096, 4 rounds, 16.5 and estimated 16.0, 384 rows,
+// 13 rounds, 38.3 and 38.5; 320 x 1216 -> 8088, 10 rounds with ragged K, 43.2 and 43.0).
+static double mx4_rows_us(int nprob, int64_t rows, int64_t O, int64_t I) {
+  const int64_t S = mx4_rows_splits(rows, I, false), nw = ((I + 511) / 512 + S - 1) / S;
+  const int64_t share = (rows + 31) / 32 * nprob * S, groups = (O + 15) / 16, fit = 256 * (8 / nw);
+  const int64_t wide = std::min(groups, std::max<int64_t>(1, fit / share));
+  const int64_t rounds = (groups + wide - 1) / wide * ((wide * share + fit - 1) / fit);
+  return 6.0 + (I % 512 ? 3.7 : 2.5) * rounds + (S > 1 ? 3.0 : 0.0);
+}
+
+// Which kernel takes a product.  The few-row kernel: up to 16 rows, and up to 512 where
+// its passes over the weight, one a tile of 32 rows, are estimated to take no longer than
+// the larger tiles.  16-bit rows on it and on those: 128 x 4096 -> 4096 16.5 and 23.4 us,
+// 40 x 8192 -> 2048 13.1 and 19.5, 256 x 4096 -> 4096 25.6 and 26.7, 32 x 4096 -> 65536
+// 52.5 and 57.3; 96 x 4096 -> 16384 41.5 and 36.2, 128 x 16384 -> 4096 51.7 and 40.0.
+// MXFP4 rows, 16 a tile, by rows x weight: 128 x 4096 -> 4096 16.6 and 19.7, 64 x 4096 ->
+// 16384 26.0 and 26.0.  And what the others' offsets cannot hold.  Else the 64- to
+// 256-row tiles.  16-bit rows from 1024
 // tiles of 256 x 256 on write the weight out in 16 bits and run the GEMM of mm8h.hip:
 // without conversions between its MFMAs it holds a higher clock over such long calls
 // (16384 x 4096 -> 16384 1636 us, on the tiles 2000), and the pass over the weight
 // is small against them (1000 rows, 256 tiles: 150 and 114).
 enum Mx4Route { MX4_ROWS, MX4_TILE, MX4_GEMM, MX4_PREFILL };
-static Mx4Route mx4_route(int64_t rows, int64_t I, int64_t O, int quantize_input) {
-  const bool few = quantize_input ? rows <= 256 && (rows + 15) / 16 * (O * I) <= 1 << 27
-                                  : rows <= 32 || (rows <= 512 && (rows + 31) / 32 * (O * I) <= 1 << 27);
-  if (rows <= 16 || few) return MX4_ROWS;
+static Mx4Route mx4_route(int nprob, int64_t rows, int64_t I, int64_t O, int quantize_input) {
+  if (rows <= 16) return MX4_ROWS;
+  if (quantize_input && rows <= 256 && (rows + 15) / 16 * (O * I) <= 1 << 27) return MX4_ROWS;
   if (quantize_input) return mx4_gemm_supported(rows, O, I) ? MX4_GEMM : MX4_ROWS;
   if ((rows + 255) / 256 * ((O + 255) / 256) >= 1024 && mx4h_supported(rows, I, O)) return MX4_PREFILL;
-  return mx4_tile_supported(rows, O, I) ? MX4_TILE : MX4_ROWS;
+  if (!mx4_tile_supported(rows, O, I)) return MX4_ROWS;
+  return rows <= 512 && mx4_rows_us(nprob, rows, O, I) <= mx4_tile_us(nprob, rows, O, I) ? MX4_ROWS : MX4_TILE;
 }
 
 }  // namespace rwkv7mi
@@ -304,7 +315,7 @@ using namespace rwkv7mi;
 extern "C" int64_t rwkv7mi_mxfp4_linear_workspace_bytes(int nprob, int64_t rows, int64_t O, int64_t I, int act_dtype,
                                                         int quantize_input) {
   if (nprob < 1 || nprob > MX4_MAXPROB || rows <= 0 || O <= 0 || I <= 0) return 0;
-  const Mx4Route route = mx4_route(rows, I, O, quantize_input);
+  const Mx4Route route = mx4_route(nprob, rows, I, O, quantize_input);
   if (route == MX4_PREFILL) return mx4h_workspace_bytes(nprob, rows, I, O);
   if (route == MX4_GEMM) return mx4_gemm_workspace_bytes(nprob, rows, O, I);
   if (route == MX4_TILE) return mx4_tile_workspace_bytes(nprob, rows, O, I);
@@ -346,7 +357,7 @@ extern "C" int rwkv7mi_mxfp4_linear(int nprob, const void* const* x, const uint8
   if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < need))
     return fail(RWKV7MI_ESIZE, w + ": workspace missing, unaligned or smaller than "
                                    "rwkv7mi_mxfp4_linear_workspace_bytes");
-  const Mx4Route route = mx4_route(rows, I, O, quantize_input);
+  const Mx4Route route = mx4_route(nprob, rows, I, O, quantize_input);
   if (route == MX4_PREFILL) return mx4h_run(b, nprob, act_dtype, ws, ws_bytes, stream);
   if (route == MX4_GEMM) return mx4_gemm_run(b, nprob, act_dtype, ws, stream);
   if (route == MX4_TILE) return mx4_tile_run(b, nprob, act_dtype, ws, stream);
