@@ -70,7 +70,7 @@ struct MhProb {
   void* y;
   int epilogue;
   int vec;  // O % 8 == 0 and y (and the residual) 16-byte aligned: 16-byte output rows
-  const float* cs;  // MX instances: a factor per column, before the bias (null: none)
+  const float* cs;  // MX instances: a factor per column, before the bias
 };
 struct MhBatch {
   MhProb p[MM8T_MAXPROB];
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(256) void mm8h_reduce_kernel(const MhBatch B) {
   }
   if constexpr (MX) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) if (P.cs && c0 + e < B.O) v[e] *= P.cs[c0 + e];
+    for (int e = 0; e < 8; ++e) if (c0 + e < B.O) v[e] *= P.cs[c0 + e];
   }
   const TA* bp = reinterpret_cast<const TA*>(P.bias);
 #pragma unroll
@@ -273,8 +273,8 @@ __global__ __launch_bounds__(256) void mm8h_reduce_kernel(const MhBatch B) {
 // FULLK: I is a multiple of 64 (no step ends inside a 16-byte chunk's range).
 // SPLIT: blockIdx.z takes B.sps of the steps and leaves fp32 partial tiles (an
 // instance of its own: the bounds and the second epilogue cost the unsplit
-// kernel 4%).  MX: the records are an MXFP4 weight's: a factor per column (fp16
-// rows are scaled by a power of two each), and relu^2 keeps a NaN
+// kernel 4%).  MX: the records are an MXFP4 weight's: a factor per column (its row is
+// scaled by a power of two), and relu^2 keeps a NaN
 template <bool FULLK, bool SPLIT, typename TA, bool MX>
 __global__ __launch_bounds__(MH_THREADS, 1) void mm8h_gemm_kernel(const MhBatch B) {
   using E = typename MhTypes<TA>::E;
@@ -452,7 +452,7 @@ __global__ __launch_bounds__(MH_THREADS, 1) void mm8h_gemm_kernel(const MhBatch 
     for (int e = 0; e < 8; ++e) bo[e] = bp && c0 + e < O ? to_f32(bp[c0 + e]) : 0.f;
     if constexpr (MX) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) co[e] = P.cs && c0 + e < O ? P.cs[c0 + e] : 1.f;
+      for (int e = 0; e < 8; ++e) co[e] = c0 + e < O ? P.cs[c0 + e] : 1.f;
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -810,17 +810,17 @@ extern "C" int rwkv7mi_dense_gemm_prefill_ws(int nprob, const void* const* x, co
 
 namespace rwkv7mi {
 
-// ---- MXFP4 weights: the same records, then the same GEMM.  fp16 rows are scaled
-// relative to their largest scale and the sums by its factor per column
-// (mx4_common.h).  16384 x 4096 -> 16384: 1.64 ms, 1.34 PFLOP/s, 40 us of it the records (170 MB).
+// ---- MXFP4 weights: the same records, then the same GEMM.  Rows are scaled by their
+// largest scale and the sums by its factor per column (mx4_common.h).  16384 x 4096 -> 16384: 1.64 ms, 1.34 PFLOP/s, 40 us of it the records (170 MB).
 struct Mx4hBatch {
   const uint8_t *codes[MX4_MAXPROB], *scales[MX4_MAXPROB];
   void* out[MX4_MAXPROB];
-  float* cs[MX4_MAXPROB];  // fp16: the columns' factors
+  float* cs[MX4_MAXPROB];  // the columns' factors
   int I, O, SB;
 };
 
-// one wave a row: the largest scale byte as the column's factor
+// one wave a row: its factor, by the largest scale byte
+template <typename TA>
 __global__ __launch_bounds__(256) void mx4h_factor_kernel(const Mx4hBatch D) {
   const int o = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, nb = D.I / MX4_BLOCK;
   if (o >= D.O) return;
@@ -829,7 +829,7 @@ __global__ __launch_bounds__(256) void mx4h_factor_kernel(const Mx4hBatch D) {
   for (int i = lane; i < nb; i += 64) m = max(m, (int)s[i]);
 #pragma unroll
   for (int d = 32; d; d >>= 1) m = max(m, __shfl_xor(m, d, 64));
-  if (lane == 0) D.cs[blockIdx.y][o] = mx4_factor((uint32_t)m);
+  if (lane == 0) D.cs[blockIdx.y][o] = mx4_run_factor<TA>((uint32_t)m);
 }
 
 // one thread per (column group, step, lane): 8 bytes of codes -> its two records.
@@ -852,10 +852,7 @@ __global__ __launch_bounds__(256) void mx4h_dequant_kernel(const Mx4hBatch D) {
   if (o < D.O && k0 < D.I) {  // I % 32 == 0: the lane's 16 inputs are of one block
     c = *reinterpret_cast<const uint2*>(D.codes[p] + (int64_t)o * (D.I / 2) + k0 / 2);
     const uint32_t e = D.scales[p][(int64_t)o * (D.I / MX4_BLOCK) + k0 / MX4_BLOCK];
-    if constexpr (std::is_same<TA, __half>::value)
-      s = mx4_relative(e, mx4_factor_emax(D.cs[p][o]));
-    else
-      s = mx4_scale(e);
+    s = mx4_scale(mx4_run_byte<TA>(e, mx4_factor_emax<TA>(D.cs[p][o])));
   }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -883,7 +880,6 @@ int64_t mx4h_workspace_bytes(int nprob, int64_t rows, int64_t I, int64_t O) {
 
 template <typename TA>
 static int mx4h_go(const Mx4Batch& m, int nprob, char* ws, int64_t ws_bytes, void* stream) {
-  constexpr bool F16 = std::is_same<TA, __half>::value;
   const std::string w("mxfp4_linear");
   const int64_t I = m.I, O = m.O, fb = mx4h_factor_bytes(nprob, O), per = mh_weight_bytes(1, I, O);
   Mx4hBatch d{};
@@ -896,11 +892,9 @@ static int mx4h_go(const Mx4Batch& m, int nprob, char* ws, int64_t ws_bytes, voi
     d.cs[i] = reinterpret_cast<float*>(ws) + i * O;
     d.out[i] = ws + fb + i * per;
   }
-  if (F16) {
-    hipLaunchKernelGGL(mx4h_factor_kernel, dim3((unsigned)((O + 3) / 4), (unsigned)nprob), dim3(256), 0,
-                       as_stream(stream), d);
-    if (int rc = check_launch("mx4h_factor_kernel")) return rc;
-  }
+  hipLaunchKernelGGL(mx4h_factor_kernel<TA>, dim3((unsigned)((O + 3) / 4), (unsigned)nprob), dim3(256), 0,
+                     as_stream(stream), d);
+  if (int rc = check_launch("mx4h_factor_kernel")) return rc;
   const int64_t recs = (2 * ((O + 31) / 32)) * (int64_t)d.SB * 64;
   hipLaunchKernelGGL(mx4h_dequant_kernel<TA>, dim3((unsigned)((recs + 255) / 256), (unsigned)nprob), dim3(256), 0,
                      as_stream(stream), d);
@@ -914,7 +908,7 @@ static int mx4h_go(const Mx4Batch& m, int nprob, char* ws, int64_t ws_bytes, voi
       if (int rc = mh_prob(w, b.p[i], static_cast<const char*>(p.x) + r * I * 2, d.out[i], p.bias,
                            res ? res + r * O * 2 : nullptr, static_cast<char*>(p.y) + r * O * 2, p.epilogue, O))
         return rc;
-      b.p[i].cs = F16 ? d.cs[i] : nullptr;
+      b.p[i].cs = d.cs[i];
     }
     if (int rc = mh_gemm_launch<TA, true>(b, nprob, std::min<int64_t>(step, m.rows - r), I, O, ws + fb, ws_bytes - fb,
                                         stream, w))

@@ -35,20 +35,36 @@ struct Mx4Batch {
 // field alone; 255 gives NaN).
 __device__ __forceinline__ float mx4_scale(uint32_t e) { return __uint_as_float(e << 23); }
 
-// fp16 weights are scaled relative to the largest scale byte emax of a run of
-// inputs: a block's codes by 2^(13 + e - emax) (at most 6 x 2^13, exact down to
-// 2^-36 of the largest scale, rounding at 2^-24 below), the sums over the run by
-// the factor 2^(emax - 127 - 13) (NaN for emax = 255) in fp32.
-__device__ __forceinline__ uint32_t mx4_relative_byte(uint32_t e, uint32_t emax) {
-  return (uint32_t)max(140 + (int)e - (int)emax, 1);
+// 16-bit weights are formed over a run of inputs whose largest scale byte is emax, their
+// codes times 2^(byte - 127), and the sums over the run take a factor in fp32 (NaN for
+// emax = 255).
+//  * fp16: scaled relative to emax, 2^(13 + e - emax) (at most 6 x 2^13, exact down to
+//    2^-36 of the largest scale, rounding at 2^-24 below).
+//  * bf16 holds a code times 2^(e - 127) exactly for e up to 252; 6 x 2^126 is past its
+//    range (and fp32's).  Runs with a byte of 253 or 254 are formed at a quarter (their
+//    bytes 0 and 1, 2^-251 of the largest at most, at no less than 2^-127).
+template <typename T>
+__device__ __forceinline__ uint32_t mx4_run_byte(uint32_t e, uint32_t emax) {
+  if constexpr (std::is_same<T, __half>::value)
+    return (uint32_t)max(140 + (int)e - (int)emax, 1);
+  else
+    return emax < 253u ? e : (uint32_t)max((int)e - 2, 0);
 }
-__device__ __forceinline__ float mx4_relative(uint32_t e, uint32_t emax) { return mx4_scale(mx4_relative_byte(e, emax)); }
-__device__ __forceinline__ float mx4_factor(uint32_t emax) {
-  return emax == 255u ? __builtin_nanf("") : ldexpf(1.f, (int)emax - 140);
+template <typename T>
+__device__ __forceinline__ float mx4_run_factor(uint32_t emax) {
+  if (emax == 255u) return __builtin_nanf("");
+  if constexpr (std::is_same<T, __half>::value)
+    return ldexpf(1.f, (int)emax - 140);
+  else
+    return emax < 253u ? 1.f : 4.f;
 }
-
-__device__ __forceinline__ uint32_t mx4_factor_emax(float f) {  // emax again
-  return f != f ? 255u : (uint32_t)(ilogbf(f) + 140);
+// an emax of that factor
+template <typename T>
+__device__ __forceinline__ uint32_t mx4_factor_emax(float f) {
+  if constexpr (std::is_same<T, __half>::value)
+    return f != f ? 255u : (uint32_t)(ilogbf(f) + 140);
+  else
+    return f == 1.f ? 0u : 254u;
 }
 
 __device__ __forceinline__ uint32_t mx4_max4(uint32_t v) {  // the largest byte

@@ -18,10 +18,9 @@
 // loads' way: a group's scales are loaded once by the workgroup, through LDS, a group
 // ahead (by each wave 1.4 us more at 1 x 4096 -> 16384, 13.1 us then), and 16-bit rows
 // by whole lines, through LDS (in the operand's layout, 16 bytes of 64 lines an
-// instruction, 17.3 us for 14.6 at 16 x 4096 -> 16384).  bf16 holds a scaled code
-// exactly.  fp16 does not for every scale, so there a step's codes are scaled relative
-// to the largest of its four scales and the step's sums by that one's factor
-// (mx4_common.h).
+// instruction, 17.3 us for 14.6 at 16 x 4096 -> 16384).  Neither 16-bit type holds a code
+// times every scale, so the codes of a step (bf16: of a unit) are scaled by its largest
+// scale and the sums by that one's factor (mx4_common.h).
 //
 // The weight's bytes bound it: 1 x 4096 -> 16384 11.9 us (36 MB; 9.5 from the caches),
 // 8 x 4096 -> 65536 35 us, 4.0 TB/s of the 5.4 that a copy reaches.
@@ -161,6 +160,8 @@ __global__ __launch_bounds__(RT > 1 ? 512 : 1024) void mx4_rows_kernel(const Mx4
     if (has) {
       if (next) load_w(g + gridDim.x, wn);
       const u32x4 e = scale[(16 * par + n) * nw + wave];
+      // bf16: the unit is the run
+      const uint32_t unit = A4 || F16 ? 0u : max(max(mx4_max4(e[0]), mx4_max4(e[1])), max(mx4_max4(e[2]), mx4_max4(e[3])));
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         const uint32_t ew = e[s], eb = (ew >> (8 * q)) & 255u;
@@ -168,8 +169,8 @@ __global__ __launch_bounds__(RT > 1 ? 512 : 1024) void mx4_rows_kernel(const Mx4
           acc[0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(a[0][s][0]), mx4_operand(w[s]), acc[0], 4, 4,
                                                                     0, (int)((ea[s] >> (8 * q)) & 255u), 0, (int)eb);
         } else {
-          const uint32_t emax = F16 ? mx4_max4(ew) : 0u;
-          const float sc = F16 ? mx4_relative(eb, emax) : mx4_scale(eb);
+          const uint32_t emax = F16 ? mx4_max4(ew) : unit;
+          const float sc = mx4_scale(mx4_run_byte<T>(eb, emax));
           f32x4 c[RT];
 #pragma unroll
           for (int t = 0; t < RT; ++t) c[t] = F16 ? (f32x4){0.f, 0.f, 0.f, 0.f} : acc[t];
@@ -181,8 +182,12 @@ __global__ __launch_bounds__(RT > 1 ? 512 : 1024) void mx4_rows_kernel(const Mx4
             for (int t = 0; t < RT; ++t) c[t] = mfma16x16x32(__builtin_bit_cast(V, a[t][s][j]), wv, c[t]);
           }
 #pragma unroll
-          for (int t = 0; t < RT; ++t) acc[t] = F16 ? acc[t] + mx4_factor(emax) * c[t] : c[t];
+          for (int t = 0; t < RT; ++t) acc[t] = F16 ? acc[t] + mx4_run_factor<T>(emax) * c[t] : c[t];
         }
+      }
+      if constexpr (!A4 && !F16) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[t] = acc[t] * mx4_run_factor<T>(unit);
       }
 #pragma unroll
       for (int s = 0; s < 4; ++s) w[s] = wn[s];

@@ -14,9 +14,9 @@
 //    16384: 2.04 ms);
 //  * W's scales: 8 steps (a superstep) at a time, global -> LDS, 16 bytes a column; for
 //    rows of scales that are not whole dwords (I % 128) from a copy that a pre-pass lays
-//    out.  fp16 columns are scaled relative to the largest scale of the workgroup's part
-//    of them (mx4_common.h), which it reads first, while the ring fills, and the sums by
-//    its factor (with the pre-pass at all sizes: 64 x 4096 -> 65536 76 us for 59, 1000 x
+//    out.  Columns are scaled by the largest scale of the workgroup's part of them
+//    (mx4_common.h), which it reads first, while the ring fills, and the sums by its
+//    factor (with the pre-pass at all sizes: 64 x 4096 -> 65536 76 us for 59, 1000 x
 //    4096 -> 16384 122.6 for 121.0, 4000 x 4096 -> 4096 116 for 120).
 // A stage of x is read to the end in its step's third sub-step: one barrier there, and
 // the loads a ring ahead go into the same stage; the barrier waits for the loads of the
@@ -54,7 +54,6 @@ static_assert(mt_lds(1) + 4 * MG_N <= 163840 && mt_lds(2) + 4 * MG_N <= 163840 &
 template <int MI, bool SPLIT, typename T>
 __global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MtArgs A) {
   const MgArgs& B = A.g;
-  constexpr bool F16 = std::is_same<T, __half>::value;
   using V = typename Mx4Types<T>::V;
   constexpr int ROWS = 64 * MI, XB = ROWS * 128, WB = MG_N * 128, SB = MG_N * 16;  // bytes of a stage of x, W, scales
   constexpr int NXS = mt_xstages(MI);
@@ -119,7 +118,7 @@ __global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MtArgs
   uint32_t emax[NJ];  // (of the lane's columns)
   auto ld_s = [&](int s, int j) {  // its scale byte
     const uint32_t e = *reinterpret_cast<const uint8_t*>(scl + (s >> 3 & 1) * SB + col(j) * 16 + 2 * (s & 7) + u);
-    return F16 ? mx4_relative_byte(e, emax[j]) : e;
+    return mx4_run_byte<T>(e, emax[j]);
   };
 
   f32x16 acc[MI][NJ];
@@ -167,7 +166,7 @@ __global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MtArgs
   for (int s = 0; s < NXS; ++s)
 #pragma unroll
     for (int v = 0; v < NX; ++v) issue_x(s, s, v);
-  if constexpr (F16) {
+  {
     // the largest scale of column tid / 2, every other 8 bytes a thread
     const int c = tid >> 1, b0 = 16 * S0 + 8 * (tid & 1), be = min(16 * S1, nb);
     uint32_t m = 0;
@@ -187,14 +186,12 @@ __global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MtArgs
       }
     }
     m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
-    if (!(tid & 1)) factor[c] = mx4_factor(m);
+    if (!(tid & 1)) factor[c] = mx4_run_factor<T>(m);
     __syncthreads();
   }
   meet(std::integral_constant<int, 0>{});
-  if constexpr (F16) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) emax[j] = mx4_factor_emax(factor[col(j)]);
-  }
+  for (int j = 0; j < NJ; ++j) emax[j] = mx4_factor_emax<T>(factor[col(j)]);
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     wc[j] = ld_w(0, j);
@@ -237,7 +234,7 @@ __global__ __launch_bounds__(64 * MT_WAVES, 1) void mx4_tile_kernel(const MtArgs
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the trailing loads have landed before the waves exit
 
-  mg_epilogue<MI, MT_WC, SPLIT, T>(B, P, smem, acc, m0, n0, F16 ? factor : nullptr);
+  mg_epilogue<MI, MT_WC, SPLIT, T>(B, P, smem, acc, m0, n0, factor);
 }
 
 // The pre-pass: the scales [superstep][column][16], 0 behind a column's end.  One thread

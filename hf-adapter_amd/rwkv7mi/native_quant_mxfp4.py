@@ -63,7 +63,8 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor,
                      out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """The values ``[..., I]`` of :func:`quantize_mxfp4`'s result, rounded to
-    ``out_dtype`` (bf16 and fp32 hold each exactly)."""
+    ``out_dtype`` (bf16 and fp32 hold each exactly below 2^128; past it they become
+    infinite, which the scales 2^126 and 2^127 reach).  Products do not form them so."""
     _check_packed(codes, scales, "dequantize_mxfp4")
     _lib.require_same_device(codes, scales, name="dequantize_mxfp4")
     codes, scales = _aligned(codes, 4), scales.contiguous()

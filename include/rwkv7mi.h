@@ -801,7 +801,8 @@ int rwkv7mi_w4_matmul_ws(const void* x, const uint8_t* packed,
 int rwkv7mi_mxfp4_quantize(const void* x, int64_t rows, int64_t I, int64_t ld,
                            int dtype, uint8_t* codes, uint8_t* scales,
                            void* stream);
-/* y [rows, I] = the values of the codes, rounded to dtype. */
+/* y [rows, I] = the values of the codes, rounded to dtype (infinite past its
+ * range, which a block of scale 2^126 or 2^127 can reach in bf16 and fp32). */
 int rwkv7mi_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales,
                              int64_t rows, int64_t I, void* y, int dtype,
                              void* stream);
