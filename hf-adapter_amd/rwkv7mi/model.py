@@ -931,7 +931,8 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
         None gives the seeded random init (as ``cls(config)`` does for the
         reference).  ``prepacked``: module name -> :class:`MM8Linear` or
         :class:`MXFP4Linear` built from a prepacked checkpoint; those modules'
-        ``.weight`` entries are not read."""
+        ``.weight`` entries are not read, and the linears that it does not hold
+        stay dense."""
         mxfp4 = bool(getattr(config, "use_native_mxfp4", False))
         if mxfp4:
             if config.use_native_mm8:
@@ -953,6 +954,8 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
                 m = prepacked[name]
                 return BlockFloatLinear(m) if isinstance(m, MXFP4Linear) else QuantLinear(m)
             w = get(name + ".weight")
+            if prepacked is not None:  # saved dense
+                return DenseLinear(w)
             if mxfp4 and int(w.shape[1]) % MXFP4_BLOCK == 0 and should_quantize_linear(
                     name, int(w.numel()), min_params=cfg.native_mxfp4_min_params, policy=cfg.native_mxfp4_policy):
                 self._replaced += 1
