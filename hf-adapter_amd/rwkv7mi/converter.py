@@ -16,10 +16,11 @@ from a directory the reference converter wrote: the same keys, its
 
 Prepacked checkpoint (the per-module loader metadata of
 docs/quantization/VLLM_QUANTIZATION_PORTING.md:411-430): the MM8 modules'
-bytes in the GEMV's blocked layout with their scales, or the MXFP4 modules' codes
-and block scales, ``prepacked.safetensors``, and ``manifest.json`` with one entry per module (format, features, dtypes,
-epilogue, sha256 of the source weight, packer version) validated before any
-GPU buffer is allocated, so loading skips quantisation.
+bytes in the GEMV's blocked layout with their scales, or the MXFP4 modules'
+codes and block scales, ``prepacked.safetensors``, and ``manifest.json`` with
+one entry per module (format, features, dtypes, epilogue, an MXFP4 module's
+``quantize_input``, sha256 of the source weight, packer version) validated
+before any GPU buffer is allocated, so loading skips quantisation.
 
 Checkpoints are read with ``torch.load(weights_only=True)`` (or safetensors):
 nothing in a file is executed.
@@ -339,6 +340,8 @@ def save_prepacked(model, output, *, source_state: Dict[str, torch.Tensor] | Non
             "epilogue": next((v for k, v in _EPILOGUE.items() if name.endswith(k)), "none"),
             "blocked_shape": list((m.codes if four else m.w_blk).shape), "packer_version": _PACKERS[fmt],
         }
+        if four:
+            entry["quantize_input"] = bool(m.quantize_input)
         if source_state is not None and name + ".weight" in source_state:
             entry["source_weight_sha256"] = _sha256(source_state[name + ".weight"])
         manifest["modules"].append(entry)
@@ -391,6 +394,8 @@ def validate_manifest(manifest: dict, cfg, dtype: torch.dtype) -> None:
         if fmt == MXFP4_FORMAT:  # codes and scales do not depend on the activations' type
             if e.get("scale_dtype") != "uint8" or i % 32:
                 raise ValueError(f"{name}: MXFP4 needs uint8 scales and inputs divisible by 32")
+            if not isinstance(e.get("quantize_input", False), bool):
+                raise ValueError(f"{name}: quantize_input {e.get('quantize_input')!r} is neither true nor false")
         else:
             if e.get("activation_dtype") != dname:
                 raise ValueError(f"{name}: packed for {e.get('activation_dtype')} activations, loading {dtype}")
@@ -408,7 +413,8 @@ def load_prepacked(path, *, device="cuda", dtype=torch.float16,
                    native_mxfp4_quantize_input: bool | None = None):
     """The model from a prepacked directory: the manifest is validated, then
     the MM8 or MXFP4 modules are built from the stored bytes (no quantisation).  Each
-    stored tensor must have the dtype the manifest declares.  With
+    stored tensor must have the dtype the manifest declares.  An MXFP4 module quantises
+    its input as the saved one did, or as ``native_mxfp4_quantize_input`` says.  With
     ``source_state`` (the unquantised HF state dict), every module's
     ``source_weight_sha256`` is checked against it."""
     from safetensors.torch import load_file
@@ -457,8 +463,10 @@ def load_prepacked(path, *, device="cuda", dtype=torch.float16,
                     or list(t["scales"].shape) != [e["output_features"], e["input_features"] // 32]):
                 raise ValueError(f"{n}: codes {list(t['codes'].shape)} and scales {list(t['scales'].shape)} do not "
                                  "match the manifest")
-            prebuilt[n] = MXFP4Linear.from_packed(t["codes"].to(device), t["scales"].to(device),
-                                                  quantize_input=cfg.native_mxfp4_quantize_input)
+            # (a manifest without the entry: the config's setting)
+            quant = (e.get("quantize_input", cfg.native_mxfp4_quantize_input) if native_mxfp4_quantize_input is None
+                     else native_mxfp4_quantize_input)
+            prebuilt[n] = MXFP4Linear.from_packed(t["codes"].to(device), t["scales"].to(device), quantize_input=quant)
             continue
         prebuilt[n] = MM8Linear.from_packed(t["w_blk"].to(device), t["mx"].to(device), t["rx"].to(device),
                                            t["my"].to(device), t["ry"].to(device), e["input_features"],

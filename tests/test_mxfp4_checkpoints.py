@@ -2,6 +2,9 @@
 (built, saved and loaded on the CPU; no kernel runs)."""
 from __future__ import annotations
 
+import json
+
+import pytest
 import torch
 
 import mx_reference as mx
@@ -59,3 +62,30 @@ def test_a_linear_saved_dense_stays_dense(tmp_path):
             assert isinstance(b, DenseLinear) and torch.equal(a.weight, b.weight), name
         else:
             assert torch.equal(a.m.codes, b.m.codes) and torch.equal(a.m.scales, b.m.scales)
+
+
+def test_every_module_keeps_its_quantize_input(tmp_path):
+    model = _pack_model({**dict.fromkeys(RKVO, True), **dict.fromkeys(FFN, True)}, head=False)
+    want = _flags(model)
+    assert len(want) == 7 and not want["lm_head"] and sum(want.values()) == 6
+    model.save_pretrained(tmp_path)
+    assert _flags(_load(tmp_path)) == want
+    assert set(_flags(_load(tmp_path, native_mxfp4_quantize_input=True)).values()) == {True}
+    # a manifest without the entry: the config's setting for every module
+    manifest = json.loads((tmp_path / "manifest.json").read_text())
+    for e in manifest["modules"]:
+        del e["quantize_input"]
+    (tmp_path / "manifest.json").write_text(json.dumps(manifest))
+    cj = json.loads((tmp_path / "config.json").read_text())
+    for setting in (True, False):
+        (tmp_path / "config.json").write_text(json.dumps({**cj, "native_mxfp4_quantize_input": setting}))
+        assert set(_flags(_load(tmp_path)).values()) == {setting}
+
+
+def test_a_manifest_entry_that_is_no_truth_value_is_refused(tmp_path):
+    _pack_model({}, head=True).save_pretrained(tmp_path)
+    manifest = json.loads((tmp_path / "manifest.json").read_text())
+    manifest["modules"][0]["quantize_input"] = "yes"
+    (tmp_path / "manifest.json").write_text(json.dumps(manifest))
+    with pytest.raises(ValueError, match="quantize_input"):
+        _load(tmp_path)
