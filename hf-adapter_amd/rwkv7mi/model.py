@@ -356,13 +356,21 @@ class BlockFloatLinear:
                             epilogue="relu2" if act == 3 else "none" if residual is None else "residual",
                             quantize_input=self.m.quantize_input)
 
+    def _as_launched(self, dtype) -> bool:
+        """Whether a launch reads the module's tensors as they are."""
+        m, b = self.m, self.m.bias
+        return (m.codes.is_contiguous() and m.scales.is_contiguous() and not m.codes.data_ptr() % 16
+                and not m.scales.data_ptr() % 4 and (b is None or (b.dtype == dtype and b.is_contiguous())))
+
     @staticmethod
     def apply_group(lins, xs, outs) -> bool:
         """``[l.apply(x, o) for ...]`` as one launch; False (nothing run) when the products
-        do not share a shape and a treatment of their inputs."""
+        do not share a shape and a treatment of their inputs, or hold what a single
+        product converts or copies first."""
         if (len(lins) > 4 or len({(l.in_features, l.out_features, l.m.quantize_input) for l in lins}) != 1
                 or any(q.dtype != xs[0].dtype or q.shape != xs[0].shape or not q.is_contiguous()
-                       or q.data_ptr() % 16 for q in xs)):
+                       or q.data_ptr() % 16 for q in xs)
+                or not all(l._as_launched(xs[0].dtype) for l in lins)):
             return False
         mxfp4_linear_multi_into(list(xs), [(l.m.codes, l.m.scales) for l in lins], list(outs),
                                 biases=[l.m.bias for l in lins], quantize_input=lins[0].m.quantize_input)

@@ -114,3 +114,24 @@ def test_rows_of_two_gigabytes():
     for r in (0, 130000, 261880, 262390):
         rs = slice(r, min(r + 16, rows))
         _within(got[rs], x[rs], w, None, residual[rs], "residual")
+
+
+@pytest.mark.parametrize("last", ["bias", "codes", "scales"])
+def test_linears_that_cannot_be_grouped_run_one_by_one(last):
+    """A bias of another type, codes and scales off their boundary, in the third of three linears
+    of a model: the results of the single products."""
+    from rwkv7mi import MXFP4Linear
+    from rwkv7mi.model import BlockFloatLinear, QuantLinear
+
+    x, codes, scales, bias, _ = (t.cuda() for t in _problem(5, 256, 40, torch.float16, 1))
+    mods = [MXFP4Linear.from_packed(codes, scales, bias) for _ in range(3)]
+    want = [m(x) for m in mods]
+    if last == "bias":
+        mods[2].bias = bias.float()
+    else:
+        t = getattr(mods[2], last)
+        moved = torch.zeros(t.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view_as(t)
+        setattr(mods[2], last, moved.copy_(t))
+    outs = [torch.empty(5, 40, dtype=torch.float16, device="cuda") for _ in range(3)]
+    QuantLinear.apply_group([BlockFloatLinear(m) for m in mods], [x, x, x], outs)
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
