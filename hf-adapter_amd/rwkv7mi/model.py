@@ -1795,11 +1795,12 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
             isinstance(v, torch.Tensor) or v != d
             for v, d in ((repetition_penalty, 1.0), (presence_penalty, 0.0), (frequency_penalty, 0.0)))
         if not plain:
+            here = lambda v: v.to(self.device) if isinstance(v, torch.Tensor) else v
             return self._generate_processed(
-                input_ids, max_new_tokens, use_graph, repetition_penalty=repetition_penalty,
-                presence_penalty=presence_penalty, frequency_penalty=frequency_penalty, penalty_decay=penalty_decay,
-                bias=None if bias is None else bias.to(self.device, torch.float32),
-                allowed=None if allowed is None else allowed.to(self.device))
+                input_ids, max_new_tokens, use_graph, repetition_penalty=here(repetition_penalty),
+                presence_penalty=here(presence_penalty), frequency_penalty=here(frequency_penalty),
+                penalty_decay=here(penalty_decay), bias=None if bias is None else bias.to(self.device, torch.float32),
+                allowed=here(allowed))
         out0 = self.forward(input_ids)
         logits, cache = out0.logits, out0.past_key_values
         nxt = argmax_rows(logits[:, -1])
