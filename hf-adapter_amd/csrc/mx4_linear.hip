@@ -313,6 +313,13 @@ static Mx4Route mx4_route(int nprob, int64_t rows, int64_t I, int64_t O, int qua
   return rows <= 512 && mx4_rows_us(nprob, rows, O, I) <= mx4_tile_us(nprob, rows, O, I) ? MX4_ROWS : MX4_TILE;
 }
 
+// The quantiser's launch of a product's rows (mx4.hip: 8 values a lane; before the GEMM
+// rows padded to whole supersteps, and the weight's scales) holds fewer than 2^32 lanes.
+static bool mx4_quantizable(Mx4Route route, int64_t rows, int64_t I, int64_t O) {
+  const int64_t NS = (I + 511) / 512;
+  return (route == MX4_GEMM ? 64 * NS * rows + 4 * NS * O : rows * (I / 8)) <= ((int64_t)1 << 32) - 1024;
+}
+
 }  // namespace rwkv7mi
 
 using namespace rwkv7mi;
@@ -321,6 +328,7 @@ extern "C" int64_t rwkv7mi_mxfp4_linear_workspace_bytes(int nprob, int64_t rows,
                                                         int quantize_input) {
   if (nprob < 1 || nprob > MX4_MAXPROB || rows <= 0 || O <= 0 || I <= 0) return 0;
   const Mx4Route route = mx4_route(nprob, rows, I, O, quantize_input);
+  if (quantize_input && !mx4_quantizable(route, rows, I, O)) return 0;
   if (route == MX4_PREFILL) return mx4h_workspace_bytes(nprob, rows, I, O);
   if (route == MX4_GEMM) return mx4_gemm_workspace_bytes(nprob, rows, O, I);
   if (route == MX4_TILE) return mx4_tile_workspace_bytes(nprob, rows, O, I);
@@ -358,11 +366,13 @@ extern "C" int rwkv7mi_mxfp4_linear(int nprob, const void* const* x, const uint8
     if (p.epilogue == RWKV7MI_EPI_RESIDUAL && !p.residual) return fail(RWKV7MI_EINVAL, w + ": residual missing");
   }
   const bool bf = act_dtype == RWKV7MI_BF16;
+  const Mx4Route route = mx4_route(nprob, rows, I, O, quantize_input);
+  if (quantize_input && !mx4_quantizable(route, rows, I, O))
+    return fail(RWKV7MI_EINVAL, w + ": too large to quantise (split the rows)");
   const int64_t need = rwkv7mi_mxfp4_linear_workspace_bytes(nprob, rows, O, I, act_dtype, quantize_input);
   if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < need))
     return fail(RWKV7MI_ESIZE, w + ": workspace missing, unaligned or smaller than "
                                    "rwkv7mi_mxfp4_linear_workspace_bytes");
-  const Mx4Route route = mx4_route(nprob, rows, I, O, quantize_input);
   if (route == MX4_PREFILL) return mx4h_run(b, nprob, act_dtype, ws, ws_bytes, stream);
   if (route == MX4_GEMM) return mx4_gemm_run(b, nprob, act_dtype, ws, stream);
   if (route == MX4_TILE) return mx4_tile_run(b, nprob, act_dtype, ws, stream);
