@@ -195,13 +195,8 @@ __global__ __launch_bounds__(256) void mm8h_dequant_kernel(const MhDeqBatch D) {
   }
 }
 
-template <bool MX>
-__device__ __forceinline__ float mh_relu(float w) {
-  return MX ? (w < 0.f ? 0.f : w) : fmaxf(w, 0.f);
-}
-
 // The tail of a column vector run: y = epilogue(v + bias), 8 columns from c0
-template <typename TA, bool MX>
+template <typename TA>
 __device__ __forceinline__ void mh_store8(const MhProb& P, int64_t row, int c0, int O, float (&v)[8]) {
   using E = typename MhTypes<TA>::E;
   using V = typename MhTypes<TA>::V;
@@ -217,7 +212,7 @@ __device__ __forceinline__ void mh_store8(const MhProb& P, int64_t row, int c0, 
     for (int e = 0; e < 8; ++e) {
       float w = v[e];
       if (P.epilogue == RWKV7MI_EPI_RELU2) {
-        w = mh_relu<MX>(w);
+        w = fmaxf(w, 0.f);
         w = w * w;
       }
       o8[e] = (E)w;
@@ -229,7 +224,7 @@ __device__ __forceinline__ void mh_store8(const MhProb& P, int64_t row, int c0, 
       if (c0 + e >= O) continue;
       float w = v[e];
       if (P.epilogue == RWKV7MI_EPI_RELU2) {
-        w = mh_relu<MX>(w);
+        w = fmaxf(w, 0.f);
         w = w * w;
       } else if (P.epilogue == RWKV7MI_EPI_RESIDUAL) {
         w += ld(reinterpret_cast<const TA*>(P.residual), oi + e);
@@ -241,7 +236,7 @@ __device__ __forceinline__ void mh_store8(const MhProb& P, int64_t row, int c0, 
 
 // S > 1: one thread adds the S fp32 partials of 8 columns of a row in split
 // order and applies the epilogue.  Memory-bound: 4 S + 2 (+ 2) bytes a value.
-template <typename TA, bool MX>
+template <typename TA>
 __global__ __launch_bounds__(256) void mm8h_reduce_kernel(const MhBatch B) {
   const MhProb& P = B.p[blockIdx.y];
   const int cols = (int)(B.ldp / 8);
@@ -260,21 +255,23 @@ __global__ __launch_bounds__(256) void mm8h_reduce_kernel(const MhBatch B) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += a[e];
   }
-  if constexpr (MX) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) if (c0 + e < B.O) v[e] *= P.cs[c0 + e];
-  }
   const TA* bp = reinterpret_cast<const TA*>(P.bias);
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] += bp && c0 + e < B.O ? to_f32(bp[c0 + e]) : 0.f;
-  mh_store8<TA, MX>(P, row, c0, B.O, v);
+  mh_store8<TA>(P, row, c0, B.O, v);
+}
+
+template <bool MX>
+__device__ __forceinline__ float mh_relu(float w) {
+  return MX ? (w < 0.f ? 0.f : w) : fmaxf(w, 0.f);
 }
 
 // FULLK: I is a multiple of 64 (no step ends inside a 16-byte chunk's range).
 // SPLIT: blockIdx.z takes B.sps of the steps and leaves fp32 partial tiles (an
 // instance of its own: the bounds and the second epilogue cost the unsplit
 // kernel 4%).  MX: the records are an MXFP4 weight's: a factor per column (its row is
-// scaled by a power of two), and relu^2 keeps a NaN
+// scaled by a power of two), and relu^2 keeps a NaN; they are used from 1024 tiles on,
+// which need no splits
 template <bool FULLK, bool SPLIT, typename TA, bool MX>
 __global__ __launch_bounds__(MH_THREADS, 1) void mm8h_gemm_kernel(const MhBatch B) {
   using E = typename MhTypes<TA>::E;
@@ -605,7 +602,7 @@ static int mh_gemm_launch(MhBatch& b, int nprob, int64_t rows, int64_t I, int64_
   // weights' bytes gets no splits)
   b.ldp = (O + 31) / 32 * 32;
   const int64_t wb = mh_weight_bytes(nprob, I, O), pb = mh_part_bytes(nprob, rows, O);
-  b.S = mh_splits(nprob, rows, I, O);
+  b.S = MX ? 1 : mh_splits(nprob, rows, I, O);
   if (ws_bytes < wb + (b.S > 1 ? b.S * pb : 0)) b.S = 1;
   b.sps = (b.SB + b.S - 1) / b.S;
   b.part = reinterpret_cast<float*>(static_cast<char*>(ws) + wb);
@@ -616,12 +613,13 @@ static int mh_gemm_launch(MhBatch& b, int nprob, int64_t rows, int64_t I, int64_
                        as_stream(stream), b);
     if (int rc = check_launch("mm8h_gemm_kernel")) return rc;
     if (b.S == 1) return (int)RWKV7MI_OK;
-    hipLaunchKernelGGL((mm8h_reduce_kernel<TA, MX>), dim3((unsigned)((rows * (b.ldp / 8) + 255) / 256), (unsigned)nprob),
+    hipLaunchKernelGGL(mm8h_reduce_kernel<TA>, dim3((unsigned)((rows * (b.ldp / 8) + 255) / 256), (unsigned)nprob),
                        dim3(256), 0, as_stream(stream), b);
     return check_launch("mm8h_reduce_kernel");
   };
   static std::atomic<uint64_t> raised[3];
-  if (b.S > 1) return launch(&mm8h_gemm_kernel<true, true, TA, MX>, raised[0]);
+  if constexpr (!MX)
+    if (b.S > 1) return launch(&mm8h_gemm_kernel<true, true, TA, MX>, raised[0]);
   return I % 64 == 0 ? launch(&mm8h_gemm_kernel<true, false, TA, MX>, raised[1])
                      : launch(&mm8h_gemm_kernel<false, false, TA, MX>, raised[2]);
 }
@@ -776,9 +774,9 @@ extern "C" int rwkv7mi_dense_gemm_prefill_ws(int nprob, const void* const* x, co
     if (S == 1) return RWKV7MI_OK;
     const dim3 rgrid((unsigned)((rows * (t.ldp / 8) + 255) / 256), (unsigned)nprob);
     if (act_dtype == RWKV7MI_BF16)
-      hipLaunchKernelGGL((mm8h_reduce_kernel<__hip_bfloat16, false>), rgrid, dim3(256), 0, as_stream(stream), t);
+      hipLaunchKernelGGL(mm8h_reduce_kernel<__hip_bfloat16>, rgrid, dim3(256), 0, as_stream(stream), t);
     else
-      hipLaunchKernelGGL((mm8h_reduce_kernel<__half, false>), rgrid, dim3(256), 0, as_stream(stream), t);
+      hipLaunchKernelGGL(mm8h_reduce_kernel<__half>, rgrid, dim3(256), 0, as_stream(stream), t);
     return check_launch("mm8h_reduce_kernel");
   }
   const int64_t per_prob = mh_weight_bytes(1, I, O);
@@ -873,9 +871,8 @@ bool mx4h_supported(int64_t rows, int64_t I, int64_t O) {
          (O + MH_N - 1) / MH_N * ((mx4h_chunk(rows, I) + MH_M - 1) / MH_M) < INT32_MAX / 64;
 }
 
-int64_t mx4h_workspace_bytes(int nprob, int64_t rows, int64_t I, int64_t O) {
-  return mx4h_factor_bytes(nprob, O) +
-         rwkv7mi_mm8t_gemm_prefill_split_ws_bytes(nprob, mx4h_chunk(rows, I), I, O);
+int64_t mx4h_workspace_bytes(int nprob, int64_t I, int64_t O) {
+  return mx4h_factor_bytes(nprob, O) + mh_weight_bytes(nprob, I, O);
 }
 
 template <typename TA>

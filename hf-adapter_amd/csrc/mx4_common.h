@@ -131,7 +131,7 @@ int mx4_tile_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, void* st
 // Products through fp16 / bf16 records of the weight and the 256 x 256 GEMM of
 // mm8h.hip: whether it takes these shapes, its workspace, its launches.
 bool mx4h_supported(int64_t rows, int64_t I, int64_t O);
-int64_t mx4h_workspace_bytes(int nprob, int64_t rows, int64_t I, int64_t O);
+int64_t mx4h_workspace_bytes(int nprob, int64_t I, int64_t O);
 int mx4h_run(const Mx4Batch& b, int nprob, int act_dtype, void* ws, int64_t ws_bytes, void* stream);
 
 }  // namespace rwkv7mi

@@ -329,7 +329,7 @@ extern "C" int64_t rwkv7mi_mxfp4_linear_workspace_bytes(int nprob, int64_t rows,
   if (nprob < 1 || nprob > MX4_MAXPROB || rows <= 0 || O <= 0 || I <= 0) return 0;
   const Mx4Route route = mx4_route(nprob, rows, I, O, quantize_input);
   if (quantize_input && !mx4_quantizable(route, rows, I, O)) return 0;
-  if (route == MX4_PREFILL) return mx4h_workspace_bytes(nprob, rows, I, O);
+  if (route == MX4_PREFILL) return mx4h_workspace_bytes(nprob, I, O);
   if (route == MX4_GEMM) return mx4_gemm_workspace_bytes(nprob, rows, O, I);
   if (route == MX4_TILE) return mx4_tile_workspace_bytes(nprob, rows, O, I);
   const int64_t part = mx4_rows_part_bytes(nprob, rows, O, I, quantize_input);

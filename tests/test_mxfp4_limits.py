@@ -26,3 +26,12 @@ def test_quantized_inputs_of_2_to_the_32_lanes(rows, n, m):
     need = lib.rwkv7mi_mxfp4_linear_workspace_bytes(1, rows // 8, m, n, _lib.F16, 1)
     assert need > 0
     assert lib.rwkv7mi_mxfp4_linear1(A, A, A, None, None, A, 0, rows // 8, m, n, _lib.F16, 1, None, 0, None) == -3
+
+
+@pytest.mark.parametrize("rows,n,m", [(262144, 1 << 21, 256), (65536, 4096, 4096), (4001, 96, 16325)])
+def test_long_batches_ask_for_the_weight_in_16_bits_alone(rows, n, m):
+    """Also for inputs so wide that a chunk of rows below 2 GiB is a single tile."""
+    from rwkv7mi import _lib
+
+    records, factors = 2 * -(-m // 32) * -(-n // 64) * 2048, -(-4 * m // 256) * 256
+    assert _lib.load().rwkv7mi_mxfp4_linear_workspace_bytes(1, rows, m, n, _lib.BF16, 0) == records + factors
