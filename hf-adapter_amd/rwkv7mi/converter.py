@@ -480,10 +480,11 @@ def convert(args: argparse.Namespace) -> Path:
     weights = torch.load(args.input, weights_only=True, map_location="cpu", mmap=bool(args.low_memory))
     cfg, state = convert_state_dict(weights, dtype)
     out = save_hf_directory(args.output, cfg, state, dtype_name=dtype_name)
-    if args.prepack_mm8 or args.prepack_mxfp4:
+    mxfp4 = bool(getattr(args, "prepack_mxfp4", False))  # (a caller's Namespace may lack it)
+    if args.prepack_mm8 or mxfp4:
         from .model import NativeRWKV7ForCausalLM
 
-        cfg.use_native_mm8, cfg.use_native_mxfp4 = bool(args.prepack_mm8), bool(args.prepack_mxfp4)
+        cfg.use_native_mm8, cfg.use_native_mxfp4 = bool(args.prepack_mm8), mxfp4
         model = NativeRWKV7ForCausalLM(cfg, state, device=args.device, dtype=dtype)
         save_prepacked(model, out, source_state=state)
     print(f"Saved RWKV-7 model to: {out}")
