@@ -477,10 +477,12 @@ def load_prepacked(path, *, device="cuda", dtype=torch.float16,
 # ------------------------------------------------------------- CLI
 def convert(args: argparse.Namespace) -> Path:
     dtype_name, dtype = DTYPES[args.precision]
+    mxfp4 = bool(getattr(args, "prepack_mxfp4", False))  # (a caller's Namespace may lack it)
+    if mxfp4 and dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"MXFP4 modules need an fp16 or bf16 model, got {args.precision}")
     weights = torch.load(args.input, weights_only=True, map_location="cpu", mmap=bool(args.low_memory))
     cfg, state = convert_state_dict(weights, dtype)
     out = save_hf_directory(args.output, cfg, state, dtype_name=dtype_name)
-    mxfp4 = bool(getattr(args, "prepack_mxfp4", False))  # (a caller's Namespace may lack it)
     if args.prepack_mm8 or mxfp4:
         from .model import NativeRWKV7ForCausalLM
 

@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import argparse
 
+import pytest
 import torch
 
 
@@ -23,3 +24,11 @@ def test_arguments_of_a_caller_that_knows_no_mxfp4(tmp_path, monkeypatch):
     torch.save({}, tmp_path / "model.pth")
     out = converter.convert(_args(tmp_path, input=str(tmp_path / "model.pth")))
     assert (out / "config.json").exists() and (out / "model.safetensors").exists()
+
+
+def test_mxfp4_of_an_fp32_checkpoint_is_refused_before_anything_is_read(tmp_path):
+    from rwkv7mi import converter
+
+    with pytest.raises(ValueError, match="fp16 or bf16"):
+        converter.convert(_args(tmp_path, precision="fp32", prepack_mxfp4=True))
+    assert not (tmp_path / "out").exists()
