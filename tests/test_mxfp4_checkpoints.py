@@ -89,3 +89,21 @@ def test_a_manifest_entry_that_is_no_truth_value_is_refused(tmp_path):
     (tmp_path / "manifest.json").write_text(json.dumps(manifest))
     with pytest.raises(ValueError, match="quantize_input"):
         _load(tmp_path)
+
+
+def test_a_prepacked_directory_is_not_taken_for_the_other_format(tmp_path):
+    """Asked for the other quantisation by name or by a config, a prepacked directory is refused."""
+    from rwkv7mi import converter as conv
+    from rwkv7mi.model import NativeRWKV7Config
+
+    _pack_model({}, head=True).save_pretrained(tmp_path)
+    assert list(_flags(_load(tmp_path, use_native_mxfp4=True))) == ["lm_head"]
+    with pytest.raises(ValueError, match="MXFP4"):
+        _load(tmp_path, use_native_mm8=True)
+    cfg = NativeRWKV7Config(vocab_size=96, hidden_size=64, num_hidden_layers=1, use_native_mm8=True)
+    with pytest.raises(ValueError, match="MXFP4"):
+        _load(tmp_path, config=cfg)
+    manifest = {"format": conv.PREPACKED_FORMAT, "packer_version": conv.PACKER_VERSION, "modules": []}
+    (tmp_path / "manifest.json").write_text(json.dumps(manifest))
+    with pytest.raises(ValueError, match="MM8"):
+        _load(tmp_path, use_native_mxfp4=True)
