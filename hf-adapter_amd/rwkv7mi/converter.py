@@ -275,9 +275,9 @@ def load_pretrained(path, *, device="cuda", dtype=torch.float16, use_native_mm8:
 
     p = Path(path)
     if (p / "manifest.json").exists():
-        four = json.loads((p / "manifest.json").read_text()).get("format") == MXFP4_FORMAT
-        if use_native_mm8 if four else use_native_mxfp4:
-            raise ValueError(f"{p} holds {'MXFP4' if four else 'MM8'} modules, not {'MM8' if four else 'MXFP4'} ones")
+        fmt = json.loads((p / "manifest.json").read_text()).get("format")
+        if (fmt == MXFP4_FORMAT and use_native_mm8) or (fmt == PREPACKED_FORMAT and use_native_mxfp4):
+            raise ValueError(f"{p} holds {'MXFP4' if fmt == MXFP4_FORMAT else 'MM8'} modules, not the ones asked for")
         return load_prepacked(p, device=device, dtype=dtype, native_mxfp4_quantize_input=native_mxfp4_quantize_input)
     cfg, state = load_hf_directory(p)
     if use_native_mm8 is not None:
