@@ -135,3 +135,22 @@ def test_linears_that_cannot_be_grouped_run_one_by_one(last):
     outs = [torch.empty(5, 40, dtype=torch.float16, device="cuda") for _ in range(3)]
     QuantLinear.apply_group([BlockFloatLinear(m) for m in mods], [x, x, x], outs)
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_modules_of_fp32_linears_run_in_16_bits():
+    """An fp32 model is quantised from its fp32 weights and converted afterwards."""
+    import rwkv7mi as mi
+
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Linear(64, 40), torch.nn.ReLU()).cuda()
+    codes, scales = mi.quantize_mxfp4(net[0].weight.data)
+    bias = net[0].bias.data.clone()
+    x = torch.randn(5, 64, device="cuda")
+    assert mi.quantize_model_mxfp4(net, min_params=1) == 1
+    with pytest.raises(ValueError, match="fp16 or bf16"):
+        net(x)
+    for dt in (torch.float16, torch.bfloat16):
+        bias = bias.to(dt)
+        y = net.to(dt)(x.to(dt))
+        assert torch.equal(net[0].bias, bias)
+        assert torch.equal(y, mi.mxfp4_linear(x.to(dt), codes, scales, bias=bias).relu())
