@@ -31,9 +31,11 @@
 // fill the chip K is split over workgroups and a second launch adds the fp32
 // partials.
 //
-// 16384 x 4096 -> 16384: 610 to 690 us with the quantiser, 3.4 PFLOP/s.  The main loop alone
-// takes 500: random codes at 4.8 PFLOP/s draw the card's power limit (7.4 with constant
-// ones), and then all CUs write their tiles, 537 MB, at about the same time.
+// 16384 x 4096 -> 16384: 640 us with the quantiser, 3.4 PFLOP/s.  By its time over K (398 us
+// at 2048 inputs, 622 at 4096, 1041 at 8192) the main loop takes 430 of them, 5.1 PFLOP/s of
+// the 6.3 of a bare loop of these MFMAs on random codes; the rest is the start and the tiles'
+// stores, 537 MB that all CUs write at about the same time.  Constant codes take 476 us (the
+// bare loop 9.1 PFLOP/s): random ones run at a lower clock.
 #include "mx4_gemm.h"
 
 namespace rwkv7mi {

@@ -22,8 +22,11 @@
 // times every scale, so the codes of a step (bf16: of a unit) are scaled by its largest
 // scale and the sums by that one's factor (mx4_common.h).
 //
-// The weight's bytes bound it: 1 x 4096 -> 16384 11.9 us (36 MB; 9.5 from the caches),
-// 8 x 4096 -> 65536 35 us, 4.0 TB/s of the 5.4 that a copy reaches.
+// 8 x 4096 -> 65536 takes 33.5 us, 4.3 TB/s of the 5.4 that a copy reaches.  Smaller
+// weights are bound by latency, a chain of x, the first codes and the sums' meeting in
+// LDS: 1 x 4096 -> 16384 11.8 us for the 6.6 of its bytes (9.5 with them in the caches),
+// 16 x 4096 -> 16384 14.6 to 15.0; with the second launch 1 x 16384 -> 4096 14.3, 16 rows
+// 17.7 (the same bytes).
 #include <algorithm>
 
 #include "mx4_common.h"
@@ -223,7 +226,7 @@ __global__ __launch_bounds__(256) void mx4_rows_reduce_kernel(const Mx4Rows R) {
 }
 
 // Workgroups that share K: up to 16 units of 512 inputs in one, 8 where there are
-// more (16 x 16384 -> 4096: 21.0 us with 8, 21.8 with 16; 1 row 15.9 and 16.7).
+// more (16 x 16384 -> 4096: 0.8 us less with 8 than with 16, and for 1 row).
 static int mx4_rows_tiles(int64_t rows, bool A4) { return rows <= 16 || A4 ? 1 : 2; }
 static int mx4_rows_splits(int64_t rows, int64_t I, bool A4) {
   return I <= (mx4_rows_tiles(rows, A4) > 1 ? 4096 : 8192) ? 1 : (int)((I + 4095) / 4096);
@@ -295,14 +298,14 @@ static double mx4_rows_us(int nprob, int64_t rows, int64_t O, int64_t I) {
 // its passes over the weight, one a tile of 32 rows, are estimated to take no longer than
 // the larger tiles.  16-bit rows on it and on those: 128 x 4096 -> 4096 16.5 and 23.4 us,
 // 40 x 8192 -> 2048 13.1 and 19.5, 256 x 4096 -> 4096 25.6 and 26.7, 32 x 4096 -> 65536
-// 52.5 and 57.3; 96 x 4096 -> 16384 41.5 and 36.2, 128 x 16384 -> 4096 51.7 and 40.0.
+// 52.5 and 57.3; 96 x 4096 -> 16384 41.5 and 34.8, 128 x 16384 -> 4096 51.7 and 39.5.
 // MXFP4 rows, 16 a tile, by rows x weight: 128 x 4096 -> 4096 16.6 and 19.7, 64 x 4096 ->
 // 16384 26.0 and 26.0.  And what the others' offsets cannot hold.  Else the 64- to
 // 256-row tiles.  16-bit rows from 1024
 // tiles of 256 x 256 on write the weight out in 16 bits and run the GEMM of mm8h.hip:
 // without conversions between its MFMAs it holds a higher clock over such long calls
 // (16384 x 4096 -> 16384 1636 us, on the tiles 2000), and the pass over the weight
-// is small against them (1000 rows, 256 tiles: 150 and 114).
+// is small against them (1000 rows, 256 tiles: 150 and 115).
 enum Mx4Route { MX4_ROWS, MX4_TILE, MX4_GEMM, MX4_PREFILL };
 static Mx4Route mx4_route(int nprob, int64_t rows, int64_t I, int64_t O, int quantize_input) {
   if (rows <= 16) return MX4_ROWS;

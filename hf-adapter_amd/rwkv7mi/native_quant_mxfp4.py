@@ -267,7 +267,9 @@ class MXFP4Linear(torch.nn.Module):
 def quantize_model_mxfp4(model, *, min_params: int = 8_000_000, policy: str = "memory",
                          quantize_input: bool = False) -> int:
     """Swap eligible ``nn.Linear`` modules for :class:`MXFP4Linear`; returns the count.
-    Linears whose ``in_features`` is not a multiple of 32 stay."""
+    Linears whose ``in_features`` is not a multiple of 32 stay.  Weights may be fp32, but
+    the modules run on fp16 or bf16 activations: an fp32 model is converted (``model.half()``
+    or ``model.bfloat16()``) before it is called."""
     policy = normalize_native_mm_policy(policy)
     targets = [n for n, m in model.named_modules()
                if isinstance(m, torch.nn.Linear) and int(m.weight.shape[1]) % BLOCK == 0

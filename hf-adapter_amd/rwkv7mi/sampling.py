@@ -105,8 +105,9 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     * a token whose bit in ``allowed`` is clear becomes ``-inf``, whatever it held
       (int32 words ``[ceil(n / 32)]`` or one row of them each; bit ``t % 32`` of word ``t // 32``).
 
-    ``history [rows, L]`` holds int32 or int64 tokens, of which the first
-    ``lengths[row]`` (int32; default all) count; entries outside ``0..n-1`` are ignored.
+    ``history [rows, L]`` (at most 2^23 a row, 65535 rows) holds int32 or int64 tokens, of
+    which the first ``lengths[row]`` (int32; default all) count; entries outside
+    ``0..n-1`` are ignored.
     The penalties are numbers or one value per row (a ``penalty_decay`` tensor is clamped
     to 0..1).  The arithmetic is fp32, rounded once to ``out``'s type: ``logits``' own
     (the default) or fp32.  ``out`` may be ``logits`` itself.
