@@ -1757,7 +1757,11 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
             given = lambda value, name: getattr(config, name, None) if value is None else value
             native_mxfp4_policy = given(native_mxfp4_policy, "native_mxfp4_policy")
             native_mxfp4_min_params = given(native_mxfp4_min_params, "native_mxfp4_min_params")
-            native_mxfp4_quantize_input = given(native_mxfp4_quantize_input, "native_mxfp4_quantize_input")
+            flag = "native_mxfp4_quantize_input"
+            # (what a prepacked directory's own config says holds for the modules its manifest is silent on)
+            if not (path / "manifest.json").exists() or getattr(config, flag, None) != json.loads(
+                    (path / "config.json").read_text()).get(flag, False):
+                native_mxfp4_quantize_input = given(native_mxfp4_quantize_input, flag)
         return load_pretrained(path, device=device, dtype=want, use_native_mm8=use_native_mm8,
                                native_mm8_policy=native_mm8_policy, native_mm8_min_params=native_mm8_min_params,
                                use_native_mxfp4=use_native_mxfp4, native_mxfp4_policy=native_mxfp4_policy,

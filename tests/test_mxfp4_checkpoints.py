@@ -107,3 +107,18 @@ def test_a_prepacked_directory_is_not_taken_for_the_other_format(tmp_path):
     (tmp_path / "manifest.json").write_text(json.dumps(manifest))
     with pytest.raises(ValueError, match="MM8"):
         _load(tmp_path, use_native_mxfp4=True)
+
+
+def test_the_directorys_own_config_keeps_each_modules_setting(tmp_path):
+    """``AutoModelForCausalLM`` hands over the config it read from the directory; a config that
+    says otherwise than the directory's is a setting for every module."""
+    from rwkv7mi.model import NativeRWKV7Config
+
+    model = _pack_model(dict.fromkeys(FFN, True), head=False)
+    model.save_pretrained(tmp_path)
+    own = NativeRWKV7Config.from_pretrained(tmp_path)
+    assert own.use_native_mxfp4 and own.native_mxfp4_quantize_input
+    assert _flags(_load(tmp_path, config=own)) == _flags(model)
+    own.native_mxfp4_quantize_input = False
+    assert set(_flags(_load(tmp_path, config=own)).values()) == {False}
+    assert set(_flags(_load(tmp_path, config=own, native_mxfp4_quantize_input=True)).values()) == {True}
