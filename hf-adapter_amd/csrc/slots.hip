@@ -38,6 +38,110 @@ __global__ __launch_bounds__(256) void slot_copy_kernel(const SlotCopy C) {
     d[i] = s ? s[i] : make_uint4(0u, 0u, 0u, 0u);
 }
 
+// Rows of several tensors moved by one index in one launch:
+//   dst[o][d(r)] = the old src[o][s(r)]   for every outer index o and every r,
+// as if all sources were read before any destination is written, so rows may
+// trade places in place; s(r) out of range (-1) writes zeros, d(r) out of range
+// nothing, and a row onto itself is left alone.
+//
+// A workgroup takes a window of the row's bytes of one tensor and outer index
+// for all rows: it gathers the rows that move into a list, loads all their
+// windows into registers, and stores them behind a barrier.  What it reads
+// it alone writes, so no launch but this one is needed, and a source with many
+// destinations comes from memory once.  The window shrinks as the rows grow
+// (THREADS x LOADS units of 16 bytes over the rows, a power of two).  HBM-bound.
+namespace {
+
+constexpr int RW_TENSORS = 24;   // of a launch
+constexpr int RW_LIST = 192;     // indices that travel with the launch
+constexpr int RW_FEW = 64;       // rows of the small workgroup
+constexpr int RW_MOST = 2048;    // rows of the large one (windows of 64 bytes)
+
+struct RwTensor {
+  const char* src;
+  char* dst;
+  int64_t src_outer, dst_outer, src_row, dst_row;  // strides in bytes
+  uint32_t units, windows;                         // of a row, units of `unit` bytes
+  int64_t outer;
+  int unit, same;                                  // same: in place
+};
+
+struct RwArgs {
+  RwTensor t[RW_TENSORS];
+  uint32_t first[RW_TENSORS + 1];  // the tensor's first workgroup
+  int n, rows, log_window, split;  // split: rows of a workgroup
+  int64_t src_rows, dst_rows;
+  const int64_t *src_index, *dst_index;  // on the device (null: the list, or the identity)
+  int listed_src, listed_dst;
+  int src_list[RW_LIST], dst_list[RW_LIST];
+};
+
+template <typename V>
+__device__ __forceinline__ void rw_hold(V& v) {  // v is in its registers here
+  if constexpr (sizeof(V) == 16)
+    asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
+  else
+    asm volatile("" : "+v"(v));
+}
+
+template <int THREADS, int LOADS, typename V, typename HELD>
+__device__ __forceinline__ void rw_window(const RwTensor& t, int64_t o, uint32_t w0, int log_window, int n, const int* src,
+                                          const int* dst) {
+  const int tid = threadIdx.x, mask = (1 << log_window) - 1;
+  HELD r[LOADS];
+#pragma unroll
+  for (int u = 0; u < LOADS; ++u) {
+    const int j = tid + THREADS * u, k = j >> log_window;
+    const uint32_t c = w0 + (uint32_t)(j & mask);
+    r[u] = HELD{};
+    if (k < n && c < t.units && src[k] >= 0)
+      r[u] = static_cast<HELD>(reinterpret_cast<const V*>(t.src + o * t.src_outer + src[k] * t.src_row)[c]);
+  }
+#pragma unroll
+  for (int u = 0; u < LOADS; ++u) rw_hold(r[u]);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < LOADS; ++u) {
+    const int j = tid + THREADS * u, k = j >> log_window;
+    const uint32_t c = w0 + (uint32_t)(j & mask);
+    if (k < n && c < t.units) reinterpret_cast<V*>(t.dst + o * t.dst_outer + dst[k] * t.dst_row)[c] = static_cast<V>(r[u]);
+  }
+}
+
+}  // namespace
+
+template <int THREADS, int LOADS, int ROWS>
+__global__ __launch_bounds__(THREADS) void rows_move_kernel(const RwArgs A) {
+  __shared__ int src[ROWS], dst[ROWS], moving;
+  int f = 0;
+  while (f + 1 < A.n && blockIdx.x >= A.first[f + 1]) ++f;
+  const RwTensor& t = A.t[f];
+  const uint32_t at = blockIdx.x - A.first[f];
+  const int64_t o = at / t.windows;
+  const uint32_t w = at % t.windows;
+  if (threadIdx.x == 0) moving = 0;
+  __syncthreads();
+  const int r1 = min(A.rows, ((int)blockIdx.y + 1) * A.split);
+  for (int r = (int)blockIdx.y * A.split + threadIdx.x; r < r1; r += THREADS) {
+    const int64_t s = A.src_index ? A.src_index[r] : A.listed_src ? A.src_list[r] : r;
+    const int64_t d = A.dst_index ? A.dst_index[r] : A.listed_dst ? A.dst_list[r] : r;
+    if (d >= 0 && d < A.dst_rows && !(t.same && s == d)) {
+      const int p = atomicAdd(&moving, 1);
+      src[p] = s >= 0 && s < A.src_rows ? (int)s : -1;
+      dst[p] = (int)d;
+    }
+  }
+  __syncthreads();
+  const int n = moving;
+  if (n == 0) return;
+  if (t.unit == 16)
+    rw_window<THREADS, LOADS, uint4, uint4>(t, o, w << A.log_window, A.log_window, n, src, dst);
+  else if (t.unit == 4)
+    rw_window<THREADS, LOADS, uint32_t, uint32_t>(t, o, w << A.log_window, A.log_window, n, src, dst);
+  else
+    rw_window<THREADS, LOADS, uint8_t, uint32_t>(t, o, w << A.log_window, A.log_window, n, src, dst);
+}
+
 }  // namespace rwkv7mi
 
 using namespace rwkv7mi;
@@ -60,4 +164,76 @@ extern "C" int rwkv7mi_slot_copy(const void* src, int64_t src_layer_stride, int6
   hipLaunchKernelGGL(slot_copy_kernel, dim3((unsigned)chunks, (unsigned)nrows, (unsigned)nlayers), dim3(256), 0,
                      as_stream(stream), c);
   return check_launch("slot_copy_kernel");
+}
+
+extern "C" int rwkv7mi_rows_move(int n, const rwkv7mi_rows* tensors, int64_t src_rows, int64_t dst_rows, int64_t nrows,
+                                 const int64_t* src_index, const int64_t* dst_index, const int64_t* src_list,
+                                 const int64_t* dst_list, int disjoint, void* stream) {
+  const std::string w("rows_move");
+  if (n < 0 || n > RW_TENSORS || (n && !tensors)) return fail(RWKV7MI_EINVAL, w + ": at most 24 tensors");
+  if (nrows < 0 || src_rows < 0 || dst_rows < 0 || src_rows > INT32_MAX || dst_rows > INT32_MAX)
+    return fail(RWKV7MI_EINVAL, w + ": bad rows");
+  if ((src_list || dst_list) && nrows > RW_LIST) return fail(RWKV7MI_EINVAL, w + ": at most 192 indices in host lists");
+  if ((src_list && src_index) || (dst_list && dst_index))
+    return fail(RWKV7MI_EINVAL, w + ": a list and a device index of the same rows");
+  RwArgs a{};
+  bool same = false;
+  for (int i = 0; i < n; ++i) {
+    const rwkv7mi_rows& t = tensors[i];
+    if (t.row_bytes < 0 || t.outer < 0) return fail(RWKV7MI_EINVAL, w + ": bad shape");
+    if (nrows == 0 || t.row_bytes == 0 || t.outer == 0) continue;
+    if (!t.src || !t.dst) return fail(RWKV7MI_EINVAL, w + ": null pointer");
+    RwTensor& q = a.t[a.n++];
+    q.src = static_cast<const char*>(t.src);
+    q.dst = static_cast<char*>(t.dst);
+    q.src_outer = t.src_outer_stride;
+    q.dst_outer = t.dst_outer_stride;
+    q.src_row = t.src_row_stride;
+    q.dst_row = t.dst_row_stride;
+    q.same = t.src == t.dst;
+    if (q.same && (q.src_outer != q.dst_outer || q.src_row != q.dst_row))
+      return fail(RWKV7MI_EINVAL, w + ": a tensor in place keeps its strides");
+    same |= q.same;
+    const uint64_t align = (uint64_t)reinterpret_cast<uintptr_t>(t.src) | (uint64_t)reinterpret_cast<uintptr_t>(t.dst) |
+                           (uint64_t)t.src_outer_stride | (uint64_t)t.dst_outer_stride | (uint64_t)t.src_row_stride |
+                           (uint64_t)t.dst_row_stride | (uint64_t)t.row_bytes;
+    q.unit = align % 16 == 0 ? 16 : align % 4 == 0 ? 4 : 1;
+    if (t.row_bytes / q.unit > INT32_MAX) return fail(RWKV7MI_EINVAL, w + ": a row is too long");
+    q.units = (uint32_t)(t.row_bytes / q.unit);
+    q.outer = t.outer;
+  }
+  if (a.n == 0) return RWKV7MI_OK;
+  if (same && !disjoint && nrows > RW_MOST)
+    return fail(RWKV7MI_EINVAL, w + ": at most 2048 rows trade places in place");
+  // rows that may trade places stay in one workgroup
+  const bool few = !same || disjoint || nrows <= RW_FEW;
+  a.rows = (int)nrows;
+  a.split = few ? RW_FEW : RW_MOST;
+  const int64_t units = few ? 256 * 8 : 1024 * 8, held = std::min<int64_t>(nrows, a.split);
+  while ((units >> (a.log_window + 1)) >= held) ++a.log_window;
+  uint64_t blocks = 0;
+  for (int i = 0; i < a.n; ++i) {
+    a.first[i] = (uint32_t)blocks;
+    a.t[i].windows = (uint32_t)(((uint64_t)a.t[i].units + (1u << a.log_window) - 1) >> a.log_window);
+    if (a.t[i].outer > INT32_MAX || (blocks += (uint64_t)a.t[i].outer * a.t[i].windows) > INT32_MAX) return fail(RWKV7MI_EINVAL, w + ": too large");
+  }
+  a.first[a.n] = (uint32_t)blocks;
+  a.src_rows = src_rows;
+  a.dst_rows = dst_rows;
+  a.src_index = src_index;
+  a.dst_index = dst_index;
+  a.listed_src = src_list != nullptr;
+  a.listed_dst = dst_list != nullptr;
+  for (int64_t r = 0; r < nrows && (src_list || dst_list); ++r) {
+    if (src_list) a.src_list[r] = (int)std::max<int64_t>(std::min<int64_t>(src_list[r], INT32_MAX), -2);
+    if (dst_list) a.dst_list[r] = (int)std::max<int64_t>(std::min<int64_t>(dst_list[r], INT32_MAX), -2);
+  }
+  const int64_t chunks = (nrows + a.split - 1) / a.split;
+  if (chunks > 65535) return fail(RWKV7MI_EINVAL, w + ": too many rows");
+  const dim3 grid((unsigned)blocks, (unsigned)chunks);
+  if (few)
+    hipLaunchKernelGGL((rows_move_kernel<256, 8, RW_FEW>), grid, dim3(256), 0, as_stream(stream), a);
+  else
+    hipLaunchKernelGGL((rows_move_kernel<1024, 8, RW_MOST>), grid, dim3(1024), 0, as_stream(stream), a);
+  return check_launch("rows_move_kernel");
 }

@@ -41,6 +41,8 @@ from .native_wkv_fp16 import (
     native_fp16_recurrent_should_use,
     native_fp16_sequence,
 )
+from .beam import BeamState, beam_select, beam_step
+from .state_rows import move_rows_, select_rows
 from .sampling import NativeLogitsProcessor, argmax_rows, process_logits
 from . import ops as _ops
 
@@ -77,6 +79,11 @@ __all__ = [
     "argmax_rows",
     "NativeLogitsProcessor",
     "process_logits",
+    "beam_select",
+    "beam_step",
+    "BeamState",
+    "select_rows",
+    "move_rows_",
     "native_fp16_recurrent_should_use",
     "native_fp16_recurrent_available",
     "native_fp16_recurrent_build_error",

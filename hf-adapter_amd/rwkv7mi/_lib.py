@@ -111,6 +111,13 @@ SIGNATURES = {
         _i32, [_c_p] * 10 + [_i64, _c_p, _c_p, _c_p, _c_p, _i64, _i64, _f32, _i32, _i32, _c_p]),
     "rwkv7mi_attn_mix_lora_chunks": (_i32, [_i64]),
     "rwkv7mi_slot_copy": (_i32, [_c_p, _i64, _i64, _c_p, _c_p, _i64, _i64, _c_p, _c_p, _i64, _i64, _i64, _c_p]),
+    "rwkv7mi_rows_move": (_i32, [_i32, _c_p, _i64, _i64, _i64] + [_c_p] * 4 + [_i32, _c_p]),
+    "rwkv7mi_beam_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "rwkv7mi_beam_select": (
+        _i32, [_c_p, _i64, _i64, _i64, _i64, _i32, _c_p, _i32, _i64, _c_p, _c_p, _c_p, _c_p, _sz, _c_p]),
+    "rwkv7mi_beam_step": (
+        _i32, [_c_p, _i64, _i64, _i64, _i64, _i32, _i32, _c_p, _i32, ctypes.c_double, _i32, _i64, _c_p, _c_p, _i64, _c_p,
+               _c_p, _c_p, _sz, _c_p]),
     "rwkv7mi_argmax_rows": (_i32, [_c_p, _i64, _i64, _i64, _i32, _c_p, _c_p, _c_p]),
     "rwkv7mi_argmax_workspace_bytes": (_sz, [_i64, _i64, _i32]),
     "rwkv7mi_argmax_rows_ws": (_i32, [_c_p, _i64, _i64, _i64, _i32, _c_p, _c_p, _c_p, _sz, _c_p]),

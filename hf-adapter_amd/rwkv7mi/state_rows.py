@@ -1,0 +1,205 @@
+"""Rows of several tensors moved by one index in one launch
+(``rwkv7mi_rows_move``): the batch edits of a recurrent cache (select, reorder,
+repeat: rwkv7_hf/model_cache.py:335-343, 368) and the state pool's forks, moves
+and fresh slots.  Byte moves, bit-exact, any dtype."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+MAX_TENSORS = 24  # of a launch
+MAX_LISTED = 192  # host indices that travel with the launch
+MAX_TRADING = 2048  # rows that may trade places in place
+
+
+def _family(t: torch.Tensor, dim: int, name: str):
+    """``(outer stride, row stride, row bytes, outer count, rows)`` of ``t`` in bytes, the
+    dimensions before ``dim`` as one and those behind it dense; None where they are not."""
+    es, shape, stride = t.element_size(), t.shape, t.stride()
+    n = len(shape)
+    if n <= dim:
+        raise ValueError(f"{name}: a tensor of {n} dimensions has no rows along dimension {dim}")
+    dense = 1
+    for i in range(n - 1, dim, -1):
+        if shape[i] != 1 and stride[i] != dense:
+            return None
+        dense *= shape[i]
+    outer, step = 1, 0
+    for i in range(dim - 1, -1, -1):
+        if shape[i] == 1:
+            continue
+        if outer > 1 and stride[i] != outer * step:
+            return None
+        if outer == 1:
+            step = stride[i]
+        outer *= shape[i]
+    rows = shape[dim]
+    return step * es, (stride[dim] if rows > 1 else dense) * es, dense * es, outer, rows
+
+
+def _apart(f) -> bool:
+    """Whether the rows of a family lie apart (they are written)."""
+    step, row, size, outer, rows = f
+    spans = sorted((abs(s), k) for s, k in ((row, rows), (step, outer)) if k > 1)
+    for s, k in spans:
+        if s < size:
+            return False
+        size = s * k
+    return True
+
+
+def _index(index, name: str):
+    """``index`` as a list of ints, or a one-dimensional int64 tensor of the GPU."""
+    if isinstance(index, torch.Tensor):
+        if index.dim() != 1 or index.is_floating_point() or index.is_complex() or index.dtype is torch.bool:
+            raise ValueError(f"{name}: an index is a one-dimensional tensor of integers")
+        return index.to(torch.int64).contiguous() if index.is_cuda else index.tolist()
+    return [int(i) for i in index]
+
+
+def _launch(families, src_rows, dst_rows, n, src, dst, disjoint, where, name):
+    """``families``: 8 numbers a tensor, as the library's ``rwkv7mi_rows``."""
+    if type(src) is list and len(src) > MAX_LISTED:
+        src = torch.tensor(src, dtype=torch.int64).to(where.device)
+    if type(dst) is list and len(dst) > MAX_LISTED:
+        dst = torch.tensor(dst, dtype=torch.int64).to(where.device)
+    on_host = lambda v: (ctypes.c_int64 * n)(*v) if type(v) is list else None  # noqa: E731
+    on_device = lambda v: v.data_ptr() if isinstance(v, torch.Tensor) else None  # noqa: E731
+    with _lib.on_device(where):
+        stream = _lib.stream_of(where)
+        for i in range(0, len(families), 8 * MAX_TENSORS):
+            part = families[i:i + 8 * MAX_TENSORS]
+            _lib.call("rwkv7mi_rows_move", len(part) // 8, (ctypes.c_int64 * len(part))(*part), src_rows, dst_rows, n,
+                      on_device(src), on_device(dst), on_host(src), on_host(dst), 1 if disjoint else 0, stream)
+
+
+def _same_rows(families, name):
+    rows = {f[4] for f in families}
+    if len(rows) != 1:
+        raise ValueError(f"{name}: tensors of {sorted(rows)} rows")
+    return rows.pop()
+
+
+def _on_gpu(tensors, index, name):
+    if not tensors:
+        raise ValueError(f"{name}: no tensors")
+    _lib.require_same_device(*tensors, *((index,) if isinstance(index, torch.Tensor) else ()), name=name)
+
+
+def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tensor]:
+    """``[t.index_select(dim, indices) for t in tensors]`` in one launch (24 tensors a
+    launch): the rows along ``dim`` of tensors that have as many.
+
+    ``indices``: integers (checked) or a one-dimensional integer tensor; -1, and on the
+    GPU any index out of range, gives a row of zeros.  ``out``: tensors to write instead of
+    new ones; they do not overlap ``tensors``.  Capturable where ``indices`` are on
+    the GPU or at most 192.
+    """
+    name = "select_rows"
+    tensors = list(tensors)
+    idx = _index(indices, name)
+    _on_gpu(tensors, idx, name)
+    if dim < 0:
+        raise ValueError(f"{name}: dim counts from the front")
+    n = len(idx) if type(idx) is list else idx.shape[0]
+    src = []
+    for i, t in enumerate(tensors):
+        f = _family(t, dim, name)
+        if f is None:
+            tensors[i] = t = t.contiguous()
+            f = _family(t, dim, name)
+        src.append(f)
+    rows = _same_rows(src, name)
+    if type(idx) is list and not all(-1 <= i < rows for i in idx):
+        raise IndexError(f"{name}: indices outside -1..{rows - 1}")
+    shapes = [(*t.shape[:dim], n, *t.shape[dim + 1:]) for t in tensors]
+    if out is None:
+        out = [t.new_empty(s) for t, s in zip(tensors, shapes)]
+        dst = [_family(o, dim, name) for o in out]
+    else:
+        out = list(out)
+        if len(out) != len(tensors):
+            raise ValueError(f"{name}: {len(out)} outputs for {len(tensors)} tensors")
+        for o, t, s in zip(out, tensors, shapes):
+            if tuple(o.shape) != s or o.dtype != t.dtype:
+                raise ValueError(f"{name}: an output is {tuple(o.shape)} {o.dtype}, not {s} {t.dtype}")
+        _on_gpu([tensors[0], *out], None, name)
+        dst = [_family(o, dim, name) for o in out]
+        if any(f is None or not _apart(f) for f in dst):
+            raise ValueError(f"{name}: the rows of an output are dense and apart")
+        if any(_lib.overlap(o, t) for o in out for t in tensors) or _lap(out):
+            raise ValueError(f"{name}: outputs overlap")
+    flat = []
+    for t, o, f, g in zip(tensors, out, src, dst):
+        flat += (t.data_ptr(), o.data_ptr(), f[0], f[1], g[0], g[1], f[2], f[3])
+    if n:
+        _launch(flat, rows, n, n, idx, None, True, tensors[0], name)
+    return out
+
+
+def _lap(tensors) -> bool:
+    """Whether the address ranges of any two meet."""
+    ends = []
+    for t in tensors:
+        if t.numel():
+            a = t.data_ptr()
+            ends.append((a, a + (1 + sum((s - 1) * k for s, k in zip(t.shape, t.stride()))) * t.element_size()))
+    ends.sort()
+    return any(b[0] < a[1] for a, b in zip(ends, ends[1:]))
+
+
+def move_rows_(tensors, sources, destinations=None, *, dim: int = 0) -> None:
+    """Row ``destinations[i]`` along ``dim`` of every tensor becomes what row
+    ``sources[i]`` was before the call, in place and in one launch (24 tensors a launch);
+    -1 makes a row of zeros.  Rows may trade places, and a source serve many times.
+
+    ``sources``: integers (checked), or a one-dimensional integer tensor of the GPU, whose
+    indices out of range make zeros too.  ``destinations``: distinct integers, known to the
+    host; default every row.  Up to 2048 rows may trade places; more where no source is
+    another row's destination.  The tensors' rows are dense, and their memory neither
+    overlaps nor interleaves.  Capturable where host indices are at most 192.
+    """
+    name = "move_rows_"
+    tensors = list(tensors)
+    src = _index(sources, name)
+    _on_gpu(tensors, src, name)
+    if dim < 0:
+        raise ValueError(f"{name}: dim counts from the front")
+    fams = [_family(t, dim, name) for t in tensors]
+    if any(f is None or not _apart(f) for f in fams):
+        raise ValueError(f"{name}: the rows of a tensor are dense and apart")
+    rows = _same_rows(fams, name)
+    if len(tensors) > 1 and _lap(tensors):
+        raise ValueError(f"{name}: tensors overlap or interleave")
+    n = len(src) if type(src) is list else src.shape[0]
+    if type(src) is list and not all(-1 <= i < rows for i in src):
+        raise IndexError(f"{name}: sources outside -1..{rows - 1}")
+    dst = None
+    if destinations is None:
+        if n != rows:
+            raise ValueError(f"{name}: {n} sources for {rows} rows")
+    else:
+        dst = _index(destinations, name)
+        if type(dst) is not list:
+            raise ValueError(f"{name}: destinations are known to the host")
+        if len(dst) != n:
+            raise ValueError(f"{name}: {n} sources for {len(dst)} destinations")
+        if not all(0 <= i < rows for i in dst):
+            raise IndexError(f"{name}: destinations outside 0..{rows - 1}")
+        if len(set(dst)) != n:
+            raise ValueError(f"{name}: destinations {sorted(dst)} repeat")
+    disjoint = type(src) is list and not {s for s, d in zip(src, dst or range(n)) if s != d} & set(dst or range(n))
+    if not disjoint and n > MAX_TRADING:
+        raise ValueError(f"{name}: at most {MAX_TRADING} rows trade places in one call")
+    flat = []
+    for t, f in zip(tensors, fams):
+        p = t.data_ptr()
+        flat += (p, p, f[0], f[1], f[0], f[1], f[2], f[3])
+    if n:
+        _launch(flat, rows, rows, n, src, dst, disjoint, tensors[0], name)
+
+
+__all__ = ["select_rows", "move_rows_"]

@@ -657,6 +657,82 @@ int rwkv7mi_slot_copy(const void* src, int64_t src_layer_stride,
                       int64_t nrows, int64_t row_bytes, int64_t nlayers,
                       void* stream);
 
+/* Rows of up to 24 tensors moved by one index in one launch: for every outer
+ * index o and every r < nrows
+ *   dst[o][d(r)] = the old src[o][s(r)]
+ * as if all sources were read before any destination is written (strides in
+ * bytes, any alignment).  s(r) and d(r) come from src_index / dst_index (device
+ * arrays), from src_list / dst_list (host arrays of at most 192, copied with
+ * the launch) or are r where both are NULL.  s(r) outside 0 .. src_rows - 1
+ * (say -1) writes zeros, d(r) outside 0 .. dst_rows - 1 nothing.  The
+ * destinations are distinct.  A tensor with src == dst is moved in place (a row
+ * onto itself is left alone); otherwise its src and dst do not overlap.  Rows
+ * that trade places in place: at most 2048; `disjoint` says that no source is
+ * another row's destination, which lifts that. */
+typedef struct {
+  const void* src;
+  void* dst;
+  int64_t src_outer_stride, src_row_stride;
+  int64_t dst_outer_stride, dst_row_stride;
+  int64_t row_bytes, outer;
+} rwkv7mi_rows;
+int rwkv7mi_rows_move(int n, const rwkv7mi_rows* tensors, int64_t src_rows,
+                      int64_t dst_rows, int64_t nrows, const int64_t* src_index,
+                      const int64_t* dst_index, const int64_t* src_list,
+                      const int64_t* dst_list, int disjoint, void* stream);
+
+/* ------------------------------------------------------------ beam search */
+
+/* The `candidates` best of each prompt's beams x vocabulary, best first, equal
+ * ones by beam, then logit, then token: x [prompts * beams, V] logits (row stride ldx
+ * elements, act dtype), scores [prompts, beams] fp32 the beams' running sums,
+ *   value = scores + (x - logsumexp(x))     (normalized: scores + x)
+ * in 64 bits, rounded once to out_scores [prompts, candidates] fp32; out_tokens
+ * the token, out_rows the row of x.  A row that holds NaN or +inf or whose score
+ * is one is NaN throughout, and NaN ranks first; a token of -inf, a row of -inf
+ * alone and a score of -inf give -inf.  At most 128 beams and candidates. */
+size_t rwkv7mi_beam_workspace_bytes(int64_t rows, int64_t V, int64_t candidates);
+int rwkv7mi_beam_select(const void* x, int64_t prompts, int64_t beams, int64_t V,
+                        int64_t ldx, int dtype, const float* scores,
+                        int normalized, int64_t candidates, float* out_scores,
+                        int64_t* out_tokens, int64_t* out_rows, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* A beam search's state: `room` tokens a row. */
+typedef struct {
+  int64_t* tokens;          /* [prompts, beams, room] the texts               */
+  int32_t* lengths;         /* [prompts * beams] tokens of each, one a prompt */
+  float* scores;            /* [prompts, beams] running sums                  */
+  int32_t* prompt_lengths;  /* [prompts]                                      */
+  int64_t* finished_tokens; /* [prompts, beams, room] hypotheses, any order   */
+  int32_t* finished_lengths;
+  float* finished_scores;   /* [prompts, beams], -inf: none                   */
+  uint8_t* done;            /* [prompts] 0 / 1                                */
+} rwkv7mi_beam_state;
+
+/* One step of a beam search: the selection of (1 + n_ends) beams candidates
+ * (at most 128) of a prompt, then, for a prompt that is not done:
+ *  - an end token (ends, host array, at most 8) among the first `beams`
+ *    candidates makes a hypothesis, value / (generated tokens)^length_penalty;
+ *    the `beams` best of these and of those so far are kept, equal ones the
+ *    earlier; newcomers, by rank, take the places of those that go, in order;
+ *  - the first `beams` candidates that are not (finite) end tokens live on: the
+ *    best child of a row stays in it, the others, by rank, take the rows without
+ *    a child, in order; next[row] is the row's token, rows[row] the row it
+ *    continues, scores and tokens follow, lengths grow by one;
+ *  - it is done where its rows are full or, early_stopping 0: no running beam at
+ *    its present length, 2: at the length that helps it most, is better than the
+ *    worst of `beams` hypotheses; 1: there are `beams` hypotheses.
+ * A done prompt stays as it is, with next = pad and rows its own.  `out` may be
+ * `in` (then only rows that change are written); otherwise no buffer is shared. */
+int rwkv7mi_beam_step(const void* x, int64_t prompts, int64_t beams, int64_t V,
+                      int64_t ldx, int dtype, int normalized,
+                      const int64_t* ends, int n_ends, double length_penalty,
+                      int early_stopping, int64_t pad,
+                      const rwkv7mi_beam_state* in, const rwkv7mi_beam_state* out,
+                      int64_t room, int64_t* next, int64_t* rows, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------- greedy selection */
 
 /* out[r] = argmax of row r of x [rows, n] (row stride ld elements, act dtype),
