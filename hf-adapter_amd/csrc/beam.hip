@@ -309,11 +309,13 @@ __device__ void beam_bookkeeping(const BmArgs& A, const BmStep& P, const BmBest&
   const double span = pow((double)max(len + 1 - prompt, 1), P.penalty);
   if (tid < K) old[tid] = P.in.finished_scores[r0 + tid], taken[tid] = -1;
   if (tid < 2) used[tid] = kept[tid] = 0;
+  const bool last = len + 1 >= P.room;  // the rows are full behind this token: all texts end
   if (tid < A.M) {
     bool end = false;
     for (int e = 0; e < P.ends; ++e) end |= best.token[tid] == P.end[e];
     is_end[tid] = end && best.value[tid] > -__builtin_inff();
-    if (tid < K) hyp[tid] = is_end[tid] ? (float)((double)best.value[tid] / span) : -__builtin_inff();
+    if (tid < K) hyp[tid] = (end || last) && best.value[tid] > -__builtin_inff() ? (float)((double)best.value[tid] / span)
+                                                                                 : -__builtin_inff();
   }
   __syncthreads();
   if (tid < A.M && !is_end[tid]) {  // the first K that do not end live on
@@ -394,7 +396,7 @@ __device__ void beam_bookkeeping(const BmArgs& A, const BmStep& P, const BmBest&
     const double ahead = P.early == 2 && P.penalty > 0 ? pow((double)max(P.room - prompt, (int64_t)1), P.penalty) : span;
     const bool over = P.early == 1 ? worst > -__builtin_inff()
                                    : !((float)((double)best.value[live[0]] / ahead) > worst);
-    P.out.done[b] = over || len + 1 >= P.room;
+    P.out.done[b] = over || last;
     P.out.prompt_lengths[b] = prompt;
   }
 }

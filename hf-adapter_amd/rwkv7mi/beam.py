@@ -149,8 +149,8 @@ class BeamState:
 
     def best(self, count: int = 1, *, length_penalty: float = 1.0):
         """``(tokens [prompts, count, room], lengths, scores)`` of each prompt's ``count`` best
-        hypotheses, best first: those that have ended, then, where they are fewer, the running
-        beams, by score / generated length ** length_penalty."""
+        texts, best first: the hypotheses, then, of a search that is not over and has fewer, the
+        running beams, by score / generated length ** length_penalty."""
         p, k, room = self.tokens.shape
         if not 1 <= count <= k:
             raise ValueError(f"BeamState.best: count must be 1..{k}")
@@ -158,7 +158,6 @@ class BeamState:
         span = (length - self.prompt_lengths[:, None]).clamp(min=1).double()
         running = (self.scores.double() / span ** float(length_penalty)).float()
         score = torch.cat([self.finished_scores, running], 1)
-        # (running beams only behind every ended one, as a search that still runs has not chosen them)
         ended = torch.cat([self.finished_scores > -math.inf, torch.zeros_like(running, dtype=torch.bool)], 1)
         order = score.sort(dim=1, descending=True, stable=True).indices
         order = order.gather(1, ended.gather(1, order).int().sort(dim=1, descending=True, stable=True).indices)[:, :count]
@@ -180,9 +179,9 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, leng
     Per prompt that is not done, :func:`beam_select` over ``(1 + ends) * beams`` candidates
     (at most 128), then:
 
-    * an end token (``eos_token_id``: none, one or up to 8) among the first ``beams`` makes a
-      hypothesis of score ``score / generated_tokens ** length_penalty``, the end token
-      included; the ``beams`` best of these and the earlier ones stay, the earlier first where
+    * an end token (``eos_token_id``: none, one or up to 8) among the first ``beams``, and each of
+      these where the rows become full, makes a hypothesis of score
+      ``score / generated_tokens ** length_penalty``, its last token included; the ``beams`` best of these and the earlier ones stay, the earlier first where
       equal; newcomers take the places of those that go;
     * the first ``beams`` others live on.  A beam's best child stays in its row, the rest take
       the rows without a child, in order: ``rows`` names as few moved rows as there can be;

@@ -40,6 +40,8 @@ from .fused_recurrent_update import fused_recurrent_output_prepare_raw
 from .native_wkv_fp16 import (native_fp16_recurrent_output_prepare_raw, native_fp16_recurrent_should_use,
                               native_fp16_sequence)
 from .fused_time_mix import fused_attn_sequence_shift_mix, fused_ffn_sequence_shift_mix
+from .beam import BeamState, beam_step, beam_workspace_bytes
+from .state_rows import MAX_TRADING, move_rows_, select_rows
 from .sampling import argmax_rows, argmax_workspace_bytes, process_logits, process_logits_workspace_bytes
 from .native_quant_mm8 import (GEMM_ROWS, GEMV_ROWS, MM8Linear, is_blocked, mm8_gemm_workspace_bytes, mm8_lnmix_multi_into,
                                mm8_many_rows_into, mm8_matmul_multi_into, mm8_matmul_multi_lora_into,
@@ -414,6 +416,24 @@ _METRIC_KEYS = ("clones", "detaches", "device_moves", "select_batch_calls", "bat
                 "native_graph_bound_selects")
 
 
+def _layer_stack(layers) -> torch.Tensor | None:
+    """``torch.stack(layers)`` without a copy, where the layers are equally spaced in one
+    allocation (None otherwise)."""
+    first = layers[0]
+    if len(layers) == 1:
+        return first[None]
+    step = layers[1].data_ptr() - first.data_ptr()
+    size = first.element_size()
+    if step <= 0 or step % size or not first.is_contiguous():
+        return None
+    home = first.untyped_storage().data_ptr()
+    for i, t in enumerate(layers):
+        if (t.data_ptr() != first.data_ptr() + i * step or t.shape != first.shape or t.dtype != first.dtype
+                or not t.is_contiguous() or t.untyped_storage().data_ptr() != home):
+            return None
+    return first.as_strided((len(layers), *first.shape), (step // size, *first.stride()))
+
+
 class NativeRWKV7Cache(_HFCache):
     """Recurrent-state cache with the reference's contract (rwkv7_hf/model_cache.py:48-466).
 
@@ -696,9 +716,46 @@ class NativeRWKV7Cache(_HFCache):
             target._rwkv7_cache_metrics["native_graph_bound_selects"] += 1
             return target
         target._invalidate_native_graph_binding()
-        target._map(lambda t: t.index_select(0, idx.to(t.device)))
+        target._take_rows(idx)
         target._rwkv7_cache_metrics["select_batch_calls"] += 1
         return target
+
+    def _stacked(self):
+        """The tensors with the rows as dimension 1: the per-layer lists as one tensor each
+        where they are equally spaced parts of one allocation (:meth:`zeros`); None where they
+        are not."""
+        out = []
+        for layers in (self._state, self._xpa, self._xpf):
+            base = _layer_stack(layers)
+            if base is None:
+                return None
+            out.append(base)
+        out.append(self._v_first[None])
+        if self._elapsed is not None:
+            out.append(self._elapsed[None])
+        return out
+
+    def _take_rows(self, index) -> None:
+        """New tensors of the rows ``index`` (a list of integers or a tensor): on the GPU in one
+        launch, the layers in one allocation again."""
+        ts = self._all_tensors()
+        if not ts or not all(t.is_cuda and t.device == ts[0].device for t in ts):
+            idx = torch.as_tensor(index, dtype=torch.long)
+            self._map(lambda t: t.index_select(0, idx.to(t.device)))
+            return
+        if isinstance(index, torch.Tensor):
+            index = index.reshape(-1).to(ts[0].device) if index.is_cuda else index.reshape(-1).tolist()
+        if isinstance(index, list) and any(i < 0 for i in index):
+            raise IndexError("NativeRWKV7Cache: index out of range")
+        stacked = self._stacked() if self._is_initialized() else None
+        if stacked is None:
+            it = iter(select_rows(ts, index))
+            self._map(lambda t: next(it))
+            return
+        new = select_rows(stacked, index, dim=1)
+        self._state, self._xpa, self._xpf = (list(t.unbind(0)) for t in new[:3])
+        self._v_first = new[3][0]
+        self._elapsed = new[4][0] if self._elapsed is not None else None
 
     def batch_select(self, indices, *, inplace: bool = True) -> "NativeRWKV7Cache":
         target = self.select_batch(indices, inplace=inplace)
@@ -723,7 +780,9 @@ class NativeRWKV7Cache(_HFCache):
         if repeats <= 0:
             raise ValueError("NativeRWKV7Cache.batch_repeat_interleave requires repeats > 0")
         self._invalidate_native_graph_binding()
-        self._map(lambda t: t.repeat_interleave(repeats, dim=0))
+        rows = self.get_batch_size()
+        if rows is not None:
+            self._take_rows([i for i in range(rows) for _ in range(repeats)])
         self._rwkv7_cache_metrics["batch_repeat_interleave_calls"] += 1
         return self
 
@@ -1819,6 +1878,70 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
             out.append(nxt[:, None])
         return torch.cat(out, 1)
 
+    @torch.no_grad()
+    def generate_beam(self, input_ids: torch.Tensor, max_new_tokens: int, *, num_beams: int = 4, eos_token_id=None,
+                      pad_token_id: int = 0, length_penalty: float = 1.0, early_stopping=False,
+                      num_return_sequences: int = 1, use_graph: bool = True, return_scores: bool = False,
+                      repetition_penalty=1.0, presence_penalty=0.0, frequency_penalty=0.0, penalty_decay=1.0,
+                      bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None):
+        """Beam search without GenerationMixin's per-step host work: after each decode step
+        :func:`~.beam.beam_step` selects and keeps the books on the device, and the cache rows
+        that change hands follow in one launch.  The sequences that
+        ``generate(num_beams=..., do_sample=False)`` gives with the same settings, rows of equal
+        score aside: ``[B * num_return_sequences, longest]``, the prompt included, padded behind the
+        end; with ``return_scores`` also their scores (sum of log-probabilities / generated
+        length ** ``length_penalty``).  The host looks every eight steps whether all prompts are done.
+
+        The penalties, ``bias`` and ``allowed`` are those of :func:`~.sampling.process_logits`, over
+        the prompt and each beam's text, on the logits before their log-softmax; per-row ones
+        hold a value for each of ``B * num_beams`` rows."""
+        B, T = (int(s) for s in input_ids.shape)
+        K, steps = int(num_beams), int(max_new_tokens)
+        if not 1 <= int(num_return_sequences) <= K or steps < 1:
+            raise ValueError("generate_beam: 1 <= num_return_sequences <= num_beams and max_new_tokens >= 1")
+        dev, V = self.device, self.config.vocab_size
+        here = lambda v: v.to(dev) if isinstance(v, torch.Tensor) else v  # noqa: E731
+        how = dict(eos_token_id=eos_token_id, length_penalty=length_penalty, early_stopping=early_stopping,
+                   pad_token_id=pad_token_id)
+        plain = bias is None and allowed is None and not any(
+            isinstance(v, torch.Tensor) or v != d
+            for v, d in ((repetition_penalty, 1.0), (presence_penalty, 0.0), (frequency_penalty, 0.0)))
+        pen = dict(repetition_penalty=here(repetition_penalty), presence_penalty=here(presence_penalty),
+                   frequency_penalty=here(frequency_penalty), penalty_decay=here(penalty_decay), allowed=here(allowed),
+                   bias=None if bias is None else bias.to(dev, torch.float32))
+        ids = input_ids.to(dev)
+        state = BeamState.start(ids, K, T + steps)
+        nxt, rows = (torch.empty(B * K, dtype=torch.long, device=dev) for _ in range(2))
+        n_ends = len(eos_token_id) if isinstance(eos_token_id, (list, tuple)) else int(eos_token_id is not None)
+        ws = torch.empty(beam_workspace_bytes(B * K, V, (1 + n_ends) * K), dtype=torch.uint8, device=dev)
+        scored = None if plain else torch.empty(B * K, V, dtype=torch.float32, device=dev)
+
+        def pick(logits):
+            if not plain:
+                logits = process_logits(logits, history=state.tokens.view(B * K, T + steps), lengths=state.lengths,
+                                        out=scored, **pen)
+            beam_step(logits, state, next_tokens=nxt, rows=rows, workspace=ws, **how)
+
+        out0 = self.forward(ids)
+        cache = out0.past_key_values
+        cache.batch_repeat_interleave(K)
+        pick(out0.logits[:, -1].repeat_interleave(K, dim=0))  # (all rows of a prompt are still the same)
+        runner = self.graph_runner(B * K) if use_graph and steps > 1 else None
+        for t in range(steps - 1):
+            if t % 8 == 7 and bool(state.done.all()):
+                break
+            if runner is not None:
+                pick(runner.replay(nxt, cache))
+            else:
+                pick(self.forward(nxt[:, None], past_key_values=cache, use_graph=False).logits[:, -1])
+            if t < steps - 2:
+                cache.reorder_cache(rows)
+        tokens, lengths, scores = state.best(int(num_return_sequences), length_penalty=length_penalty)
+        n = int(lengths.max())
+        tokens = torch.where(torch.arange(n, device=dev) < lengths[..., None], tokens[..., :n], pad_token_id)
+        tokens = tokens.reshape(B * int(num_return_sequences), n)
+        return (tokens, scores.reshape(-1)) if return_scores else tokens
+
     def _generate_processed(self, input_ids, max_new_tokens, use_graph, **how):
         """:meth:`generate_greedy` through :func:`process_logits`: the ids returned are the
         history buffer it appends to."""
@@ -1930,6 +2053,7 @@ class NativeGraphRunner(_OwnsGraph):
         dev = model.device
         model.reserve_workspace(self.batch)
         self.cache = model.new_cache(self.batch)
+        self._rows = self.cache._stacked()
         self.tokens = torch.zeros(self.batch, dtype=torch.long, device=dev)
         self.logits = torch.empty(self.batch, model.config.vocab_size, device=dev, dtype=model.dtype)
         self.next_tokens = torch.zeros(self.batch, dtype=torch.long, device=dev)
@@ -1995,11 +2119,19 @@ class NativeGraphRunner(_OwnsGraph):
 
     def reorder_batch_inplace(self, indices: torch.Tensor) -> bool:
         """Permute the bound batch rows in place (beam search on a bound cache)."""
-        idx = indices.to(device=self.model.device, dtype=torch.long)
-        if int(idx.numel()) != self.batch:
+        if int(indices.numel()) != self.batch:
             return False
-        for t in self.cache._all_tensors():
-            t.copy_(t.index_select(0, idx))
+        idx = indices.reshape(-1)
+        if idx.is_cuda:
+            idx = idx.to(self.model.device)
+        elif bool((idx < 0).any()):
+            raise IndexError("NativeRWKV7Cache: index out of range")
+        if self.batch > MAX_TRADING:
+            idx = idx.to(device=self.model.device, dtype=torch.long)
+            for t in self.cache._all_tensors():
+                t.copy_(t.index_select(0, idx))
+            return True
+        move_rows_(self._rows, idx, dim=1)
         return True
 
     def replay(self, tokens: torch.Tensor, cache: NativeRWKV7Cache) -> torch.Tensor:

@@ -12,14 +12,16 @@ semantics):
 * ``allocate`` returns zeroed, uniquely owned slots with a generation;
   ``free`` checks the generation and bumps it, so a stale handle cannot
   touch a reassigned slot; ``reset`` / ``clone`` / ``gather`` / ``scatter`` /
-  ``snapshot`` / ``restore`` as the ABI lists them;
+  ``snapshot`` / ``restore`` as the ABI lists them; ``fork`` (one slot to many),
+  ``reorder`` (beams), ``compact`` and ``resize`` move slots in one launch for
+  every tensor and layer;
 * :class:`PooledDecoder` runs one decode step for any list of live slots:
   the rows are gathered into a graph bucket's layer-major batch cache (one
   ``rwkv7mi_slot_copy`` launch per tensor family for all layers), the
   bucket's captured hipGraph replays, and only the active rows are
   scattered back; padding rows use the scratch slot with active = 0.
 
-Every copy is the HIP slot-copy kernel (byte moves, bit-exact).
+Every copy is a HIP kernel (slot-copy or moved rows: byte moves, bit-exact).
 """
 from __future__ import annotations
 
@@ -29,6 +31,7 @@ import hashlib
 import torch
 
 from . import _lib
+from .state_rows import move_rows_, select_rows
 
 LAYOUT_VERSION = "rwkv7mi.state_pool.v1"
 
@@ -79,6 +82,7 @@ class RWKV7StatePool:
         self.generation = [0] * C
         self.allocated = [False] * C
         self.owner: dict[int, object] = {}
+        self._retired: dict[int, int] = {}  # generations of the slots that a smaller capacity left out
         self.scratch_slot = self.capacity
 
     # ------------------------------------------------------------ bookkeeping
@@ -110,9 +114,8 @@ class RWKV7StatePool:
                                  f"{self.generation[s]})")
 
     # ------------------------------------------------------------ allocator
-    def allocate(self, request_ids) -> list[tuple[int, int]]:
-        """Zeroed, uniquely owned slots: ``[(slot, generation), ...]``."""
-        request_ids = list(request_ids)
+    def _take(self, request_ids) -> list[int]:
+        """The lowest free slots, now owned by the requests; their state is what it was."""
         free = [s for s in range(self.capacity) if not self.allocated[s]]
         if len(free) < len(request_ids):
             raise RuntimeError(f"state pool full: {len(request_ids)} requested, {len(free)} free")
@@ -120,6 +123,11 @@ class RWKV7StatePool:
         for s, rid in zip(slots, request_ids):
             self.allocated[s] = True
             self.owner[s] = rid
+        return slots
+
+    def allocate(self, request_ids) -> list[tuple[int, int]]:
+        """Zeroed, uniquely owned slots: ``[(slot, generation), ...]``."""
+        slots = self._take(list(request_ids))
         self.reset(slots)
         return [(s, self.generation[s]) for s in slots]
 
@@ -131,28 +139,15 @@ class RWKV7StatePool:
             self.allocated[int(s)] = False
             self.owner.pop(int(s), None)
 
-    def _rows(self, slots, *, zero=False, src_slots=None):
-        """One slot-copy launch per tensor family: pool rows ``src_slots`` (or
-        zeros) into pool rows ``slots``."""
-        n = len(slots)
-        if n == 0:
-            return
-        dst = self._idx(slots)
-        src = None if zero else self._idx(src_slots)
-        st = _lib.stream_of(self.state)
-        for t in (self.state, self.xpa, self.xpf):
-            row = t[0, 0].numel() * t.element_size()
-            layer = t[0].numel() * t.element_size()
-            _slot_copy(None if zero else t.data_ptr(), layer, row, src, t.data_ptr(), layer, row, dst, None, n, row,
-                       t.shape[0], st)
-        vrow = self.v_first[0].numel() * self.v_first.element_size()
-        _slot_copy(None if zero else self.v_first.data_ptr(), 0, vrow, src, self.v_first.data_ptr(), 0, vrow, dst,
-                   None, n, vrow, 1, st)
+    def _tensors(self):
+        """Every tensor of the pool, the slots as dimension 1."""
+        return [self.state, self.xpa, self.xpf, self.v_first[None]]
 
     def reset(self, slots) -> None:
         """Exact new-request state (zeros, seen_tokens 0)."""
         self.check(slots)
-        self._rows(list(slots), zero=True)
+        slots = [int(s) for s in slots]
+        move_rows_(self._tensors(), [-1] * len(slots), slots, dim=1)
         for s in slots:
             self.seen_tokens[int(s)] = 0
 
@@ -162,9 +157,88 @@ class RWKV7StatePool:
         self.check(destination_slots)
         if set(map(int, source_slots)) & set(map(int, destination_slots)):
             raise ValueError("clone: source and destination slots overlap")
-        self._rows(list(destination_slots), src_slots=list(source_slots))
+        if len(source_slots) != len(destination_slots):
+            raise ValueError("clone: as many sources as destinations")
+        move_rows_(self._tensors(), [int(s) for s in source_slots], [int(d) for d in destination_slots], dim=1)
         for s, d in zip(source_slots, destination_slots):
             self.seen_tokens[int(d)] = self.seen_tokens[int(s)]
+
+    def fork(self, slot: int, generation: int, request_ids) -> list[tuple[int, int]]:
+        """A new slot for each request with a copy of ``slot``'s state (one prompt to many
+        continuations), in one launch that reads it once: ``[(slot, generation), ...]``."""
+        self.check([slot], [generation])
+        slot = int(slot)
+        slots = self._take(list(request_ids))
+        move_rows_(self._tensors(), [slot] * len(slots), slots, dim=1)
+        for s in slots:
+            self.seen_tokens[s] = self.seen_tokens[slot]
+        return [(s, self.generation[s]) for s in slots]
+
+    def reorder(self, slots, generations, parents) -> None:
+        """``slots[i]`` takes the state that ``slots[parents[i]]`` had before the call, all at
+        once and in one launch: the beams of a search.  ``parents``: positions in ``slots``,
+        as many, on the host, or an integer tensor of the GPU (:func:`~.beam.beam_step`'s rows),
+        for which the slots have seen as many tokens (a position out of range on the GPU
+        zeroes the slot's state)."""
+        self.check(slots, generations)
+        slots = [int(s) for s in slots]
+        n = len(slots)
+        if isinstance(parents, torch.Tensor) and parents.is_cuda:
+            if parents.dim() != 1 or parents.shape[0] != n or parents.is_floating_point():
+                raise ValueError(f"reorder: parents must be {n} integers")
+            if len({self.seen_tokens[s] for s in slots}) > 1:
+                raise ValueError("reorder: slots of unequal seen_tokens need parents on the host")
+            if n:
+                at = parents.to(torch.int64)
+                here = self._idx(slots)[at.clamp(0, n - 1)]
+                move_rows_(self._tensors(), torch.where((at >= 0) & (at < n), here, -1), slots, dim=1)
+            return
+        parents = [int(p) for p in parents]
+        if len(parents) != n or not all(0 <= p < n for p in parents):
+            raise ValueError(f"reorder: parents must be {n} positions in slots")
+        sources = [slots[p] for p in parents]
+        move_rows_(self._tensors(), sources, slots, dim=1)
+        seen = [self.seen_tokens[s] for s in sources]
+        for d, t in zip(slots, seen):
+            self.seen_tokens[d] = t
+
+    def compact(self) -> dict[int, tuple[int, int]]:
+        """Move the live slots down to 0 .. live - 1, the highest into the holes, in one launch:
+        ``{old slot: (new slot, generation)}`` of those that moved (their old handles are
+        stale; the others keep theirs)."""
+        live = sum(self.allocated[:self.capacity])
+        holes = [s for s in range(live) if not self.allocated[s]]
+        above = [s for s in range(live, self.capacity) if self.allocated[s]]
+        move_rows_(self._tensors(), above, holes, dim=1)
+        moved = {}
+        for s, d in zip(above, holes):
+            self.allocated[s], self.allocated[d] = False, True
+            self.seen_tokens[d] = self.seen_tokens[s]
+            self.generation[s] += 1
+            if s in self.owner:
+                self.owner[d] = self.owner.pop(s)
+            moved[s] = (d, self.generation[d])
+        return moved
+
+    def resize(self, capacity: int) -> None:
+        """Room for ``capacity`` slots, in new storage; live slots keep their numbers and handles,
+        so all of them have to lie below ``capacity`` (:meth:`compact`)."""
+        capacity = int(capacity)
+        if capacity < 1:
+            raise ValueError("capacity must be positive")
+        if any(self.allocated[capacity:]):
+            raise ValueError(f"resize: live slots above {capacity - 1} (compact first)")
+        keep = [s if s < self.capacity and self.allocated[s] else -1 for s in range(capacity)] + [-1]
+        self.state, self.xpa, self.xpf, v_first = select_rows(self._tensors(), keep, dim=1)
+        self.v_first = v_first[0]
+        # (a number that comes back after the pool has shrunk keeps counting: no old handle fits)
+        self._retired = {**self._retired, **{s: self.generation[s] for s in range(capacity, self.capacity)}}
+        more = range(self.capacity, capacity)
+        scratch = capacity
+        self.generation = self.generation[:min(capacity, self.capacity)] + [self._retired.get(s, 0) for s in more] + [0]
+        self.seen_tokens = [self.seen_tokens[s] if k >= 0 else 0 for s, k in enumerate(keep)]
+        self.allocated = [k >= 0 for k in keep]
+        self.capacity, self.scratch_slot = capacity, scratch
 
     # ------------------------------------------------------------ per layer
     def gather(self, layer_id: int, slot_ids):

@@ -713,8 +713,8 @@ typedef struct {
 /* One step of a beam search: the selection of (1 + n_ends) beams candidates
  * (at most 128) of a prompt, then, for a prompt that is not done:
  *  - an end token (ends, host array, at most 8) among the first `beams`
- *    candidates makes a hypothesis, value / (generated tokens)^length_penalty;
- *    the `beams` best of these and of those so far are kept, equal ones the
+ *    candidates, and each of them where the rows become full, makes a
+ *    hypothesis, value / (generated tokens)^length_penalty; the `beams` best of these and of those so far are kept, equal ones the
  *    earlier; newcomers, by rank, take the places of those that go, in order;
  *  - the first `beams` candidates that are not (finite) end tokens live on: the
  *    best child of a row stays in it, the others, by rank, take the rows without

@@ -51,12 +51,12 @@ def step(found, state, ends, penalty, early, pad=0):
         pool = [(float(v), 0, i) for i, v in enumerate(s["finished_scores"][b])]
         live = []
         for r in range(len(val)):
-            if tok[r] in ends and val[r] > -np.inf:
-                if r < k:
-                    h = float(np.float32(np.float64(val[r]) / np.float64(gen) ** penalty))
-                    if h > -np.inf:
-                        pool.append((h, 1, r))
-            elif len(live) < k:
+            end = tok[r] in ends and val[r] > -np.inf
+            if r < k and (end or (at + 1 >= room and val[r] > -np.inf)):
+                h = float(np.float32(np.float64(val[r]) / np.float64(gen) ** penalty))
+                if h > -np.inf:
+                    pool.append((h, 1, r))
+            if not end and len(live) < k:
                 live.append(r)
         best = sorted(pool, key=lambda e: (-e[0], e[1], e[2]))[:k]
         stay = {i for _, new, i in best if not new}
