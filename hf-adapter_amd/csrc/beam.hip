@@ -51,10 +51,10 @@ struct BmArgs {
   int64_t ldx;
   int V, beams, S, M, normalized;
   const float* scores;
-  // the slices' results: [rows][S][M] values and tokens, [rows][S] maxima and sums
-  float* pv;
-  int* pt;
-  float *pm, *ps;
+  // the slices' results: [rows][S][M] values (high) and beams and tokens (low), best first;
+  // [rows][S] maxima and sums
+  uint64_t* got;
+  float2* sums;
   float* out_scores;  // the selection's own outputs (null in a step)
   int64_t *out_tokens, *out_rows;
 };
@@ -83,13 +83,17 @@ __device__ __forceinline__ uint64_t bm_key(double x) {
 __device__ __forceinline__ double bm_value(uint64_t k) {
   return __longlong_as_double((long long)(k >> 63 ? k ^ 0x8000000000000000ull : ~k));
 }
+constexpr uint32_t BM_NONE = 0x007fffffu;  // the key of -inf: nothing to choose
+// a slice's candidate: the logit's key, the beam (7 bits), the token (23)
+__device__ __forceinline__ uint64_t bm_pack(uint32_t key, int beam, int token) {
+  return (uint64_t)key << 32 | (uint32_t)(beam << 23 | token);
+}
 // what decides between equal values: the beam (7 bits), the logit, the token (23)
-__device__ __forceinline__ uint64_t bm_place(int beam, float logit, int token) {
-  return (uint64_t)beam << 55 | (uint64_t) ~bm_key(logit) << 23 | (uint32_t)token;
+__device__ __forceinline__ uint64_t bm_place(uint64_t c) {
+  return (c & 0x3f800000u) << 32 | (uint64_t) ~(uint32_t)(c >> 32) << 23 | (c & 0x7fffffu);
 }
 __device__ __forceinline__ int bm_beam(uint64_t p) { return (int)(p >> 55); }
 __device__ __forceinline__ int bm_token(uint64_t p) { return (int)(p & 0x7fffff); }
-constexpr uint32_t BM_NONE = 0x007fffffu;  // the key of -inf: nothing to choose
 
 __device__ __forceinline__ uint32_t bm_wave_max(uint32_t v) {
 #pragma unroll
@@ -128,7 +132,7 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
   __shared__ uint32_t top[BM_THREADS];
   __shared__ uint32_t bound, wave_top[BM_THREADS / 64];
   __shared__ float wave_sum_[BM_THREADS / 64];
-  __shared__ int count, bad;
+  __shared__ int count;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.y;
   const T* x = static_cast<const T*>(A.x) + row * A.ldx;
@@ -153,61 +157,64 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
       for (int e = 0; e < E; ++e) v[u][e] = i + e >= 0 && i + e < A.V ? to_f32(x[i + e]) : -__builtin_inff();
     }
   }
-  if (tid == 0) count = bad = 0;
-  float best = -__builtin_inff();
-  bool odd = false;
+  if (tid == 0) count = 0;
+  float run_best[RUNS], best = -__builtin_inff();
 #pragma unroll
-  for (int u = 0; u < RUNS; ++u)
+  for (int u = 0; u < RUNS; ++u) {
+    run_best[u] = v[u][0];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      odd |= !(v[u][e] < __builtin_inff());  // NaN or +inf
-      best = fmaxf(best, v[u][e]);
-    }
+    for (int e = 1; e < E; ++e) run_best[u] = fmaxf(run_best[u], v[u][e]);
+    best = fmaxf(best, run_best[u]);
+  }
   const uint32_t mine = bm_key(best);
   top[tid] = mine;
   const uint32_t wtop = bm_wave_max(mine);
   if ((tid & 63) == 0) wave_top[tid >> 6] = wtop;
   __syncthreads();
-  if (__any(odd) && (tid & 63) == 0) bad = 1;
+  uint32_t all = wave_top[0];
+#pragma unroll
+  for (int w = 1; w < BM_THREADS / 64; ++w) all = max(all, wave_top[w]);
   if (tid < 64) {
     const uint32_t t = bm_bound<BM_THREADS / 64, LOW>(top, A.M);
     if (tid == 0) bound = t;
   }
-  uint32_t all = wave_top[0];
-#pragma unroll
-  for (int w = 1; w < BM_THREADS / 64; ++w) all = max(all, wave_top[w]);
   const float m = bm_value(all);
+  // NaN and +inf make the sum NaN (a slice of -inf and NaN alone: asked for)
   float s = 0.f;
   if (all > BM_NONE) {
 #pragma unroll
     for (int u = 0; u < RUNS; ++u)
 #pragma unroll
       for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v[u][e] - m) * 1.44269504f);
+  } else {
+#pragma unroll
+    for (int u = 0; u < RUNS; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) s = v[u][e] != v[u][e] ? __builtin_nanf("") : s;
   }
   s = wave_sum(s);
   if ((tid & 63) == 0) wave_sum_[tid >> 6] = s;
   __syncthreads();
   const uint32_t at_least = bound;
+  const float reach = bm_value(at_least);
   const int64_t slice = row * A.S + blockIdx.x;
+  const int beam = (int)(row % A.beams);
   if (tid == 0) {
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < BM_THREADS / 64; ++w) sum += wave_sum_[w];
-    A.pm[slice] = m;
-    A.ps[slice] = bad ? __builtin_nanf("") : sum;
+    A.sums[slice] = make_float2(m, sum);
   }
-  float* pv = A.pv + slice * A.M;
-  int* pt = A.pt + slice * A.M;
-  if (mine >= at_least) {
+  uint64_t* out = A.got + slice * A.M;
+  const int t0 = c0 + E * tid;
 #pragma unroll
-    for (int u = 0; u < RUNS; ++u)
+  for (int u = 0; u < RUNS; ++u) {
+    if (!(run_best[u] >= reach)) continue;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const uint32_t k = bm_key(v[u][e]);
-        if (k >= at_least) {
-          const int p = atomicAdd(&count, 1);
-          if (p < BM_CAP) got[p] = (uint64_t)k << 32 | (uint32_t) ~(c0 + E * (BM_THREADS * u + tid) + e);
-        }
+    for (int e = 0; e < E; ++e)
+      if (v[u][e] >= reach) {
+        const int p = atomicAdd(&count, 1);
+        if (p < BM_CAP) got[p] = (uint64_t)bm_key(v[u][e]) << 32 | (uint32_t) ~(t0 + E * BM_THREADS * u + e);
       }
   }
   __syncthreads();
@@ -217,12 +224,9 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
       const uint64_t k = got[i];
       int r = 0;
       for (int j = 0; j < n; ++j) r += got[j] > k;
-      if (r < A.M) {
-        pv[r] = bm_value((uint32_t)(k >> 32));
-        pt[r] = (int)~(uint32_t)k;
-      }
+      if (r < A.M) out[r] = bm_pack((uint32_t)(k >> 32), beam, (int)~(uint32_t)k);
     }
-    for (int r = n + tid; r < A.M; r += BM_THREADS) pv[r] = -__builtin_inff(), pt[r] = -1;
+    for (int r = n + tid; r < A.M; r += BM_THREADS) out[r] = 0;
     return;
   }
   // too many reach the bound: M times the best below the last
@@ -233,8 +237,8 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
     for (int u = 0; u < RUNS; ++u)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const uint64_t c = (uint64_t)bm_key(v[u][e]) << 32 | (uint32_t) ~(c0 + E * (BM_THREADS * u + tid) + e);
-        if (c < last && c > k) k = c;
+        const uint64_t c = (uint64_t)bm_key(v[u][e]) << 32 | (uint32_t) ~(t0 + E * BM_THREADS * u + e);
+        if (v[u][e] >= reach && c < last && c > k) k = c;
       }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -247,10 +251,7 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
 #pragma unroll
     for (int w = 0; w < BM_THREADS / 64; ++w) k = max(k, got[w]);
     last = k;
-    if (tid == 0) {
-      pv[r] = bm_value((uint32_t)(k >> 32));
-      pt[r] = (int)~(uint32_t)k;
-    }
+    if (tid == 0) out[r] = bm_pack((uint32_t)(k >> 32), beam, (int)~(uint32_t)k);
   }
 }
 
@@ -268,8 +269,18 @@ __device__ __forceinline__ int bm_clear_bit(const uint64_t* mask, int n, int q) 
   return n;
 }
 
-__device__ __forceinline__ void bm_copy(int64_t* dst, const int64_t* src, int64_t n) {
-  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) dst[i] = src[i];
+// a row of n tokens by one wave, eight loads in flight
+__device__ __forceinline__ void bm_copy(int64_t* dst, const int64_t* src, int n) {
+  const int lane = threadIdx.x & 63;
+  for (int i0 = lane; i0 < n; i0 += 512) {
+    int64_t t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i0 + 64 * u < n) t[u] = src[i0 + 64 * u];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i0 + 64 * u < n) dst[i0 + 64 * u] = t[u];
+  }
 }
 
 }  // namespace
@@ -284,21 +295,25 @@ __device__ void beam_bookkeeping(const BmArgs& A, const BmStep& P, const BmBest&
   const bool was = P.in.done[b];
   const int len = P.in.lengths[r0], prompt = P.in.prompt_lengths[b];
   const bool full = len < 0 || len >= P.room;  // (no room: nothing can follow)
+  const int waves = blockDim.x >> 6, wave = tid >> 6;
+  const auto held = [&](int k) { return min(max(P.in.finished_lengths[r0 + k], 0), (int)P.room); };
   if (was || full) {
-    for (int k = 0; k < K; ++k) {
-      if (!P.in_place) {
-        bm_copy(P.out.tokens + (r0 + k) * P.room, P.in.tokens + (r0 + k) * P.room, min((int64_t)max(len, 0), P.room));
-        const int64_t fl = min((int64_t)max(P.in.finished_lengths[r0 + k], 0), P.room);
-        bm_copy(P.out.finished_tokens + (r0 + k) * P.room, P.in.finished_tokens + (r0 + k) * P.room, fl);
+    if (!P.in_place)
+      for (int j = wave; j < 2 * K; j += waves) {
+        const int64_t at = (r0 + (j >> 1)) * P.room;
+        if (j & 1)
+          bm_copy(P.out.finished_tokens + at, P.in.finished_tokens + at, held(j >> 1));
+        else
+          bm_copy(P.out.tokens + at, P.in.tokens + at, min(max(len, 0), (int)P.room));
       }
-      if (tid == 0) {
-        P.next[r0 + k] = P.pad;
-        P.rows[r0 + k] = r0 + k;
-        P.out.lengths[r0 + k] = P.in.lengths[r0 + k];
-        P.out.scores[r0 + k] = P.in.scores[r0 + k];
-        P.out.finished_lengths[r0 + k] = P.in.finished_lengths[r0 + k];
-        P.out.finished_scores[r0 + k] = P.in.finished_scores[r0 + k];
-      }
+    if (tid < K) {
+      const int64_t r = r0 + tid;
+      P.next[r] = P.pad;
+      P.rows[r] = r;
+      P.out.lengths[r] = P.in.lengths[r];
+      P.out.scores[r] = P.in.scores[r];
+      P.out.finished_lengths[r] = P.in.finished_lengths[r];
+      P.out.finished_scores[r] = P.in.finished_scores[r];
     }
     if (tid == 0) {
       P.out.done[b] = 1;
@@ -356,56 +371,60 @@ __device__ void beam_bookkeeping(const BmArgs& A, const BmStep& P, const BmBest&
     place[tid] = twin[tid] ? bm_clear_bit(used, K, q) : best.beam[live[tid]];
   }
   __syncthreads();
-  // hypotheses first: in place, a row whose only child ended may be taken below
-  for (int k = 0; k < K; ++k) {
+  // the texts: a wave a row; hypotheses first: in place, a row whose only child ended may be taken
+  for (int k = wave; k < K; k += waves) {
     const int h = taken[k];
     int64_t* dst = P.out.finished_tokens + (r0 + k) * P.room;
-    if (h >= 0) {
+    if (h >= 0)
       bm_copy(dst, P.in.tokens + (r0 + best.beam[h]) * P.room, len);
-      if (tid == 0) {
-        dst[len] = best.token[h];
-        P.out.finished_lengths[r0 + k] = len + 1;
-        P.out.finished_scores[r0 + k] = hyp[h];
-      }
-    } else if (!P.in_place) {
-      const int fl = P.in.finished_lengths[r0 + k];
-      bm_copy(dst, P.in.finished_tokens + (r0 + k) * P.room, min((int64_t)max(fl, 0), P.room));
-      if (tid == 0) {
-        P.out.finished_lengths[r0 + k] = fl;
-        P.out.finished_scores[r0 + k] = old[k];
-      }
-    }
+    else if (!P.in_place)
+      bm_copy(dst, P.in.finished_tokens + (r0 + k) * P.room, held(k));
   }
-  __syncthreads();
-  for (int i = 0; i < K; ++i) {
+  if (P.in_place) __syncthreads();
+  for (int i = wave; i < K; i += waves) {
     const int c = live[i], k = place[i];
-    int64_t* dst = P.out.tokens + (r0 + k) * P.room;
-    if (!P.in_place || k != best.beam[c]) bm_copy(dst, P.in.tokens + (r0 + best.beam[c]) * P.room, len);
-    if (tid == 0) {
-      dst[len] = best.token[c];
-      P.next[r0 + k] = best.token[c];
-      P.rows[r0 + k] = r0 + best.beam[c];
-      P.out.lengths[r0 + k] = len + 1;
-      P.out.scores[r0 + k] = best.value[c];
+    if (!P.in_place || k != best.beam[c])
+      bm_copy(P.out.tokens + (r0 + k) * P.room, P.in.tokens + (r0 + best.beam[c]) * P.room, len);
+  }
+  if (tid < K) {
+    const int c = live[tid], h = taken[tid];
+    const int64_t r = r0 + place[tid], f = r0 + tid;
+    P.out.tokens[r * P.room + len] = best.token[c];
+    P.next[r] = best.token[c];
+    P.rows[r] = r0 + best.beam[c];
+    P.out.lengths[r] = len + 1;
+    P.out.scores[r] = best.value[c];
+    if (h >= 0) {
+      P.out.finished_tokens[f * P.room + len] = best.token[h];
+      P.out.finished_lengths[f] = len + 1;
+      P.out.finished_scores[f] = hyp[h];
+    } else if (!P.in_place) {
+      P.out.finished_lengths[f] = P.in.finished_lengths[f];
+      P.out.finished_scores[f] = old[tid];
     }
   }
-  if (tid == 0) {
+  if (tid < 64) {
     float worst = __builtin_inff();
-    for (int k = 0; k < K; ++k) worst = fminf(worst, taken[k] >= 0 ? hyp[taken[k]] : old[k]);
-    // early 0: at the present length; 1: as soon as there are K hypotheses; 2: at the length that helps most
-    const double ahead = P.early == 2 && P.penalty > 0 ? pow((double)max(P.room - prompt, (int64_t)1), P.penalty) : span;
-    const bool over = P.early == 1 ? worst > -__builtin_inff()
-                                   : !((float)((double)best.value[live[0]] / ahead) > worst);
-    P.out.done[b] = over || last;
-    P.out.prompt_lengths[b] = prompt;
+    for (int k = tid; k < K; k += 64) worst = fminf(worst, taken[k] >= 0 ? hyp[taken[k]] : old[k]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) worst = fminf(worst, __shfl_xor(worst, o, 64));
+    if (tid == 0) {
+      // early 0: at the present length; 1: as soon as there are K hypotheses; 2: at the length that helps most
+      const double ahead = P.early == 2 && P.penalty > 0 ? pow((double)max(P.room - prompt, (int64_t)1), P.penalty) : span;
+      const bool over = P.early == 1 ? worst > -__builtin_inff()
+                                     : !((float)((double)best.value[live[0]] / ahead) > worst);
+      P.out.done[b] = over || last;
+      P.out.prompt_lengths[b] = prompt;
+    }
   }
 }
 
 template <int NT, bool STEP>
 __global__ __launch_bounds__(NT) void beam_merge_kernel(const BmArgs A, const BmStep P) {
+  constexpr int HOLD = 4;  // candidates that a lane keeps; further ones are read twice
   __shared__ uint64_t got[BM_CAP];
   __shared__ uint64_t got_at[BM_CAP];  // what decides where values are equal (bm_place), the least first
-  __shared__ uint32_t top[NT];
+  __shared__ uint32_t top[256];
   __shared__ double lse[BM_MOST];
   __shared__ float score[BM_MOST];
   __shared__ int nan_rows[BM_MOST];  // the rows of NaN, in order; then the others
@@ -415,31 +434,37 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(const BmArgs A, const Bm
   __shared__ BmBest best;
   const int tid = threadIdx.x, lane = tid & 63, K = A.beams, M = A.M;
   const int64_t r0 = (int64_t)blockIdx.x * K;
+  const int L = K * A.S, N = L * M;  // lists, candidates
+  const uint64_t* list = A.got + r0 * A.S * M;
+  // the candidates on their way while lse is formed
+  uint64_t held[HOLD], head = 0;
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i) held[i] = tid + NT * i < N ? list[tid + NT * i] : 0;
+  if (tid < 256 && L <= 256 && tid / L < M) head = list[(tid % L) * M + tid / L];
   if (tid < 2) poison[tid] = 0;
   if (tid == 0) count = 0;
   __syncthreads();
   for (int k = tid >> 6; k < K; k += NT / 64) {  // a wave a row
-    const float* pm = A.pm + (r0 + k) * A.S;
-    const float* ps = A.ps + (r0 + k) * A.S;
+    const float2* sums = A.sums + (r0 + k) * A.S;
+    const float own = A.scores[r0 + k];
     float m = -__builtin_inff();
-    for (int j = lane; j < A.S; j += 64) m = fmaxf(m, pm[j]);
+    for (int j = lane; j < A.S; j += 64) m = fmaxf(m, sums[j].x);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     double s = 0.0;
-    bool odd = false;
     for (int j = lane; j < A.S; j += 64) {
-      odd |= ps[j] != ps[j];
-      if (pm[j] > -__builtin_inff()) s += (double)ps[j] * exp((double)pm[j] - (double)m);
+      const float2 q = sums[j];
+      s += q.x > -__builtin_inff() ? (double)q.y * exp((double)q.x - (double)m) : (double)q.y;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (__any(odd) || !(A.scores[r0 + k] < __builtin_inff())) {
-      if (lane == 0) atomicOr((unsigned long long*)&poison[k >> 6], 1ull << (k & 63));
-      s = 1.0;
-    }
     if (lane == 0) {
+      if (s != s || !(own < __builtin_inff())) {
+        atomicOr((unsigned long long*)&poison[k >> 6], 1ull << (k & 63));
+        s = 1.0;
+      }
       lse[k] = A.normalized || !(s > 0.0) ? 0.0 : (double)m + log(s);
-      score[k] = A.scores[r0 + k];
+      score[k] = own;
     }
   }
   __syncthreads();
@@ -456,37 +481,36 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(const BmArgs A, const Bm
   const int bad = __popcll(poison[0]) + __popcll(poison[1]);
   const int first = (int)min((int64_t)bad * A.V, (int64_t)M);  // NaN ranks first
   const int want = M - first;
-  const int N = K * A.S * M;
-  const auto entry = [&](int j, double& v, uint64_t& at) {  // false: nothing to choose
-    const float l = A.pv[r0 * A.S * M + j];
-    const int k = j / (A.S * M);
-    v = (double)score[k] + ((double)l - lse[k]);
-    if (!(v > -__builtin_inf()) || (poison[k >> 6] >> (k & 63) & 1)) return false;
-    at = bm_place(k, l, A.pt[r0 * A.S * M + j]);
-    return true;
+  const auto value = [&](uint64_t c) {  // -inf: nothing to choose
+    const int k = (int)(c >> 23 & 0x7f);
+    if ((uint32_t)(c >> 32) <= BM_NONE || (poison[k >> 6] >> (k & 63) & 1)) return -__builtin_inf();
+    return (double)score[k] + ((double)bm_value((uint32_t)(c >> 32)) - lse[k]);
   };
-  uint32_t mine = BM_NONE;
-  for (int j = tid; j < N; j += NT) {
-    double v;
-    uint64_t at;
-    if (entry(j, v, at)) mine = max(mine, bm_key((float)v));
+  // 256 candidates give the bound: the best of every list and, where lists are few, the next ones
+  if (tid < 256) {
+    uint32_t mine = bm_key((float)value(head));
+    if (L > 256)
+      for (int l = tid; l < L; l += 256) mine = max(mine, bm_key((float)value(list[(int64_t)l * M])));
+    top[tid] = mine;
   }
-  top[tid] = mine;
   __syncthreads();
   if (tid < 64) {
-    const uint32_t t = bm_bound<NT / 64, 0>(top, max(want, 1));
+    const uint32_t t = bm_bound<4, 0>(top, max(want, 1));
     if (tid == 0) bound = t;
   }
   __syncthreads();
   const uint32_t at_least = bound;
-  for (int j = tid; j < N; j += NT) {
-    double v;
-    uint64_t at;
-    if (entry(j, v, at) && bm_key((float)v) >= at_least) {
+  const auto gather = [&](uint64_t c) {
+    const double v = value(c);
+    if (bm_key((float)v) >= at_least) {
       const int p = atomicAdd(&count, 1);
-      if (p < BM_CAP) got[p] = bm_key(v), got_at[p] = at;
+      if (p < BM_CAP) got[p] = bm_key(v), got_at[p] = bm_place(c);
     }
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i)
+    if (held[i]) gather(held[i]);
+  for (int j = tid + NT * HOLD; j < N; j += NT) gather(list[j]);
   __syncthreads();
   int n = count;
   const auto put = [&](int r, float v, int beam, int token) {
@@ -507,10 +531,9 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(const BmArgs A, const Bm
     for (int r = 0; r < want; ++r) {
       uint64_t k = 0, a = ~0ull;
       for (int j = tid; j < N; j += NT) {
-        double v;
-        uint64_t at;
-        if (!entry(j, v, at)) continue;
-        const uint64_t c = bm_key(v);
+        const double v = value(list[j]);
+        if (!(v > -__builtin_inf())) continue;
+        const uint64_t c = bm_key(v), at = bm_place(list[j]);
         if ((c < lk || (c == lk && at > la)) && (c > k || (c == k && at < a))) k = c, a = at;
       }
 #pragma unroll
@@ -577,10 +600,8 @@ int bm_run(BmArgs& a, const BmStep* step, int64_t prompts, int dtype, void* work
   const size_t need = (size_t)(rows * a.S) * (8u * (size_t)a.M + 8u);
   if (!workspace || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))
     return fail(RWKV7MI_ESIZE, w + ": workspace missing, unaligned or smaller than rwkv7mi_beam_workspace_bytes");
-  a.pv = static_cast<float*>(workspace);
-  a.pt = reinterpret_cast<int*>(a.pv + rows * a.S * a.M);
-  a.pm = reinterpret_cast<float*>(a.pt + rows * a.S * a.M);
-  a.ps = a.pm + rows * a.S;
+  a.got = static_cast<uint64_t*>(workspace);
+  a.sums = reinterpret_cast<float2*>(a.got + rows * a.S * a.M);
   const int rc = dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int RUNS = 32 / (16 / (int)sizeof(T));
@@ -589,9 +610,9 @@ int bm_run(BmArgs& a, const BmStep* step, int64_t prompts, int dtype, void* work
   });
   if (rc) return rc;
   if (step)
-    hipLaunchKernelGGL((beam_merge_kernel<256, true>), dim3((unsigned)prompts), dim3(256), 0, stream, a, *step);
+    hipLaunchKernelGGL((beam_merge_kernel<1024, true>), dim3((unsigned)prompts), dim3(1024), 0, stream, a, *step);
   else
-    hipLaunchKernelGGL((beam_merge_kernel<256, false>), dim3((unsigned)prompts), dim3(256), 0, stream, a, BmStep{});
+    hipLaunchKernelGGL((beam_merge_kernel<1024, false>), dim3((unsigned)prompts), dim3(1024), 0, stream, a, BmStep{});
   return check_launch("beam_merge_kernel");
 }
 
