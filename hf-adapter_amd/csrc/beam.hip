@@ -31,7 +31,9 @@ namespace rwkv7mi {
 namespace {
 
 constexpr int BM_THREADS = 256;
+constexpr int BM_MERGE = 1024;    // lanes that join a prompt's slices
 constexpr int BM_CAP = 1024;      // candidates that a workgroup gathers
+constexpr int BM_RANKED = 320;    // of them ranked without a second bound
 constexpr int BM_MOST = 128;      // candidates of a prompt
 constexpr int BM_ENDS = 8;        // end tokens
 
@@ -95,17 +97,50 @@ __device__ __forceinline__ uint64_t bm_place(uint64_t c) {
 __device__ __forceinline__ int bm_beam(uint64_t p) { return (int)(p >> 55); }
 __device__ __forceinline__ int bm_token(uint64_t p) { return (int)(p & 0x7fffff); }
 
-__device__ __forceinline__ uint32_t bm_wave_max(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+// the wave's maximum, in every lane (NaN counts as nothing)
+__device__ __forceinline__ float bm_wave_max(float v) {
+  v = fmaxf(v, dpp_row_ror<8>(v));
+  v = fmaxf(v, dpp_row_ror<4>(v));
+  v = fmaxf(v, dpp_row_ror<2>(v));
+  v = fmaxf(v, dpp_row_ror<1>(v));
+  return fmaxf(fmaxf(lane_f(v, 0), lane_f(v, 16)), fmaxf(lane_f(v, 32), lane_f(v, 48)));
+}
+
+// the maximum and the total over the 16 lanes of a row, in each of them
+__device__ __forceinline__ float bm_row_max(float v) {
+  v = fmaxf(v, dpp_row_ror<8>(v));
+  v = fmaxf(v, dpp_row_ror<4>(v));
+  v = fmaxf(v, dpp_row_ror<2>(v));
+  return fmaxf(v, dpp_row_ror<1>(v));
+}
+template <int N>
+__device__ __forceinline__ double bm_turn(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, 0x120 + N, 0xF, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), 0x120 + N, 0xF, 0xF, false);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ double bm_row_sum(double v) {
+  v += bm_turn<8>(v);
+  v += bm_turn<4>(v);
+  v += bm_turn<2>(v);
+  return v + bm_turn<1>(v);
+}
+// the total over the 16 lanes of a row, in each of them
+__device__ __forceinline__ int bm_row_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x124, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x122, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x121, 0xF, 0xF, false);
   return v;
 }
 
-// The largest t such that M of the n keys in LDS (64 Q of them, all above
-// BM_NONE or equal to it) reach t, as far as bits LOW and up tell; BM_NONE + 1 where
-// fewer than M are above BM_NONE.  One wave.
+// A bound that at least M of the 64 Q keys in LDS reach, and no more than M + SLACK of them where bits
+// LOW and up can tell (the largest such, bit by bit from the top); BM_NONE + 1 where fewer than M are
+// above BM_NONE.  One wave.
 template <int Q, int LOW>
 __device__ __forceinline__ uint32_t bm_bound(const uint32_t* keys, int M) {
+  constexpr int SLACK = 16;
   uint32_t k[Q];
 #pragma unroll
   for (int q = 0; q < Q; ++q) k[q] = keys[64 * q + (threadIdx.x & 63)];
@@ -116,115 +151,191 @@ __device__ __forceinline__ uint32_t bm_bound(const uint32_t* keys, int M) {
 #pragma unroll
     for (int q = 0; q < Q; ++q) n += __popcll(__ballot(k[q] >= c));
     if (n >= M) t = c;
-    if (n == M) break;
+    if (n >= M && n <= M + SLACK) break;
   }
   return max(t, BM_NONE + 1);
 }
 
 }  // namespace
 
-// RUNS 16-byte runs a lane.
+namespace {
+
+// element e of a run of 16 bytes
+template <typename T>
+__device__ __forceinline__ float bm_element(const uint32_t (&d)[4], int e) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(d[e]);
+  } else {
+    const uint32_t w = d[e / 2];
+    return to_f32(__builtin_bit_cast(T, (uint16_t)(e & 1 ? w >> 16 : w & 0xffffu)));
+  }
+}
+
+// that element less m (minus: -m), exactly as its fp32 value less m
+template <typename T>
+__device__ __forceinline__ float bm_less(const uint32_t (&d)[4], int e, float minus) {
+  if constexpr (std::is_same<T, __half>::value) {
+    float r;  // (the conversion inside the addition)
+    const uint32_t w = d[e / 2];
+    if (e & 1)
+      asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(minus));
+    else
+      asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(minus));
+    return r;
+  } else {
+    return bm_element<T>(d, e) + minus;
+  }
+}
+
+// the largest element of a run (NaN counts as nothing, or as the largest)
+template <typename T>
+__device__ __forceinline__ float bm_run_max(const uint32_t (&d)[4]) {
+  if constexpr (std::is_same<T, __half>::value) {
+    f16x2 h[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t w = d[q];
+      h[q] = __builtin_bit_cast(f16x2, w);
+    }
+    const f16x2 t = __builtin_elementwise_max(__builtin_elementwise_max(h[0], h[1]), __builtin_elementwise_max(h[2], h[3]));
+    return fmaxf((float)t[0], (float)t[1]);
+  } else {
+    float t = bm_element<T>(d, 0);
+#pragma unroll
+    for (int e = 1; e < 16 / (int)sizeof(T); ++e) t = fmaxf(t, bm_element<T>(d, e));
+    return t;
+  }
+}
+
+}  // namespace
+
+// RUNS 16-byte runs a lane, kept as they are in memory.
 template <typename T, int RUNS>
 __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) {
-  constexpr int E = 16 / (int)sizeof(T), SLICE = BM_THREADS * RUNS * E;
+  constexpr int E = 16 / (int)sizeof(T), SLICE = BM_THREADS * RUNS * E, WAVES = BM_THREADS / 64;
   constexpr int LOW = std::is_same<T, __half>::value ? 13 : sizeof(T) == 2 ? 16 : 0;  // bits that T's values have
   __shared__ uint64_t got[BM_CAP];
   __shared__ uint32_t top[BM_THREADS];
-  __shared__ uint32_t bound, wave_top[BM_THREADS / 64];
-  __shared__ float wave_sum_[BM_THREADS / 64];
+  __shared__ uint32_t bound;
+  __shared__ float wave_top[WAVES], wave_sums[WAVES];
   __shared__ int count;
-  const int tid = threadIdx.x;
-  const int64_t row = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int beam = (int)blockIdx.y;
+  const int64_t row = (int64_t)blockIdx.z * A.beams + beam;
   const T* x = static_cast<const T*>(A.x) + row * A.ldx;
   const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int c0 = (int)blockIdx.x * SLICE - shift;  // the slice's first token (before the row in the first slice)
-  float v[RUNS][E];
+  const int t0 = c0 + E * tid;
+  // whole runs all at once (others read as zeros), then what the row's two ends need
+  const __amdgpu_buffer_rsrc_t mem = make_rsrc(x - shift, (uint32_t)(shift + A.V) * (uint32_t)sizeof(T));
+  uint32_t d[RUNS][4];
 #pragma unroll
   for (int u = 0; u < RUNS; ++u) {
-    const int i = c0 + E * (BM_THREADS * u + tid);
-    if (i >= 0 && i + E <= A.V) {
-      const uint4 d = *reinterpret_cast<const uint4*>(x + i);
-      const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+    const int i = t0 + E * BM_THREADS * u;
+    const u32x4 w = buf_ld16(mem, i >= 0 && i + E <= A.V ? (uint32_t)(i + shift) * (uint32_t)sizeof(T) : BUF_OOB);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) d[u][q] = w[q];
+  }
+  if (c0 < 0 || c0 + SLICE > A.V) {
+    for (int u = 0; u < RUNS; ++u) {
+      const int i = t0 + E * BM_THREADS * u;
+      if (i >= 0 && i + E <= A.V) continue;
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
       for (int e = 0; e < E; ++e) {
+        const bool in = i + e >= 0 && i + e < A.V;
         if constexpr (sizeof(T) == 4)
-          v[u][e] = __uint_as_float(w[e]);
+          w[e] = in ? __float_as_uint(x[i + e]) : 0xff800000u;
         else
-          v[u][e] = to_f32(__builtin_bit_cast(T, (uint16_t)(w[e / 2] >> (16 * (e & 1)))));
+          w[e / 2] |= (uint32_t)(in ? __builtin_bit_cast(uint16_t, x[i + e]) : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u)
+                      << (16 * (e & 1));
       }
-    } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[u][e] = i + e >= 0 && i + e < A.V ? to_f32(x[i + e]) : -__builtin_inff();
+      for (int q = 0; q < RUNS; ++q)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[q][j] = q == u ? w[j] : d[q][j];
     }
   }
-  if (tid == 0) count = 0;
   float run_best[RUNS], best = -__builtin_inff();
 #pragma unroll
   for (int u = 0; u < RUNS; ++u) {
-    run_best[u] = v[u][0];
-#pragma unroll
-    for (int e = 1; e < E; ++e) run_best[u] = fmaxf(run_best[u], v[u][e]);
+    run_best[u] = bm_run_max<T>(d[u]);
     best = fmaxf(best, run_best[u]);
   }
-  const uint32_t mine = bm_key(best);
-  top[tid] = mine;
-  const uint32_t wtop = bm_wave_max(mine);
-  if ((tid & 63) == 0) wave_top[tid >> 6] = wtop;
+  if (tid == 0) count = 0;
+  top[tid] = bm_key(best);
+  best = bm_wave_max(best);
+  if (lane == 0) wave_top[wave] = best;
   __syncthreads();
-  uint32_t all = wave_top[0];
+  float m = wave_top[0];
 #pragma unroll
-  for (int w = 1; w < BM_THREADS / 64; ++w) all = max(all, wave_top[w]);
-  if (tid < 64) {
-    const uint32_t t = bm_bound<BM_THREADS / 64, LOW>(top, A.M);
+  for (int w = 1; w < WAVES; ++w) m = fmaxf(m, wave_top[w]);
+  if (wave == 0) {
+    const uint32_t t = bm_bound<WAVES, LOW>(top, A.M);
     if (tid == 0) bound = t;
   }
-  const float m = bm_value(all);
   // NaN and +inf make the sum NaN (a slice of -inf and NaN alone: asked for)
   float s = 0.f;
-  if (all > BM_NONE) {
+  if (m > -__builtin_inff()) {
 #pragma unroll
-    for (int u = 0; u < RUNS; ++u)
+    for (int u = 0; u < RUNS; ++u) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v[u][e] - m) * 1.44269504f);
+      for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(bm_less<T>(d[u], e, -m) * 1.44269504f);
+      __builtin_amdgcn_sched_barrier(0);  // (one run's exponentials at a time: registers)
+    }
   } else {
 #pragma unroll
     for (int u = 0; u < RUNS; ++u)
 #pragma unroll
-      for (int e = 0; e < E; ++e) s = v[u][e] != v[u][e] ? __builtin_nanf("") : s;
+      for (int e = 0; e < E; ++e) {
+        const float v = bm_element<T>(d[u], e);
+        s = v != v ? v : s;
+        __builtin_amdgcn_sched_barrier(0);
+      }
   }
   s = wave_sum(s);
-  if ((tid & 63) == 0) wave_sum_[tid >> 6] = s;
+  if (lane == 0) wave_sums[wave] = s;
   __syncthreads();
-  const uint32_t at_least = bound;
-  const float reach = bm_value(at_least);
+  const float reach = bm_value(bound);
   const int64_t slice = row * A.S + blockIdx.x;
-  const int beam = (int)(row % A.beams);
+  uint64_t* out = A.got + slice * A.M;
+  // the runs that hold one that reaches: most lanes none, few lanes two
+  uint32_t runs = 0;
+#pragma unroll
+  for (int u = 0; u < RUNS; ++u) runs |= (run_best[u] >= reach ? 1u : 0u) << u;
+  while (runs) {
+    const int u = __builtin_ctz(runs);
+    runs &= runs - 1;
+    uint32_t w[4] = {d[0][0], d[0][1], d[0][2], d[0][3]}, hits = 0;
+#pragma unroll
+    for (int q = 1; q < RUNS; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = q == u ? d[q][j] : w[j];
+#pragma unroll
+    for (int e = 0; e < E; ++e) hits |= (bm_element<T>(w, e) >= reach ? 1u : 0u) << e;
+    for (; hits; hits &= hits - 1) {
+      const int p = atomicAdd(&count, 1), e = __builtin_ctz(hits), q = sizeof(T) == 4 ? e : e >> 1;
+      uint32_t one[4] = {q & 2 ? (q & 1 ? w[3] : w[2]) : (q & 1 ? w[1] : w[0])};
+      if (sizeof(T) == 2 && e & 1) one[0] >>= 16;
+      if (p < BM_CAP)
+        got[p] = (uint64_t)bm_key(bm_element<T>(one, 0)) << 32 | (uint32_t) ~(t0 + E * BM_THREADS * u + e);
+    }
+  }
+  __syncthreads();
   if (tid == 0) {
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < BM_THREADS / 64; ++w) sum += wave_sum_[w];
+    for (int w = 0; w < WAVES; ++w) sum += wave_sums[w];
     A.sums[slice] = make_float2(m, sum);
   }
-  uint64_t* out = A.got + slice * A.M;
-  const int t0 = c0 + E * tid;
-#pragma unroll
-  for (int u = 0; u < RUNS; ++u) {
-    if (!(run_best[u] >= reach)) continue;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (v[u][e] >= reach) {
-        const int p = atomicAdd(&count, 1);
-        if (p < BM_CAP) got[p] = (uint64_t)bm_key(v[u][e]) << 32 | (uint32_t) ~(t0 + E * BM_THREADS * u + e);
-      }
-  }
-  __syncthreads();
   const int n = count;
   if (n <= BM_CAP) {
-    for (int i = tid; i < n; i += BM_THREADS) {
+    for (int i = tid >> 4; i < n; i += BM_THREADS / 16) {  // 16 lanes a candidate
       const uint64_t k = got[i];
       int r = 0;
-      for (int j = 0; j < n; ++j) r += got[j] > k;
-      if (r < A.M) out[r] = bm_pack((uint32_t)(k >> 32), beam, (int)~(uint32_t)k);
+      for (int j = tid & 15; j < n; j += 16) r += got[j] > k;
+      r = bm_row_sum(r);
+      if (r < A.M && (tid & 15) == 0) out[r] = bm_pack((uint32_t)(k >> 32), beam, (int)~(uint32_t)k);
     }
     for (int r = n + tid; r < A.M; r += BM_THREADS) out[r] = 0;
     return;
@@ -233,23 +344,30 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
   uint64_t last = ~0ull;
   for (int r = 0; r < A.M; ++r) {
     uint64_t k = 0;
+    int t = t0;
 #pragma unroll
-    for (int u = 0; u < RUNS; ++u)
+    for (int u = 0; u < RUNS; ++u) {
+      asm volatile("" : "+v"(t));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(d[u][q]));  // (converted anew each time: registers)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const uint64_t c = (uint64_t)bm_key(v[u][e]) << 32 | (uint32_t) ~(t0 + E * BM_THREADS * u + e);
-        if (v[u][e] >= reach && c < last && c > k) k = c;
+        const float v = bm_element<T>(d[u], e);
+        const uint64_t c = (uint64_t)bm_key(v) << 32 | (uint32_t) ~(t + E * BM_THREADS * u + e);
+        if (v >= reach && c < last && c > k) k = c;
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       const uint64_t c = __shfl_xor((unsigned long long)k, o, 64);
       k = max(k, c);
     }
     __syncthreads();
-    if ((tid & 63) == 0) got[tid >> 6] = k;
+    if (lane == 0) got[wave] = k;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < BM_THREADS / 64; ++w) k = max(k, got[w]);
+    for (int w = 0; w < WAVES; ++w) k = max(k, got[w]);
     last = k;
     if (tid == 0) out[r] = bm_pack((uint32_t)(k >> 32), beam, (int)~(uint32_t)k);
   }
@@ -262,12 +380,19 @@ struct BmBest {  // a prompt's candidates, best first
   int token[BM_MOST], beam[BM_MOST];
 };
 
-// the position of the q-th (from 0) clear bit of the first n of mask; n where there is none
-__device__ __forceinline__ int bm_clear_bit(const uint64_t* mask, int n, int q) {
-  for (int i = 0; i < n; ++i)
-    if (!(mask[i >> 6] >> (i & 63) & 1) && q-- == 0) return i;
-  return n;
+// what the lanes of a wave wrote to LDS is there for the others
+__device__ __forceinline__ void bm_wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
+
+struct BmBook {  // what one wave decides and all copy by
+  int live[BM_MOST], place[BM_MOST], taken[BM_MOST];  // taken: the hypothesis of a slot, -1: as before
+  float hyp[BM_MOST], old[BM_MOST];
+  int old_length[BM_MOST];
+  int list[BM_MOST], owner[BM_MOST];
+  double span;
+};
 
 // a row of n tokens by one wave, eight loads in flight
 __device__ __forceinline__ void bm_copy(int64_t* dst, const int64_t* src, int n) {
@@ -285,24 +410,88 @@ __device__ __forceinline__ void bm_copy(int64_t* dst, const int64_t* src, int n)
 
 }  // namespace
 
-__device__ void beam_bookkeeping(const BmArgs& A, const BmStep& P, const BmBest& best) {
-  __shared__ int live[BM_MOST], place[BM_MOST], taken[BM_MOST];  // taken: the hypothesis of a slot, -1: as before
-  __shared__ float hyp[BM_MOST], old[BM_MOST];
-  __shared__ uint64_t used[2], kept[2];
-  __shared__ int is_end[BM_MOST], twin[BM_MOST];
-  const int tid = threadIdx.x, K = A.beams;
+// One wave: which candidates live on, where, and which texts end.
+__device__ __forceinline__ void beam_decide(const BmArgs& A, const BmStep& P, const BmBest& best, BmBook& k, bool last) {
+  const int lane = threadIdx.x & 63, K = A.beams;
+  const uint64_t below = (1ull << lane) - 1;
+  int lives = 0, newcomers = 0;
+  bool any = false;
+  for (int r0 = 0; r0 < A.M; r0 += 64) {
+    const int r = r0 + lane;
+    const bool in = r < A.M;
+    const float v = in ? best.value[r] : -__builtin_inff();
+    bool end = false;
+    for (int e = 0; e < P.ends; ++e) end |= in && best.token[r] == P.end[e];
+    end = end && v > -__builtin_inff();
+    // the first K that do not end live on
+    const uint64_t on = __ballot(in && !end);
+    const int rank = lives + __popcll(on & below);
+    if (in && !end && rank < K) k.live[rank] = r;
+    lives += __popcll(on);
+    if (r < K) {
+      const float h = (end || last) && v > -__builtin_inff() ? (float)((double)v / k.span) : -__builtin_inff();
+      k.hyp[r] = h;
+      k.owner[r] = K;
+      k.taken[r] = -1;
+      any |= h > -__builtin_inff();
+    }
+  }
+  bm_wave_sync();
+  if (__any(any)) {
+    // the K best of the hypotheses so far and of those that end here, earlier ones first
+    uint64_t kept[2] = {0, 0};
+    for (int q = 0; q < 2 && 64 * q < K; ++q) {
+      const int r = 64 * q + lane;
+      const float o = r < K ? k.old[r] : 0.f, h = r < K ? k.hyp[r] : -__builtin_inff();
+      int ro = r < K ? 0 : K, rh = 0;
+      for (int j = 0; j < K; ++j) {
+        const float oj = k.old[j], hj = k.hyp[j];
+        ro += (oj > o || (oj == o && j < r)) + (hj > o);
+        rh += (oj >= h) + (hj > h || (hj == h && j < r));
+      }
+      kept[q] = __ballot(ro < K);
+      const uint64_t in = __ballot(h > -__builtin_inff() && rh < K);
+      if (in >> lane & 1) k.list[newcomers + __popcll(in & below)] = r;
+      newcomers += __popcll(in);
+    }
+    bm_wave_sync();
+    for (int q = 0, gone = 0; q < 2 && 64 * q < K; ++q) {
+      const int r = 64 * q + lane;
+      const uint64_t go = __ballot(r < K && !(kept[q] >> lane & 1));
+      const int at = gone + __popcll(go & below);
+      if ((go >> lane & 1) && at < newcomers) k.taken[r] = k.list[at];
+      gone += __popcll(go);
+    }
+  }
+  // a beam's first child keeps its row, the others take the rows that are left
+  for (int r = lane; r < K; r += 64) atomicMin(&k.owner[best.beam[k.live[r]]], r);
+  bm_wave_sync();
+  for (int r0 = 0, spare = 0; r0 < K; r0 += 64) {
+    const int r = r0 + lane;
+    const uint64_t free = __ballot(r < K && k.owner[r] == K);
+    if (free >> lane & 1) k.list[spare + __popcll(free & below)] = r;
+    spare += __popcll(free);
+  }
+  bm_wave_sync();
+  for (int r0 = 0, twins = 0; r0 < K; r0 += 64) {
+    const int r = r0 + lane, beam = r < K ? best.beam[k.live[r]] : 0;
+    const uint64_t twin = __ballot(r < K && k.owner[beam] != r);
+    if (r < K) k.place[r] = twin >> lane & 1 ? k.list[twins + __popcll(twin & below)] : beam;
+    twins += __popcll(twin);
+  }
+}
+
+// All waves: the step behind the selection.  was, len and prompt are the prompt's.
+__device__ __forceinline__ void beam_bookkeeping(const BmArgs& A, const BmStep& P, const BmBest& best, BmBook& book, bool was,
+                                                 int len, int prompt) {
+  const int tid = threadIdx.x, K = A.beams, waves = blockDim.x >> 6, wave = tid >> 6;
   const int64_t b = blockIdx.x, r0 = b * K;
-  const bool was = P.in.done[b];
-  const int len = P.in.lengths[r0], prompt = P.in.prompt_lengths[b];
-  const bool full = len < 0 || len >= P.room;  // (no room: nothing can follow)
-  const int waves = blockDim.x >> 6, wave = tid >> 6;
-  const auto held = [&](int k) { return min(max(P.in.finished_lengths[r0 + k], 0), (int)P.room); };
-  if (was || full) {
+  if (was || len < 0 || len >= P.room) {  // (no room: nothing can follow)
     if (!P.in_place)
       for (int j = wave; j < 2 * K; j += waves) {
         const int64_t at = (r0 + (j >> 1)) * P.room;
         if (j & 1)
-          bm_copy(P.out.finished_tokens + at, P.in.finished_tokens + at, held(j >> 1));
+          bm_copy(P.out.finished_tokens + at, P.in.finished_tokens + at, book.old_length[j >> 1]);
         else
           bm_copy(P.out.tokens + at, P.in.tokens + at, min(max(len, 0), (int)P.room));
       }
@@ -321,56 +510,11 @@ __device__ void beam_bookkeeping(const BmArgs& A, const BmStep& P, const BmBest&
     }
     return;
   }
-  const double span = pow((double)max(len + 1 - prompt, 1), P.penalty);
-  if (tid < K) old[tid] = P.in.finished_scores[r0 + tid], taken[tid] = -1;
-  if (tid < 2) used[tid] = kept[tid] = 0;
   const bool last = len + 1 >= P.room;  // the rows are full behind this token: all texts end
-  if (tid < A.M) {
-    bool end = false;
-    for (int e = 0; e < P.ends; ++e) end |= best.token[tid] == P.end[e];
-    is_end[tid] = end && best.value[tid] > -__builtin_inff();
-    if (tid < K) hyp[tid] = (end || last) && best.value[tid] > -__builtin_inff() ? (float)((double)best.value[tid] / span)
-                                                                                 : -__builtin_inff();
-  }
+  if (wave == 0) beam_decide(A, P, best, book, last);
   __syncthreads();
-  if (tid < A.M && !is_end[tid]) {  // the first K that do not end live on
-    int r = 0;
-    for (int j = 0; j < tid; ++j) r += !is_end[j];
-    if (r < K) live[r] = tid;
-  }
-  if (tid < K) {
-    // the K best of the hypotheses so far and those that end here, earlier ones first
-    const float o = old[tid], h = hyp[tid];
-    int ro = 0, rh = 0;
-    for (int j = 0; j < K; ++j) {
-      ro += (old[j] > o || (old[j] == o && j < tid)) + (hyp[j] > o);
-      rh += (old[j] >= h) + (hyp[j] > h || (hyp[j] == h && j < tid));
-    }
-    if (ro < K) atomicOr((unsigned long long*)&kept[tid >> 6], 1ull << (tid & 63));
-    place[tid] = h > -__builtin_inff() && rh < K;  // (as a flag; places of the beams below)
-  }
-  __syncthreads();
-  if (tid < K && place[tid]) {
-    int q = 0;
-    for (int j = 0; j < tid; ++j) q += place[j];
-    const int slot = bm_clear_bit(kept, K, q);
-    if (slot < K) taken[slot] = tid;
-  }
-  if (tid < K) atomicOr((unsigned long long*)&used[best.beam[live[tid]] >> 6], 1ull << (best.beam[live[tid]] & 63));
-  __syncthreads();
-  if (tid < K) {
-    int t = 0;
-    for (int j = 0; j < tid; ++j) t |= best.beam[live[j]] == best.beam[live[tid]];
-    twin[tid] = t;
-  }
-  __syncthreads();
-  if (tid < K) {
-    // a beam's first child keeps its row, the others take the rows that are left
-    int q = 0;
-    for (int j = 0; j < tid; ++j) q += twin[j];
-    place[tid] = twin[tid] ? bm_clear_bit(used, K, q) : best.beam[live[tid]];
-  }
-  __syncthreads();
+  const int *live = book.live, *place = book.place, *taken = book.taken;
+  const float *hyp = book.hyp, *old = book.old;
   // the texts: a wave a row; hypotheses first: in place, a row whose only child ended may be taken
   for (int k = wave; k < K; k += waves) {
     const int h = taken[k];
@@ -378,10 +522,10 @@ __device__ void beam_bookkeeping(const BmArgs& A, const BmStep& P, const BmBest&
     if (h >= 0)
       bm_copy(dst, P.in.tokens + (r0 + best.beam[h]) * P.room, len);
     else if (!P.in_place)
-      bm_copy(dst, P.in.finished_tokens + (r0 + k) * P.room, held(k));
+      bm_copy(dst, P.in.finished_tokens + (r0 + k) * P.room, book.old_length[k]);
   }
   if (P.in_place) __syncthreads();
-  for (int i = wave; i < K; i += waves) {
+  for (int i = P.in_place ? wave : (wave + waves - K % waves) % waves; i < K; i += waves) {
     const int c = live[i], k = place[i];
     if (!P.in_place || k != best.beam[c])
       bm_copy(P.out.tokens + (r0 + k) * P.room, P.in.tokens + (r0 + best.beam[c]) * P.room, len);
@@ -403,14 +547,14 @@ __device__ void beam_bookkeeping(const BmArgs& A, const BmStep& P, const BmBest&
       P.out.finished_scores[f] = old[tid];
     }
   }
-  if (tid < 64) {
+  if (wave == waves - 1) {
     float worst = __builtin_inff();
-    for (int k = tid; k < K; k += 64) worst = fminf(worst, taken[k] >= 0 ? hyp[taken[k]] : old[k]);
+    for (int k = tid & 63; k < K; k += 64) worst = fminf(worst, taken[k] >= 0 ? hyp[taken[k]] : old[k]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) worst = fminf(worst, __shfl_xor(worst, o, 64));
-    if (tid == 0) {
+    if ((tid & 63) == 0) {
       // early 0: at the present length; 1: as soon as there are K hypotheses; 2: at the length that helps most
-      const double ahead = P.early == 2 && P.penalty > 0 ? pow((double)max(P.room - prompt, (int64_t)1), P.penalty) : span;
+      const double ahead = P.early == 2 && P.penalty > 0 ? pow((double)max(P.room - prompt, (int64_t)1), P.penalty) : book.span;
       const bool over = P.early == 1 ? worst > -__builtin_inff()
                                      : !((float)((double)best.value[live[0]] / ahead) > worst);
       P.out.done[b] = over || last;
@@ -419,88 +563,117 @@ __device__ void beam_bookkeeping(const BmArgs& A, const BmStep& P, const BmBest&
   }
 }
 
-template <int NT, bool STEP>
-__global__ __launch_bounds__(NT) void beam_merge_kernel(const BmArgs A, const BmStep P) {
+template <bool STEP>
+__global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, const BmStep P) {
+  constexpr int NT = BM_MERGE;
   constexpr int HOLD = 4;  // candidates that a lane keeps; further ones are read twice
   __shared__ uint64_t got[BM_CAP];
   __shared__ uint64_t got_at[BM_CAP];  // what decides where values are equal (bm_place), the least first
-  __shared__ uint32_t top[256];
+  __shared__ uint32_t keys[BM_CAP];  // of a sample of the candidates, then of those gathered
   __shared__ double lse[BM_MOST];
   __shared__ float score[BM_MOST];
-  __shared__ int nan_rows[BM_MOST];  // the rows of NaN, in order; then the others
-  __shared__ uint64_t poison[2];
+  __shared__ int by_kind[BM_MOST];  // the rows of NaN, in order; then the others
+  __shared__ bool odd[BM_MOST];      // rows of NaN
+  __shared__ float offset[BM_MOST];  // score - lse in fp32
   __shared__ uint32_t bound;
   __shared__ int count;
   __shared__ BmBest best;
+  __shared__ BmBook book;
   const int tid = threadIdx.x, lane = tid & 63, K = A.beams, M = A.M;
   const int64_t r0 = (int64_t)blockIdx.x * K;
   const int L = K * A.S, N = L * M;  // lists, candidates
   const uint64_t* list = A.got + r0 * A.S * M;
-  // the candidates on their way while lse is formed
+  // candidates by chunks: the next 2^chunk of every list (they are in order), as many as fit HOLD a lane
+  int chunk = 0;
+  while (1 << chunk < M && (L << (chunk + 1)) <= NT * HOLD) ++chunk;
+  const int wide = L << chunk;
+  const auto at = [&](int j, int rank0) {  // candidate j of a chunk
+    const int r = rank0 + (j & ((1 << chunk) - 1));
+    return j < wide && r < M ? list[(int64_t)(j >> chunk) * M + r] : 0;
+  };
+  // a sample of 64 or 256 gives the bound: the best of every list and, where lists are few, the next ones.
+  // (64 cost half the time for a bound that lets a few more through: M of them have to reach it)
+  const int sample = M <= 24 ? 64 : 256;
+  // everything that is read is on its way while lse is formed
+  const int row = tid >> 4, part0 = tid & 15;  // 16 lanes a row
+  float own = row < K ? A.scores[r0 + row] : 0.f;
+  const auto sums_of = [&](int k, int j) {
+    return k < K && j < A.S ? A.sums[(r0 + k) * A.S + j] : make_float2(-__builtin_inff(), 0.f);
+  };
+  float2 sums = sums_of(row, part0);
   uint64_t held[HOLD], head = 0;
+  if (tid < sample && L <= sample && tid / L < M) head = list[(tid % L) * M + tid / L];
 #pragma unroll
-  for (int i = 0; i < HOLD; ++i) held[i] = tid + NT * i < N ? list[tid + NT * i] : 0;
-  if (tid < 256 && L <= 256 && tid / L < M) head = list[(tid % L) * M + tid / L];
-  if (tid < 2) poison[tid] = 0;
+  for (int i = 0; i < HOLD; ++i) held[i] = at(tid + NT * i, 0);
+  bool was = false;
+  int len = 0, prompt = 0;
+  if constexpr (STEP) {
+    was = P.in.done[blockIdx.x];
+    len = P.in.lengths[r0];
+    prompt = P.in.prompt_lengths[blockIdx.x];
+    const int k = tid - (NT - BM_MOST);  // (the last waves have no row of sums, as a rule)
+    if (k >= 0 && k < K) {
+      book.old[k] = P.in.finished_scores[r0 + k];
+      book.old_length[k] = min(max(P.in.finished_lengths[r0 + k], 0), (int)P.room);
+    }
+    if (tid == NT - 1) {
+      const double gen = max(len + 1 - prompt, 1);
+      book.span = P.penalty == 1.0 ? gen : pow(gen, P.penalty);
+    }
+  }
   if (tid == 0) count = 0;
-  __syncthreads();
-  for (int k = tid >> 6; k < K; k += NT / 64) {  // a wave a row
-    const float2* sums = A.sums + (r0 + k) * A.S;
-    const float own = A.scores[r0 + k];
-    float m = -__builtin_inff();
-    for (int j = lane; j < A.S; j += 64) m = fmaxf(m, sums[j].x);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    double s = 0.0;
-    for (int j = lane; j < A.S; j += 64) {
-      const float2 q = sums[j];
-      s += q.x > -__builtin_inff() ? (double)q.y * exp((double)q.x - (double)m) : (double)q.y;
+  for (int k = row; k < K; k += NT / 16) {
+    if (k != row) {
+      own = A.scores[r0 + k];
+      sums = sums_of(k, part0);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (lane == 0) {
-      if (s != s || !(own < __builtin_inff())) {
-        atomicOr((unsigned long long*)&poison[k >> 6], 1ull << (k & 63));
-        s = 1.0;
-      }
-      lse[k] = A.normalized || !(s > 0.0) ? 0.0 : (double)m + log(s);
-      score[k] = own;
+    float m = sums.x;
+    for (int j = part0 + 16; j < A.S; j += 16) m = fmaxf(m, sums_of(k, j).x);
+    m = bm_row_max(m);
+    const auto part = [&](float2 q) {
+      return q.x > -__builtin_inff() ? (double)q.y * exp((double)q.x - (double)m) : (double)q.y;
+    };
+    double s = part(sums);
+    for (int j = part0 + 16; j < A.S; j += 16) s += part(sums_of(k, j));
+    s = bm_row_sum(s);
+    const bool nan = s != s || !(own < __builtin_inff());
+    if (part0 == 0) {
+      const double l = A.normalized || nan || !(s > 0.0) ? 0.0 : (double)m + log(s);
+      lse[k] = l;
+      odd[k] = nan;
+      score[k] = nan ? -__builtin_inff() : own;  // (nothing to choose by value)
+      offset[k] = nan ? -__builtin_inff() : (float)((double)own - l);
     }
   }
   __syncthreads();
-  if (tid < K) {
-    const bool p = poison[tid >> 6] >> (tid & 63) & 1;
-    int q = 0, all = 0;
-    for (int j = 0; j < K; ++j) {
-      const bool o = poison[j >> 6] >> (j & 63) & 1;
-      q += j < tid && o == p;
-      all += o;
-    }
-    nan_rows[p ? q : all + q] = tid;
-  }
-  const int bad = __popcll(poison[0]) + __popcll(poison[1]);
+  const uint64_t nan0 = __ballot(lane < K && odd[lane & (BM_MOST - 1)]);
+  const uint64_t nan1 = K > 64 ? __ballot(lane + 64 < K && odd[lane + 64]) : 0;
+  const int bad = __popcll(nan0) + __popcll(nan1);
   const int first = (int)min((int64_t)bad * A.V, (int64_t)M);  // NaN ranks first
   const int want = M - first;
   const auto value = [&](uint64_t c) {  // -inf: nothing to choose
     const int k = (int)(c >> 23 & 0x7f);
-    if ((uint32_t)(c >> 32) <= BM_NONE || (poison[k >> 6] >> (k & 63) & 1)) return -__builtin_inf();
-    return (double)score[k] + ((double)bm_value((uint32_t)(c >> 32)) - lse[k]);
+    if ((uint32_t)(c >> 32) <= BM_NONE) return -__builtin_inf();
+    return fmax((double)score[k] + ((double)bm_value((uint32_t)(c >> 32)) - lse[k]), -__builtin_inf());
   };
-  // 256 candidates give the bound: the best of every list and, where lists are few, the next ones
-  if (tid < 256) {
+  if (tid < sample) {
     uint32_t mine = bm_key((float)value(head));
-    if (L > 256)
-      for (int l = tid; l < L; l += 256) mine = max(mine, bm_key((float)value(list[(int64_t)l * M])));
-    top[tid] = mine;
+    if (L > sample)
+      for (int l = tid; l < L; l += sample) mine = max(mine, bm_key((float)value(list[(int64_t)l * M])));
+    keys[tid] = mine;
   }
   __syncthreads();
   if (tid < 64) {
-    const uint32_t t = bm_bound<4, 0>(top, max(want, 1));
+    const uint32_t t = sample == 64 ? bm_bound<1, 0>(keys, max(want, 1)) : bm_bound<4, 0>(keys, max(want, 1));
     if (tid == 0) bound = t;
   }
   __syncthreads();
   const uint32_t at_least = bound;
+  const float reach = bm_value(at_least);
   const auto gather = [&](uint64_t c) {
+    const float l = bm_value((uint32_t)(c >> 32)), o = offset[c >> 23 & 0x7f];
+    // (fp32, less than four roundings off; false for -inf and what is not there)
+    if (!(l + o + 0x1p-21f * (fabsf(l) + fabsf(o)) >= reach) || (uint32_t)(c >> 32) <= BM_NONE) return;
     const double v = value(c);
     if (bm_key((float)v) >= at_least) {
       const int p = atomicAdd(&count, 1);
@@ -509,21 +682,51 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(const BmArgs A, const Bm
   };
 #pragma unroll
   for (int i = 0; i < HOLD; ++i)
-    if (held[i]) gather(held[i]);
-  for (int j = tid + NT * HOLD; j < N; j += NT) gather(list[j]);
+    if (NT * i < wide) gather(held[i]);
+  for (int j = tid + NT * HOLD; j < wide; j += NT) gather(at(j, 0));
+  // further chunks only behind lists whose last candidate so far reaches the bound
+  for (int rank = 1 << chunk; rank < M; rank += 1 << chunk) {
+    bool more = false;
+    for (int l = tid; l < L; l += NT) more |= bm_key((float)value(list[(int64_t)l * M + rank - 1])) >= at_least;
+    if (!__syncthreads_or(more)) break;
+    for (int j = tid; j < wide; j += NT) gather(at(j, rank));
+  }
   __syncthreads();
   int n = count;
+  // (ranking by counting reads n entries for each: many are cut down by a bound of their own first)
+  if (n > BM_RANKED && n <= BM_CAP) {
+    uint64_t k = 0, p = 0;
+    if (tid < n) k = got[tid], p = got_at[tid];
+    const uint32_t key = tid < n ? bm_key((float)bm_value(k)) : 0u;
+    keys[tid] = key;
+    __syncthreads();
+    if (tid < 64) {
+      const uint32_t t = bm_bound<BM_CAP / 64, 0>(keys, max(want, 1));
+      if (tid == 0) bound = t, count = 0;
+    }
+    __syncthreads();
+    if (key >= bound) {
+      const int q = atomicAdd(&count, 1);
+      got[q] = k, got_at[q] = p;
+    }
+    __syncthreads();
+    n = count;
+  }
   const auto put = [&](int r, float v, int beam, int token) {
     best.value[r] = v;
     best.beam[r] = beam;
     best.token[r] = token;
   };
   if (n <= BM_CAP) {
-    for (int i = tid; i < n; i += NT) {
+    for (int i = tid >> 4; i < n; i += NT / 16) {  // 16 lanes a candidate
       const uint64_t k = got[i], at = got_at[i];
       int r = 0;
-      for (int j = 0; j < n; ++j) r += got[j] > k || (got[j] == k && got_at[j] < at);
-      if (r < want) put(first + r, (float)bm_value(k), bm_beam(at), bm_token(at));
+      for (int j = tid & 15; j < n; j += 16) {
+        const uint64_t c = got[j], ca = got_at[j];
+        r += (c > k) | ((c == k) & (ca < at));
+      }
+      r = bm_row_sum(r);
+      if (r < want && (tid & 15) == 0) put(first + r, (float)bm_value(k), bm_beam(at), bm_token(at));
     }
   } else {
     uint64_t lk = ~0ull, la = 0;
@@ -554,29 +757,36 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(const BmArgs A, const Bm
       if (tid == 0) put(first + r, (float)bm_value(k), bm_beam(a), bm_token(a));
     }
   }
-  __syncthreads();
-  // the NaN rows' tokens, and behind what can be chosen the -inf ones by their index
-  if (tid < first) put(tid, __builtin_nanf(""), nan_rows[tid / A.V], tid % A.V);
   const int found = min(n, want);
-  if (found < want && tid < 64) {
-    int r = first + found;
-    for (int j0 = 0; r < M; j0 += 64) {
-      const int j = j0 + lane;
-      const int ord = bad + j / A.V;  // (M values are there: bad V + others V >= M)
-      const bool there = ord < K;
-      const int beam = there ? nan_rows[ord] : 0, token = j % A.V;
-      bool free = there;
-      for (int i = 0; i < found && free; ++i) free = best.beam[first + i] != beam || best.token[first + i] != token;
-      const uint64_t f = __ballot(free);
-      const int p = r + __popcll(f & ((1ull << lane) - 1));
-      if (free && p < M) put(p, -__builtin_inff(), beam, token);
-      r += __popcll(f);
-      if (!__any(there)) break;
+  if (first || found < want) {
+    // the rows of NaN give their tokens, and behind what can be chosen the others their -inf ones, both
+    // by index: M values are there
+    if (tid < K) {
+      int q = 0;
+      for (int j = 0; j < tid; ++j) q += odd[j] == odd[tid];
+      by_kind[odd[tid] ? q : bad + q] = tid;
+    }
+    __syncthreads();
+    if (tid < first) put(tid, __builtin_nanf(""), by_kind[tid / A.V], tid % A.V);
+    if (found < want && tid < 64) {
+      int r = first + found;
+      for (int j0 = 0; r < M; j0 += 64) {
+        const int j = j0 + lane, kind = bad + j / A.V;
+        const bool there = kind < K;
+        const int beam = there ? by_kind[kind] : 0, token = j % A.V;
+        bool free = there;
+        for (int i = 0; i < found && free; ++i) free = best.beam[first + i] != beam || best.token[first + i] != token;
+        const uint64_t f = __ballot(free);
+        const int p = r + __popcll(f & ((1ull << lane) - 1));
+        if (free && p < M) put(p, -__builtin_inff(), beam, token);
+        r += __popcll(f);
+        if (!__any(there)) break;
+      }
     }
   }
   __syncthreads();
   if constexpr (STEP) {
-    beam_bookkeeping(A, P, best);
+    beam_bookkeeping(A, P, best, book, was, len, prompt);
   } else {
     if (tid < M) {
       const int64_t o = (int64_t)blockIdx.x * M + tid;
@@ -589,14 +799,21 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(const BmArgs A, const Bm
 
 namespace {
 
-constexpr int BM_SLICE = BM_THREADS * 32;  // tokens of a workgroup
-
-int64_t bm_slices(int64_t V) { return (V + 7 + BM_SLICE - 1) / BM_SLICE; }
+// 8 runs a lane where that still fills the card, else 2: 64 x 8 rows of 65536 fp16 logits with their
+// selection take 25.7 us with 8 and 30.3 with 2, 7 x 5 rows of 50277 bf16 15.8 and 13.5
+constexpr int BM_RUNS_MANY = 8, BM_RUNS_FEW = 2, BM_MANY = 512;
+int64_t bm_slice(int dtype, int runs) { return (int64_t)BM_THREADS * runs * (dtype == RWKV7MI_F32 ? 4 : 8); }
+int64_t bm_slices(int64_t V, int dtype, int runs) { return (V + bm_slice(dtype, runs) - 1) / bm_slice(dtype, runs); }
 
 int bm_run(BmArgs& a, const BmStep* step, int64_t prompts, int dtype, void* workspace, size_t bytes, hipStream_t stream,
            const std::string& w) {
   const int64_t rows = prompts * a.beams;
-  a.S = (int)bm_slices(a.V);
+  // (a row starts up to 7 elements behind a boundary)
+  const bool straight = !(reinterpret_cast<uintptr_t>(a.x) & 15) &&
+                        (rows == 1 || a.ldx * (dtype == RWKV7MI_F32 ? 4 : 2) % 16 == 0);
+  const int64_t width = a.V + (straight ? 0 : 7);
+  const bool many = rows * bm_slices(width, dtype, BM_RUNS_MANY) >= BM_MANY;
+  a.S = (int)bm_slices(width, dtype, many ? BM_RUNS_MANY : BM_RUNS_FEW);
   const size_t need = (size_t)(rows * a.S) * (8u * (size_t)a.M + 8u);
   if (!workspace || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))
     return fail(RWKV7MI_ESIZE, w + ": workspace missing, unaligned or smaller than rwkv7mi_beam_workspace_bytes");
@@ -604,15 +821,18 @@ int bm_run(BmArgs& a, const BmStep* step, int64_t prompts, int dtype, void* work
   a.sums = reinterpret_cast<float2*>(a.got + rows * a.S * a.M);
   const int rc = dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    constexpr int RUNS = 32 / (16 / (int)sizeof(T));
-    hipLaunchKernelGGL((beam_slice_kernel<T, RUNS>), dim3((unsigned)a.S, (unsigned)rows), dim3(BM_THREADS), 0, stream, a);
+    const dim3 grid((unsigned)a.S, (unsigned)a.beams, (unsigned)prompts);
+    if (many)
+      hipLaunchKernelGGL((beam_slice_kernel<T, BM_RUNS_MANY>), grid, dim3(BM_THREADS), 0, stream, a);
+    else
+      hipLaunchKernelGGL((beam_slice_kernel<T, BM_RUNS_FEW>), grid, dim3(BM_THREADS), 0, stream, a);
     return check_launch("beam_slice_kernel");
   });
   if (rc) return rc;
   if (step)
-    hipLaunchKernelGGL((beam_merge_kernel<1024, true>), dim3((unsigned)prompts), dim3(1024), 0, stream, a, *step);
+    hipLaunchKernelGGL(beam_merge_kernel<true>, dim3((unsigned)prompts), dim3(BM_MERGE), 0, stream, a, *step);
   else
-    hipLaunchKernelGGL((beam_merge_kernel<1024, false>), dim3((unsigned)prompts), dim3(1024), 0, stream, a, BmStep{});
+    hipLaunchKernelGGL(beam_merge_kernel<false>, dim3((unsigned)prompts), dim3(BM_MERGE), 0, stream, a, BmStep{});
   return check_launch("beam_merge_kernel");
 }
 
@@ -636,7 +856,7 @@ using namespace rwkv7mi;
 
 extern "C" size_t rwkv7mi_beam_workspace_bytes(int64_t rows, int64_t V, int64_t candidates) {
   if (rows <= 0 || V <= 0 || candidates <= 0) return 0;
-  return (size_t)(rows * bm_slices(V)) * (8u * (size_t)candidates + 8u);
+  return (size_t)(rows * bm_slices(V + 7, RWKV7MI_F32, BM_RUNS_FEW)) * (8u * (size_t)candidates + 8u);
 }
 
 extern "C" int rwkv7mi_beam_select(const void* x, int64_t prompts, int64_t beams, int64_t V, int64_t ldx, int dtype,
