@@ -32,7 +32,7 @@ namespace {
 
 constexpr int BM_THREADS = 256;
 constexpr int BM_MERGE = 1024;    // lanes that join a prompt's slices
-constexpr int BM_CAP = 1024;      // candidates that a workgroup gathers
+constexpr int BM_CAP = 1024;      // candidates that a workgroup gathers, whole 64s
 constexpr int BM_RANKED = 320;    // of them ranked without a second bound
 constexpr int BM_MOST = 128;      // candidates of a prompt
 constexpr int BM_ENDS = 8;        // end tokens
@@ -68,6 +68,8 @@ struct BmStep {
   double penalty;
   int early, ends, in_place;
   int64_t end[BM_ENDS];
+  int* plan;  // [prompts][2 beams] where the texts of the rows and of the hypotheses come from, for
+              // beam_texts_kernel (null: copied with the decision): a row of the prompt, -1 as it was
 };
 
 // a float's order as an unsigned number (-0 as 0)
@@ -263,6 +265,8 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
     best = fmaxf(best, run_best[u]);
   }
   if (tid == 0) count = 0;
+#pragma unroll
+  for (int i = 0; i < BM_CAP / BM_THREADS; ++i) got[BM_THREADS * i + tid] = 0;
   top[tid] = bm_key(best);
   best = bm_wave_max(best);
   if (lane == 0) wave_top[wave] = best;
@@ -333,7 +337,7 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
     for (int i = tid >> 4; i < n; i += BM_THREADS / 16) {  // 16 lanes a candidate
       const uint64_t k = got[i];
       int r = 0;
-      for (int j = tid & 15; j < n; j += 16) r += got[j] > k;
+      for (int j = tid & 15; j < n; j += 64) r += (got[j] > k) + (got[j + 16] > k) + (got[j + 32] > k) + (got[j + 48] > k);
       r = bm_row_sum(r);
       if (r < A.M && (tid & 15) == 0) out[r] = bm_pack((uint32_t)(k >> 32), beam, (int)~(uint32_t)k);
     }
@@ -386,83 +390,66 @@ __device__ __forceinline__ void bm_wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
-struct BmBook {  // what one wave decides and all copy by
+struct BmBook {  // what two waves decide and all copy by
   int live[BM_MOST], place[BM_MOST], taken[BM_MOST];  // taken: the hypothesis of a slot, -1: as before
   float hyp[BM_MOST], old[BM_MOST];
   int old_length[BM_MOST];
-  int list[BM_MOST], owner[BM_MOST];
+  int list[BM_MOST], owner[BM_MOST], newcomer[BM_MOST];
   double span;
 };
 
-// a row of n tokens by one wave, eight loads in flight
+template <typename V>
+__device__ __forceinline__ void bm_copy_units(V* dst, const V* src, int n) {
+  int i = threadIdx.x & 63;
+  for (; i + 448 < n; i += 512) {
+    V t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) t[u] = src[i + 64 * u];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) dst[i + 64 * u] = t[u];
+  }
+  V t[8] = {};
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    if (i + 64 * u < n) t[u] = src[i + 64 * u];
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    if (i + 64 * u < n) dst[i + 64 * u] = t[u];
+}
+// a row of n tokens by one wave, eight loads in flight, of two tokens where the rows' alignment allows it
 __device__ __forceinline__ void bm_copy(int64_t* dst, const int64_t* src, int n) {
-  const int lane = threadIdx.x & 63;
-  for (int i0 = lane; i0 < n; i0 += 512) {
-    int64_t t[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (i0 + 64 * u < n) t[u] = src[i0 + 64 * u];
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (i0 + 64 * u < n) dst[i0 + 64 * u] = t[u];
+  if (((reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(src)) & 15) == 0) {
+    bm_copy_units(reinterpret_cast<u32x4*>(dst), reinterpret_cast<const u32x4*>(src), n / 2);
+    if (n & 1 && (threadIdx.x & 63) == 0) dst[n - 1] = src[n - 1];
+  } else {
+    bm_copy_units(dst, src, n);
   }
 }
 
 }  // namespace
 
-// One wave: which candidates live on, where, and which texts end.
-__device__ __forceinline__ void beam_decide(const BmArgs& A, const BmStep& P, const BmBest& best, BmBook& k, bool last) {
+// whether candidate r ends its text
+__device__ __forceinline__ bool bm_ends(const BmStep& P, const BmBest& best, int r) {
+  bool end = false;
+  for (int e = 0; e < P.ends; ++e) end |= best.token[r] == P.end[e];
+  return end && best.value[r] > -__builtin_inff();
+}
+
+// One wave: which candidates live on, and where.
+__device__ __forceinline__ void beam_live(const BmArgs& A, const BmStep& P, const BmBest& best, BmBook& k) {
   const int lane = threadIdx.x & 63, K = A.beams;
   const uint64_t below = (1ull << lane) - 1;
-  int lives = 0, newcomers = 0;
-  bool any = false;
-  for (int r0 = 0; r0 < A.M; r0 += 64) {
+  // the first K that do not end
+  for (int r0 = 0, lives = 0; r0 < A.M && lives < K; r0 += 64) {
     const int r = r0 + lane;
-    const bool in = r < A.M;
-    const float v = in ? best.value[r] : -__builtin_inff();
-    bool end = false;
-    for (int e = 0; e < P.ends; ++e) end |= in && best.token[r] == P.end[e];
-    end = end && v > -__builtin_inff();
-    // the first K that do not end live on
-    const uint64_t on = __ballot(in && !end);
+    const bool stays = r < A.M && !bm_ends(P, best, r);
+    const uint64_t on = __ballot(stays);
     const int rank = lives + __popcll(on & below);
-    if (in && !end && rank < K) k.live[rank] = r;
+    if (stays && rank < K) k.live[rank] = r;
     lives += __popcll(on);
-    if (r < K) {
-      const float h = (end || last) && v > -__builtin_inff() ? (float)((double)v / k.span) : -__builtin_inff();
-      k.hyp[r] = h;
-      k.owner[r] = K;
-      k.taken[r] = -1;
-      any |= h > -__builtin_inff();
-    }
   }
+  for (int r = lane; r < K; r += 64) k.owner[r] = K;
   bm_wave_sync();
-  if (__any(any)) {
-    // the K best of the hypotheses so far and of those that end here, earlier ones first
-    uint64_t kept[2] = {0, 0};
-    for (int q = 0; q < 2 && 64 * q < K; ++q) {
-      const int r = 64 * q + lane;
-      const float o = r < K ? k.old[r] : 0.f, h = r < K ? k.hyp[r] : -__builtin_inff();
-      int ro = r < K ? 0 : K, rh = 0;
-      for (int j = 0; j < K; ++j) {
-        const float oj = k.old[j], hj = k.hyp[j];
-        ro += (oj > o || (oj == o && j < r)) + (hj > o);
-        rh += (oj >= h) + (hj > h || (hj == h && j < r));
-      }
-      kept[q] = __ballot(ro < K);
-      const uint64_t in = __ballot(h > -__builtin_inff() && rh < K);
-      if (in >> lane & 1) k.list[newcomers + __popcll(in & below)] = r;
-      newcomers += __popcll(in);
-    }
-    bm_wave_sync();
-    for (int q = 0, gone = 0; q < 2 && 64 * q < K; ++q) {
-      const int r = 64 * q + lane;
-      const uint64_t go = __ballot(r < K && !(kept[q] >> lane & 1));
-      const int at = gone + __popcll(go & below);
-      if ((go >> lane & 1) && at < newcomers) k.taken[r] = k.list[at];
-      gone += __popcll(go);
-    }
-  }
   // a beam's first child keeps its row, the others take the rows that are left
   for (int r = lane; r < K; r += 64) atomicMin(&k.owner[best.beam[k.live[r]]], r);
   bm_wave_sync();
@@ -481,13 +468,56 @@ __device__ __forceinline__ void beam_decide(const BmArgs& A, const BmStep& P, co
   }
 }
 
+// Another wave: the K best of the hypotheses so far and of those that end here, earlier ones first.
+__device__ __forceinline__ void beam_end(const BmArgs& A, const BmStep& P, const BmBest& best, BmBook& k, bool last) {
+  const int lane = threadIdx.x & 63, K = A.beams;
+  const uint64_t below = (1ull << lane) - 1;
+  bool any = false;
+  for (int r = lane; r < K; r += 64) {
+    const float v = best.value[r];
+    const bool ends = bm_ends(P, best, r) || (last && v > -__builtin_inff());
+    const float h = ends ? (float)((double)v / k.span) : -__builtin_inff();
+    k.hyp[r] = h;
+    k.taken[r] = -1;
+    any |= h > -__builtin_inff();
+  }
+  if (!__any(any)) return;
+  bm_wave_sync();
+  uint64_t kept[2] = {0, 0};
+  int newcomers = 0;
+  for (int q = 0; q < 2 && 64 * q < K; ++q) {
+    const int r = 64 * q + lane;
+    const float o = r < K ? k.old[r] : 0.f, h = r < K ? k.hyp[r] : -__builtin_inff();
+    int ro = r < K ? 0 : K, rh = 0;
+#pragma unroll 4
+    for (int j = 0; j < K; ++j) {
+      const float oj = k.old[j], hj = k.hyp[j];
+      ro += ((oj > o) | ((oj == o) & (j < r))) + (hj > o);
+      rh += (oj >= h) + ((hj > h) | ((hj == h) & (j < r)));
+    }
+    kept[q] = __ballot(ro < K);
+    const uint64_t in = __ballot(h > -__builtin_inff() && rh < K);
+    if (in >> lane & 1) k.newcomer[newcomers + __popcll(in & below)] = r;
+    newcomers += __popcll(in);
+  }
+  bm_wave_sync();
+  for (int q = 0, gone = 0; q < 2 && 64 * q < K; ++q) {
+    const int r = 64 * q + lane;
+    const uint64_t go = __ballot(r < K && !(kept[q] >> lane & 1));
+    const int at = gone + __popcll(go & below);
+    if ((go >> lane & 1) && at < newcomers) k.taken[r] = k.newcomer[at];
+    gone += __popcll(go);
+  }
+}
+
 // All waves: the step behind the selection.  was, len and prompt are the prompt's.
 __device__ __forceinline__ void beam_bookkeeping(const BmArgs& A, const BmStep& P, const BmBest& best, BmBook& book, bool was,
                                                  int len, int prompt) {
   const int tid = threadIdx.x, K = A.beams, waves = blockDim.x >> 6, wave = tid >> 6;
   const int64_t b = blockIdx.x, r0 = b * K;
   if (was || len < 0 || len >= P.room) {  // (no room: nothing can follow)
-    if (!P.in_place)
+    if (P.plan && tid < 2 * K) P.plan[2 * r0 + tid] = -1;
+    if (!P.in_place && !P.plan)
       for (int j = wave; j < 2 * K; j += waves) {
         const int64_t at = (r0 + (j >> 1)) * P.room;
         if (j & 1)
@@ -511,12 +541,17 @@ __device__ __forceinline__ void beam_bookkeeping(const BmArgs& A, const BmStep& 
     return;
   }
   const bool last = len + 1 >= P.room;  // the rows are full behind this token: all texts end
-  if (wave == 0) beam_decide(A, P, best, book, last);
+  if (wave == 0) beam_live(A, P, best, book);
+  if (wave == 1) beam_end(A, P, best, book, last);
   __syncthreads();
   const int *live = book.live, *place = book.place, *taken = book.taken;
   const float *hyp = book.hyp, *old = book.old;
+  if (P.plan && tid < K) {
+    P.plan[2 * r0 + place[tid]] = best.beam[live[tid]];
+    P.plan[2 * r0 + K + tid] = taken[tid] >= 0 ? best.beam[taken[tid]] : -1;
+  }
   // the texts: a wave a row; hypotheses first: in place, a row whose only child ended may be taken
-  for (int k = wave; k < K; k += waves) {
+  for (int k = wave; k < K && !P.plan; k += waves) {
     const int h = taken[k];
     int64_t* dst = P.out.finished_tokens + (r0 + k) * P.room;
     if (h >= 0)
@@ -525,7 +560,7 @@ __device__ __forceinline__ void beam_bookkeeping(const BmArgs& A, const BmStep& 
       bm_copy(dst, P.in.finished_tokens + (r0 + k) * P.room, book.old_length[k]);
   }
   if (P.in_place) __syncthreads();
-  for (int i = P.in_place ? wave : (wave + waves - K % waves) % waves; i < K; i += waves) {
+  for (int i = P.in_place ? wave : (wave + waves - K % waves) % waves; i < K && !P.plan; i += waves) {
     const int c = live[i], k = place[i];
     if (!P.in_place || k != best.beam[c])
       bm_copy(P.out.tokens + (r0 + k) * P.room, P.in.tokens + (r0 + best.beam[c]) * P.room, len);
@@ -622,6 +657,7 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
     }
   }
   if (tid == 0) count = 0;
+  got[tid] = 0;
   for (int k = row; k < K; k += NT / 16) {
     if (k != row) {
       own = A.scores[r0 + k];
@@ -670,26 +706,26 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
   __syncthreads();
   const uint32_t at_least = bound;
   const float reach = bm_value(at_least);
-  const auto gather = [&](uint64_t c) {
+  const auto gather = [&](uint64_t c) {  // whether it reaches the bound
     const float l = bm_value((uint32_t)(c >> 32)), o = offset[c >> 23 & 0x7f];
     // (fp32, less than four roundings off; false for -inf and what is not there)
-    if (!(l + o + 0x1p-21f * (fabsf(l) + fabsf(o)) >= reach) || (uint32_t)(c >> 32) <= BM_NONE) return;
+    if (!(l + o + 0x1p-21f * (fabsf(l) + fabsf(o)) >= reach) || (uint32_t)(c >> 32) <= BM_NONE) return false;
     const double v = value(c);
-    if (bm_key((float)v) >= at_least) {
-      const int p = atomicAdd(&count, 1);
-      if (p < BM_CAP) got[p] = bm_key(v), got_at[p] = bm_place(c);
-    }
+    if (bm_key((float)v) < at_least) return false;
+    const int p = atomicAdd(&count, 1);
+    if (p < BM_CAP) got[p] = bm_key(v), got_at[p] = bm_place(c);
+    return true;
   };
+  // further chunks only behind lists whose last candidate so far reaches the bound
+  const int last = (1 << chunk) - 1;
+  bool more = false;
 #pragma unroll
   for (int i = 0; i < HOLD; ++i)
-    if (NT * i < wide) gather(held[i]);
-  for (int j = tid + NT * HOLD; j < wide; j += NT) gather(at(j, 0));
-  // further chunks only behind lists whose last candidate so far reaches the bound
-  for (int rank = 1 << chunk; rank < M; rank += 1 << chunk) {
-    bool more = false;
-    for (int l = tid; l < L; l += NT) more |= bm_key((float)value(list[(int64_t)l * M + rank - 1])) >= at_least;
-    if (!__syncthreads_or(more)) break;
-    for (int j = tid; j < wide; j += NT) gather(at(j, rank));
+    if (NT * i < wide) more |= gather(held[i]) && ((tid + NT * i) & last) == last;
+  for (int j = tid + NT * HOLD; j < wide; j += NT) more |= gather(at(j, 0)) && (j & last) == last;
+  for (int rank = 1 << chunk; rank < M && __syncthreads_or(more); rank += 1 << chunk) {
+    more = false;
+    for (int j = tid; j < wide; j += NT) more |= gather(at(j, rank)) && (j & last) == last;
   }
   __syncthreads();
   int n = count;
@@ -700,6 +736,7 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
     const uint32_t key = tid < n ? bm_key((float)bm_value(k)) : 0u;
     keys[tid] = key;
     __syncthreads();
+    got[tid] = 0;
     if (tid < 64) {
       const uint32_t t = bm_bound<BM_CAP / 64, 0>(keys, max(want, 1));
       if (tid == 0) bound = t, count = 0;
@@ -720,11 +757,14 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
   if (n <= BM_CAP) {
     for (int i = tid >> 4; i < n; i += NT / 16) {  // 16 lanes a candidate
       const uint64_t k = got[i], at = got_at[i];
-      int r = 0;
-      for (int j = tid & 15; j < n; j += 16) {
-        const uint64_t c = got[j], ca = got_at[j];
-        r += (c > k) | ((c == k) & (ca < at));
+      int r = 0, same = 0;
+      for (int j = tid & 15; j < n; j += 64) {  // (zeros behind the n)
+        const uint64_t c0 = got[j], c1 = got[j + 16], c2 = got[j + 32], c3 = got[j + 48];
+        r += (c0 > k) + (c1 > k) + (c2 > k) + (c3 > k);
+        same += (c0 == k) + (c1 == k) + (c2 == k) + (c3 == k);
       }
+      if (bm_row_sum(same) > 1)
+        for (int j = tid & 15; j < n; j += 16) r += got[j] == k && got_at[j] < at;
       r = bm_row_sum(r);
       if (r < want && (tid & 15) == 0) put(first + r, (float)bm_value(k), bm_beam(at), bm_token(at));
     }
@@ -797,6 +837,23 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
   }
 }
 
+// The texts of a step into another state: one workgroup a row or hypothesis.  (The step's own
+// workgroups, one a prompt, leave most of the card idle.  Steps over 8192 logits with this launch and
+// with the copies in the step's: 1 x 32 texts of 1024 tokens of room 23.3 us and 27.5, 1 x 32 of 4096
+// 24.0 and 40.3, 64 x 8 of 4096 25.7 and 26.9; 1 x 4 of 4096 13.6 and 12.9, 64 x 8 of 500 19.7 and 17.6.)
+__global__ __launch_bounds__(256) void beam_texts_kernel(const BmStep P, int beams) {
+  const int64_t b = blockIdx.y, row = b * beams + blockIdx.x % beams;
+  const bool finished = (int)blockIdx.x >= beams;
+  const int from = P.plan[2 * b * beams + blockIdx.x], room = (int)P.room;
+  const int64_t* src = (finished && from < 0 ? P.in.finished_tokens : P.in.tokens) + (from < 0 ? row : b * beams + from) * P.room;
+  int n = finished && from < 0 ? P.in.finished_lengths[row] : P.in.lengths[b * beams];
+  n = min(max(n, 0), room);
+  int64_t* dst = (finished ? P.out.finished_tokens : P.out.tokens) + row * P.room;
+  // (a wave takes a run of whole 16-byte units)
+  const int part = ((n + 3) / 4 + 1) & ~1, at = min((int)(threadIdx.x >> 6) * part, n);
+  bm_copy(dst + at, src + at, min(part, n - at));
+}
+
 namespace {
 
 // 8 runs a lane where that still fills the card, else 2: 64 x 8 rows of 65536 fp16 logits with their
@@ -805,7 +862,9 @@ constexpr int BM_RUNS_MANY = 8, BM_RUNS_FEW = 2, BM_MANY = 512;
 int64_t bm_slice(int dtype, int runs) { return (int64_t)BM_THREADS * runs * (dtype == RWKV7MI_F32 ? 4 : 8); }
 int64_t bm_slices(int64_t V, int dtype, int runs) { return (V + bm_slice(dtype, runs) - 1) / bm_slice(dtype, runs); }
 
-int bm_run(BmArgs& a, const BmStep* step, int64_t prompts, int dtype, void* workspace, size_t bytes, hipStream_t stream,
+constexpr int64_t BM_TEXTS = 1 << 15;  // tokens of room a prompt from which a launch of their own copies the texts
+
+int bm_run(BmArgs& a, BmStep* step, int64_t prompts, int dtype, void* workspace, size_t bytes, hipStream_t stream,
            const std::string& w) {
   const int64_t rows = prompts * a.beams;
   // (a row starts up to 7 elements behind a boundary)
@@ -814,7 +873,7 @@ int bm_run(BmArgs& a, const BmStep* step, int64_t prompts, int dtype, void* work
   const int64_t width = a.V + (straight ? 0 : 7);
   const bool many = rows * bm_slices(width, dtype, BM_RUNS_MANY) >= BM_MANY;
   a.S = (int)bm_slices(width, dtype, many ? BM_RUNS_MANY : BM_RUNS_FEW);
-  const size_t need = (size_t)(rows * a.S) * (8u * (size_t)a.M + 8u);
+  const size_t need = (size_t)(rows * a.S) * (8u * (size_t)a.M + 8u) + 8u * (size_t)rows;
   if (!workspace || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))
     return fail(RWKV7MI_ESIZE, w + ": workspace missing, unaligned or smaller than rwkv7mi_beam_workspace_bytes");
   a.got = static_cast<uint64_t*>(workspace);
@@ -829,10 +888,17 @@ int bm_run(BmArgs& a, const BmStep* step, int64_t prompts, int dtype, void* work
     return check_launch("beam_slice_kernel");
   });
   if (rc) return rc;
-  if (step)
-    hipLaunchKernelGGL(beam_merge_kernel<true>, dim3((unsigned)prompts), dim3(BM_MERGE), 0, stream, a, *step);
-  else
+  if (!step) {
     hipLaunchKernelGGL(beam_merge_kernel<false>, dim3((unsigned)prompts), dim3(BM_MERGE), 0, stream, a, BmStep{});
+    return check_launch("beam_merge_kernel");
+  }
+  if (!step->in_place && a.beams * step->room >= BM_TEXTS) step->plan = reinterpret_cast<int*>(a.sums + rows * a.S);
+  hipLaunchKernelGGL(beam_merge_kernel<true>, dim3((unsigned)prompts), dim3(BM_MERGE), 0, stream, a, *step);
+  if (step->plan) {
+    if (const int e = check_launch("beam_merge_kernel")) return e;
+    hipLaunchKernelGGL(beam_texts_kernel, dim3(2u * (unsigned)a.beams, (unsigned)prompts), dim3(256), 0, stream, *step, a.beams);
+    return check_launch("beam_texts_kernel");
+  }
   return check_launch("beam_merge_kernel");
 }
 
@@ -856,7 +922,7 @@ using namespace rwkv7mi;
 
 extern "C" size_t rwkv7mi_beam_workspace_bytes(int64_t rows, int64_t V, int64_t candidates) {
   if (rows <= 0 || V <= 0 || candidates <= 0) return 0;
-  return (size_t)(rows * bm_slices(V + 7, RWKV7MI_F32, BM_RUNS_FEW)) * (8u * (size_t)candidates + 8u);
+  return (size_t)(rows * bm_slices(V + 7, RWKV7MI_F32, BM_RUNS_FEW)) * (8u * (size_t)candidates + 8u) + 8u * (size_t)rows;
 }
 
 extern "C" int rwkv7mi_beam_select(const void* x, int64_t prompts, int64_t beams, int64_t V, int64_t ldx, int dtype,

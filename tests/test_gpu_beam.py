@@ -269,6 +269,47 @@ def test_step_follows_the_definition(prompts, beams, n, room, ends, penalty, ear
     assert bool(state.done.all())
 
 
+@pytest.mark.parametrize("prompts,beams,room", [(3, 4, 700), (2, 16, 2049), (1, 32, 1024), (3, 40, 999), (2, 8, 4096)])
+def test_step_into_another_state_is_the_step_in_place(prompts, beams, room):
+    """Long texts and hypotheses of all lengths, prompts that are done and full ones: the same state in
+    place and into another one, whichever way its texts are copied, and the rest of the rows as it was."""
+    import rwkv7mi as mi
+
+    rng = np.random.default_rng(beams * room)
+    n, ends = 400, [3, 5]
+    length = rng.integers(room // 2, room, prompts)
+    if prompts > 1:
+        length[1] = room
+    held = rng.integers(0, room + 1, (prompts, beams))
+    has = rng.random((prompts, beams)) < 0.7
+    arrays = dict(tokens=rng.integers(0, n, (prompts, beams, room)), lengths=np.repeat(length, beams).astype(np.int32),
+                  scores=(rng.standard_normal((prompts, beams)) - 9).astype(np.float32),
+                  prompt_lengths=(length // 2).astype(np.int32), finished_tokens=rng.integers(0, n, (prompts, beams, room)),
+                  finished_lengths=held.astype(np.int32),
+                  finished_scores=np.where(has, rng.standard_normal((prompts, beams)) * 0.02 - 0.05, -np.inf).astype(np.float32),
+                  done=np.arange(prompts) == 2)
+    x = rng.standard_normal((prompts * beams, n)) * 2
+    x[:, ends] += 4.0 * (rng.random((prompts * beams, 1)) < 0.3)
+    x = torch.from_numpy(x).half().cuda()
+    ends = ends[: 2 if beams <= 40 else 1]
+    here, there = _state(mi, arrays), _state(mi, arrays)
+    other = _state(mi, {k: np.full_like(v, 7) if v.dtype != bool else v for k, v in arrays.items()})
+    a = mi.beam_step(x, here, eos_token_id=ends)
+    b = mi.beam_step(x, there, eos_token_id=ends, out=other)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for k in KEYS:
+        assert np.array_equal(getattr(there, k).cpu().numpy(), arrays[k]), k
+        got, want = getattr(other, k).cpu().numpy(), getattr(here, k).cpu().numpy()
+        if k.endswith("tokens"):
+            lens = (here.lengths.view(prompts, beams) if k == "tokens" else here.finished_lengths).cpu().numpy()
+            want = np.where(np.arange(room) < lens[..., None], want, 7)
+        assert np.array_equal(got, want), k
+    val, tok, row = (t.cpu().numpy() for t in mi.beam_select(x, there.scores, (1 + len(ends)) * beams))
+    nxt, rows, want = ref.step((val, tok, row - beams * np.arange(prompts)[:, None]), arrays, tuple(ends), 1.0, False)
+    assert np.array_equal(a[0].cpu().numpy(), nxt) and np.array_equal(a[1].cpu().numpy(), rows)
+    _same(here, want)
+
+
 def test_step_one_end_token_as_a_number_and_logits_per_prompt():
     import rwkv7mi as mi
 
