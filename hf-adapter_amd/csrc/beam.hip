@@ -704,8 +704,8 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
     if (tid == 0) bound = t;
   }
   __syncthreads();
-  const uint32_t at_least = bound;
-  const float reach = bm_value(at_least);
+  uint32_t at_least = bound;
+  float reach = bm_value(at_least);
   const auto gather = [&](uint64_t c) {  // whether it reaches the bound
     const float l = bm_value((uint32_t)(c >> 32)), o = offset[c >> 23 & 0x7f];
     // (fp32, less than four roundings off; false for -inf and what is not there)
@@ -716,19 +716,36 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
     if (p < BM_CAP) got[p] = bm_key(v), got_at[p] = bm_place(c);
     return true;
   };
-  // further chunks only behind lists whose last candidate so far reaches the bound
-  const int last = (1 << chunk) - 1;
-  bool more = false;
+  int n;
+  for (;;) {
+    // further chunks only behind lists whose last candidate so far reaches the bound
+    const int last = (1 << chunk) - 1;
+    bool more = false;
 #pragma unroll
-  for (int i = 0; i < HOLD; ++i)
-    if (NT * i < wide) more |= gather(held[i]) && ((tid + NT * i) & last) == last;
-  for (int j = tid + NT * HOLD; j < wide; j += NT) more |= gather(at(j, 0)) && (j & last) == last;
-  for (int rank = 1 << chunk; rank < M && __syncthreads_or(more); rank += 1 << chunk) {
-    more = false;
-    for (int j = tid; j < wide; j += NT) more |= gather(at(j, rank)) && (j & last) == last;
+    for (int i = 0; i < HOLD; ++i)
+      if (NT * i < wide) more |= gather(held[i]) && ((tid + NT * i) & last) == last;
+    for (int j = tid + NT * HOLD; j < wide; j += NT) more |= gather(at(j, 0)) && (j & last) == last;
+    for (int rank = 1 << chunk; rank < M && __syncthreads_or(more); rank += 1 << chunk) {
+      more = false;
+      for (int j = tid; j < wide; j += NT) more |= gather(at(j, rank)) && (j & last) == last;
+    }
+    __syncthreads();
+    n = count;
+    if (n <= BM_CAP) break;
+    // too many, as where the best beams have most of the best candidates: those gathered, whichever they
+    // are, give a better bound (unless they are equal: then they are drawn one by one)
+    keys[tid] = bm_key((float)bm_value(got[tid]));
+    __syncthreads();
+    if (tid < 64) {
+      const uint32_t t = bm_bound<BM_CAP / 64, 0>(keys, max(want, 1));
+      if (tid == 0) bound = t, count = 0;
+    }
+    got[tid] = 0;
+    __syncthreads();
+    if (bound <= at_least) break;
+    at_least = bound;
+    reach = bm_value(at_least);
   }
-  __syncthreads();
-  int n = count;
   // (ranking by counting reads n entries for each: many are cut down by a bound of their own first)
   if (n > BM_RANKED && n <= BM_CAP) {
     uint64_t k = 0, p = 0;
@@ -856,11 +873,17 @@ __global__ __launch_bounds__(256) void beam_texts_kernel(const BmStep P, int bea
 
 namespace {
 
-// 8 runs a lane where that still fills the card, else 2: 64 x 8 rows of 65536 fp16 logits with their
-// selection take 25.7 us with 8 and 30.3 with 2, 7 x 5 rows of 50277 bf16 15.8 and 13.5
-constexpr int BM_RUNS_MANY = 8, BM_RUNS_FEW = 2, BM_MANY = 512;
 int64_t bm_slice(int dtype, int runs) { return (int64_t)BM_THREADS * runs * (dtype == RWKV7MI_F32 ? 4 : 8); }
 int64_t bm_slices(int64_t V, int dtype, int runs) { return (V + bm_slice(dtype, runs) - 1) / bm_slice(dtype, runs); }
+
+// Runs of a lane: 8, whose slices share the bound and the ranking among the most logits, where there are
+// logits for 512 such workgroups, 4 down to 128 and 2 below, which fill the card sooner.  us with 2, 4, 8
+// runs, rows of 65536 fp16 logits: 16 rows 8.8, 9.3, 10.0; 32 10.0, 9.6, 10.0; 128 14.9, 13.3, 13.0; 512
+// 35.0, 29.7, 24.0.
+int bm_runs(int64_t rows, int64_t V, int dtype, int64_t M) {
+  const int64_t logits = rows * V, unit = bm_slice(dtype, 8);
+  return logits >= 512 * unit ? 8 : logits >= 128 * unit ? 4 : 2;
+}
 
 constexpr int64_t BM_TEXTS = 1 << 15;  // tokens of room a prompt from which a launch of their own copies the texts
 
@@ -871,8 +894,8 @@ int bm_run(BmArgs& a, BmStep* step, int64_t prompts, int dtype, void* workspace,
   const bool straight = !(reinterpret_cast<uintptr_t>(a.x) & 15) &&
                         (rows == 1 || a.ldx * (dtype == RWKV7MI_F32 ? 4 : 2) % 16 == 0);
   const int64_t width = a.V + (straight ? 0 : 7);
-  const bool many = rows * bm_slices(width, dtype, BM_RUNS_MANY) >= BM_MANY;
-  a.S = (int)bm_slices(width, dtype, many ? BM_RUNS_MANY : BM_RUNS_FEW);
+  const int runs = bm_runs(rows, a.V, dtype, a.M);
+  a.S = (int)bm_slices(width, dtype, runs);
   const size_t need = (size_t)(rows * a.S) * (8u * (size_t)a.M + 8u) + 8u * (size_t)rows;
   if (!workspace || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))
     return fail(RWKV7MI_ESIZE, w + ": workspace missing, unaligned or smaller than rwkv7mi_beam_workspace_bytes");
@@ -881,10 +904,12 @@ int bm_run(BmArgs& a, BmStep* step, int64_t prompts, int dtype, void* workspace,
   const int rc = dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const dim3 grid((unsigned)a.S, (unsigned)a.beams, (unsigned)prompts);
-    if (many)
-      hipLaunchKernelGGL((beam_slice_kernel<T, BM_RUNS_MANY>), grid, dim3(BM_THREADS), 0, stream, a);
+    if (runs == 8)
+      hipLaunchKernelGGL((beam_slice_kernel<T, 8>), grid, dim3(BM_THREADS), 0, stream, a);
+    else if (runs == 4)
+      hipLaunchKernelGGL((beam_slice_kernel<T, 4>), grid, dim3(BM_THREADS), 0, stream, a);
     else
-      hipLaunchKernelGGL((beam_slice_kernel<T, BM_RUNS_FEW>), grid, dim3(BM_THREADS), 0, stream, a);
+      hipLaunchKernelGGL((beam_slice_kernel<T, 2>), grid, dim3(BM_THREADS), 0, stream, a);
     return check_launch("beam_slice_kernel");
   });
   if (rc) return rc;
@@ -922,7 +947,7 @@ using namespace rwkv7mi;
 
 extern "C" size_t rwkv7mi_beam_workspace_bytes(int64_t rows, int64_t V, int64_t candidates) {
   if (rows <= 0 || V <= 0 || candidates <= 0) return 0;
-  return (size_t)(rows * bm_slices(V + 7, RWKV7MI_F32, BM_RUNS_FEW)) * (8u * (size_t)candidates + 8u) + 8u * (size_t)rows;
+  return (size_t)(rows * bm_slices(V + 7, RWKV7MI_F32, 2)) * (8u * (size_t)candidates + 8u) + 8u * (size_t)rows;
 }
 
 extern "C" int rwkv7mi_beam_select(const void* x, int64_t prompts, int64_t beams, int64_t V, int64_t ldx, int dtype,

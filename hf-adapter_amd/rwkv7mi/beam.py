@@ -71,7 +71,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | No
     m = 2 * beams if candidates is None else int(candidates)
     _lib.require_same_device(logits, scores, *(out or ()), workspace, name=name)
     if out is None:
-        out = (scores.new_empty((prompts, m)), *(scores.new_empty((prompts, m), dtype=torch.int64) for _ in range(2)))
+        out = (scores.new_empty((prompts, m)), scores.new_empty((prompts, m), dtype=torch.int64),
+               scores.new_empty((prompts, m), dtype=torch.int64))
     else:
         out = tuple(out)
         for t, want in zip(out, (torch.float32, torch.int64, torch.int64)):
@@ -112,18 +113,20 @@ class BeamState:
                  ("finished_tokens", finished_tokens, torch.int64, shape),
                  ("finished_lengths", finished_lengths, torch.int32, (p, k)),
                  ("finished_scores", finished_scores, torch.float32, (p, k)), ("done", done, torch.bool, (p,)))
-        put = object.__setattr__
-        ends = []
+        put, where = object.__setattr__, tokens.get_device()
+        ends, at = [], []
         for key, t, dtype, want in given:
-            if t.dtype is not dtype or t.shape != want or not t.is_contiguous() or t.device != tokens.device:
+            if t.dtype is not dtype or t.shape != want or not t.is_contiguous() or t.get_device() != where:
                 raise ValueError(f"{name}: {key} must be a contiguous {dtype} tensor {list(want)} on {tokens.device}")
             put(self, key, t)
-            at = t.data_ptr()
-            ends.append((at, at + t.numel() * t.element_size()))
-        put(self, "_pointers", (ctypes.c_void_p * 8)(*[e[0] for e in ends]))
-        put(self, "_ends", sorted(e for e in ends if e[1] > e[0]))
-        if any(b[0] < a[1] for a, b in zip(self._ends, self._ends[1:])):
+            p = t.data_ptr()
+            at.append(p)
+            ends.append((p, p + t.nbytes))
+        ends.sort()
+        if any([b[0] < a[1] for a, b in zip(ends, ends[1:])]):
             raise ValueError(f"{name}: tensors overlap")
+        put(self, "_pointers", (ctypes.c_void_p * 8)(*at))
+        put(self, "_ends", ends)
 
     def __setattr__(self, key, value):
         raise AttributeError(f"BeamState.{key} is not replaced (write into the tensor)")
@@ -215,7 +218,7 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, leng
         if to.tokens.shape != state.tokens.shape:
             raise ValueError(f"{name}: out has {list(to.tokens.shape)} tokens, state {list(state.tokens.shape)}")
         every = sorted(state._ends + to._ends)
-        if any(b[0] < a[1] for a, b in zip(every, every[1:])):
+        if any([b[0] < a[1] for a, b in zip(every, every[1:])]):
             raise ValueError(f"{name}: out shares memory with state")
     total = prompts * beams
     for t in (next_tokens, rows):

@@ -5,6 +5,7 @@ and fresh slots.  Byte moves, bit-exact, any dtype."""
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -16,14 +17,18 @@ MAX_TRADING = 2048  # rows that may trade places in place
 
 
 def _family(t: torch.Tensor, dim: int, name: str):
-    """``(outer stride, row stride, row bytes, outer count, rows)`` of ``t`` in bytes, the
-    dimensions before ``dim`` as one and those behind it dense; None where they are not."""
-    es, shape, stride = t.element_size(), t.shape, t.stride()
-    n = len(shape)
-    if n <= dim:
-        raise ValueError(f"{name}: a tensor of {n} dimensions has no rows along dimension {dim}")
-    dense = 1
-    for i in range(n - 1, dim, -1):
+    """``(address, outer stride, row stride, row bytes, outer count, rows, end)`` of ``t`` in
+    bytes, the dimensions before ``dim`` as one and those behind it dense; None where they are
+    not."""
+    es, shape, at = t.element_size(), t.shape, t.data_ptr()
+    if len(shape) <= dim:
+        raise ValueError(f"{name}: a tensor of {len(shape)} dimensions has no rows along dimension {dim}")
+    rows = shape[dim]
+    if t.is_contiguous():
+        size = math.prod(shape[dim + 1:]) * es
+        return at, rows * size, size, size, math.prod(shape[:dim]), rows, at + t.numel() * es
+    stride, dense = t.stride(), 1
+    for i in range(len(shape) - 1, dim, -1):
         if shape[i] != 1 and stride[i] != dense:
             return None
         dense *= shape[i]
@@ -36,19 +41,26 @@ def _family(t: torch.Tensor, dim: int, name: str):
         if outer == 1:
             step = stride[i]
         outer *= shape[i]
-    rows = shape[dim]
-    return step * es, (stride[dim] if rows > 1 else dense) * es, dense * es, outer, rows
+    end = at + (1 + sum((k - 1) * s for k, s in zip(shape, stride))) * es if t.numel() else at
+    return at, step * es, (stride[dim] if rows > 1 else dense) * es, dense * es, outer, rows, end
 
 
 def _apart(f) -> bool:
     """Whether the rows of a family lie apart (they are written)."""
-    step, row, size, outer, rows = f
-    spans = sorted((abs(s), k) for s, k in ((row, rows), (step, outer)) if k > 1)
+    _, step, row, size, outer, rows, _ = f
+    spans = ((row, rows), (step, outer)) if row <= step else ((step, outer), (row, rows))
     for s, k in spans:
-        if s < size:
-            return False
-        size = s * k
+        if k > 1:
+            if s < size:
+                return False
+            size = s * k
     return True
+
+
+def _lap(families) -> bool:
+    """Whether the address ranges of any two meet."""
+    ends = sorted([(f[0], f[6]) for f in families if f[6] > f[0]])
+    return any([b[0] < a[1] for a, b in zip(ends, ends[1:])])
 
 
 def _index(index, name: str):
@@ -77,10 +89,11 @@ def _launch(families, src_rows, dst_rows, n, src, dst, disjoint, where, name):
 
 
 def _same_rows(families, name):
-    rows = {f[4] for f in families}
-    if len(rows) != 1:
-        raise ValueError(f"{name}: tensors of {sorted(rows)} rows")
-    return rows.pop()
+    rows = families[0][5]
+    for f in families:
+        if f[5] != rows:
+            raise ValueError(f"{name}: tensors of {sorted({f[5] for f in families})} rows")
+    return rows
 
 
 def _on_gpu(tensors, index, name):
@@ -130,25 +143,14 @@ def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tenso
         dst = [_family(o, dim, name) for o in out]
         if any(f is None or not _apart(f) for f in dst):
             raise ValueError(f"{name}: the rows of an output are dense and apart")
-        if any(_lib.overlap(o, t) for o in out for t in tensors) or _lap(out):
+        if _lap(dst) or any(_lap((f, g)) for f in src for g in dst):
             raise ValueError(f"{name}: outputs overlap")
     flat = []
-    for t, o, f, g in zip(tensors, out, src, dst):
-        flat += (t.data_ptr(), o.data_ptr(), f[0], f[1], g[0], g[1], f[2], f[3])
+    for f, g in zip(src, dst):
+        flat += (f[0], g[0], f[1], f[2], g[1], g[2], f[3], f[4])
     if n:
         _launch(flat, rows, n, n, idx, None, True, tensors[0], name)
     return out
-
-
-def _lap(tensors) -> bool:
-    """Whether the address ranges of any two meet."""
-    ends = []
-    for t in tensors:
-        if t.numel():
-            a = t.data_ptr()
-            ends.append((a, a + (1 + sum((s - 1) * k for s, k in zip(t.shape, t.stride()))) * t.element_size()))
-    ends.sort()
-    return any(b[0] < a[1] for a, b in zip(ends, ends[1:]))
 
 
 def move_rows_(tensors, sources, destinations=None, *, dim: int = 0) -> None:
@@ -169,10 +171,11 @@ def move_rows_(tensors, sources, destinations=None, *, dim: int = 0) -> None:
     if dim < 0:
         raise ValueError(f"{name}: dim counts from the front")
     fams = [_family(t, dim, name) for t in tensors]
-    if any(f is None or not _apart(f) for f in fams):
-        raise ValueError(f"{name}: the rows of a tensor are dense and apart")
+    for f in fams:
+        if f is None or not _apart(f):
+            raise ValueError(f"{name}: the rows of a tensor are dense and apart")
     rows = _same_rows(fams, name)
-    if len(tensors) > 1 and _lap(tensors):
+    if len(fams) > 1 and _lap(fams):
         raise ValueError(f"{name}: tensors overlap or interleave")
     n = len(src) if type(src) is list else src.shape[0]
     if type(src) is list and not all(-1 <= i < rows for i in src):
@@ -195,9 +198,8 @@ def move_rows_(tensors, sources, destinations=None, *, dim: int = 0) -> None:
     if not disjoint and n > MAX_TRADING:
         raise ValueError(f"{name}: at most {MAX_TRADING} rows trade places in one call")
     flat = []
-    for t, f in zip(tensors, fams):
-        p = t.data_ptr()
-        flat += (p, p, f[0], f[1], f[0], f[1], f[2], f[3])
+    for f in fams:
+        flat += (f[0], f[0], f[1], f[2], f[1], f[2], f[3], f[4])
     if n:
         _launch(flat, rows, rows, n, src, dst, disjoint, tensors[0], name)
 

@@ -127,6 +127,20 @@ def test_select_sorted_and_shifted_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+def test_select_where_few_beams_hold_the_best(dtype):
+    """All that is wanted comes from one or two of many beams, more of it than a workgroup gathers."""
+    import rwkv7mi as mi
+
+    rng = np.random.default_rng(9)
+    for beams, n, good in ((64, 65536, 2), (64, 30001, 1), (128, 9000, 9), (40, 65536, 3)):
+        x, s = _case(rng, 2, beams, n, dtype, 0.5 if good == 9 else 3.0)
+        s[:] = s - 500.0
+        s[:, rng.choice(beams, good, replace=False)] = -3.0
+        for m in (128, 60):
+            _check(mi.beam_select(x.cuda(), s.cuda(), m), x, s, m)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 def test_select_masks(dtype):
     """Masks that leave a few tokens, one, or none; the type's lowest value; beams that have not begun."""
     import rwkv7mi as mi
