@@ -72,20 +72,28 @@ def _index(index, name: str):
     return [int(i) for i in index]
 
 
-def _launch(families, src_rows, dst_rows, n, src, dst, disjoint, where, name):
+def _launch(families, src_rows, dst_rows, n, src, dst, disjoint, where):
     """``families``: 8 numbers a tensor, as the library's ``rwkv7mi_rows``."""
-    if type(src) is list and len(src) > MAX_LISTED:
+    src_at = dst_at = src_list = dst_list = None
+    if type(src) is not list:
+        src_at = src.data_ptr()
+    elif n <= MAX_LISTED:
+        src_list = (ctypes.c_int64 * n)(*src)
+    else:
         src = torch.tensor(src, dtype=torch.int64).to(where.device)
-    if type(dst) is list and len(dst) > MAX_LISTED:
-        dst = torch.tensor(dst, dtype=torch.int64).to(where.device)
-    on_host = lambda v: (ctypes.c_int64 * n)(*v) if type(v) is list else None  # noqa: E731
-    on_device = lambda v: v.data_ptr() if isinstance(v, torch.Tensor) else None  # noqa: E731
+        src_at = src.data_ptr()
+    if dst is not None:
+        if n <= MAX_LISTED:
+            dst_list = (ctypes.c_int64 * n)(*dst)
+        else:
+            dst = torch.tensor(dst, dtype=torch.int64).to(where.device)
+            dst_at = dst.data_ptr()
     with _lib.on_device(where):
         stream = _lib.stream_of(where)
         for i in range(0, len(families), 8 * MAX_TENSORS):
             part = families[i:i + 8 * MAX_TENSORS]
             _lib.call("rwkv7mi_rows_move", len(part) // 8, (ctypes.c_int64 * len(part))(*part), src_rows, dst_rows, n,
-                      on_device(src), on_device(dst), on_host(src), on_host(dst), 1 if disjoint else 0, stream)
+                      src_at, dst_at, src_list, dst_list, 1 if disjoint else 0, stream)
 
 
 def _same_rows(families, name):
@@ -128,28 +136,32 @@ def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tenso
     rows = _same_rows(src, name)
     if type(idx) is list and not all(-1 <= i < rows for i in idx):
         raise IndexError(f"{name}: indices outside -1..{rows - 1}")
-    shapes = [(*t.shape[:dim], n, *t.shape[dim + 1:]) for t in tensors]
+    flat = []
     if out is None:
-        out = [t.new_empty(s) for t, s in zip(tensors, shapes)]
-        dst = [_family(o, dim, name) for o in out]
+        out = []
+        for t, f in zip(tensors, src):
+            shape, size = t.shape, f[3]
+            o = t.new_empty((*shape[:dim], n, *shape[dim + 1:]))
+            out.append(o)
+            flat += (f[0], o.data_ptr(), f[1], f[2], n * size, size, size, f[4])
     else:
         out = list(out)
         if len(out) != len(tensors):
             raise ValueError(f"{name}: {len(out)} outputs for {len(tensors)} tensors")
-        for o, t, s in zip(out, tensors, shapes):
-            if tuple(o.shape) != s or o.dtype != t.dtype:
-                raise ValueError(f"{name}: an output is {tuple(o.shape)} {o.dtype}, not {s} {t.dtype}")
+        for o, t in zip(out, tensors):
+            want = (*t.shape[:dim], n, *t.shape[dim + 1:])
+            if tuple(o.shape) != want or o.dtype != t.dtype:
+                raise ValueError(f"{name}: an output is {tuple(o.shape)} {o.dtype}, not {want} {t.dtype}")
         _on_gpu([tensors[0], *out], None, name)
         dst = [_family(o, dim, name) for o in out]
         if any(f is None or not _apart(f) for f in dst):
             raise ValueError(f"{name}: the rows of an output are dense and apart")
         if _lap(dst) or any(_lap((f, g)) for f in src for g in dst):
             raise ValueError(f"{name}: outputs overlap")
-    flat = []
-    for f, g in zip(src, dst):
-        flat += (f[0], g[0], f[1], f[2], g[1], g[2], f[3], f[4])
+        for f, g in zip(src, dst):
+            flat += (f[0], g[0], f[1], f[2], g[1], g[2], f[3], f[4])
     if n:
-        _launch(flat, rows, n, n, idx, None, True, tensors[0], name)
+        _launch(flat, rows, n, n, idx, None, True, tensors[0])
     return out
 
 
@@ -201,7 +213,7 @@ def move_rows_(tensors, sources, destinations=None, *, dim: int = 0) -> None:
     for f in fams:
         flat += (f[0], f[0], f[1], f[2], f[1], f[2], f[3], f[4])
     if n:
-        _launch(flat, rows, rows, n, src, dst, disjoint, tensors[0], name)
+        _launch(flat, rows, rows, n, src, dst, disjoint, tensors[0])
 
 
 __all__ = ["select_rows", "move_rows_"]
