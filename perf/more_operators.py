@@ -35,9 +35,8 @@ MODELS = {"0.1B": (12, 768), "1.5B": (24, 2048), "2.9B": (32, 2560), "7.2B": (32
 
 def _own():
     """This package's entry points (imported only where they are measured)."""
-    path = str(Path.cwd() / "hf-adapter_amd")
-    if path not in sys.path:
-        sys.path.insert(0, path)
+    if "rwkv7mi" not in sys.modules:
+        sys.path.insert(0, str(Path.cwd() / "hf-adapter_amd"))
     import rwkv7mi
 
     return rwkv7mi
