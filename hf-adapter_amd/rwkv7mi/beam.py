@@ -88,6 +88,19 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | No
     return out
 
 
+_Pointers = ctypes.c_void_p * 8
+
+
+def _meet(ranges) -> bool:
+    """Whether two of the sorted address ranges meet."""
+    last = 0
+    for start, end in ranges:
+        if start < last:
+            return True
+        last = end
+    return False
+
+
 class BeamState:
     """The state of a beam search over ``prompts`` prompts with ``beams`` beams each, on one
     GPU: contiguous tensors, checked once and not replaced afterwards.
@@ -123,9 +136,9 @@ class BeamState:
             at.append(p)
             ends.append((p, p + t.nbytes))
         ends.sort()
-        if any([b[0] < a[1] for a, b in zip(ends, ends[1:])]):
+        if _meet(ends):
             raise ValueError(f"{name}: tensors overlap")
-        put(self, "_pointers", (ctypes.c_void_p * 8)(*at))
+        put(self, "_pointers", _Pointers(*at))
         put(self, "_ends", ends)
 
     def __setattr__(self, key, value):
@@ -217,8 +230,7 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, leng
     if to is not state:
         if to.tokens.shape != state.tokens.shape:
             raise ValueError(f"{name}: out has {list(to.tokens.shape)} tokens, state {list(state.tokens.shape)}")
-        every = sorted(state._ends + to._ends)
-        if any([b[0] < a[1] for a, b in zip(every, every[1:])]):
+        if _meet(sorted(state._ends + to._ends)):
             raise ValueError(f"{name}: out shares memory with state")
     total = prompts * beams
     for t in (next_tokens, rows):
