@@ -57,6 +57,12 @@ SCHEMAS = {
         "process_logits(Tensor logits, Tensor? history, Tensor? lengths, float repetition_penalty,"
         " float presence_penalty, float frequency_penalty, float penalty_decay, Tensor? bias, Tensor? allowed)"
         " -> (Tensor, Tensor)",
+    "beam_select":
+        "beam_select(Tensor logits, Tensor scores, int candidates, bool normalized) -> (Tensor, Tensor, Tensor)",
+    "select_rows":
+        "select_rows(Tensor[] tensors, Tensor indices, int dim) -> Tensor[]",
+    "move_rows_":
+        "move_rows_(Tensor(a!)[] tensors, Tensor sources, int dim) -> ()",
     "w4_groupwise_linear":
         "w4_groupwise_linear(Tensor x, Tensor q, Tensor scales, int out_features, int in_features, int group_size)"
         " -> Tensor",
@@ -83,7 +89,7 @@ SCHEMAS = {
 
 def _cuda_impls():
     from . import fused_decode_norm_mix as fdm
-    from . import fused_lora, fused_output, fused_prefill, fused_time_mix, native_quant_mm8, native_quant_mxfp4, sampling, sm70_quant
+    from . import beam, fused_lora, fused_output, fused_prefill, fused_time_mix, native_quant_mm8, native_quant_mxfp4, sampling, sm70_quant, state_rows
     from .fused_recurrent_update import fused_recurrent_output_prepare_raw, fused_recurrent_update
     from .self_chunk_rwkv7 import _run_chunk
     from .fused_recurrent_update import _as_bthn, _check_state
@@ -146,6 +152,15 @@ def _cuda_impls():
                                        presence_penalty=pres, frequency_penalty=freq, penalty_decay=decay, bias=bias,
                                        allowed=allowed, next_tokens=nxt), nxt
 
+    def beams(logits, scores, candidates, normalized):
+        return beam.beam_select(logits, scores, candidates, normalized=normalized)
+
+    def rows(tensors, indices, dim):
+        return state_rows.select_rows(tensors, indices, dim=dim)
+
+    def rows_(tensors, sources, dim):
+        state_rows.move_rows_(tensors, sources, dim=dim)
+
     def w4g(x, q, scales, out_features, in_features, group_size):
         return sm70_quant.w4_groupwise_linear(x, q, scales, out_features, in_features, group_size=group_size)
 
@@ -177,7 +192,8 @@ def _cuda_impls():
         "fused_recurrent_output_prepare_raw": prep_raw, "fused_recurrent_output_prepare_raw_": prep_raw_,
         "chunk_scan": chunk, "chunk_scan_": chunk_, "mm8_matmul": mm8, "mm8_matmul_out": mm8_out,
         "quantize_mm8": quant8, "quantize_mxfp4": quant4, "dequantize_mxfp4": dequant4, "mxfp4_linear": linear4,
-        "process_logits": logits_step, "w4_groupwise_linear": w4g, "attn_norm_mix6_": mix6_,
+        "process_logits": logits_step, "beam_select": beams, "select_rows": rows, "move_rows_": rows_,
+        "w4_groupwise_linear": w4g, "attn_norm_mix6_": mix6_,
         "ffn_add_norm_mix_": ffn_mix_, "wavg_lora": wavg, "state_prep": sprep, "output_prepare": oprep,
         "seq_shift_mix": shift,
     }
@@ -218,6 +234,13 @@ def _fake_impls():
     def logits_step(logits, history, lengths, rep, pres, freq, decay, bias, allowed):
         return logits.new_empty(logits.shape), logits.new_empty(logits.shape[0], dtype=torch.long)
 
+    def beams(logits, scores, candidates, normalized):
+        shape = (scores.shape[0], candidates)
+        return scores.new_empty(shape), *(scores.new_empty(shape, dtype=torch.long) for _ in range(2))
+
+    def rows(tensors, indices, dim):
+        return [t.new_empty((*t.shape[:dim], indices.shape[0], *t.shape[dim + 1:])) for t in tensors]
+
     def w4g(x, q, scales, out_features, in_features, group_size):
         return x.new_empty((*x.shape[:-1], int(out_features)))
 
@@ -240,7 +263,8 @@ def _fake_impls():
         "fused_recurrent_output_prepare_raw": prep_raw, "fused_recurrent_output_prepare_raw_": none,
         "chunk_scan": chunk, "chunk_scan_": none, "mm8_matmul": mm8, "mm8_matmul_out": none,
         "quantize_mm8": quant8, "quantize_mxfp4": quant4, "dequantize_mxfp4": dequant4, "mxfp4_linear": linear4,
-        "process_logits": logits_step, "w4_groupwise_linear": w4g, "attn_norm_mix6_": none, "ffn_add_norm_mix_": none,
+        "process_logits": logits_step, "beam_select": beams, "select_rows": rows, "move_rows_": none,
+        "w4_groupwise_linear": w4g, "attn_norm_mix6_": none, "ffn_add_norm_mix_": none,
         "wavg_lora": wavg, "state_prep": sprep, "output_prepare": oprep, "seq_shift_mix": shift,
     }
 

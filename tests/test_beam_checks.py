@@ -218,3 +218,16 @@ def test_the_plain_step():
     # (of two empty places the first stays empty)
     assert new["finished_tokens"][0, 1].tolist() == [7, 1, 0] and new["finished_lengths"][0].tolist() == [0, 2]
     assert np.isclose(new["finished_scores"][0, 1], np.log(0.3) - 1.0) and not new["done"][0]
+
+
+def test_custom_ops_give_shapes():
+    import rwkv7mi  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        out = torch.ops.rwkv7mi.beam_select(torch.empty(6, 50), torch.empty(2, 3), 7, False)
+        assert [t.shape for t in out] == [(2, 7)] * 3 and out[1].dtype is torch.int64
+        rows = torch.ops.rwkv7mi.select_rows([torch.empty(2, 5, 3), torch.empty(1, 5)], torch.zeros(4, dtype=torch.long), 1)
+        assert [t.shape for t in rows] == [(2, 4, 3), (1, 4)]
+    with pytest.raises(RuntimeError, match="GPU only"):
+        torch.ops.rwkv7mi.move_rows_([torch.zeros(3, 2)], torch.zeros(3, dtype=torch.long), 0)

@@ -158,3 +158,15 @@ def test_move_rows_on_a_stream_and_captured():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(ts, want))
         assert all(torch.equal(a, b[:, [3, 3, 0]]) for a, b in zip(new, want))
+
+
+def test_custom_ops():
+    import rwkv7mi as mi
+
+    ts = _tensors(5)
+    idx = torch.tensor([4, 0, 0, 1, 2], device="cuda")
+    new = torch.ops.rwkv7mi.select_rows(ts, idx, 1)
+    torch.ops.rwkv7mi.move_rows_(ts, idx, 1)
+    assert all(torch.equal(a, b) for a, b in zip(new, ts))
+    x, s = torch.randn(6, 300, device="cuda"), torch.zeros(2, 3, device="cuda")
+    assert all(torch.equal(a, b) for a, b in zip(torch.ops.rwkv7mi.beam_select(x, s, 5, False), mi.beam_select(x, s, 5)))
