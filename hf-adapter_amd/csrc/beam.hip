@@ -33,6 +33,7 @@ namespace {
 constexpr int BM_THREADS = 256;
 constexpr int BM_MERGE = 1024;    // lanes that join a prompt's slices
 constexpr int BM_CAP = 1024;      // candidates that a workgroup gathers, whole 64s
+constexpr int BM_WAVE_RUNS = 128; // runs of them that a wave gathers
 constexpr int BM_RANKED = 320;    // of them ranked without a second bound
 constexpr int BM_MOST = 128;      // candidates of a prompt
 constexpr int BM_ENDS = 8;        // end tokens
@@ -106,6 +107,12 @@ __device__ __forceinline__ float bm_wave_max(float v) {
   v = fmaxf(v, dpp_row_ror<2>(v));
   v = fmaxf(v, dpp_row_ror<1>(v));
   return fmaxf(fmaxf(lane_f(v, 0), lane_f(v, 16)), fmaxf(lane_f(v, 32), lane_f(v, 48)));
+}
+
+// what the lanes of a wave wrote to LDS is there for the others
+__device__ __forceinline__ void bm_wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 // the maximum and the total over the 16 lanes of a row, in each of them
@@ -220,6 +227,8 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
   __shared__ uint32_t top[BM_THREADS];
   __shared__ uint32_t bound;
   __shared__ float wave_top[WAVES], wave_sums[WAVES];
+  __shared__ u32x4 run[WAVES][BM_WAVE_RUNS];
+  __shared__ uint16_t run_at[WAVES][BM_WAVE_RUNS];
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int beam = (int)blockIdx.y;
@@ -303,26 +312,30 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
   const float reach = bm_value(bound);
   const int64_t slice = row * A.S + blockIdx.x;
   uint64_t* out = A.got + slice * A.M;
-  // the runs that hold one that reaches: most lanes none, few lanes two
-  uint32_t runs = 0;
+  // the runs that hold one that reaches go to LDS as they are, and the wave's lanes take their elements:
+  // no lane waits for what another one found
+  int held = 0;
 #pragma unroll
-  for (int u = 0; u < RUNS; ++u) runs |= (run_best[u] >= reach ? 1u : 0u) << u;
-  while (runs) {
-    const int u = __builtin_ctz(runs);
-    runs &= runs - 1;
-    uint32_t w[4] = {d[0][0], d[0][1], d[0][2], d[0][3]}, hits = 0;
-#pragma unroll
-    for (int q = 1; q < RUNS; ++q)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = q == u ? d[q][j] : w[j];
-#pragma unroll
-    for (int e = 0; e < E; ++e) hits |= (bm_element<T>(w, e) >= reach ? 1u : 0u) << e;
-    for (; hits; hits &= hits - 1) {
-      const int p = atomicAdd(&count, 1), e = __builtin_ctz(hits), q = sizeof(T) == 4 ? e : e >> 1;
-      uint32_t one[4] = {q & 2 ? (q & 1 ? w[3] : w[2]) : (q & 1 ? w[1] : w[0])};
-      if (sizeof(T) == 2 && e & 1) one[0] >>= 16;
-      if (p < BM_CAP)
-        got[p] = (uint64_t)bm_key(bm_element<T>(one, 0)) << 32 | (uint32_t) ~(t0 + E * BM_THREADS * u + e);
+  for (int u = 0; u < RUNS; ++u) {
+    const bool hit = run_best[u] >= reach;
+    const uint64_t hits = __ballot(hit);
+    const int p = held + __popcll(hits & ((1ull << lane) - 1));
+    if (hit && p < BM_WAVE_RUNS) {
+      run[wave][p] = u32x4{d[u][0], d[u][1], d[u][2], d[u][3]};
+      run_at[wave][p] = (uint16_t)(BM_THREADS * u + tid);
+    }
+    held += __popcll(hits);
+  }
+  bm_wave_sync();
+  if (held > BM_WAVE_RUNS) {  // (drawn one by one)
+    if (lane == 0) atomicAdd(&count, BM_CAP + 1);
+  } else {
+    for (int i = lane / E; i < held; i += 64 / E) {
+      const float v = to_f32(reinterpret_cast<const T*>(&run[wave][i])[lane % E]);
+      if (v >= reach) {
+        const int p = atomicAdd(&count, 1);
+        if (p < BM_CAP) got[p] = (uint64_t)bm_key(v) << 32 | (uint32_t) ~(c0 + E * run_at[wave][i] + lane % E);
+      }
     }
   }
   __syncthreads();
@@ -383,12 +396,6 @@ struct BmBest {  // a prompt's candidates, best first
   float value[BM_MOST];
   int token[BM_MOST], beam[BM_MOST];
 };
-
-// what the lanes of a wave wrote to LDS is there for the others
-__device__ __forceinline__ void bm_wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
 
 struct BmBook {  // what two waves decide and all copy by
   int live[BM_MOST], place[BM_MOST], taken[BM_MOST];  // taken: the hypothesis of a slot, -1: as before
