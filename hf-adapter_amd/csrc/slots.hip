@@ -215,7 +215,8 @@ extern "C" int rwkv7mi_rows_move(int n, const rwkv7mi_rows* tensors, int64_t src
   for (int i = 0; i < a.n; ++i) {
     a.first[i] = (uint32_t)blocks;
     a.t[i].windows = (uint32_t)(((uint64_t)a.t[i].units + (1u << a.log_window) - 1) >> a.log_window);
-    if (a.t[i].outer > INT32_MAX || (blocks += (uint64_t)a.t[i].outer * a.t[i].windows) > INT32_MAX) return fail(RWKV7MI_EINVAL, w + ": too large");
+    if (a.t[i].outer > INT32_MAX ||
+        (blocks += (uint64_t)a.t[i].outer * a.t[i].windows) > UINT32_MAX / (few ? 256u : 1024u)) return fail(RWKV7MI_EINVAL, w + ": too large");
   }
   a.first[a.n] = (uint32_t)blocks;
   a.src_rows = src_rows;

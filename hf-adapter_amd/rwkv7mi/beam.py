@@ -69,14 +69,18 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | No
     logits = _logits(logits, prompts, beams, name)
     dt = _lib.dtype_code(logits)
     m = 2 * beams if candidates is None else int(candidates)
+    if m < 1:
+        raise ValueError(f"{name}: candidates must be positive")
     _lib.require_same_device(logits, scores, *(out or ()), workspace, name=name)
     if out is None:
         out = (scores.new_empty((prompts, m)), scores.new_empty((prompts, m), dtype=torch.int64),
                scores.new_empty((prompts, m), dtype=torch.int64))
     else:
         out = tuple(out)
+        if len(out) != 3 or _lib.overlap(out[1], out[2]) or any(_lib.overlap(out[0], t) for t in out[1:]):
+            raise ValueError(f"{name}: out must be three tensors apart from each other")
         for t, want in zip(out, (torch.float32, torch.int64, torch.int64)):
-            if len(out) != 3 or tuple(t.shape) != (prompts, m) or t.dtype is not want or not t.is_contiguous():
+            if tuple(t.shape) != (prompts, m) or t.dtype is not want or not t.is_contiguous():
                 raise ValueError(f"{name}: out must be contiguous fp32, int64, int64 [prompts, candidates]")
     rows, n = logits.shape
     need = _workspace(rows, n, m)
@@ -182,6 +186,16 @@ class BeamState:
                 torch.cat([self.finished_lengths, length], 1).gather(1, order), score.gather(1, order))
 
 
+def end_tokens(eos_token_id) -> list[int]:
+    """The end tokens that ``eos_token_id`` names: none, one, or several (a sequence or a
+    tensor)."""
+    if eos_token_id is None:
+        return []
+    if isinstance(eos_token_id, torch.Tensor):
+        eos_token_id = eos_token_id.reshape(-1).tolist()
+    return [int(t) for t in eos_token_id] if isinstance(eos_token_id, (list, tuple)) else [int(eos_token_id)]
+
+
 def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, length_penalty: float = 1.0,
               early_stopping=False, pad_token_id: int = 0, normalized: bool = False, out: BeamState | None = None,
               next_tokens: torch.Tensor | None = None, rows: torch.Tensor | None = None,
@@ -213,8 +227,7 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, leng
     prompts, beams, room = state.tokens.shape
     logits = _logits(logits, prompts, beams, name)
     dt = _lib.dtype_code(logits)
-    ends = [] if eos_token_id is None else [int(t) for t in (
-        eos_token_id if isinstance(eos_token_id, (list, tuple)) else (eos_token_id,))]
+    ends = end_tokens(eos_token_id)
     m = (1 + len(ends)) * beams
     if len(ends) > MAX_ENDS or m > MAX_CANDIDATES:
         raise ValueError(f"{name}: at most {MAX_ENDS} end tokens and {MAX_CANDIDATES} candidates, "
@@ -236,6 +249,8 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, leng
     for t in (next_tokens, rows):
         if t is not None and (t.dtype is not torch.int64 or t.numel() != total or not t.is_contiguous()):
             raise ValueError(f"{name}: next_tokens and rows must be contiguous int64 tensors of one entry per row")
+    if next_tokens is not None and rows is not None and total and _lib.overlap(next_tokens, rows):
+        raise ValueError(f"{name}: next_tokens and rows overlap")
     if next_tokens is None:
         next_tokens = state.tokens.new_empty(total)
     if rows is None:

@@ -40,7 +40,7 @@ from .fused_recurrent_update import fused_recurrent_output_prepare_raw
 from .native_wkv_fp16 import (native_fp16_recurrent_output_prepare_raw, native_fp16_recurrent_should_use,
                               native_fp16_sequence)
 from .fused_time_mix import fused_attn_sequence_shift_mix, fused_ffn_sequence_shift_mix
-from .beam import BeamState, beam_step, beam_workspace_bytes
+from .beam import BeamState, beam_step, beam_workspace_bytes, end_tokens
 from .state_rows import MAX_TRADING, move_rows_, select_rows
 from .sampling import argmax_rows, argmax_workspace_bytes, process_logits, process_logits_workspace_bytes
 from .native_quant_mm8 import (GEMM_ROWS, GEMV_ROWS, MM8Linear, is_blocked, mm8_gemm_workspace_bytes, mm8_lnmix_multi_into,
@@ -744,6 +744,8 @@ class NativeRWKV7Cache(_HFCache):
             self._map(lambda t: t.index_select(0, idx.to(t.device)))
             return
         if isinstance(index, torch.Tensor):
+            if index.dim() > 1:
+                raise IndexError("NativeRWKV7Cache: a one-dimensional index is wanted")
             index = index.reshape(-1).to(ts[0].device) if index.is_cuda else index.reshape(-1).tolist()
         if isinstance(index, list) and any(i < 0 for i in index):
             raise IndexError("NativeRWKV7Cache: index out of range")
@@ -1901,7 +1903,8 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
             raise ValueError("generate_beam: 1 <= num_return_sequences <= num_beams and max_new_tokens >= 1")
         dev, V = self.device, self.config.vocab_size
         here = lambda v: v.to(dev) if isinstance(v, torch.Tensor) else v  # noqa: E731
-        how = dict(eos_token_id=eos_token_id, length_penalty=length_penalty, early_stopping=early_stopping,
+        ends = end_tokens(eos_token_id)
+        how = dict(eos_token_id=ends, length_penalty=length_penalty, early_stopping=early_stopping,
                    pad_token_id=pad_token_id)
         plain = bias is None and allowed is None and not any(
             isinstance(v, torch.Tensor) or v != d
@@ -1912,8 +1915,7 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
         ids = input_ids.to(dev)
         state = BeamState.start(ids, K, T + steps)
         nxt, rows = (torch.empty(B * K, dtype=torch.long, device=dev) for _ in range(2))
-        n_ends = len(eos_token_id) if isinstance(eos_token_id, (list, tuple)) else int(eos_token_id is not None)
-        ws = torch.empty(beam_workspace_bytes(B * K, V, (1 + n_ends) * K), dtype=torch.uint8, device=dev)
+        ws = torch.empty(beam_workspace_bytes(B * K, V, (1 + len(ends)) * K), dtype=torch.uint8, device=dev)
         scored = None if plain else torch.empty(B * K, V, dtype=torch.float32, device=dev)
 
         def pick(logits):

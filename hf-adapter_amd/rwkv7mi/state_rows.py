@@ -63,6 +63,18 @@ def _lap(families) -> bool:
     return any([b[0] < a[1] for a, b in zip(ends, ends[1:])])
 
 
+def _within(index, families) -> bool:
+    """Whether an index of the GPU lies in memory that is written."""
+    if type(index) is list:
+        return False
+    a = index.data_ptr()
+    b = a + 8 * index.numel()
+    for f in families:
+        if f[0] < b and a < f[6]:
+            return True
+    return False
+
+
 def _index(index, name: str):
     """``index`` as a list of ints, or a one-dimensional int64 tensor of the GPU."""
     if isinstance(index, torch.Tensor):
@@ -156,7 +168,7 @@ def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tenso
         dst = [_family(o, dim, name) for o in out]
         if any(f is None or not _apart(f) for f in dst):
             raise ValueError(f"{name}: the rows of an output are dense and apart")
-        if _lap(dst) or any(_lap((f, g)) for f in src for g in dst):
+        if _lap(dst) or any(_lap((f, g)) for f in src for g in dst) or _within(idx, dst):
             raise ValueError(f"{name}: outputs overlap")
         for f, g in zip(src, dst):
             flat += (f[0], g[0], f[1], f[2], g[1], g[2], f[3], f[4])
@@ -187,6 +199,8 @@ def move_rows_(tensors, sources, destinations=None, *, dim: int = 0) -> None:
         if f is None or not _apart(f):
             raise ValueError(f"{name}: the rows of a tensor are dense and apart")
     rows = _same_rows(fams, name)
+    if _within(src, fams):
+        src = src.clone()  # (as if it was read first, like the rows)
     if len(fams) > 1 and _lap(fams):
         raise ValueError(f"{name}: tensors overlap or interleave")
     n = len(src) if type(src) is list else src.shape[0]

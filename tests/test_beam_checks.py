@@ -103,7 +103,8 @@ def test_beam_select_refuses(calls):
     x, s = torch.zeros(6, 50), torch.zeros(2, 3)
     for args, kw in (((x, s.double()), {}), ((x, s[0]), {}), ((x[:5], s), {}), ((x.view(3, 2, 50), s), {}),
                      ((x.to(torch.float64), s), {}), ((x[:, :0], s), {}), ((x, s), dict(out=(s, s, s))),
-                     ((x, s), dict(workspace=torch.zeros(8, dtype=torch.uint8)))):
+                     ((x, s), dict(workspace=torch.zeros(8, dtype=torch.uint8))), ((x, s, 0), {}), ((x, s, -3), {}),
+                     ((x, s), dict(out=(torch.zeros(2, 6), *[torch.zeros(2, 6, dtype=torch.int64)] * 2)))):
         with pytest.raises(ValueError):
             mi.beam_select(*args, **kw)
     assert not calls
@@ -147,12 +148,19 @@ def test_beam_step_refuses(calls):
                dict(rows=torch.zeros(6, dtype=torch.int32)), dict(workspace=torch.zeros(4, dtype=torch.uint8))):
         with pytest.raises(ValueError):
             mi.beam_step(x, s, **kw)
+    both = torch.zeros(7, dtype=torch.int64)
+    with pytest.raises(ValueError, match="overlap"):
+        mi.beam_step(x, s, next_tokens=both[:6], rows=both[1:])
     with pytest.raises(ValueError):
         mi.beam_step(torch.zeros(80, 50), mi.BeamState.start(torch.zeros(1, 2, dtype=torch.int64), 80, 9), eos_token_id=1)
     with pytest.raises(ValueError):
         mi.beam_step(x[:4], s)
     assert not calls
     assert mi.beam_step(x, s)[2] is s and len(calls) == 1
+    for eos in (3, [3, 4], (3, 4), torch.tensor([3, 4]), torch.tensor(3)):  # (the library's 9th and 8th arguments)
+        mi.beam_step(x, s, eos_token_id=eos)
+        args = calls[-1][1]
+        assert list(args[7]) == ([3] if args[8] == 1 else [3, 4])
 
 
 def test_rows_refuse(calls):

@@ -184,7 +184,8 @@ def test_cache_rows(state):
             c.batch_repeat_interleave(3)
             assert all(torch.equal(a, b[at].repeat_interleave(3, 0)) for a, b in zip(c._all_tensors(), old))
     c = _cache(model, 4)
-    for bad in ([4], [-1], torch.tensor([0, -1])):
+    assert c.select_batch([], inplace=False).get_batch_size() == 0
+    for bad in ([4], [-1], torch.tensor([0, -1]), torch.zeros(1, 2, dtype=torch.long, device="cuda")):
         with pytest.raises(IndexError):
             c.select_batch(bad)
 

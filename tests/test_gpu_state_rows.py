@@ -160,6 +160,20 @@ def test_move_rows_on_a_stream_and_captured():
         assert all(torch.equal(a, b[:, [3, 3, 0]]) for a, b in zip(new, want))
 
 
+def test_an_index_among_what_is_moved():
+    """The index's own rows move too: it counts as it was before the call."""
+    import rwkv7mi as mi
+
+    for _ in range(3):
+        t = torch.randn(500, 3000, device="cuda")
+        idx = torch.randperm(500, device="cuda")
+        want = (t[idx], idx[idx])
+        mi.move_rows_([t, idx], idx)
+        assert torch.equal(t, want[0]) and torch.equal(idx, want[1])
+    with pytest.raises(ValueError):
+        mi.select_rows([t[:, 0].long().contiguous()], idx, out=[idx])
+
+
 def test_custom_ops():
     import rwkv7mi as mi
 
