@@ -5,7 +5,7 @@
 //   value(k, t) = s + (x[t] - lse),  lse = m + log sum_t exp(x[t] - m)
 // in 64 bits (so that which of two close candidates comes first does not hang on
 // fp32's last bits), rounded once to fp32.  The M best of the K V values, best
-// first, equal ones by (k, t).  A row that holds NaN or +inf, or whose score is
+// first, equal ones by beam, then logit, then token.  A row that holds NaN or +inf, or whose score is
 // one, is NaN throughout, and NaN ranks first, as in the argmax; a token of
 // logit -inf, and every token of a row that is -inf throughout or whose score
 // is, has the value -inf.
@@ -20,22 +20,23 @@
 // hold one go through LDS to the wave's lanes, and what reaches the bound is
 // ranked by counting.  -inf is never gathered: a masked row costs no more than
 // another.  Values in numbers that LDS does not hold (long ties) are drawn one by
-// one instead.  HBM-bound for many rows (67 MB in 17 us, vector instructions in
-// two thirds of them), latency-bound for few (4.6 us for 4 rows).  (The least of
-// the maxima of 16 groups of lanes as the bound, without the search: 26.6 us for
-// 24.0 at 64 x 8 rows; fp32 values in registers: 33.)
+// one instead.  Bound by memory and vector instructions together for many rows:
+// 67 MB in 18.4 us, 3.6 TB/s, the vector units busy for two thirds of the busy
+// cycles; latency-bound for few (4.6 us for 4 rows).  (The least of the maxima of
+// 16 groups of lanes as the bound, without the search: a selection of 64 x 8 rows
+// 26.6 us against 24.9.)
 //
 // beam_merge_kernel: one workgroup per prompt joins the slices' sums to lse, in
 // 64 bits, and selects among their K S M candidates the same way, the bound from
 // the lists' heads; the step's bookkeeping (ends, hypotheses, places of the
 // beams) follows in the same workgroup, two of its waves deciding without a
-// barrier.  Latency-bound: 3.6 us for one prompt of 4 beams (lse 1900 cycles, the
-// bound 1300, gathering and ranking 900 each), 6 for 64 of 8; 4 x 32 beams with 64
-// candidates 9 to 14, the ranking of 100 to 300 gathered ones; the step's
-// decisions 2300 cycles more.
+// barrier.  Latency-bound, a chain of short phases: 4.6 us for one prompt of 4
+// beams, 7.9 for 64 of 8, 9 to 14 (by what reaches the bound) for 4 of 32 with 64
+// candidates; as a step's 7.8 and 17.5 for the first two.
 //
-// Whole selections in a captured graph: 1 x 4 rows of 65536 fp16 logits 8.4 us,
-// 64 x 8 24.2 (floor 13.7), 4 x 32 fp32 25.7; steps 11 and 43.
+// Whole selections in a captured graph: 1 x 4 rows of 65536 fp16 logits 8.8 us,
+// 64 x 8 24.6 (12.5 at the rate of a large copy), 4 x 32 fp32 25.8; steps of the
+// first two 11.5 and 44.2, texts of 4096 tokens of room included in the second.
 #include "common.h"
 
 namespace rwkv7mi {
@@ -899,7 +900,7 @@ int64_t bm_slices(int64_t V, int dtype, int runs) { return (V + bm_slice(dtype, 
 // logits for 512 such workgroups, 4 down to 128 and 2 below, which fill the card sooner.  us with 2, 4, 8
 // runs, rows of 65536 fp16 logits: 16 rows 8.8, 9.3, 10.0; 32 10.0, 9.6, 10.0; 128 14.9, 13.3, 13.0; 512
 // 35.0, 29.7, 24.0.
-int bm_runs(int64_t rows, int64_t V, int dtype, int64_t M) {
+int bm_runs(int64_t rows, int64_t V, int dtype) {
   const int64_t logits = rows * V, unit = bm_slice(dtype, 8);
   return logits >= 512 * unit ? 8 : logits >= 128 * unit ? 4 : 2;
 }
@@ -913,7 +914,7 @@ int bm_run(BmArgs& a, BmStep* step, int64_t prompts, int dtype, void* workspace,
   const bool straight = !(reinterpret_cast<uintptr_t>(a.x) & 15) &&
                         (rows == 1 || a.ldx * (dtype == RWKV7MI_F32 ? 4 : 2) % 16 == 0);
   const int64_t width = a.V + (straight ? 0 : 7);
-  const int runs = bm_runs(rows, a.V, dtype, a.M);
+  const int runs = bm_runs(rows, a.V, dtype);
   a.S = (int)bm_slices(width, dtype, runs);
   const size_t need = (size_t)(rows * a.S) * (8u * (size_t)a.M + 8u) + 8u * (size_t)rows;
   if (!workspace || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))

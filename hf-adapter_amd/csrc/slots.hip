@@ -58,7 +58,8 @@ __global__ __launch_bounds__(256) void slot_copy_kernel(const SlotCopy C) {
 // MB a row): 8 chats of 4 beams in place, 0.99 GB, 177 [188]; one row to 8, 0.31
 // GB, 51 [64]; two rows to four each in new tensors, 0.34 GB, 52 [72]; the 2.9B
 // model's fp16 pool of 33, 9 rows moved and 5 made zero, 0.25 GB, 51 [59]; 4 rows
-// of the 0.1B model 4.5 [4.6].  (4 or 16 loads a lane: 10 to 15% more.)
+// of the 0.1B model 4.5 [4.6].  (Behind ordinary stores, 4 loads a lane: 8% less to
+// 13% more, the largest moves losing; 16: up to a third more.)
 namespace {
 
 constexpr int RW_TENSORS = 24;   // of a launch
