@@ -3,8 +3,9 @@
 //
 // For prompt b, beam k with running score s and logits x[0 .. V-1]:
 //   value(k, t) = s + (x[t] - lse),  lse = m + log sum_t exp(x[t] - m)
-// in 64 bits (so that which of two close candidates comes first does not hang on
-// fp32's last bits), rounded once to fp32.  The M best of the K V values, best
+// in 64 bits, rounded once to fp32 (close candidates are not equal for that); the
+// exponentials and their sums over a slice are fp32, the slices' sums joined in 64
+// bits.  The M best of the K V values, best
 // first, equal ones by beam, then logit, then token.  A row that holds NaN or +inf, or whose score is
 // one, is NaN throughout, and NaN ranks first, as in the argmax; a token of
 // logit -inf, and every token of a row that is -inf throughout or whose score
@@ -678,6 +679,11 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
   }
   if (tid == 0) count = 0;
   got[tid] = 0;
+  if (tid < BM_MOST) {  // (what a workspace that another call writes leaves unset points into the prompt too)
+    best.value[tid] = -__builtin_inff();
+    best.beam[tid] = best.token[tid] = 0;
+    if constexpr (STEP) book.live[tid] = 0;
+  }
   for (int k = row; k < K; k += NT / 16) {
     if (k != row) {
       own = A.scores[r0 + k];
@@ -788,7 +794,7 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
   }
   const auto put = [&](int r, float v, int beam, int token) {
     best.value[r] = v;
-    best.beam[r] = beam;
+    best.beam[r] = min(beam, K - 1);
     best.token[r] = token;
   };
   if (n <= BM_CAP) {
@@ -881,7 +887,7 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
 __global__ __launch_bounds__(256) void beam_texts_kernel(const BmStep P, int beams) {
   const int64_t b = blockIdx.y, row = b * beams + blockIdx.x % beams;
   const bool finished = (int)blockIdx.x >= beams;
-  const int from = P.plan[2 * b * beams + blockIdx.x], room = (int)P.room;
+  const int from = min(P.plan[2 * b * beams + blockIdx.x], beams - 1), room = (int)P.room;
   const int64_t* src = (finished && from < 0 ? P.in.finished_tokens : P.in.tokens) + (from < 0 ? row : b * beams + from) * P.room;
   int n = finished && from < 0 ? P.in.finished_lengths[row] : P.in.lengths[b * beams];
   n = min(max(n, 0), room);
@@ -955,7 +961,7 @@ int bm_check(const std::string& w, const void* x, int64_t prompts, int64_t beams
   if (V > INT32_MAX / 256) return fail(RWKV7MI_EINVAL, w + ": too large");
   if (reinterpret_cast<uintptr_t>(x) & (dtype == RWKV7MI_F32 ? 3 : 1)) return fail(RWKV7MI_EINVAL, w + ": unaligned logits");
   if (M > beams * V) return fail(RWKV7MI_EINVAL, w + ": more candidates than there are");
-  if (prompts * beams > 65535) return fail(RWKV7MI_EINVAL, w + ": at most 65535 rows");
+  if (prompts > 65535 / beams) return fail(RWKV7MI_EINVAL, w + ": at most 65535 rows");
   return RWKV7MI_OK;
 }
 

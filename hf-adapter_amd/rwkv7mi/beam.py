@@ -55,8 +55,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | No
 
     Returns ``(scores fp32, tokens int64, rows int64)``, each ``[prompts, candidates]``, best
     first, equal ones by beam, then logit, then token; ``rows`` are rows of ``logits``.  A continuation's
-    score is ``scores + (logit - logsumexp(row))`` in 64 bits, rounded once
-    (``normalized``: the logits are log-probabilities as they are).  A row that holds NaN
+    score is ``scores + (logit - logsumexp(row))`` in 64 bits (the exponentials and their sums over
+    parts of a row in 32), rounded once (``normalized``: the logits are log-probabilities as they are).  A row that holds NaN
     or +inf, or whose score is one, counts as NaN throughout, which ranks first; a logit of
     -inf, a row of nothing else and a score of -inf (a beam that has not begun) give -inf, in
     the order of their indices.  No host synchronisation; capturable.  ``out``: three tensors

@@ -30,6 +30,13 @@ def test_select_entry_refuses(kw):
     assert _select(**kw) == -1
 
 
+@pytest.mark.parametrize("prompts,beams", [(2 ** 57, 128), (2 ** 62, 4), (16384, 4), (65536, 1)])
+def test_entries_count_rows_without_wrapping(prompts, beams):
+    for call in (_select, lambda **kw: _step(ends=(), **kw)):
+        assert call(prompts=prompts, beams=beams) == -1
+        assert b"65535 rows" in _lib().rwkv7mi_last_error()
+
+
 def test_select_entry_wants_its_workspace():
     need = _lib().rwkv7mi_beam_workspace_bytes(6, 100, 6)
     assert need >= 6 * 6 * 8
