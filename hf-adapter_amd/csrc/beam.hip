@@ -194,19 +194,22 @@ __device__ __forceinline__ float bm_element(const uint32_t (&d)[4], int e) {
   }
 }
 
-// that element less m (minus: -m), exactly as its fp32 value less m
+constexpr float BM_LOG2E = 1.44269504f;
+// log2(e) times that element less m, to be exponentiated.  fp16: less base = fp32(log2(e) m), in one
+// instruction (the product exact; what base was rounded by is put right in the sum); the others, whose
+// products could overflow: the difference first.
 template <typename T>
-__device__ __forceinline__ float bm_less(const uint32_t (&d)[4], int e, float minus) {
+__device__ __forceinline__ float bm_less(const uint32_t (&d)[4], int e, float m, float base) {
   if constexpr (std::is_same<T, __half>::value) {
-    float r;  // (the conversion inside the addition)
+    float r;  // (the conversion inside)
     const uint32_t w = d[e / 2];
     if (e & 1)
-      asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(minus));
+      asm("v_fma_mix_f32 %0, %1, %2, -%3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(BM_LOG2E), "v"(base));
     else
-      asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(minus));
+      asm("v_fma_mix_f32 %0, %1, %2, -%3 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(BM_LOG2E), "v"(base));
     return r;
   } else {
-    return bm_element<T>(d, e) + minus;
+    return (bm_element<T>(d, e) - m) * BM_LOG2E;
   }
 }
 
@@ -251,34 +254,30 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
   const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int c0 = (int)blockIdx.x * SLICE - shift;  // the slice's first token (before the row in the first slice)
   const int t0 = c0 + E * tid;
-  // whole runs all at once (others read as zeros), then what the row's two ends need
-  const __amdgpu_buffer_rsrc_t mem = make_rsrc(x - shift, (uint32_t)(shift + A.V) * (uint32_t)sizeof(T));
+  // aligned units of 16 bytes that hold a token of the row (no such unit crosses a page), all at once; what
+  // of them lies outside the row is nothing
+  const __amdgpu_buffer_rsrc_t mem = make_rsrc(x - shift, ((uint32_t)(shift + A.V) * (uint32_t)sizeof(T) + 15u) & ~15u);
   uint32_t d[RUNS][4];
 #pragma unroll
   for (int u = 0; u < RUNS; ++u) {
     const int i = t0 + E * BM_THREADS * u;
-    const u32x4 w = buf_ld16(mem, i >= 0 && i + E <= A.V ? (uint32_t)(i + shift) * (uint32_t)sizeof(T) : BUF_OOB);
+    const u32x4 w = buf_ld16(mem, (uint32_t)(i + shift) * (uint32_t)sizeof(T));
 #pragma unroll
     for (int q = 0; q < 4; ++q) d[u][q] = w[q];
   }
   if (c0 < 0 || c0 + SLICE > A.V) {
+    constexpr uint32_t NOTHING = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
     for (int u = 0; u < RUNS; ++u) {
       const int i = t0 + E * BM_THREADS * u;
       if (i >= 0 && i + E <= A.V) continue;
-      uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const bool in = i + e >= 0 && i + e < A.V;
-        if constexpr (sizeof(T) == 4)
-          w[e] = in ? __float_as_uint(x[i + e]) : 0xff800000u;
-        else
-          w[e / 2] |= (uint32_t)(in ? __builtin_bit_cast(uint16_t, x[i + e]) : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u)
-                      << (16 * (e & 1));
+        const uint32_t mask = sizeof(T) == 4 ? ~0u : 0xffffu << (16 * (e & 1));
+        uint32_t& w = d[u][e * (int)sizeof(T) / 4];
+        w = in ? w : (w & ~mask) | (NOTHING & mask);
       }
-#pragma unroll
-      for (int q = 0; q < RUNS; ++q)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) d[q][j] = q == u ? w[j] : d[q][j];
     }
   }
   float run_best[RUNS], best = -__builtin_inff();
@@ -302,12 +301,13 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
     if (tid == 0) bound = t;
   }
   // NaN and +inf make the sum NaN (a slice of -inf and NaN alone: asked for)
+  const float base = m * BM_LOG2E;
   float s = 0.f;
   if (m > -__builtin_inff()) {
 #pragma unroll
     for (int u = 0; u < RUNS; ++u) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(bm_less<T>(d[u], e, -m) * 1.44269504f);
+      for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(bm_less<T>(d[u], e, m, base));
       __builtin_amdgcn_sched_barrier(0);  // (one run's exponentials at a time: registers)
     }
   } else {
@@ -357,6 +357,7 @@ __global__ __launch_bounds__(BM_THREADS) void beam_slice_kernel(const BmArgs A) 
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) sum += wave_sums[w];
+    if (std::is_same<T, __half>::value && m > -__builtin_inff()) sum *= __builtin_amdgcn_exp2f(fmaf(-m, BM_LOG2E, base));
     A.sums[slice] = make_float2(m, sum);
   }
   const int n = count;
