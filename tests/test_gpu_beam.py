@@ -84,6 +84,25 @@ def test_select_rows_anywhere_in_memory(dtype):
     _check(mi.beam_select(x, s, 4), x.cpu(), s.cpu(), 4)
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_select_takes_nothing_from_around_a_row(dtype):
+    """NaN or +inf in the elements before and behind every row, at each alignment; logits of large
+    magnitude too (they leave no rounding of their own: the differences are exact)."""
+    import rwkv7mi as mi
+
+    rng = np.random.default_rng(9)
+    for n in (1, 3, 16, 4097, 16385):
+        for offset in range(9):
+            for poison, shift in ((float("nan"), 0.0), (INF, 30000.0), (INF, -30000.0)):
+                x = torch.from_numpy(rng.standard_normal((4, n)) * 3 + shift).to(DTYPES[dtype])
+                big = torch.full((16 + offset + 4 * (n + 17) + 16,), poison, dtype=DTYPES[dtype], device="cuda")
+                rows = big.as_strided((4, n), (n + 17, 1), 16 + offset)
+                rows.copy_(x)
+                s = torch.from_numpy(rng.standard_normal((2, 2)) - 5).float()
+                m = min(4, 2 * n)
+                _check(mi.beam_select(rows, s.cuda(), m), x, s, m)
+
+
 def test_select_equal_values_by_index():
     """Equal beams, equal logits, more of them than a workgroup gathers: exactly the first indices."""
     import rwkv7mi as mi
