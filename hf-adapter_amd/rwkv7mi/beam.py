@@ -169,21 +169,29 @@ class BeamState:
 
     def best(self, count: int = 1, *, length_penalty: float = 1.0):
         """``(tokens [prompts, count, room], lengths, scores)`` of each prompt's ``count`` best
-        texts, best first: the hypotheses, then, of a search that is not over and has fewer, the
-        running beams, by score / generated length ** length_penalty."""
+        texts, best first: the hypotheses, then, of a search that is not over (or ended without a
+        hypothesis) and has fewer, the running beams, by score / generated length ** length_penalty.
+        Where there are not as many texts, the rest are the prompt alone, with the score -inf."""
         p, k, room = self.tokens.shape
         if not 1 <= count <= k:
             raise ValueError(f"BeamState.best: count must be 1..{k}")
         length = self.lengths.view(p, k)
         span = (length - self.prompt_lengths[:, None]).clamp(min=1).double()
         running = (self.scores.double() / span ** float(length_penalty)).float()
+        ended = self.finished_scores > -math.inf
+        # (what still ran when the last step filled the rows is among the hypotheses)
+        open_ = ~(self.done & ended.any(1))[:, None] & (self.scores != -math.inf)
+        kind = torch.cat([ended.int() * 2, open_.int()], 1)  # 2: a hypothesis, 1: a running text, 0: none
         score = torch.cat([self.finished_scores, running], 1)
-        ended = torch.cat([self.finished_scores > -math.inf, torch.zeros_like(running, dtype=torch.bool)], 1)
         order = score.sort(dim=1, descending=True, stable=True).indices
-        order = order.gather(1, ended.gather(1, order).int().sort(dim=1, descending=True, stable=True).indices)[:, :count]
-        pick = order[..., None].expand(p, count, room)
-        return (torch.cat([self.finished_tokens, self.tokens], 1).gather(1, pick),
-                torch.cat([self.finished_lengths, length], 1).gather(1, order), score.gather(1, order))
+        order = order.gather(1, kind.gather(1, order).sort(dim=1, descending=True, stable=True).indices)[:, :count]
+        none = kind.gather(1, order) == 0
+        order = order.masked_fill(none, k)  # (every running text begins with the prompt)
+        tokens = torch.cat([self.finished_tokens, self.tokens], 1).gather(1, order[..., None].expand(p, count, room))
+        lengths = torch.cat([self.finished_lengths, length], 1).gather(1, order)
+        lengths = torch.where(none, self.prompt_lengths[:, None], lengths)
+        tokens = tokens.masked_fill(none[..., None] & (torch.arange(room, device=tokens.device) >= lengths[..., None]), 0)
+        return tokens, lengths, score.gather(1, order).masked_fill(none, -math.inf)
 
 
 def end_tokens(eos_token_id) -> list[int]:

@@ -1,0 +1,86 @@
+"""Beam search and moved rows at their limits, on the CPU: searches with fewer texts than beams, states and buffers
+that a call has to refuse, caches that the kernels do not serve."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import beam_reference as ref
+
+KEYS = ("tokens", "lengths", "scores", "prompt_lengths", "finished_tokens", "finished_lengths", "finished_scores", "done")
+
+
+def _search(mi, ids, beams, room, logits, ends=(), steps=None):
+    """The state behind ``steps`` steps (default: until the rows are full) over ``logits [beams, n]``."""
+    start = mi.BeamState.start(torch.tensor(ids), beams, room)
+    s = {k: getattr(start, k).numpy().copy() for k in KEYS}
+    prompts = len(ids)
+    x = np.broadcast_to(np.asarray(logits, np.float64), (prompts, beams, len(logits[0]) if np.ndim(logits) > 1 else len(logits)))
+    for _ in range(room - len(ids[0]) if steps is None else steps):
+        val, tok, beam = ref.select(ref.values(x, s["scores"]), (1 + len(ends)) * beams)
+        _, _, s = ref.step((val.astype(np.float32), tok, beam), s, ends, 1.0, False)
+    return mi.BeamState(**{k: torch.from_numpy(v) for k, v in s.items()})
+
+
+def _texts(found, prompt=0):
+    tokens, lengths, scores = found
+    return [(t[:n].tolist(), float(s)) for t, n, s in zip(tokens[prompt], lengths[prompt], scores[prompt])]
+
+
+ONE = np.where(np.arange(8) == 5, 0.0, -np.inf)  # one token can follow
+
+
+def test_best_of_a_full_search_gives_no_text_twice():
+    import rwkv7mi as mi
+
+    s = _search(mi, [[1, 2]], 3, 4, ONE)
+    assert s.done.all()
+    # one text in all: the places that are left hold the prompt
+    assert _texts(s.best(3)) == [([1, 2, 5, 5], 0.0), ([1, 2], -np.inf), ([1, 2], -np.inf)]
+    assert _texts(s.best(1)) == [([1, 2, 5, 5], 0.0)]
+
+
+def test_best_of_a_search_that_ended_early():
+    import rwkv7mi as mi
+
+    s = _search(mi, [[1, 2], [3, 4]], 3, 9, ONE, ends=(5,))
+    assert s.done.all()
+    for b, prompt in enumerate(([1, 2], [3, 4])):
+        assert _texts(s.best(3), b) == [(prompt + [5], 0.0), (prompt, -np.inf), (prompt, -np.inf)]
+
+
+def test_best_of_a_running_search_with_fewer_texts_than_beams():
+    import rwkv7mi as mi
+
+    s = _search(mi, [[1, 2]], 3, 9, ONE, steps=2)
+    assert not s.done.any()
+    assert _texts(s.best(3)) == [([1, 2, 5, 5], 0.0), ([1, 2], -np.inf), ([1, 2], -np.inf)]
+    # before the first step: the prompt itself
+    assert _texts(mi.BeamState.start(torch.tensor([[1, 2]]), 3, 9).best(2)) == [([1, 2], 0.0), ([1, 2], -np.inf)]
+
+
+def test_best_where_the_logits_are_nan():
+    """A search that met NaN is over without hypotheses: its texts, their scores NaN, not rows of nothing."""
+    import rwkv7mi as mi
+
+    s = _search(mi, [[1, 2]], 3, 9, np.full(8, np.nan), steps=1)
+    assert s.done.all()
+    got = _texts(s.best(2))
+    assert all(t[:2] == [1, 2] and len(t) == 3 and np.isnan(v) for t, v in got) and got[0][0] != got[1][0]
+
+
+def test_best_without_room_for_a_token():
+    import rwkv7mi as mi
+
+    s = mi.BeamState.start(torch.tensor([[1, 2]]), 2, 2)
+    s.done.fill_(True)
+    assert _texts(s.best(2)) == [([1, 2], 0.0), ([1, 2], -np.inf)]
+
+
+def test_best_where_the_penalty_outgrows_fp32():
+    """Running texts whose scores round to -inf under the penalty are texts all the same."""
+    import rwkv7mi as mi
+
+    s = _search(mi, [[1, 2]], 2, 9, np.array([0.0, 1.0, 2.0]), steps=3)
+    assert [len(t) for t, _ in _texts(s.best(2, length_penalty=-400.0))] == [5, 5]
