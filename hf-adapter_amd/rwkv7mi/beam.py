@@ -227,8 +227,8 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, leng
       its present length, ``"never"``: at the length that helps it most, beats the worst of
       ``beams`` hypotheses; True: there are ``beams`` hypotheses.
 
-    A done prompt keeps its state; its next tokens are ``pad_token_id``, its rows their own. No host
-    synchronisation; capturable.  ``next_tokens``, ``rows`` and ``workspace``
+    A done prompt keeps its state; its next tokens are ``pad_token_id`` (one that the
+    model takes, where they are fed to it), its rows their own. No host synchronisation; capturable.  ``next_tokens``, ``rows`` and ``workspace``
     (:func:`beam_workspace_bytes`) are allocated when not given.
     """
     name = "beam_step"

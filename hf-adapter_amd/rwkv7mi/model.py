@@ -1891,7 +1891,8 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
         that change hands follow in one launch.  The sequences that
         ``generate(num_beams=..., do_sample=False)`` gives with the same settings, rows of equal
         score aside: ``[B * num_return_sequences, longest]``, the prompt included, padded behind the
-        end; with ``return_scores`` also their scores (sum of log-probabilities / generated
+        end (``pad_token_id``: any number, the model is not fed it; a prompt with fewer texts than asked
+        for has itself, with score -inf, in the other places); with ``return_scores`` also their scores (sum of log-probabilities / generated
         length ** ``length_penalty``).  The host looks every eight steps whether all prompts are done.
 
         The penalties, ``bias`` and ``allowed`` are those of :func:`~.sampling.process_logits`, over
@@ -1904,8 +1905,8 @@ class NativeRWKV7ForCausalLM(_PreTrainedModel, _GenerationMixin):
         dev, V = self.device, self.config.vocab_size
         here = lambda v: v.to(dev) if isinstance(v, torch.Tensor) else v  # noqa: E731
         ends = end_tokens(eos_token_id)
-        how = dict(eos_token_id=ends, length_penalty=length_penalty, early_stopping=early_stopping,
-                   pad_token_id=pad_token_id)
+        # (a done prompt's rows run on with a token that the embedding has, whatever the filler is)
+        how = dict(eos_token_id=ends, length_penalty=length_penalty, early_stopping=early_stopping, pad_token_id=0)
         plain = bias is None and allowed is None and not any(
             isinstance(v, torch.Tensor) or v != d
             for v, d in ((repetition_penalty, 1.0), (presence_penalty, 0.0), (frequency_penalty, 0.0)))

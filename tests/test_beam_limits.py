@@ -84,3 +84,51 @@ def test_best_where_the_penalty_outgrows_fp32():
 
     s = _search(mi, [[1, 2]], 2, 9, np.array([0.0, 1.0, 2.0]), steps=3)
     assert [len(t) for t, _ in _texts(s.best(2, length_penalty=-400.0))] == [5, 5]
+
+
+class _Searcher:
+    """What ``generate_beam`` needs of a model, on the CPU: logits that end prompt 0 at once, and a record of
+    the tokens that it is fed."""
+
+    class config:
+        vocab_size = 8
+
+    device = torch.device("cpu")
+
+    def __init__(self):
+        self.fed = []
+
+    def forward(self, ids, past_key_values=None, use_graph=None):
+        from types import SimpleNamespace as Of
+
+        self.fed.append(ids.clone())
+        x = torch.full((ids.shape[0], 1, 8), -2.0)
+        first = (ids == 1).any(1) if past_key_values is None else torch.arange(ids.shape[0]) < ids.shape[0] // 2
+        x[first, :, 7] = 9.0
+        cache = Of(batch_repeat_interleave=lambda k: None, reorder_cache=lambda rows: None)
+        return Of(logits=x, past_key_values=cache)
+
+
+@pytest.mark.parametrize("pad", [-100, -1, 0, 7, 1 << 40])
+def test_generate_beam_feeds_the_model_tokens_of_its_own(monkeypatch, pad):
+    """A filler of any value: done prompts are padded with it, and the model never sees it."""
+    import rwkv7mi as mi
+    from rwkv7mi import model as module
+
+    def step(logits, state, *, next_tokens, rows, workspace, eos_token_id, length_penalty, early_stopping, pad_token_id):
+        s = {k: getattr(state, k).numpy() for k in KEYS}
+        x = logits.double().numpy().reshape(*s["scores"].shape, -1)
+        val, tok, beam = ref.select(ref.values(x, s["scores"]), (1 + len(eos_token_id)) * s["scores"].shape[1])
+        nxt, at, new = ref.step((val.astype(np.float32), tok, beam), s, eos_token_id, length_penalty, early_stopping,
+                                pad_token_id)
+        for k, v in new.items():
+            getattr(state, k).copy_(torch.from_numpy(v))
+        next_tokens.copy_(torch.from_numpy(nxt))
+        rows.copy_(torch.from_numpy(at))
+
+    monkeypatch.setattr(module, "beam_step", step)
+    model = _Searcher()
+    got = mi.model.NativeRWKV7ForCausalLM.generate_beam(model, torch.tensor([[1, 1], [2, 2]]), 5, num_beams=1, eos_token_id=7,
+                                                        pad_token_id=pad, use_graph=False)
+    assert got[0].tolist() == [1, 1, 7] + [pad] * 4 and got[1, :2].tolist() == [2, 2] and got.shape == (2, 7)
+    assert len(model.fed) == 5 and all(((0 <= t) & (t < 8)).all() for t in model.fed)

@@ -41,3 +41,13 @@ def test_generate_beam_of_nan_logits_keeps_the_prompt():
     bias[3] = float("nan")
     got, scores = model.generate_beam(ids, 4, num_beams=2, num_return_sequences=2, bias=bias, return_scores=True)
     assert got.shape[1] == 6 and torch.equal(got[:, :5], ids.repeat_interleave(2, 0)) and scores.isnan().all()
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_generate_beam_with_a_filler_outside_the_vocabulary(use_graph):
+    """Prompts that end at different steps: the filler stands in the result alone."""
+    model = _model()
+    ids = _ids(3)
+    want = model.generate_beam(ids, 12, num_beams=2, eos_token_id=80, pad_token_id=0, use_graph=use_graph, return_scores=True)
+    got = model.generate_beam(ids, 12, num_beams=2, eos_token_id=80, pad_token_id=-100, use_graph=use_graph, return_scores=True)
+    assert torch.equal(torch.where(got[0] == -100, 0, got[0]), want[0]) and torch.equal(got[1], want[1])
