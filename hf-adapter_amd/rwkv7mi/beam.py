@@ -107,7 +107,8 @@ def _meet(ranges) -> bool:
 
 class BeamState:
     """The state of a beam search over ``prompts`` prompts with ``beams`` beams each, on one
-    GPU: contiguous tensors, checked once and not replaced afterwards.
+    GPU: contiguous tensors, checked once and not replaced afterwards (a step refuses a state
+    whose tensors were given other memory).
 
     ``tokens`` int64 ``[prompts, beams, room]`` and ``lengths`` int32 ``[prompts * beams]``
     (the beams of a prompt are equally long): the texts, prompt included (also a history
@@ -117,7 +118,7 @@ class BeamState:
     hypotheses that have ended, in no order; ``done`` bool ``[prompts]``."""
 
     __slots__ = ("tokens", "lengths", "scores", "prompt_lengths", "finished_tokens", "finished_lengths",
-                 "finished_scores", "done", "_pointers", "_ends")
+                 "finished_scores", "done", "_pointers", "_addresses", "_shape", "_ends")
 
     def __init__(self, *, tokens, lengths, scores, prompt_lengths, finished_tokens, finished_lengths, finished_scores,
                  done):
@@ -143,7 +144,18 @@ class BeamState:
         if _meet(ends):
             raise ValueError(f"{name}: tensors overlap")
         put(self, "_pointers", _Pointers(*at))
+        put(self, "_addresses", tuple(at))
+        put(self, "_shape", shape)
         put(self, "_ends", ends)
+
+    def _check(self, name: str) -> None:
+        """The tensors lie where they did when they were checked (``resize_``, ``set_`` and ``.data`` move
+        them), with the room that they had."""
+        at = (self.tokens.data_ptr(), self.lengths.data_ptr(), self.scores.data_ptr(), self.prompt_lengths.data_ptr(),
+              self.finished_tokens.data_ptr(), self.finished_lengths.data_ptr(), self.finished_scores.data_ptr(),
+              self.done.data_ptr())
+        if at != self._addresses or self.tokens.shape != self._shape:
+            raise ValueError(f"{name}: a tensor of the BeamState was given other memory or another shape")
 
     def __setattr__(self, key, value):
         raise AttributeError(f"BeamState.{key} is not replaced (write into the tensor)")
@@ -232,7 +244,7 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, leng
     (:func:`beam_workspace_bytes`) are allocated when not given.
     """
     name = "beam_step"
-    prompts, beams, room = state.tokens.shape
+    prompts, beams, room = state._shape
     logits = _logits(logits, prompts, beams, name)
     dt = _lib.dtype_code(logits)
     ends = end_tokens(eos_token_id)
@@ -248,9 +260,11 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, leng
         raise ValueError(f"{name}: length_penalty = {lp}")
     to = state if out is None else out
     _lib.require_same_device(logits, state.tokens, to.tokens, next_tokens, rows, workspace, name=name)
+    state._check(name)
     if to is not state:
-        if to.tokens.shape != state.tokens.shape:
-            raise ValueError(f"{name}: out has {list(to.tokens.shape)} tokens, state {list(state.tokens.shape)}")
+        to._check(name)
+        if to._shape != state._shape:
+            raise ValueError(f"{name}: out has {list(to._shape)} tokens, state {list(state._shape)}")
         if _meet(sorted(state._ends + to._ends)):
             raise ValueError(f"{name}: out shares memory with state")
     total = prompts * beams

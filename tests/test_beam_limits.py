@@ -132,3 +132,45 @@ def test_generate_beam_feeds_the_model_tokens_of_its_own(monkeypatch, pad):
                                                         pad_token_id=pad, use_graph=False)
     assert got[0].tolist() == [1, 1, 7] + [pad] * 4 and got[1, :2].tolist() == [2, 2] and got.shape == (2, 7)
     assert len(model.fed) == 5 and all(((0 <= t) & (t < 8)).all() for t in model.fed)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The library calls, recorded instead of run."""
+    from rwkv7mi import _lib
+
+    made = []
+    monkeypatch.setattr(_lib, "require_same_device", lambda *t, name: None)
+    monkeypatch.setattr(_lib, "stream_of", lambda t: 0)
+    monkeypatch.setattr(_lib, "on_device", lambda t: _lib._HERE)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: made.append((name, args)))
+    return made
+
+
+def _state(mi, room=9):
+    return mi.BeamState.start(torch.zeros(2, 4, dtype=torch.int64), 3, room)
+
+
+@pytest.mark.parametrize("key", KEYS)
+def test_a_state_whose_memory_was_replaced_is_refused(calls, key):
+    """resize_, set_ and .data give a tensor other memory or another room: the state's addresses are not its own."""
+    import rwkv7mi as mi
+
+    x = torch.zeros(6, 50)
+    for change in (lambda t: t.resize_(4096), lambda t: t.set_(t.clone()), lambda t: setattr(t, "data", t.clone()),
+                   lambda t: t.untyped_storage().resize_(0)):
+        for side in ("in", "out"):
+            s, o = _state(mi), _state(mi)
+            change(getattr(s if side == "in" else o, key))
+            with pytest.raises(ValueError, match="BeamState"):
+                mi.beam_step(x, s, out=o)
+    assert not calls
+    s = _state(mi)
+    s.tokens.resize_(2, 3, 5)  # (less room in the same memory)
+    with pytest.raises(ValueError, match="BeamState"):
+        mi.beam_step(x, s)
+    assert not calls
+    s = _state(mi)
+    s.tokens.fill_(3)  # (written into: still its own)
+    mi.beam_step(x, s)
+    assert len(calls) == 1
