@@ -160,6 +160,10 @@ class BeamState:
     def __setattr__(self, key, value):
         raise AttributeError(f"BeamState.{key} is not replaced (write into the tensor)")
 
+    def __reduce__(self):
+        """Copied and pickled by its tensors: a copy of other tensors has addresses of its own."""
+        return _rebuilt, tuple(getattr(self, key) for key in self.__slots__[:8])
+
     @classmethod
     def start(cls, input_ids: torch.Tensor, beams: int, room: int, *, lengths=None) -> "BeamState":
         """The state behind the prompts ``input_ids [prompts, T]`` (the first ``lengths``
@@ -204,6 +208,10 @@ class BeamState:
         lengths = torch.where(none, self.prompt_lengths[:, None], lengths)
         tokens = tokens.masked_fill(none[..., None] & (torch.arange(room, device=tokens.device) >= lengths[..., None]), 0)
         return tokens, lengths, score.gather(1, order).masked_fill(none, -math.inf)
+
+
+def _rebuilt(*tensors) -> BeamState:
+    return BeamState(**dict(zip(BeamState.__slots__, tensors)))
 
 
 def end_tokens(eos_token_id) -> list[int]:

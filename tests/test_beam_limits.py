@@ -174,3 +174,20 @@ def test_a_state_whose_memory_was_replaced_is_refused(calls, key):
     s.tokens.fill_(3)  # (written into: still its own)
     mi.beam_step(x, s)
     assert len(calls) == 1
+
+
+def test_a_state_is_copied_and_pickled():
+    import copy
+    import pickle
+
+    import rwkv7mi as mi
+
+    s = _state(mi)
+    s.tokens.random_(0, 9)
+    same = copy.copy(s)
+    assert type(same) is mi.BeamState and all(getattr(same, k).data_ptr() == getattr(s, k).data_ptr() for k in KEYS)
+    for other in (copy.deepcopy(s), pickle.loads(pickle.dumps(s))):
+        assert type(other) is mi.BeamState and other._addresses != s._addresses and other._shape == s._shape
+        assert all(torch.equal(getattr(other, k), getattr(s, k)) for k in KEYS)
+        other.tokens.zero_()
+        assert s.tokens.any()
