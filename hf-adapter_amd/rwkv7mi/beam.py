@@ -5,6 +5,7 @@
 search is ``NativeRWKV7ForCausalLM.generate_beam``."""
 from __future__ import annotations
 
+import bisect
 import ctypes
 import functools
 import math
@@ -47,6 +48,26 @@ def _scratch(workspace, need, like, name):
     return workspace
 
 
+def _range(t: torch.Tensor, size: int | None = None):
+    """The addresses of ``t`` (rows of any distance), or of its first ``size`` bytes."""
+    at = t.data_ptr()
+    if size is None:
+        size = (sum((k - 1) * s for k, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else 0
+    return at, at + size
+
+
+def _clear(name: str, written, read, states=()) -> None:
+    """Refuses ranges that are written and meet another one: of ``written``, of ``read``, or of the
+    states' (sorted, apart from each other)."""
+    for i, (a, b) in enumerate(written):
+        hit = any(c < b and a < d for c, d in (*written[:i], *read))
+        for ends in states:
+            k = bisect.bisect_left(ends, (b,))
+            hit |= k > 0 and ends[k - 1][1] > a
+        if hit and a < b:
+            raise ValueError(f"{name}: outputs or workspace overlap each other or what is read")
+
+
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | None = None, *, normalized: bool = False,
                 out=None, workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The ``candidates`` (default twice the beams, at most 128) best continuations of each
@@ -60,7 +81,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | No
     or +inf, or whose score is one, counts as NaN throughout, which ranks first; a logit of
     -inf, a row of nothing else and a score of -inf (a beam that has not begun) give -inf, in
     the order of their indices.  No host synchronisation; capturable.  ``out``: three tensors
-    to write; ``workspace`` (:func:`beam_workspace_bytes`) is allocated when not given.
+    to write; ``workspace`` (:func:`beam_workspace_bytes`) is allocated when not given.  They share no
+    memory with each other, the logits or the scores.
     """
     name = "beam_select"
     if scores.dim() != 2 or scores.dtype is not torch.float32:
@@ -72,18 +94,25 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | No
     if m < 1:
         raise ValueError(f"{name}: candidates must be positive")
     _lib.require_same_device(logits, scores, *(out or ()), workspace, name=name)
+    given = ()
     if out is None:
         out = (scores.new_empty((prompts, m)), scores.new_empty((prompts, m), dtype=torch.int64),
                scores.new_empty((prompts, m), dtype=torch.int64))
     else:
         out = tuple(out)
-        if len(out) != 3 or _lib.overlap(out[1], out[2]) or any(_lib.overlap(out[0], t) for t in out[1:]):
-            raise ValueError(f"{name}: out must be three tensors apart from each other")
+        if len(out) != 3:
+            raise ValueError(f"{name}: out must be three tensors")
         for t, want in zip(out, (torch.float32, torch.int64, torch.int64)):
             if tuple(t.shape) != (prompts, m) or t.dtype is not want or not t.is_contiguous():
                 raise ValueError(f"{name}: out must be contiguous fp32, int64, int64 [prompts, candidates]")
+        given = out
     rows, n = logits.shape
     need = _workspace(rows, n, m)
+    if given or workspace is not None:
+        written = [_range(t) for t in given]
+        if workspace is not None:
+            written.append(_range(workspace, need))
+        _clear(name, written, (_range(logits), _range(scores)))
     workspace = _scratch(workspace, need, logits, name)
     with _lib.on_device(logits):
         _lib.call("rwkv7mi_beam_select", logits.data_ptr(), prompts, beams, n, logits.stride(0), dt,
@@ -249,7 +278,8 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, leng
 
     A done prompt keeps its state; its next tokens are ``pad_token_id`` (one that the
     model takes, where they are fed to it), its rows their own. No host synchronisation; capturable.  ``next_tokens``, ``rows`` and ``workspace``
-    (:func:`beam_workspace_bytes`) are allocated when not given.
+    (:func:`beam_workspace_bytes`) are allocated when not given; they share no memory with each
+    other, the logits or a state.
     """
     name = "beam_step"
     prompts, beams, room = state._shape
@@ -279,14 +309,17 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, leng
     for t in (next_tokens, rows):
         if t is not None and (t.dtype is not torch.int64 or t.numel() != total or not t.is_contiguous()):
             raise ValueError(f"{name}: next_tokens and rows must be contiguous int64 tensors of one entry per row")
-    if next_tokens is not None and rows is not None and total and _lib.overlap(next_tokens, rows):
-        raise ValueError(f"{name}: next_tokens and rows overlap")
+    n = logits.shape[1]
+    need = _workspace(total, n, m)
+    written = [_range(t) for t in (next_tokens, rows) if t is not None]
+    if workspace is not None:
+        written.append(_range(workspace, need))
+    if written:
+        _clear(name, written, (_range(logits),), (state._ends,) if to is state else (state._ends, to._ends))
     if next_tokens is None:
         next_tokens = state.tokens.new_empty(total)
     if rows is None:
         rows = state.tokens.new_empty(total)
-    n = logits.shape[1]
-    need = _workspace(total, n, m)
     workspace = _scratch(workspace, need, logits, name)
     with _lib.on_device(logits):
         _lib.call("rwkv7mi_beam_step", logits.data_ptr(), prompts, beams, n, logits.stride(0), dt, 1 if normalized else 0,

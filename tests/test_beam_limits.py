@@ -191,3 +191,53 @@ def test_a_state_is_copied_and_pickled():
         assert all(torch.equal(getattr(other, k), getattr(s, k)) for k in KEYS)
         other.tokens.zero_()
         assert s.tokens.any()
+
+
+def test_beam_select_refuses_outputs_among_what_it_reads(calls):
+    import rwkv7mi as mi
+
+    s = torch.zeros(2, 3)
+    tok, row = (torch.zeros(2, 6, dtype=torch.int64) for _ in range(2))
+    need = mi.beam.beam_workspace_bytes(6, 50, 6)
+    big = torch.zeros(1 << 16)
+    x = big[:300].view(6, 50)
+    bytes_ = big.view(torch.uint8)
+    for args, kw in (((x, big[400:406].view(2, 3)), dict(out=(big[400:412].view(2, 6), tok, row))),  # the scores
+                     ((x, s), dict(out=(big[290:302].view(2, 6), tok, row))),                        # the logits
+                     ((x, s), dict(workspace=bytes_[:need])),
+                     ((x, big[402:408].view(2, 3)), dict(workspace=bytes_[1600:])),
+                     ((x, s), dict(out=(big[500:512].view(2, 6), tok, row), workspace=bytes_[2000:])),
+                     ((x, s), dict(out=(big[500:512].view(2, 6), *torch.zeros(1, 24, dtype=torch.int64).expand(2, 24).reshape(-1)
+                                        .as_strided((2, 2, 6), (6, 6, 1)).unbind(0))))):
+        with pytest.raises(ValueError, match="overlap"):
+            mi.beam_select(*args, **kw)
+    assert not calls
+    mi.beam_select(x, s, out=(big[500:512].view(2, 6), tok, row), workspace=bytes_[2048:])
+    mi.beam_select(x[:0], s[:0], out=(big[:0].view(0, 6), tok[:0], row[:0]))
+    assert len(calls) == 2
+
+
+def test_beam_step_refuses_buffers_among_its_state(calls):
+    import rwkv7mi as mi
+
+    x, s, o = torch.zeros(6, 50), _state(mi), _state(mi)
+    need = mi.beam.beam_workspace_bytes(6, 50, 3)
+    room = torch.zeros(need + 4096, dtype=torch.int64)
+    for kw in (dict(next_tokens=s.tokens.view(-1)[:6]), dict(rows=s.tokens.view(-1)[5:11]),
+               dict(rows=s.finished_tokens.view(-1)[-6:]), dict(out=o, next_tokens=o.tokens.view(-1)[:6]),
+               dict(workspace=room.view(torch.uint8), rows=room[:6]), dict(workspace=room.view(torch.uint8), next_tokens=room[9:15]),
+               dict(next_tokens=room[:6], rows=room[5:11])):
+        with pytest.raises(ValueError, match="overlap"):
+            mi.beam_step(x, s, **kw)
+    shared = torch.zeros(1 << 16, dtype=torch.uint8)
+    parts = dict(scores=shared[64:88].view(torch.float32).view(2, 3))
+    in_shared = mi.BeamState(**{**{k: getattr(_state(mi), k) for k in KEYS}, **parts})
+    for args, kw in (((x, in_shared), dict(workspace=shared)),
+                     ((shared[:1200].view(torch.float32).view(6, 50), s), dict(workspace=shared)),
+                     ((shared[:1200].view(torch.float32).view(6, 50), s), dict(rows=shared[800:848].view(torch.int64)))):
+        with pytest.raises(ValueError, match="overlap"):
+            mi.beam_step(*args, **kw)
+    assert not calls
+    mi.beam_step(x, s, out=o, workspace=room.view(torch.uint8)[128:], rows=room[:6], next_tokens=room[6:12])
+    mi.beam_step(x, in_shared, workspace=shared[88:], rows=shared[:48].view(torch.int64))
+    assert len(calls) == 2
