@@ -196,14 +196,20 @@ class BeamState:
     @classmethod
     def start(cls, input_ids: torch.Tensor, beams: int, room: int, *, lengths=None) -> "BeamState":
         """The state behind the prompts ``input_ids [prompts, T]`` (the first ``lengths``
-        tokens of each, default all), with one live beam each and rows of ``room`` tokens."""
+        tokens of each, default all; read on the host), with one live beam each and rows of ``room``
+        tokens."""
         if input_ids.dim() != 2 or input_ids.shape[1] > room or beams < 1:
             raise ValueError("BeamState.start: input_ids must be [prompts, T] with T <= room, beams positive")
         dev, (p, t) = input_ids.device, input_ids.shape
         tokens = torch.zeros(p, beams, room, dtype=torch.int64, device=dev)
         tokens[:, :, :t] = input_ids[:, None]
-        n = torch.full((p,), t, dtype=torch.int32, device=dev) if lengths is None else \
-            torch.as_tensor(lengths, dtype=torch.int32, device=dev).clone()
+        if lengths is None:
+            n = torch.full((p,), t, dtype=torch.int32, device=dev)
+        else:
+            held = torch.as_tensor(lengths).tolist()
+            if not isinstance(held, list) or len(held) != p or not all(isinstance(v, int) and 0 <= v <= t for v in held):
+                raise ValueError(f"BeamState.start: lengths must be {p} numbers of 0..{t}")
+            n = torch.tensor(held, dtype=torch.int32, device=dev)
         scores = torch.full((p, beams), -math.inf, device=dev)
         scores[:, 0] = 0.0
         return cls(tokens=tokens, lengths=n.repeat_interleave(beams), scores=scores,

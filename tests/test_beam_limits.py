@@ -241,3 +241,15 @@ def test_beam_step_refuses_buffers_among_its_state(calls):
     mi.beam_step(x, s, out=o, workspace=room.view(torch.uint8)[128:], rows=room[:6], next_tokens=room[6:12])
     mi.beam_step(x, in_shared, workspace=shared[88:], rows=shared[:48].view(torch.int64))
     assert len(calls) == 2
+
+
+def test_lengths_lie_within_the_ids():
+    import rwkv7mi as mi
+
+    ids = torch.zeros(2, 4, dtype=torch.int64)
+    for bad in ([5, 2], [2, 9], [50, 1], [-1, 2], torch.tensor([2, 5]), np.array([2, -3]), [2], [1, 2, 3], 2, [[1, 2]], [1 << 33, 1]):
+        with pytest.raises((ValueError, OverflowError)):
+            mi.BeamState.start(ids, 3, 9, lengths=bad)
+    for good in ([4, 0], torch.tensor([1, 4], dtype=torch.int32), np.array([2, 3])):
+        s = mi.BeamState.start(ids, 3, 9, lengths=good)
+        assert s.prompt_lengths.tolist() == [int(n) for n in good] and s.lengths.tolist() == [int(n) for n in good for _ in range(3)]
