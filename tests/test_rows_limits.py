@@ -1,0 +1,44 @@
+"""Moved rows and the caches that use them at their limits, on the CPU: tensors of other kinds, layouts and lifetimes."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The library calls, recorded instead of run."""
+    from rwkv7mi import _lib
+
+    made = []
+    monkeypatch.setattr(_lib, "require_same_device", lambda *t, name: None)
+    monkeypatch.setattr(_lib, "stream_of", lambda t: 0)
+    monkeypatch.setattr(_lib, "on_device", lambda t: _lib._HERE)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: made.append((name, args)))
+    return made
+
+
+def _config(layers=2):
+    from rwkv7mi.model import NativeRWKV7Config
+
+    return NativeRWKV7Config(vocab_size=64, hidden_size=128, num_hidden_layers=layers, intermediate_size=256,
+                             decay_low_rank_dim=32, a_low_rank_dim=32, gate_low_rank_dim=64, v_low_rank_dim=32)
+
+
+@pytest.mark.parametrize("state", [torch.float32, torch.float16])
+def test_cache_edits_of_fake_tensors_give_shapes(calls, state):
+    """A GPU cache under a fake mode: its tensors have no memory that a kernel could read."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from rwkv7mi.model import NativeRWKV7Cache
+
+    with FakeTensorMode():
+        c = NativeRWKV7Cache.zeros(_config(), 3, "cuda", state_dtype=state)
+        c.batch_repeat_interleave(2)
+        assert c.get_batch_size() == 6 and all(t.shape[0] == 6 for t in c._all_tensors())
+        d = c.select_batch([4, 0], inplace=False)
+        assert d.get_batch_size() == 2 and c.get_batch_size() == 6
+        c.reorder_cache(torch.tensor([5, 5, 1, 0], device="cuda"))
+        assert [t.shape[0] for t in c._all_tensors()] == [4] * len(c._all_tensors())
+        assert c._state[1].shape == (4, 2, 64, 64) and c._state[1].dtype is state
+    assert not calls
