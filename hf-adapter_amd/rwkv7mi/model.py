@@ -737,11 +737,12 @@ class NativeRWKV7Cache(_HFCache):
 
     def _take_rows(self, index) -> None:
         """New tensors of the rows ``index`` (a list of integers or a tensor): on the GPU in one
-        launch, the layers in one allocation again; by torch's indexing elsewhere, and where a tensor
-        is of another class (a fake one has no memory to read)."""
+        launch, the layers in one allocation again; by torch's indexing elsewhere, where a gradient is
+        wanted, and where a tensor is of another class (a fake one has no memory to read)."""
         ts = self._all_tensors()
         where = ts[0].get_device() if ts else -1
-        if where < 0 or not all(type(t) is torch.Tensor and t.get_device() == where for t in ts):
+        if (where < 0 or not all(type(t) is torch.Tensor and t.get_device() == where for t in ts)
+                or (torch.is_grad_enabled() and any(t.requires_grad for t in ts))):
             idx = torch.as_tensor(index, dtype=torch.long)
             self._map(lambda t: t.index_select(0, idx.to(t.device)))
             return

@@ -42,3 +42,24 @@ def test_cache_edits_of_fake_tensors_give_shapes(calls, state):
         assert [t.shape[0] for t in c._all_tensors()] == [4] * len(c._all_tensors())
         assert c._state[1].shape == (4, 2, 64, 64) and c._state[1].dtype is state
     assert not calls
+
+
+def test_cache_edits_keep_the_graph(calls, monkeypatch):
+    """Cache tensors that require grad: selection and repeat are differentiable (CPU tensors in the place of GPU
+    ones); without grad mode they are moved."""
+    from rwkv7mi.model import NativeRWKV7Cache
+
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    c = NativeRWKV7Cache.zeros(_config(), 3, "cpu")
+    c._map(lambda t: t.float().requires_grad_())
+    leaves = c._all_tensors()
+    c.batch_repeat_interleave(2)
+    c.select_batch([0, 0, 5, 2])
+    sum((t * (i + 1)).sum() for i, t in enumerate(c._all_tensors())).backward()
+    for i, t in enumerate(leaves):
+        want = torch.tensor([2.0, 1.0, 1.0]) * (i + 1)  # rows 0, 0, 2, 1 of the three
+        assert torch.equal(t.grad, want.view(3, *[1] * (t.dim() - 1)).expand_as(t))
+    assert not calls
+    with torch.no_grad():
+        c.select_batch([1, 0])
+    assert calls and not any(t.requires_grad for t in c._all_tensors())
