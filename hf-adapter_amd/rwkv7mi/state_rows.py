@@ -122,9 +122,20 @@ def _on_gpu(tensors, index, name):
     _lib.require_same_device(*tensors, *((index,) if isinstance(index, torch.Tensor) else ()), name=name)
 
 
+def _no_gradient(tensors, name):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{name}: no gradient flows through moved rows (a tensor requires grad)")
+
+
+_changed = torch.autograd.graph.increment_version  # (tells autograd that the tensors are written)
+
+
 def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tensor]:
     """``[t.index_select(dim, indices) for t in tensors]`` in one launch (24 tensors a
-    launch): the rows along ``dim`` of tensors that have as many.
+    launch): the rows along ``dim`` of tensors that have as many.  No gradient flows through:
+    in grad mode tensors that require grad are refused.
 
     ``indices``: integers (checked) or a one-dimensional integer tensor; -1, and on the
     GPU any index out of range, gives a row of zeros.  ``out``: tensors to write instead of
@@ -135,6 +146,7 @@ def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tenso
     tensors = list(tensors)
     idx = _index(indices, name)
     _on_gpu(tensors, idx, name)
+    _no_gradient(tensors, name)
     if dim < 0:
         raise ValueError(f"{name}: dim counts from the front")
     n = len(idx) if type(idx) is list else idx.shape[0]
@@ -165,6 +177,7 @@ def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tenso
             if tuple(o.shape) != want or o.dtype != t.dtype:
                 raise ValueError(f"{name}: an output is {tuple(o.shape)} {o.dtype}, not {want} {t.dtype}")
         _on_gpu([tensors[0], *out], None, name)
+        _no_gradient(out, name)
         dst = [_family(o, dim, name) for o in out]
         if any(f is None or not _apart(f) for f in dst):
             raise ValueError(f"{name}: the rows of an output are dense and apart")
@@ -172,6 +185,8 @@ def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tenso
             raise ValueError(f"{name}: outputs overlap")
         for f, g in zip(src, dst):
             flat += (f[0], g[0], f[1], f[2], g[1], g[2], f[3], f[4])
+        if n:
+            _changed(out)
     if n:
         _launch(flat, rows, n, n, idx, None, True, tensors[0])
     return out
@@ -186,12 +201,14 @@ def move_rows_(tensors, sources, destinations=None, *, dim: int = 0) -> None:
     indices out of range make zeros too.  ``destinations``: distinct integers, known to the
     host; default every row.  Up to 2048 rows may trade places; more where no source is
     another row's destination.  The tensors' rows are dense, and their memory neither
-    overlaps nor interleaves.  Capturable where host indices are at most 192.
+    overlaps nor interleaves.  Capturable where host indices are at most 192.  No gradient flows
+    through: in grad mode tensors that require grad are refused, others count as changed.
     """
     name = "move_rows_"
     tensors = list(tensors)
     src = _index(sources, name)
     _on_gpu(tensors, src, name)
+    _no_gradient(tensors, name)
     if dim < 0:
         raise ValueError(f"{name}: dim counts from the front")
     fams = [_family(t, dim, name) for t in tensors]
@@ -227,6 +244,7 @@ def move_rows_(tensors, sources, destinations=None, *, dim: int = 0) -> None:
     for f in fams:
         flat += (f[0], f[0], f[1], f[2], f[1], f[2], f[3], f[4])
     if n:
+        _changed(tensors)
         _launch(flat, rows, rows, n, src, dst, disjoint, tensors[0])
 
 

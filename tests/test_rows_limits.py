@@ -63,3 +63,37 @@ def test_cache_edits_keep_the_graph(calls, monkeypatch):
     with torch.no_grad():
         c.select_batch([1, 0])
     assert calls and not any(t.requires_grad for t in c._all_tensors())
+
+
+def test_moved_rows_have_no_gradient_and_say_so(calls):
+    import rwkv7mi as mi
+
+    t, u = torch.zeros(3, 4), torch.zeros(3, 5, requires_grad=True)
+    for f in (lambda: mi.select_rows([t, u], [0, 1]), lambda: mi.move_rows_([t, u * 2], [1, 0, 2]),
+              lambda: mi.select_rows([t], [0], out=[torch.zeros(1, 4, requires_grad=True)])):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            f()
+    assert not calls
+    with torch.no_grad():
+        assert not mi.select_rows([t, u], [0, 1])[1].requires_grad
+        mi.move_rows_([t, u], [1, 0, 2])
+    assert len(calls) == 2
+
+
+def test_rows_moved_in_place_are_a_change_to_autograd(calls):
+    """A tensor that a backward pass saved and whose rows then move: an error, as for torch's own in-place operations."""
+    import rwkv7mi as mi
+
+    x, w, aside = torch.ones(3, 4), torch.ones(3, 4, requires_grad=True), torch.ones(2, 3)
+    y = (w * x).sum()
+    mi.move_rows_([x], [1, 0, 2])
+    assert x._version == 1 and aside._version == 0
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    out = torch.empty(2, 4)
+    mi.select_rows([x], [1, 0], out=[out])
+    assert out._version == 1 and x._version == 1
+    mi.move_rows_([x], [], [])
+    with torch.inference_mode():
+        mi.move_rows_([torch.zeros(3, 4)], [1, 0, 2])
+    assert len(calls) == 3
