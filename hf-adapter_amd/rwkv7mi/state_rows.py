@@ -152,6 +152,8 @@ def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tenso
     n = len(idx) if type(idx) is list else idx.shape[0]
     src = []
     for i, t in enumerate(tensors):
+        if t.is_neg() or t.is_conj():  # (its bytes are not its values)
+            tensors[i] = t = t.resolve_conj().resolve_neg()
         f = _family(t, dim, name)
         if f is None:
             tensors[i] = t = t.contiguous()
@@ -178,6 +180,8 @@ def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tenso
                 raise ValueError(f"{name}: an output is {tuple(o.shape)} {o.dtype}, not {want} {t.dtype}")
         _on_gpu([tensors[0], *out], None, name)
         _no_gradient(out, name)
+        if any(o.is_neg() or o.is_conj() for o in out):
+            raise ValueError(f"{name}: an output is a conjugate or negative view")
         dst = [_family(o, dim, name) for o in out]
         if any(f is None or not _apart(f) for f in dst):
             raise ValueError(f"{name}: the rows of an output are dense and apart")

@@ -97,3 +97,21 @@ def test_rows_moved_in_place_are_a_change_to_autograd(calls):
     with torch.inference_mode():
         mi.move_rows_([torch.zeros(3, 4)], [1, 0, 2])
     assert len(calls) == 3
+
+
+def test_conjugate_and_negative_views_are_selected_by_value(calls):
+    """The bytes of such a view are not its values: they are taken from a plain copy, and written nowhere."""
+    import rwkv7mi as mi
+
+    x = torch.randn(4, 3, dtype=torch.complex64)
+    for view in (x.conj(), x.conj().imag):
+        assert view.is_conj() or view.is_neg()
+        (out,) = mi.select_rows([view], [1, 0])
+        assert not out.is_conj() and not out.is_neg()
+        address, end = calls[-1][1][1][0], view.data_ptr() + view.untyped_storage().nbytes()
+        assert not view.data_ptr() <= address < end  # (not the view's own memory)
+        with pytest.raises(ValueError, match="conjugate"):
+            mi.select_rows([view.clone()], [1, 0], out=[view[:2]])
+    y = x.conj()
+    mi.move_rows_([y], [1, 0, 2, 3])  # (rows of one view: its bytes trade places as its values do)
+    assert list(calls[-1][1][1][:2]) == [x.data_ptr()] * 2
