@@ -53,7 +53,7 @@ def _apart(f) -> bool:
         if k > 1:
             if s < size:
                 return False
-            size = s * k
+            size += s * (k - 1)
     return True
 
 

@@ -1,0 +1,52 @@
+"""Moved rows at their limits, on the GPU: layouts, indices out of range, empty tensors, gradients."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_beam_model import _cache, _model
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.uint8])
+def test_rows_apart_move_in_place(dtype):
+    import rwkv7mi as mi
+
+    g = torch.Generator("cuda").manual_seed(2)
+    for rows, width in ((5, 12), (7, 33), (9, 4096)):
+        base = torch.randint(0, 99, (3, rows, width), device="cuda", generator=g).to(dtype)
+        view, keep = base[:, ::2], base.clone()
+        n = view.shape[1]
+        idx = list(range(1, n)) + [-1]
+        for index in (idx, torch.tensor(idx, device="cuda")):
+            base.copy_(keep)
+            mi.move_rows_([view], index, dim=1)
+            assert torch.equal(view[:, :-1], keep[:, 2::2]) and not view[:, -1].any()
+            assert torch.equal(base[:, 1::2], keep[:, 1::2])
+
+
+def test_conjugate_and_negative_views():
+    import rwkv7mi as mi
+
+    x = torch.randn(4, 3, dtype=torch.complex64, device="cuda")
+    for view in (x.conj(), x.conj().imag):
+        (got,) = mi.select_rows([view], [2, -1, 0])
+        assert torch.equal(got[[0, 2]], view[[2, 0]]) and not got[1].any()
+    y = x.clone().conj()
+    want = y[[3, 0, 1, 2]].clone()
+    mi.move_rows_([y], [3, 0, 1, 2])
+    assert torch.equal(y, want)
+
+
+def test_cache_edits_are_differentiable():
+    model = _model()
+    c = _cache(model, 3)
+    c._map(lambda t: t.float().requires_grad_())
+    leaves = c._all_tensors()
+    c.batch_repeat_interleave(2)
+    c.reorder_cache(torch.tensor([0, 0, 5, 2], device="cuda"))
+    sum(t.sum() for t in c._all_tensors()).backward()
+    for t in leaves:
+        want = torch.tensor([2.0, 1.0, 1.0], device="cuda").view(3, *[1] * (t.dim() - 1)).expand_as(t)
+        assert torch.equal(t.grad, want)

@@ -115,3 +115,25 @@ def test_conjugate_and_negative_views_are_selected_by_value(calls):
     y = x.conj()
     mi.move_rows_([y], [1, 0, 2, 3])  # (rows of one view: its bytes trade places as its values do)
     assert list(calls[-1][1][1][:2]) == [x.data_ptr()] * 2
+
+
+def test_rows_apart_are_moved_whatever_follows_them(calls):
+    """Every other row of an odd number: the last one ends before the next part begins."""
+    import rwkv7mi as mi
+
+    for rows in range(1, 8):
+        for step in (1, 2, 3):
+            base = torch.zeros(3, rows, 4)
+            view = base[:, ::step]
+            mi.move_rows_([view], list(range(view.shape[1] - 1, -1, -1)), dim=1)
+            mi.select_rows([base], [0] * view.shape[1], dim=1, out=[view.clone()])
+    # rows outermost in memory, parts of them in use
+    view = torch.zeros(5, 7, 4).transpose(0, 1)[::3, ::2]
+    mi.move_rows_([view], [2, 1, 0], dim=1)
+    done = len(calls)
+    for bad in (torch.zeros(30).as_strided((3, 3, 4), (8, 4, 1)),      # a part's last row is the next one's first
+                torch.zeros(30).as_strided((3, 3, 4), (7, 4, 1)), torch.zeros(30).as_strided((3, 2, 4), (4, 4, 1)),
+                torch.zeros(40).as_strided((3, 3, 4), (12, 3, 1))):
+        with pytest.raises(ValueError, match="apart"):
+            mi.move_rows_([bad], [0] * bad.shape[1], dim=1)
+    assert len(calls) == done
