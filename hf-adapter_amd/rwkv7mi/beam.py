@@ -114,9 +114,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | No
             written.append(_range(workspace, need))
         _clear(name, written, (_range(logits), _range(scores)))
     workspace = _scratch(workspace, need, logits, name)
+    scores = scores.contiguous()  # (a copy lives until the launch)
     with _lib.on_device(logits):
         _lib.call("rwkv7mi_beam_select", logits.data_ptr(), prompts, beams, n, logits.stride(0), dt,
-                  scores.contiguous().data_ptr(), 1 if normalized else 0, m, out[0].data_ptr(), out[1].data_ptr(),
+                  scores.data_ptr(), 1 if normalized else 0, m, out[0].data_ptr(), out[1].data_ptr(),
                   out[2].data_ptr(), workspace.data_ptr(), need, _lib.stream_of(logits))
     return out
 

@@ -253,3 +253,23 @@ def test_lengths_lie_within_the_ids():
     for good in ([4, 0], torch.tensor([1, 4], dtype=torch.int32), np.array([2, 3])):
         s = mi.BeamState.start(ids, 3, 9, lengths=good)
         assert s.prompt_lengths.tolist() == [int(n) for n in good] and s.lengths.tolist() == [int(n) for n in good for _ in range(3)]
+
+
+def test_scores_made_contiguous_live_until_the_launch(monkeypatch, calls):
+    import weakref
+
+    import rwkv7mi as mi
+    from rwkv7mi import _lib
+
+    made, alive = [], []
+    plain = torch.Tensor.contiguous
+
+    def contiguous(t, *args, **kw):
+        out = plain(t, *args, **kw)
+        made.append((weakref.ref(out), out.data_ptr()))
+        return out
+
+    monkeypatch.setattr(torch.Tensor, "contiguous", contiguous)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: alive.extend(r() is not None for r, at in made if at in args))
+    mi.beam_select(torch.zeros(6, 50), torch.zeros(3, 2).t())
+    assert alive == [True]
