@@ -704,7 +704,9 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
       lse[k] = l;
       odd[k] = nan;
       score[k] = nan ? -__builtin_inff() : own;  // (nothing to choose by value)
-      offset[k] = nan ? -__builtin_inff() : (float)((double)own - l);
+      // (finite where own is: what it is cut off by is covered by the allowance in gather, or that is infinite)
+      offset[k] = nan || own == -__builtin_inff() ? -__builtin_inff()
+                                                  : fminf(fmaxf((float)((double)own - l), -__FLT_MAX__), __FLT_MAX__);
     }
   }
   __syncthreads();
@@ -734,8 +736,9 @@ __global__ __launch_bounds__(BM_MERGE) void beam_merge_kernel(const BmArgs A, co
   float reach = bm_value(at_least);
   const auto gather = [&](uint64_t c) {  // whether it reaches the bound
     const float l = bm_value((uint32_t)(c >> 32)), o = offset[c >> 23 & 0x7f];
-    // (fp32, less than four roundings off; false for -inf and what is not there)
-    if (!(l + o + 0x1p-21f * (fabsf(l) + fabsf(o)) >= reach) || (uint32_t)(c >> 32) <= BM_NONE) return false;
+    // (fp32, less than four roundings off, and no bound where it is not finite; false for -inf and what is not there)
+    if (l + o + 0x1p-21f * (fabsf(l) + fabsf(o)) < reach || o == -__builtin_inff() || (uint32_t)(c >> 32) <= BM_NONE)
+      return false;
     const double v = value(c);
     if (bm_key((float)v) < at_least) return false;
     const int p = atomicAdd(&count, 1);
