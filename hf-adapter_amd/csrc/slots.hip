@@ -197,7 +197,7 @@ extern "C" int rwkv7mi_rows_move(int n, const rwkv7mi_rows* tensors, int64_t src
     const rwkv7mi_rows& t = tensors[i];
     if (t.row_bytes < 0 || t.outer < 0) return fail(RWKV7MI_EINVAL, w + ": bad shape");
     if (nrows == 0 || t.row_bytes == 0 || t.outer == 0) continue;
-    if (!t.src || !t.dst) return fail(RWKV7MI_EINVAL, w + ": null pointer");
+    if ((!t.src && src_rows) || !t.dst) return fail(RWKV7MI_EINVAL, w + ": null pointer");
     RwTensor& q = a.t[a.n++];
     q.src = static_cast<const char*>(t.src);
     q.dst = static_cast<char*>(t.dst);

@@ -666,9 +666,10 @@ int rwkv7mi_slot_copy(const void* src, int64_t src_layer_stride,
  * the launch) or are r where both are NULL.  s(r) outside 0 .. src_rows - 1
  * (say -1) writes zeros, d(r) outside 0 .. dst_rows - 1 nothing.  The
  * destinations are distinct.  A tensor with src == dst is moved in place (a row
- * onto itself is left alone); otherwise its src and dst do not overlap.  Rows
+ * onto itself is left alone); otherwise its src and dst do not overlap (src may
+ * be NULL where src_rows is 0).  No device index lies in what is written.  Rows
  * that trade places in place: at most 2048; `disjoint` says that no source is
- * another row's destination, which lifts that. */
+ * another row's destination, which lifts that.  At most 4194240 rows a call. */
 typedef struct {
   const void* src;
   void* dst;

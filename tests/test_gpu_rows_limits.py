@@ -50,3 +50,14 @@ def test_cache_edits_are_differentiable():
     for t in leaves:
         want = torch.tensor([2.0, 1.0, 1.0], device="cuda").view(3, *[1] * (t.dim() - 1)).expand_as(t)
         assert torch.equal(t.grad, want)
+
+
+def test_rows_of_empty_tensors_are_zeros():
+    """A tensor without rows has no memory: every index is out of range."""
+    import rwkv7mi as mi
+
+    e, full = torch.empty(3, 0, 5, device="cuda"), torch.empty(2, 0, 40, device="cuda", dtype=torch.half)
+    for index in ([-1, -1], torch.tensor([-1, 3], device="cuda")):
+        got = mi.select_rows([e, full], index, dim=1)
+        assert [t.shape for t in got] == [(3, 2, 5), (2, 2, 40)] and not any(t.any() for t in got)
+    mi.move_rows_([e, full], [], dim=1)
