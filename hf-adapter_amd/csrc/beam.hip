@@ -50,6 +50,7 @@ constexpr int BM_WAVE_RUNS = 128; // runs of them that a wave gathers
 constexpr int BM_RANKED = 320;    // of them ranked without a second bound
 constexpr int BM_MOST = 128;      // candidates of a prompt
 constexpr int BM_ENDS = 8;        // end tokens
+constexpr int64_t BM_ROOM = 1 << 30;  // tokens of room (a copy's offsets, in steps of 512, are 32 bits wide)
 
 struct BmState {
   int64_t* tokens;
@@ -1002,8 +1003,8 @@ extern "C" int rwkv7mi_beam_step(const void* x, int64_t prompts, int64_t beams, 
   const std::string w("beam_step");
   if (n_ends < 0 || n_ends > BM_ENDS || (n_ends && !ends)) return fail(RWKV7MI_EINVAL, w + ": at most 8 end tokens");
   if (int rc = bm_check(w, x, prompts, beams, V, ldx, dtype, beams > BM_MOST ? beams : (1 + n_ends) * beams)) return rc;
-  if (early_stopping < 0 || early_stopping > 2 || room <= 0 || room > INT32_MAX - 1)
-    return fail(RWKV7MI_EINVAL, w + ": bad early_stopping or room");
+  if (early_stopping < 0 || early_stopping > 2 || room <= 0 || room > BM_ROOM)
+    return fail(RWKV7MI_EINVAL, w + ": bad early_stopping, or a room outside 1 .. 2^30");
   if (!(length_penalty == length_penalty)) return fail(RWKV7MI_EINVAL, w + ": length_penalty is NaN");
   if (prompts == 0) return RWKV7MI_OK;
   if (!x || !next || !rows || !in || !out) return fail(RWKV7MI_EINVAL, w + ": null pointer");

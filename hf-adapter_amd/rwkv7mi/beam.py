@@ -140,7 +140,7 @@ class BeamState:
     GPU: contiguous tensors, checked once and not replaced afterwards (a step refuses a state
     whose tensors were given other memory).
 
-    ``tokens`` int64 ``[prompts, beams, room]`` and ``lengths`` int32 ``[prompts * beams]``
+    ``tokens`` int64 ``[prompts, beams, room]`` (room at most 2^30) and ``lengths`` int32 ``[prompts * beams]``
     (the beams of a prompt are equally long): the texts, prompt included (also a history
     that :func:`~.sampling.process_logits` takes); ``scores`` fp32 ``[prompts, beams]`` their
     log-probabilities; ``prompt_lengths`` int32 ``[prompts]``; ``finished_tokens``,

@@ -699,7 +699,7 @@ int rwkv7mi_beam_select(const void* x, int64_t prompts, int64_t beams, int64_t V
                         int64_t* out_tokens, int64_t* out_rows, void* workspace,
                         size_t workspace_bytes, void* stream);
 
-/* A beam search's state: `room` tokens a row. */
+/* A beam search's state: `room` tokens a row, at most 2^30. */
 typedef struct {
   int64_t* tokens;          /* [prompts, beams, room] the texts               */
   int32_t* lengths;         /* [prompts * beams] tokens of each, one a prompt */

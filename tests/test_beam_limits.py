@@ -273,3 +273,18 @@ def test_scores_made_contiguous_live_until_the_launch(monkeypatch, calls):
     monkeypatch.setattr(_lib, "call", lambda name, *args: alive.extend(r() is not None for r, at in made if at in args))
     mi.beam_select(torch.zeros(6, 50), torch.zeros(3, 2).t())
     assert alive == [True]
+
+
+@pytest.mark.parametrize("room", [(1 << 30) + 1, 2 ** 31 - 512, 2 ** 31 - 2])
+def test_rooms_that_pass_32_bits_are_refused(room):
+    """(the lanes' offsets into a text, steps of 512 tokens, are 32 bits wide)"""
+    import ctypes
+
+    from rwkv7mi import _lib
+
+    state = (ctypes.c_void_p * 8)(*[(1 << 20) + 4096 * i for i in range(8)])
+    other = (ctypes.c_void_p * 8)(*[(1 << 21) + 4096 * i for i in range(8)])
+    at = 1 << 22
+    assert _lib.load().rwkv7mi_beam_step(at, 2, 3, 100, 100, 1, 0, None, 0, 1.0, 0, 0, state, other, room, at, at, at, 1 << 20,
+                                         None) == -1
+    assert b"room" in _lib.load().rwkv7mi_last_error()
