@@ -41,8 +41,9 @@ __global__ __launch_bounds__(256) void slot_copy_kernel(const SlotCopy C) {
 // Rows of several tensors moved by one index in one launch:
 //   dst[o][d(r)] = the old src[o][s(r)]   for every outer index o and every r,
 // as if all sources were read before any destination is written, so rows may
-// trade places in place; s(r) out of range (-1) writes zeros, d(r) out of range
-// nothing, and a row onto itself is left alone.
+// trade places in place; s(r) out of range (-1) writes zeros (or bytes of 0xff:
+// NaN in fp16, bf16 and fp32), d(r) out of range nothing, and a row onto itself is
+// left alone.
 //
 // A workgroup takes a window of the row's bytes of one tensor and outer index
 // for all rows: it gathers the rows that move into a list, loads all their
@@ -83,6 +84,7 @@ struct RwArgs {
   int64_t src_rows, dst_rows;
   const int64_t *src_index, *dst_index;  // on the device (null: the list, or the identity)
   int listed_src, listed_dst;
+  uint32_t fill;  // what a source out of range writes
   int src_list[RW_LIST], dst_list[RW_LIST];
 };
 
@@ -93,17 +95,24 @@ __device__ __forceinline__ void rw_hold(V& v) {  // v is in its registers here
   else
     asm volatile("" : "+v"(v));
 }
+template <typename V>
+__device__ __forceinline__ V rw_filled(uint32_t f) {
+  if constexpr (sizeof(V) == 16)
+    return make_uint4(f, f, f, f);
+  else
+    return f;
+}
 
 template <int THREADS, int LOADS, typename V, typename HELD>
 __device__ __forceinline__ void rw_window(const RwTensor& t, int64_t o, uint32_t w0, int log_window, int n, const int* src,
-                                          const int* dst) {
+                                          const int* dst, uint32_t fill) {
   const int tid = threadIdx.x, mask = (1 << log_window) - 1;
   HELD r[LOADS];
 #pragma unroll
   for (int u = 0; u < LOADS; ++u) {
     const int j = tid + THREADS * u, k = j >> log_window;
     const uint32_t c = w0 + (uint32_t)(j & mask);
-    r[u] = HELD{};
+    r[u] = rw_filled<HELD>(fill);
     if (k < n && c < t.units && src[k] >= 0)
       r[u] = static_cast<HELD>(reinterpret_cast<const V*>(t.src + o * t.src_outer + src[k] * t.src_row)[c]);
   }
@@ -150,11 +159,11 @@ __global__ __launch_bounds__(THREADS) void rows_move_kernel(const RwArgs A) {
   const int n = moving;
   if (n == 0) return;
   if (t.unit == 16)
-    rw_window<THREADS, LOADS, uint4, uint4>(t, o, w << A.log_window, A.log_window, n, src, dst);
+    rw_window<THREADS, LOADS, uint4, uint4>(t, o, w << A.log_window, A.log_window, n, src, dst, A.fill);
   else if (t.unit == 4)
-    rw_window<THREADS, LOADS, uint32_t, uint32_t>(t, o, w << A.log_window, A.log_window, n, src, dst);
+    rw_window<THREADS, LOADS, uint32_t, uint32_t>(t, o, w << A.log_window, A.log_window, n, src, dst, A.fill);
   else
-    rw_window<THREADS, LOADS, uint8_t, uint32_t>(t, o, w << A.log_window, A.log_window, n, src, dst);
+    rw_window<THREADS, LOADS, uint8_t, uint32_t>(t, o, w << A.log_window, A.log_window, n, src, dst, A.fill);
 }
 
 }  // namespace rwkv7mi
@@ -183,7 +192,7 @@ extern "C" int rwkv7mi_slot_copy(const void* src, int64_t src_layer_stride, int6
 
 extern "C" int rwkv7mi_rows_move(int n, const rwkv7mi_rows* tensors, int64_t src_rows, int64_t dst_rows, int64_t nrows,
                                  const int64_t* src_index, const int64_t* dst_index, const int64_t* src_list,
-                                 const int64_t* dst_list, int disjoint, void* stream) {
+                                 const int64_t* dst_list, int flags, void* stream) {
   const std::string w("rows_move");
   if (n < 0 || n > RW_TENSORS || (n && !tensors)) return fail(RWKV7MI_EINVAL, w + ": at most 24 tensors");
   if (nrows < 0 || src_rows < 0 || dst_rows < 0 || src_rows > INT32_MAX || dst_rows > INT32_MAX)
@@ -191,7 +200,10 @@ extern "C" int rwkv7mi_rows_move(int n, const rwkv7mi_rows* tensors, int64_t src
   if ((src_list || dst_list) && nrows > RW_LIST) return fail(RWKV7MI_EINVAL, w + ": at most 192 indices in host lists");
   if ((src_list && src_index) || (dst_list && dst_index))
     return fail(RWKV7MI_EINVAL, w + ": a list and a device index of the same rows");
+  if (flags & ~3) return fail(RWKV7MI_EINVAL, w + ": unknown flags");
+  const bool disjoint = flags & RWKV7MI_ROWS_DISJOINT;
   RwArgs a{};
+  a.fill = flags & RWKV7MI_ROWS_POISON ? ~0u : 0u;
   bool same = false;
   for (int i = 0; i < n; ++i) {
     const rwkv7mi_rows& t = tensors[i];

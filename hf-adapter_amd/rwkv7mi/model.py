@@ -738,7 +738,8 @@ class NativeRWKV7Cache(_HFCache):
     def _take_rows(self, index) -> None:
         """New tensors of the rows ``index`` (a list of integers or a tensor): on the GPU in one
         launch, the layers in one allocation again; by torch's indexing elsewhere, where a gradient is
-        wanted, and where a tensor is of another class (a fake one has no memory to read)."""
+        wanted, and where a tensor is of another class (a fake one has no memory to read).  An index
+        out of range raises on the host; on the GPU, where nothing waits to look, its row is NaN."""
         ts = self._all_tensors()
         where = ts[0].get_device() if ts else -1
         if (where < 0 or not all(type(t) is torch.Tensor and t.get_device() == where for t in ts)
@@ -754,10 +755,10 @@ class NativeRWKV7Cache(_HFCache):
             raise IndexError("NativeRWKV7Cache: index out of range")
         stacked = self._stacked() if self._is_initialized() else None
         if stacked is None:
-            it = iter(select_rows(ts, index))
+            it = iter(select_rows(ts, index, poison=True))
             self._map(lambda t: next(it))
             return
-        new = select_rows(stacked, index, dim=1)
+        new = select_rows(stacked, index, dim=1, poison=True)
         self._state, self._xpa, self._xpf = (list(t.unbind(0)) for t in new[:3])
         self._v_first = new[3][0]
         self._elapsed = new[4][0] if self._elapsed is not None else None
@@ -2137,7 +2138,7 @@ class NativeGraphRunner(_OwnsGraph):
             for t in self.cache._all_tensors():
                 t.copy_(t.index_select(0, idx))
             return True
-        move_rows_(self._rows, idx, dim=1)
+        move_rows_(self._rows, idx, dim=1, poison=True)
         return True
 
     def replay(self, tokens: torch.Tensor, cache: NativeRWKV7Cache) -> torch.Tensor:

@@ -84,7 +84,7 @@ def _index(index, name: str):
     return [int(i) for i in index]
 
 
-def _launch(families, src_rows, dst_rows, n, src, dst, disjoint, where):
+def _launch(families, src_rows, dst_rows, n, src, dst, disjoint, poison, where):
     """``families``: 8 numbers a tensor, as the library's ``rwkv7mi_rows``."""
     src_at = dst_at = src_list = dst_list = None
     if type(src) is not list:
@@ -105,7 +105,7 @@ def _launch(families, src_rows, dst_rows, n, src, dst, disjoint, where):
         for i in range(0, len(families), 8 * MAX_TENSORS):
             part = families[i:i + 8 * MAX_TENSORS]
             _lib.call("rwkv7mi_rows_move", len(part) // 8, (ctypes.c_int64 * len(part))(*part), src_rows, dst_rows, n,
-                      src_at, dst_at, src_list, dst_list, 1 if disjoint else 0, stream)
+                      src_at, dst_at, src_list, dst_list, (1 if disjoint else 0) + (2 if poison else 0), stream)
 
 
 def _same_rows(families, name):
@@ -132,15 +132,16 @@ def _no_gradient(tensors, name):
 _changed = torch.autograd.graph.increment_version  # (tells autograd that the tensors are written)
 
 
-def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tensor]:
+def select_rows(tensors, indices, *, dim: int = 0, out=None, poison: bool = False) -> list[torch.Tensor]:
     """``[t.index_select(dim, indices) for t in tensors]`` in one launch (24 tensors a
     launch): the rows along ``dim`` of tensors that have as many.  No gradient flows through:
     in grad mode tensors that require grad are refused.
 
     ``indices``: integers (checked) or a one-dimensional integer tensor; -1, and on the
-    GPU any index out of range, gives a row of zeros.  ``out``: tensors to write instead of
-    new ones; they do not overlap ``tensors``.  Capturable where ``indices`` are on
-    the GPU or at most 192.
+    GPU any index out of range, gives a row of zeros; with ``poison`` one of bytes of 0xff, NaN
+    in fp16, bf16 and fp32.  ``out``: tensors to write instead of new ones, whose ranges of
+    memory do not meet those of ``tensors``.  At most 4194240 indices.  Capturable where
+    ``indices`` are on the GPU or at most 192.
     """
     name = "select_rows"
     tensors = list(tensors)
@@ -192,17 +193,18 @@ def select_rows(tensors, indices, *, dim: int = 0, out=None) -> list[torch.Tenso
         if n:
             _changed(out)
     if n:
-        _launch(flat, rows, n, n, idx, None, True, tensors[0])
+        _launch(flat, rows, n, n, idx, None, True, poison, tensors[0])
     return out
 
 
-def move_rows_(tensors, sources, destinations=None, *, dim: int = 0) -> None:
+def move_rows_(tensors, sources, destinations=None, *, dim: int = 0, poison: bool = False) -> None:
     """Row ``destinations[i]`` along ``dim`` of every tensor becomes what row
     ``sources[i]`` was before the call, in place and in one launch (24 tensors a launch);
-    -1 makes a row of zeros.  Rows may trade places, and a source serve many times.
+    -1 makes a row of zeros (with ``poison`` of bytes of 0xff, NaN in fp16, bf16 and fp32).
+    Rows may trade places, and a source serve many times.
 
     ``sources``: integers (checked), or a one-dimensional integer tensor of the GPU, whose
-    indices out of range make zeros too.  ``destinations``: distinct integers, known to the
+    indices out of range do the same.  ``destinations``: distinct integers, known to the
     host; default every row.  Up to 2048 rows may trade places; more where no source is
     another row's destination.  The tensors' rows are dense, and their memory neither
     overlaps nor interleaves.  Capturable where host indices are at most 192.  No gradient flows
@@ -249,7 +251,7 @@ def move_rows_(tensors, sources, destinations=None, *, dim: int = 0) -> None:
         flat += (f[0], f[0], f[1], f[2], f[1], f[2], f[3], f[4])
     if n:
         _changed(tensors)
-        _launch(flat, rows, rows, n, src, dst, disjoint, tensors[0])
+        _launch(flat, rows, rows, n, src, dst, disjoint, poison, tensors[0])
 
 
 __all__ = ["select_rows", "move_rows_"]

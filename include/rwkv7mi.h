@@ -664,12 +664,14 @@ int rwkv7mi_slot_copy(const void* src, int64_t src_layer_stride,
  * bytes, any alignment).  s(r) and d(r) come from src_index / dst_index (device
  * arrays), from src_list / dst_list (host arrays of at most 192, copied with
  * the launch) or are r where both are NULL.  s(r) outside 0 .. src_rows - 1
- * (say -1) writes zeros, d(r) outside 0 .. dst_rows - 1 nothing.  The
+ * (say -1) writes zeros, or, with the flag RWKV7MI_ROWS_POISON, bytes of 0xff
+ * (NaN in fp16, bf16 and fp32); d(r) outside 0 .. dst_rows - 1 nothing.  The
  * destinations are distinct.  A tensor with src == dst is moved in place (a row
  * onto itself is left alone); otherwise its src and dst do not overlap (src may
  * be NULL where src_rows is 0).  No device index lies in what is written.  Rows
- * that trade places in place: at most 2048; `disjoint` says that no source is
- * another row's destination, which lifts that.  At most 4194240 rows a call. */
+ * that trade places in place: at most 2048; the flag RWKV7MI_ROWS_DISJOINT says
+ * that no source is another row's destination, which lifts that.  At most 4194240
+ * rows a call. */
 typedef struct {
   const void* src;
   void* dst;
@@ -677,10 +679,11 @@ typedef struct {
   int64_t dst_outer_stride, dst_row_stride;
   int64_t row_bytes, outer;
 } rwkv7mi_rows;
+enum { RWKV7MI_ROWS_DISJOINT = 1, RWKV7MI_ROWS_POISON = 2 };
 int rwkv7mi_rows_move(int n, const rwkv7mi_rows* tensors, int64_t src_rows,
                       int64_t dst_rows, int64_t nrows, const int64_t* src_index,
                       const int64_t* dst_index, const int64_t* src_list,
-                      const int64_t* dst_list, int disjoint, void* stream);
+                      const int64_t* dst_list, int flags, void* stream);
 
 /* ------------------------------------------------------------ beam search */
 

@@ -61,3 +61,51 @@ def test_rows_of_empty_tensors_are_zeros():
         got = mi.select_rows([e, full], index, dim=1)
         assert [t.shape for t in got] == [(3, 2, 5), (2, 2, 40)] and not any(t.any() for t in got)
     mi.move_rows_([e, full], [], dim=1)
+
+
+@pytest.mark.parametrize("state", [torch.float32, torch.float16])
+def test_cache_edits_by_a_wrong_index_on_the_gpu(state):
+    """Nothing waits to look at an index on the GPU: a row out of range is NaN, not a state to go on with."""
+    model = _model()
+    model.state_dtype = state
+    for scattered in (False, True):
+        c = _cache(model, 4)
+        if scattered:
+            c._map(lambda t: t.clone())
+        old = [t.clone() for t in c._all_tensors()]
+        c.reorder_cache(torch.tensor([2, 4, -1, 0, 1 << 40], device="cuda"))
+        for t, o in zip(c._all_tensors(), old):
+            assert torch.equal(t[[0, 3]], o[[2, 0]])
+            bad = t[[1, 2, 4]]
+            assert bad.isnan().all() if t.is_floating_point() else (bad == -1).all()
+    runner = model.graph_runner(3)
+    c = _cache(model, 3)
+    runner.replay(torch.zeros(3, dtype=torch.long, device="cuda"), c)
+    old = [t.clone() for t in runner.cache._all_tensors()]
+    c.reorder_cache(torch.tensor([1, 3, 1], device="cuda"))
+    assert c._native_graph_bound_to(runner)
+    for t, o in zip(runner.cache._all_tensors(), old):
+        assert torch.equal(t[[0, 2]], o[[1, 1]])
+        assert t[1].isnan().all() if t.is_floating_point() else (t[1] == -1).all()
+    logits = runner.replay(torch.zeros(3, dtype=torch.long, device="cuda"), c)
+    assert logits[1].isnan().all() and not logits[[0, 2]].isnan().any()
+    runner.cache.zero_()
+
+
+def test_rows_of_all_kinds_poisoned():
+    import rwkv7mi as mi
+    from test_gpu_state_rows import _tensors
+
+    for rows in (3, 70, 200):
+        ts = _tensors(rows)
+        idx = torch.arange(rows, device="cuda").flip(0)
+        idx[1::3] = torch.tensor([-1, rows, -5, 1 << 50], device="cuda").repeat(rows)[:len(idx[1::3])]
+        good = (idx >= 0) & (idx < rows)
+        old = [t.clone() for t in ts]
+        new = mi.select_rows(ts, idx, dim=1, poison=True)
+        mi.move_rows_(ts, idx, dim=1, poison=True)
+        for a, b, o in zip(new, ts, old):
+            assert torch.equal(a[:, good], o[:, idx[good]]) and torch.equal(b[:, good], o[:, idx[good]])
+            for t in (a[:, ~good], b[:, ~good]):
+                assert t.isnan().all() if t.is_floating_point() else (t == -1).all()
+        assert not any(t[:, ~good].any() for t in mi.select_rows(old, idx, dim=1))

@@ -137,3 +137,23 @@ def test_rows_apart_are_moved_whatever_follows_them(calls):
         with pytest.raises(ValueError, match="apart"):
             mi.move_rows_([bad], [0] * bad.shape[1], dim=1)
     assert len(calls) == done
+
+
+def test_an_index_out_of_range_is_marked_in_cache_edits(calls, monkeypatch):
+    from rwkv7mi.model import NativeRWKV7Cache
+
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    c = NativeRWKV7Cache.zeros(_config(), 3, "cpu")
+    c.select_batch([1, 0])
+    assert calls[-1][1][9] == 3  # (poison, and nothing trades places)
+    c._map(lambda t: t.clone())
+    c.select_batch([1, 0])
+    assert calls[-1][1][9] == 3
+    import rwkv7mi as mi
+
+    mi.select_rows([torch.zeros(3, 4)], [0, -1])
+    assert calls[-1][1][9] == 1
+    mi.move_rows_([torch.zeros(3, 4)], [1, 0, -1])
+    assert calls[-1][1][9] == 0
+    mi.move_rows_([torch.zeros(3, 4)], [1, 0, -1], poison=True)
+    assert calls[-1][1][9] == 2
