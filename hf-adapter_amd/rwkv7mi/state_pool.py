@@ -176,10 +176,10 @@ class RWKV7StatePool:
 
     def reorder(self, slots, generations, parents) -> None:
         """``slots[i]`` takes the state that ``slots[parents[i]]`` had before the call, all at
-        once and in one launch: the beams of a search.  ``parents``: positions in ``slots``,
-        as many, on the host, or an integer tensor of the GPU (:func:`~.beam.beam_step`'s rows),
-        for which the slots have seen as many tokens (a position out of range on the GPU
-        zeroes the slot's state)."""
+        once: the beams of a search.  ``parents``: positions in ``slots``, as many, on the host
+        (one launch), or an integer tensor of the GPU (:func:`~.beam.beam_step`'s rows; a few small
+        operations look the slots up before the launch), for which the slots have seen as many
+        tokens (a position out of range on the GPU zeroes the slot's state)."""
         self.check(slots, generations)
         slots = [int(s) for s in slots]
         n = len(slots)
