@@ -48,6 +48,8 @@ def _family(t: torch.Tensor, dim: int, name: str):
 def _apart(f) -> bool:
     """Whether the rows of a family lie apart (they are written)."""
     _, step, row, size, outer, rows, _ = f
+    if not (size and outer and rows):
+        return True
     spans = ((row, rows), (step, outer)) if row <= step else ((step, outer), (row, rows))
     for s, k in spans:
         if k > 1:

@@ -157,3 +157,13 @@ def test_an_index_out_of_range_is_marked_in_cache_edits(calls, monkeypatch):
     assert calls[-1][1][9] == 0
     mi.move_rows_([torch.zeros(3, 4)], [1, 0, -1], poison=True)
     assert calls[-1][1][9] == 2
+
+
+def test_no_rows_are_moved(calls):
+    """Tensors without rows, without parts, or with rows of nothing: all apart, and nothing is launched for no index."""
+    import rwkv7mi as mi
+
+    for t in (torch.empty(3, 0, 5), torch.empty(0, 4, 5), torch.empty(3, 4, 0), torch.empty(3, 8, 5)[:, 8:]):
+        mi.move_rows_([t], list(range(t.shape[1])), dim=1)
+        mi.move_rows_([t], [], [], dim=1)
+        mi.select_rows([torch.empty(3, 2, 5)[:, :0], ], [], dim=1, out=[torch.empty(3, 0, 5)])
