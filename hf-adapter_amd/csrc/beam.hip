@@ -907,9 +907,14 @@ int64_t bm_slice(int dtype, int runs) { return (int64_t)BM_THREADS * runs * (dty
 int64_t bm_slices(int64_t V, int dtype, int runs) { return (V + bm_slice(dtype, runs) - 1) / bm_slice(dtype, runs); }
 
 // Runs of a lane: 8, whose slices share the bound and the ranking among the most logits, where there are
-// logits for 512 such workgroups, 4 down to 128 and 2 below, which fill the card sooner.  us with 2, 4, 8
-// runs, rows of 65536 fp16 logits: 16 rows 8.8, 9.3, 10.0; 32 10.0, 9.6, 10.0; 128 14.9, 13.3, 13.0; 512
-// 35.0, 29.7, 24.0.
+// logits for 512 such workgroups, 4 down to 128 and 2 below, which fill the card sooner.  us of a selection
+// with 2, 4, 8 runs, rows of 65536 logits (the rule takes 2 below 32 rows, 4 below 128, 8 from there; of fp32
+// below 16 and 64):
+//   rows      4              32              128               256               512
+//   fp16  8.7 9.0 9.6   9.7 9.8 10.2   14.5 13.7 13.9   18.8 18.5 17.3   27.0 22.3 21.6
+//   bf16  8.9 9.3 10.5  9.7 9.7 10.6   15.4 14.6 14.6   19.9 20.6 18.1   28.0 24.2 23.8
+//   fp32  9.4 8.8 9.5  10.4 9.6 9.9    18.5 15.7 15.8   25.6 20.4 20.6   42.4 31.9 32.7
+// (It was fitted to fp16.  fp32 would take 4 runs throughout: 1 to 8% less.)
 int bm_runs(int64_t rows, int64_t V, int dtype) {
   const int64_t logits = rows * V, unit = bm_slice(dtype, 8);
   return logits >= 512 * unit ? 8 : logits >= 128 * unit ? 4 : 2;

@@ -70,9 +70,10 @@ def _clear(name: str, written, read, states=()) -> None:
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | None = None, *, normalized: bool = False,
                 out=None, workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """The ``candidates`` (default twice the beams, at most 128) best continuations of each
-    prompt: ``logits [prompts * beams, n]`` (fp16, bf16 or fp32; or ``[prompts, beams, n]``),
-    ``scores [prompts, beams]`` (fp32) the beams' running sums of log-probabilities.
+    """The ``candidates`` (default twice the beams; 128, and the continuations there are, at most)
+    best continuations of each prompt: ``logits [prompts * beams, n]`` (fp16, bf16 or fp32; or
+    ``[prompts, beams, n]``; at most 65535 rows), ``scores [prompts, beams]`` (fp32) the beams'
+    running sums of log-probabilities.
 
     Returns ``(scores fp32, tokens int64, rows int64)``, each ``[prompts, candidates]``, best
     first, equal ones by beam, then logit, then token; ``rows`` are rows of ``logits``.  A continuation's
