@@ -48,24 +48,33 @@ def _scratch(workspace, need, like, name):
     return workspace
 
 
-def _range(t: torch.Tensor, size: int | None = None):
-    """The addresses of ``t`` (rows of any distance), or of its first ``size`` bytes."""
-    at = t.data_ptr()
-    if size is None:
-        size = (sum((k - 1) * s for k, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else 0
-    return at, at + size
+def _rows_range(t: torch.Tensor):
+    """The addresses of a matrix whose rows are any distance apart."""
+    at, (rows, n) = t.data_ptr(), t.shape
+    return at, at + (((rows - 1) * t.stride(0) + (n - 1) * t.stride(1) + 1) * t.element_size() if rows and n else 0)
 
 
-def _clear(name: str, written, read, states=()) -> None:
-    """Refuses ranges that are written and meet another one: of ``written``, of ``read``, or of the
-    states' (sorted, apart from each other)."""
-    for i, (a, b) in enumerate(written):
-        hit = any(c < b and a < d for c, d in (*written[:i], *read))
-        for ends in states:
-            k = bisect.bisect_left(ends, (b,))
-            hit |= k > 0 and ends[k - 1][1] > a
-        if hit and a < b:
-            raise ValueError(f"{name}: outputs or workspace overlap each other or what is read")
+def _clear(name: str, written, sizes, read, states=()) -> None:
+    """Refuses tensors of ``written`` (None: not given; dense, of which ``sizes`` bytes count) that meet another one,
+    a range of ``read``, or one of the states' (sorted, apart from each other)."""
+    taken = list(read)
+    for t, size in zip(written, sizes):
+        if t is None or not size:
+            continue
+        a = t.data_ptr()
+        b = a + size
+        for c, d in taken:
+            if c < b and a < d:
+                break
+        else:
+            for ends in states:
+                k = bisect.bisect_left(ends, (b,))
+                if k and ends[k - 1][1] > a:
+                    break
+            else:
+                taken.append((a, b))
+                continue
+        raise ValueError(f"{name}: outputs or workspace overlap each other or what is read")
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | None = None, *, normalized: bool = False,
@@ -95,7 +104,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | No
     if m < 1:
         raise ValueError(f"{name}: candidates must be positive")
     _lib.require_same_device(logits, scores, *(out or ()), workspace, name=name)
-    given = ()
+    given = out is not None
     if out is None:
         out = (scores.new_empty((prompts, m)), scores.new_empty((prompts, m), dtype=torch.int64),
                scores.new_empty((prompts, m), dtype=torch.int64))
@@ -106,14 +115,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int | No
         for t, want in zip(out, (torch.float32, torch.int64, torch.int64)):
             if tuple(t.shape) != (prompts, m) or t.dtype is not want or not t.is_contiguous():
                 raise ValueError(f"{name}: out must be contiguous fp32, int64, int64 [prompts, candidates]")
-        given = out
     rows, n = logits.shape
     need = _workspace(rows, n, m)
     if given or workspace is not None:
-        written = [_range(t) for t in given]
-        if workspace is not None:
-            written.append(_range(workspace, need))
-        _clear(name, written, (_range(logits), _range(scores)))
+        size = 8 * prompts * m
+        _clear(name, (*out, workspace) if given else (None, None, None, workspace), (size // 2, size, size, need),
+               (_rows_range(logits), _rows_range(scores)))
     workspace = _scratch(workspace, need, logits, name)
     scores = scores.contiguous()  # (a copy lives until the launch)
     with _lib.on_device(logits):
@@ -319,11 +326,9 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id=None, leng
             raise ValueError(f"{name}: next_tokens and rows must be contiguous int64 tensors of one entry per row")
     n = logits.shape[1]
     need = _workspace(total, n, m)
-    written = [_range(t) for t in (next_tokens, rows) if t is not None]
-    if workspace is not None:
-        written.append(_range(workspace, need))
-    if written:
-        _clear(name, written, (_range(logits),), (state._ends,) if to is state else (state._ends, to._ends))
+    if next_tokens is not None or rows is not None or workspace is not None:
+        _clear(name, (next_tokens, rows, workspace), (8 * total, 8 * total, need), (_rows_range(logits),),
+               (state._ends,) if to is state else (state._ends, to._ends))
     if next_tokens is None:
         next_tokens = state.tokens.new_empty(total)
     if rows is None:
