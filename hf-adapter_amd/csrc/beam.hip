@@ -21,8 +21,8 @@
 // ranked by counting.  -inf is never gathered: a masked row costs no more than
 // another.  Values in numbers that LDS does not hold (long ties) are drawn one by
 // one instead.  Bound by memory and vector instructions together for many rows:
-// 67 MB in 17.7 us, 3.8 TB/s, the vector units busy for 57% of the busy cycles;
-// latency-bound for few (4.6 us for 4 rows).  (The least of the maxima of
+// 67 MB in 17.1 us, 3.9 TB/s, the vector units busy for 57% of the busy cycles;
+// latency-bound for few (4.4 us for 4 rows).  (The least of the maxima of
 // 16 groups of lanes as the bound, without the search: a selection of 64 x 8 rows
 // 26.6 us against 24.9.)
 //
@@ -30,13 +30,13 @@
 // 64 bits, and selects among their K S M candidates the same way, the bound from
 // the lists' heads; the step's bookkeeping (ends, hypotheses, places of the
 // beams) follows in the same workgroup, two of its waves deciding without a
-// barrier.  Latency-bound, a chain of short phases: 4.7 us for one prompt of 4
-// beams, 8.2 for 64 of 8, 9 to 14 (by what reaches the bound) for 4 of 32 with 64
-// candidates; as a step's 7.9 and 16.8 for the first two.
+// barrier.  Latency-bound, a chain of short phases: 4.8 us for one prompt of 4
+// beams, 7.8 for 64 of 8, 9 to 15 (by what reaches the bound) for 4 of 32 with 64
+// candidates; as a step's 8.1 and 17.2 for the first two.
 //
-// Whole selections in a captured graph: 1 x 4 rows of 65536 fp16 logits 8.7 us,
-// 64 x 8 24.0 (12.5 at the rate of a large copy), 4 x 32 fp32 25.8; steps of the
-// first two 11.5 and 43.1, texts of 4096 tokens of room included in the second.
+// Whole selections in a captured graph: 1 x 4 rows of 65536 fp16 logits 8.7 to
+// 9.0 us, 64 x 8 24.0 (12.5 at the rate of a large copy), 4 x 32 fp32 25.8; steps of
+// the first two 11.5 and 42.7, texts of 4096 tokens of room included in the second.
 #include "common.h"
 
 namespace rwkv7mi {

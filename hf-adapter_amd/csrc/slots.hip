@@ -53,14 +53,15 @@ __global__ __launch_bounds__(256) void slot_copy_kernel(const SlotCopy C) {
 // (THREADS x LOADS units of 16 bytes over the rows, a power of two).
 //
 // HBM-bound.  The stores go past the caches: behind ordinary ones (in brackets)
-// the same moves of states that the caches do not hold take up to 1.4 times as
-// long, and where they hold them, with a pass over the states behind the move,
-// both are the same within 2%.  us for the fp32 states of the 7.2B model (33.5
-// MB a row): 8 chats of 4 beams in place, 0.99 GB, 177 [188]; one row to 8, 0.31
-// GB, 51 [64]; two rows to four each in new tensors, 0.34 GB, 52 [72]; the 2.9B
-// model's fp16 pool of 33, 9 rows moved and 5 made zero, 0.25 GB, 51 [59]; 4 rows
-// of the 0.1B model 4.5 [4.6].  (Behind ordinary stores, 4 loads a lane: 8% less to
-// 13% more, the largest moves losing; 16: up to a third more.)
+// the same moves of states that the caches do not hold take up to 1.3 times as
+// long.  us for the fp32 states of the 7.2B model (33.5 MB a row): 8 chats of 4
+// beams in place, 0.99 GB, 183 [189]; one row to 8, 0.31 GB, 50 [64]; two rows to
+// four each in new tensors, 0.34 GB, 51 [67]; the 2.9B model's fp16 pool of 33, 9
+// rows moved and 5 made zero, 0.25 GB, 48 [58]; 4 rows of the 0.1B model 4.2 [4.3].
+// (Rows trading places in pairs, states of 9 to 537 MB: 0 to 9% more than behind
+// ordinary stores, with a pass over the states behind the move up to 2%.  In an
+// earlier build, behind ordinary stores, 4 loads a lane: 8% less to 13% more, the
+// largest moves losing; 16: up to a third more.)
 namespace {
 
 constexpr int RW_TENSORS = 24;   // of a launch
